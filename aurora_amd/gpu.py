@@ -23,7 +23,8 @@ from ._lib import AuroraError
 __all__ = [
     "AuroraError", "GpuContext", "GpuBuffer", "GemmKernel", "GemmTransposeBKernel",
     "OuterProductAccumKernel", "CausalMhaForwardKernel", "CausalMhaBackwardKernel",
-    "MhaKvCacheKernel",
+    "MhaKvCacheKernel", "PagedKvCache", "PagedBatch", "RotaryTableKernel", "PagedKvAppendKernel",
+    "PagedMhaKernel",
 ]
 
 
@@ -253,3 +254,116 @@ class MhaKvCacheKernel(_Kernel):
         _need("MhaKvCacheKernel scratch", self.scratch_len(n_head, max_len, b), scratch)
         ctx.call("aur_mha_kv_step_batched", _p(q_new), _p(k_history), _p(v_history),
                  _p(out), _p(scratch), _p(t_total_dev), t_max, b, n_head, d_head, max_len)
+
+
+class _PagedCacheStruct(C.Structure):
+    """aur_paged_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_uint32), ("page_len", C.c_uint32),
+                ("n_kv_head", C.c_uint32), ("d_head", C.c_uint32), ("dtype", C.c_uint32)]
+
+
+class _PagedBatchStruct(C.Structure):
+    """aur_paged_batch."""
+    _fields_ = [("tok_off", C.c_void_p), ("own_len", C.c_void_p), ("pages", C.c_void_p),
+                ("prefix_pages", C.c_void_p), ("b", C.c_uint32), ("max_pages", C.c_uint32),
+                ("n_tok", C.c_uint32), ("max_tok", C.c_uint32), ("max_own", C.c_uint32),
+                ("n_prefix_pages", C.c_uint32), ("prefix_len", C.c_uint32)]
+
+
+class PagedKvCache:
+    """A paged K/V cache (aur_paged_cache): two pools [n_pages, page_len, n_kv_head*d_head] of "f32"
+    or "bf16" elements that the caller owns."""
+
+    DTYPES = {"f32": 0, "bf16": 1}
+
+    def __init__(self, k, v, n_pages, page_len, n_kv_head, d_head, dtype="f32"):
+        if dtype not in self.DTYPES:
+            raise ValueError(f"PagedKvCache: dtype {dtype!r}, one of {sorted(self.DTYPES)}")
+        self.k, self.v, self.dtype = k, v, dtype
+        self.n_pages, self.page_len, self.n_kv_head, self.d_head = n_pages, page_len, n_kv_head, d_head
+        size = 4 if dtype == "f32" else 2
+        for b in (k, v):
+            if isinstance(b, GpuBuffer) and b.nbytes < size * self.elements:
+                raise ValueError(f"PagedKvCache: pool of {b.nbytes} bytes, {size * self.elements} needed")
+        self._struct = _PagedCacheStruct(_p(k), _p(v), n_pages, page_len, n_kv_head, d_head, self.DTYPES[dtype])
+        self.ref = C.addressof(self._struct)
+
+    @property
+    def elements(self) -> int:
+        """Elements of one pool."""
+        return self.n_pages * self.page_len * self.n_kv_head * self.d_head
+
+    @classmethod
+    def zeros(cls, ctx: GpuContext, n_pages, page_len, n_kv_head, d_head, dtype="f32") -> "PagedKvCache":
+        n = n_pages * page_len * n_kv_head * d_head
+        np_type = np.float32 if dtype == "f32" else np.uint16
+        return cls(GpuBuffer.zeros(ctx, n, np_type), GpuBuffer.zeros(ctx, n, np_type), n_pages, page_len,
+                   n_kv_head, d_head, dtype)
+
+    def free(self) -> None:
+        for b in (self.k, self.v):
+            if isinstance(b, GpuBuffer):
+                b.free()
+
+
+class PagedBatch:
+    """A batch of sequences on a paged cache (aur_paged_batch): device arrays tok_off [b+1], own_len
+    [b], pages [b, max_pages] and prefix_pages, int32, and the host's bounds on what they hold."""
+
+    def __init__(self, tok_off, own_len, pages, b, max_pages, n_tok, max_tok, max_own, prefix_pages=0,
+                 n_prefix_pages=0, prefix_len=0):
+        _need("PagedBatch tok_off", b + 1, tok_off)
+        _need("PagedBatch own_len", b, own_len)
+        _need("PagedBatch pages", b * max_pages, pages)
+        _need("PagedBatch prefix_pages", n_prefix_pages, prefix_pages)
+        self.tok_off, self.own_len, self.pages, self.prefix_pages = tok_off, own_len, pages, prefix_pages
+        self.b, self.n_tok, self.max_own, self.prefix_len = b, n_tok, max_own, prefix_len
+        self._struct = _PagedBatchStruct(_p(tok_off), _p(own_len), _p(pages), _p(prefix_pages), b, max_pages,
+                                         n_tok, max_tok, max_own, n_prefix_pages, prefix_len)
+        self.ref = C.addressof(self._struct)
+
+
+class RotaryTableKernel(_Kernel):
+    """table [n_pos, rot_dim/2, 2] = (cos, sin)(position·θ^(-2u/rot_dim))."""
+
+    def dispatch_into(self, ctx, table, n_pos, rot_dim, theta=10000.0):
+        _need("RotaryTableKernel table", n_pos * rot_dim, table)
+        ctx.call("aur_rotary_table", _p(table), n_pos, rot_dim, theta)
+
+
+def _rows(n, ld, d) -> int:
+    """Elements from the first row's start to the last one's end."""
+    return (n - 1) * ld + d if n > 0 else 0
+
+
+class PagedKvAppendKernel(_Kernel):
+    """Appends k and v of the batch's new tokens to the cache, k rotated by its position, and puts the
+    rotated q into q_out (q = q_out = 0: no q)."""
+
+    def dispatch_into(self, ctx, cache, batch, q, ld_q, k, v, ld_kv, q_out, ld_qo, table, n_pos, rot_dim,
+                      n_head, pairs=False):
+        n, row = batch.n_tok, cache.n_kv_head * cache.d_head
+        _need("PagedKvAppendKernel q", _rows(n, ld_q, n_head * cache.d_head), q)
+        _need("PagedKvAppendKernel q_out", _rows(n, ld_qo, n_head * cache.d_head), q_out)
+        _need("PagedKvAppendKernel k/v", _rows(n, ld_kv, row), k, v)
+        _need("PagedKvAppendKernel table", n_pos * rot_dim, table)
+        ctx.call("aur_kv_append_paged", cache.ref, batch.ref, _p(q), ld_q, _p(k), _p(v), ld_kv, _p(q_out), ld_qo,
+                 _p(table), n_pos, rot_dim, n_head, 1 if pairs else 0)
+
+
+class PagedMhaKernel(_Kernel):
+    """Attention of the batch's new tokens over the shared prefix and their own keys (lse = 0: none)."""
+
+    @staticmethod
+    def scratch_len(cache, batch, n_head) -> int:
+        return (_lib.load().aur_mha_paged_ws_bytes(cache.ref, batch.ref, n_head) + 3) // 4
+
+    def dispatch_into(self, ctx, cache, batch, q, ld_q, out, ld_o, lse, scratch, scratch_len, n_head):
+        d = n_head * cache.d_head
+        _need("PagedMhaKernel q", _rows(batch.n_tok, ld_q, d), q)
+        _need("PagedMhaKernel out", _rows(batch.n_tok, ld_o, d), out)
+        if lse:
+            _need("PagedMhaKernel lse", batch.n_tok * n_head, lse)
+        _need("PagedMhaKernel scratch", scratch_len, scratch)
+        ctx.call("aur_mha_paged", cache.ref, batch.ref, _p(q), ld_q, _p(out), ld_o, _p(lse), _p(scratch),
+                 4 * scratch_len, n_head)

@@ -211,6 +211,79 @@ int aur_mha_kv_step_batched(aur_ctx* ctx, const float* q_new,
                             uint32_t t_max, uint32_t b, uint32_t n_head,
                             uint32_t d_head, uint32_t max_len);
 
+/* ---- paged K/V cache --------------------------------------------------------
+ * No reference counterpart (its KvCacheGpu keeps one contiguous history per
+ * sequence, src/gpu/kv_cache.rs:21-92): a pool of pages that sequences take as
+ * they grow, and a prefix that the sequences of a batch share, held once.
+ *
+ * A cache is two pools [n_pages, page_len, n_kv_head*d_head] of fp32 or bf16,
+ * 16-byte aligned (a key's head h at column offset h*d_head).  page_len is a
+ * power of two; d_head a multiple of 8 up to 128 (AUR_ELIMIT otherwise).
+ *
+ * A batch is `b` sequences with new tokens.  Rows tok_off[s] .. tok_off[s+1] of
+ * the token tensors are sequence s's n_s new tokens; rows from tok_off[b] on
+ * belong to none and are left as they are.  own_len[s] counts its tokens in the
+ * cache, the new ones among them; row j of them lies in page
+ * pages[s*max_pages + j/page_len].  In front of every sequence stand the
+ * prefix_len tokens of prefix_pages.  New token i of a sequence has the own
+ * index j = own_len - n_s + i and the position prefix_len + j.  A prefix is
+ * itself written as a batch of one sequence without a prefix.
+ * The arrays lie on the device, so a captured step sees their new values; the
+ * host's max_tok, max_own, max_pages and n_tok bound them: n_s <= max_tok,
+ * own_len <= max_own <= max_pages*page_len, tok_off[b] <= n_tok, tok_off
+ * ascending.  Values beyond the bounds are cut to them, so that nothing out of
+ * range is touched (results then mean nothing); page numbers outside
+ * [0, n_pages) read and write nothing: the keys count as not there. */
+#define AUR_PAGED_F32 0u
+#define AUR_PAGED_BF16 1u
+typedef struct {
+  void* k;
+  void* v;
+  uint32_t n_pages, page_len, n_kv_head, d_head, dtype;
+} aur_paged_cache;
+typedef struct {
+  const int32_t* tok_off;
+  const int32_t* own_len;
+  const int32_t* pages;
+  const int32_t* prefix_pages;
+  uint32_t b, max_pages, n_tok, max_tok, max_own, n_prefix_pages, prefix_len;
+} aur_paged_batch;
+
+/* table[n_pos][rot_dim/2][2] = (cos, sin)(position * theta^(-2u/rot_dim)),
+ * angles in 64 bits. */
+int aur_rotary_table(aur_ctx* ctx, float* table, uint32_t n_pos, uint32_t rot_dim, float theta);
+
+/* Appends the new tokens' k and v [n_tok, n_kv_head*d_head] (row stride ld_kv)
+ * to the cache; k, and q [n_tok, n_head*d_head] on its way to q_out, are first
+ * rotated by their positions: columns (u, u + rot_dim/2) of each head as a pair,
+ * or with pairs != 0 columns (2u, 2u + 1); columns from rot_dim on are copied.
+ * rot_dim is a multiple of 8 up to d_head, 0 for no rotation (table may be NULL
+ * then); the table holds n_pos >= prefix_len + max_own positions.  q and q_out
+ * may be one buffer, or both NULL.  bf16 pools take the nearest value, ties to
+ * even.  Rows 16-byte aligned, strides multiples of 4.  A token with j < 0
+ * (own_len below n_s) is skipped, q_out included. */
+int aur_kv_append_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,
+                        const float* q, uint32_t ld_q, const float* k, const float* v,
+                        uint32_t ld_kv, float* q_out, uint32_t ld_qo, const float* table,
+                        uint32_t n_pos, uint32_t rot_dim, uint32_t n_head, int pairs);
+
+/* Attention of the new tokens over prefix and own keys: query token i of a
+ * sequence sees the whole prefix and own keys 0 .. j.  q, out [n_tok,
+ * n_head*d_head] fp32 (row strides ld_q, ld_o), n_head a multiple of n_kv_head
+ * (query head h reads K/V head h / (n_head/n_kv_head)), scale 1/sqrt(d_head).
+ * lse [n_tok, n_head] receives the log-sum-exp of the scaled scores (may be
+ * NULL).  A row whose keys all have score -inf, or that sees none, gets out 0
+ * and lse -inf; values at keys that a row does not see never reach it.
+ * `scratch` is caller-owned, 16-byte aligned, of scratch_bytes >=
+ * aur_mha_paged_ws_bytes(cache, batch, n_head) (0: it may be NULL), which goes
+ * by the host's fields alone; calls that overlap in time need a scratch each.
+ * Sums are fp32 and joined in a fixed order: the same call gives the same bits. */
+size_t aur_mha_paged_ws_bytes(const aur_paged_cache* cache, const aur_paged_batch* batch,
+                              uint32_t n_head);
+int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,
+                  const float* q, uint32_t ld_q, float* out, uint32_t ld_o, float* lse,
+                  float* scratch, size_t scratch_bytes, uint32_t n_head);
+
 /* ---- model: DecoderTransformerGpu / KvCacheGpu ----------------------------
  * The caller of the hot path (src/gpu/transformer.rs:32-116, 949-2640),
  * running B sequences through every GEMM together (M = B·T rows).  The
