@@ -23,8 +23,11 @@
 // consecutive columns of V are rows of four MFMAs (row r of MFMA c is column
 // 4r + c), so V needs no transposition.
 #include "attention.hpp"
+#include "attention_split.hpp"
 #include "common.hpp"
 #include "paged.hpp"
+
+#include <type_traits>
 
 using namespace aurattn;
 using namespace aurpaged;
@@ -51,245 +54,521 @@ struct MhaArgs {
   int p_items;                    // items 0 .. p_items-1 are the prefix's
 };
 
-__device__ __forceinline__ floatx4 load4(const float* p) { return *reinterpret_cast<const floatx4*>(p); }
-__device__ __forceinline__ floatx4 load4(const __bf16* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  return floatx4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                 __uint_as_float(u.y & 0xffff0000u)};
+typedef unsigned uint2v __attribute__((ext_vector_type(2)));
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+
+// ---------------------------------------------------------------- an item
+
+struct Item {
+  int s, hk, part;
+  int row0, n_rows, tok0;  // first query row, how many rows there are, the token of row 0
+  int x0, x1;              // keys of the axis
+  int pre, first;          // the axis's prefix keys; keys that row 0's token sees
+  bool of_prefix;
+};
+
+// Key x of the axis is the prefix's while x < pre, then the sequence's own.  The page's number can
+// be asked for before the sequence's length is known: the table is read inside its bounds anyway.
+__device__ __forceinline__ int page_of(const MhaArgs& a, int s, int pre, int x) {
+  if (x < pre) return a.b.prefix_pages[min(x, a.b.prefix_len - 1) >> a.sh];
+  return a.b.max_own > 0 ? a.b.pages[(size_t)s * a.b.max_pages + min((x - pre) >> a.sh, a.b.max_pages - 1)] : -1;
+}
+// Pool row of key x, or −1 where there is none.
+__device__ __forceinline__ int row_of(const MhaArgs& a, const Item& it, int x, int page) {
+  const int i = x < it.pre ? x : x - it.pre;
+  return x < it.x1 && (unsigned)page < (unsigned)a.n_pages ? (page << a.sh) + (i & ((1 << a.sh) - 1)) : -1;
 }
 
-// DT: d_head in blocks of 16 columns, rounded up.
-template <class T, int DT, int RT>
-__global__ void __launch_bounds__(64 * NW) paged_mha_kernel(MhaArgs a) {
-  constexpr int VB = (DT + 3) / 4;  // blocks of 64 columns of V
-  constexpr int KT = STEP / 16;
-  constexpr int R = 16 * RT, OS = 64 * VB + 4;
-  __shared__ float sm[NW][R], sl[NW][R];
-  __shared__ __attribute__((aligned(16))) float so[R][OS];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int g = lane >> 4, l16 = lane & 15;
-  const float sl2 = a.scale * LOG2E;
-
-  // Which rows, which keys.  Key x < pre of the item's axis is the prefix's x, others are own.
-  int item = blockIdx.x, s = 0, part, x0, x1, row0, n_rows, tok0, pre, first = 0;
-  const bool of_prefix = item < a.p_items;
-  int hk;
-  if (of_prefix) {
-    hk = item % a.Hkv;
+// The block's item; `page` is the page of key x0 + lead.  False: nothing to do.
+template <int R>
+__device__ __forceinline__ bool take_item(const MhaArgs& a, Item& it, int lead, int& page) {
+  int item = blockIdx.x;
+  it.of_prefix = item < a.p_items;
+  it.s = 0;
+  it.tok0 = 0;
+  it.first = 0;
+  if (it.of_prefix) {
+    it.hk = item % a.Hkv;
     item /= a.Hkv;
-    const int tile = item % a.p_tiles;
-    part = item / a.p_tiles;
-    tok0 = 0;
-    row0 = tile * R;
-    n_rows = a.b.n_tok * a.G;
-    pre = a.b.prefix_len;
-    x0 = part * a.p_keys;
-    x1 = min(x0 + a.p_keys, pre);
-  } else {
-    item -= a.p_items;
-    hk = item % a.Hkv;
-    item /= a.Hkv;
-    const int tile = item % a.o_tiles;
-    item /= a.o_tiles;
-    s = item % a.b.b;
-    part = item / a.b.b;
-    const Seq q = sequence(a.b, s);
-    tok0 = q.lo;
-    row0 = tile * R;
-    n_rows = q.n * a.G;
-    pre = a.pooled ? 0 : a.b.prefix_len;
-    x0 = part * a.o_keys;
-    if (row0 >= n_rows || (part > 0 && x0 >= pre + q.len)) return;
-    first = pre + q.len - q.n + 1;  // keys that the sequence's first new token sees
-    x1 = min(x0 + a.o_keys, max(first + (min(row0 + R, n_rows) - 1) / a.G, pre));
-    if (a.pooled) part += a.p_splits;
+    it.row0 = item % a.p_tiles * R;
+    it.part = item / a.p_tiles;
+    it.n_rows = a.b.n_tok * a.G;
+    it.pre = a.b.prefix_len;
+    it.x0 = it.part * a.p_keys;
+    it.x1 = min(it.x0 + a.p_keys, it.pre);
+    page = page_of(a, 0, it.pre, it.x0 + lead);
+    return true;
   }
+  item -= a.p_items;
+  it.hk = item % a.Hkv;
+  item /= a.Hkv;
+  it.row0 = item % a.o_tiles * R;
+  item /= a.o_tiles;
+  it.s = item % a.b.b;
+  it.part = item / a.b.b;
+  it.pre = a.pooled ? 0 : a.b.prefix_len;
+  it.x0 = it.part * a.o_keys;
+  page = page_of(a, it.s, it.pre, it.x0 + lead);
+  const Seq q = sequence(a.b, it.s);
+  it.tok0 = q.lo;
+  it.n_rows = q.n * a.G;
+  if (it.row0 >= it.n_rows || (it.part > 0 && it.x0 >= it.pre + q.len)) return false;
+  it.first = it.pre + q.len - q.n + 1;
+  it.x1 = min(it.x0 + a.o_keys, max(it.first + (min(it.row0 + R, it.n_rows) - 1) / a.G, it.pre));
+  if (a.pooled) it.part += a.p_splits;
+  return true;
+}
 
-  // Rows of this lane (one per tile of 16): token, head and how many keys of the axis it sees.
-  int vis[RT];
-  floatx4 qf[RT][DT];
-  int vmin = 0x7fffffff;
+// The lane's rows, one of each tile of 16: the query's address, and how many keys of the axis it sees.
+template <int RT>
+struct Rows {
+  const float* q[RT];  // null: no row
+  int vis[RT], vmin;   // vmin: the fewest that a row of the item's tile sees
+};
+template <int RT>
+__device__ __forceinline__ void take_rows(const MhaArgs& a, const Item& it, int row0, int l16, Rows<RT>& r) {
+  r.vmin = 0x7fffffff;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = row0 + 16 * r + l16;
-    const bool live = row < n_rows;
-    const int t = live ? row / a.G : 0, h = hk * a.G + (live ? row - t * a.G : 0);
-    vis[r] = !live ? 0 : of_prefix ? pre : max(first + t, pre);
-    if (live) vmin = min(vmin, vis[r]);
-    const float* qp = a.q + (size_t)(tok0 + t) * a.ld_q + (size_t)h * a.dh;
-#pragma unroll
-    for (int c = 0; c < DT; ++c) {
-      const int col = 16 * c + 4 * g;
-      qf[r][c] = live && col < a.dh ? load4(qp + col) * sl2 : floatx4{0.f, 0.f, 0.f, 0.f};
-    }
+  for (int i = 0; i < RT; ++i) {
+    const int row = row0 + 16 * i + l16, t = row / a.G;
+    const bool live = row < it.n_rows;
+    r.q[i] = live ? a.q + (size_t)(it.tok0 + t) * a.ld_q + (size_t)(it.hk * a.G + row - t * a.G) * a.dh : nullptr;
+    r.vis[i] = !live ? 0 : it.of_prefix ? it.pre : max(it.first + t, it.pre);
+    if (live) r.vmin = min(r.vmin, r.vis[i]);
   }
 #pragma unroll
-  for (int m = 1; m < 16; m *= 2) vmin = min(vmin, __shfl_xor(vmin, m, 64));
+  for (int m = 1; m < 16; m *= 2) r.vmin = min(r.vmin, __shfl_xor(r.vmin, m, 64));
+}
 
-  const T* kp = static_cast<const T*>(a.k);
-  const T* vp = static_cast<const T*>(a.v);
-  const size_t ld = (size_t)a.Hkv * a.dh;
-  const size_t head = (size_t)hk * a.dh;
-  // Pool row of key x, or −1 where there is none.
-  auto place = [&](int x) {
-    if (x >= x1) return -1;
-    const bool p = x < pre;
-    const int i = p ? x : x - pre;
-    const int page = p ? a.b.prefix_pages[i >> a.sh] : a.b.pages[(size_t)s * a.b.max_pages + (i >> a.sh)];
-    return (unsigned)page < (unsigned)a.n_pages ? (page << a.sh) + (i & ((1 << a.sh) - 1)) : -1;
-  };
-  floatx4 kf[KT][DT], vf[KT][4][VB];
-  auto load_k = [&](int at) {
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const T* p = kp + (size_t)max(__shfl(at, 16 * kt + l16, 64), 0) * ld + head;
-#pragma unroll
-      for (int c = 0; c < DT; ++c) {
-        const int col = 16 * c + 4 * g;
-        kf[kt][c] = DT * 16 == a.dh || col < a.dh ? load4(p + col) : floatx4{0.f, 0.f, 0.f, 0.f};
-      }
-    }
-  };
-  auto load_v = [&](int at) {
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = __shfl(at, 16 * kt + 4 * g + e, 64);
-        const T* p = vp + (size_t)max(row, 0) * ld + head;
-#pragma unroll
-        for (int b = 0; b < VB; ++b) {
-          const int col = 64 * b + 4 * l16;
-          // a key that is not there adds nothing, whatever lies in the row
-          vf[kt][e][b] = row >= 0 && col < a.dh ? load4(p + col) : floatx4{0.f, 0.f, 0.f, 0.f};
-        }
-      }
-  };
-
-  floatx4 acc[RT][VB][4];
+// Running maximum (log2 domain), sum and unnormalised output of RT tiles of 16 rows: lane (g, l16) has row
+// l16's m, its own keys' share of l, and in acc[.][b][c][i] the columns 64b + 16g + 4i + c.
+template <int DT, int RT>
+struct Sums {
+  static constexpr int VB = (DT + 3) / 4;
   float m[RT], l[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int b = 0; b < VB; ++b)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[r][b][c] = floatx4{0.f, 0.f, 0.f, 0.f};
-  }
-  int x = x0 + STEP * w;
-  int at = place(x + (lane & 31));
-  if (x < x1) load_k(at);
-  for (; x < x1; x += STEP * NW) {
-    load_v(at);
-    const unsigned long long there = __ballot(at >= 0);
-    const int at_next = place(x + STEP * NW + (lane & 31));
-    floatx4 st[RT][KT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        st[r][kt] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < DT; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) st[r][kt] = mfma16x16x4(kf[kt][c][e], qf[r][c][e], st[r][kt]);
-      }
-    if (x + STEP * NW < x1) load_k(at_next);
-    at = at_next;
-    const bool mixed = x + STEP > vmin;  // some row does not see some key
-    bool odd = false;                    // … and a value that 0 times would not remove is there
-    if (mixed) {
-      float z = 0.f;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int b = 0; b < VB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z += 0.f * vf[kt][e][b][i];
-      odd = __ballot(!(z == 0.f)) != 0;
-    }
-    const bool masked = mixed || there != ~0ull;
+  floatx4 acc[RT][VB][4];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      if (masked) {
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = 16 * kt + 4 * g + e;
-            if (x + key >= vis[r] || !(there >> key & 1)) st[r][kt][e] = -INFINITY;
-          }
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-        mx = fmaxf(mx, fmaxf(fmaxf(st[r][kt][0], st[r][kt][1]), fmaxf(st[r][kt][2], st[r][kt][3])));
-      const float m_new = fmaxf(m[r], rows4_max(mx));
-      const float ms = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m[r] - ms);
-      m[r] = m_new;
-      float ps = 0.f;
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          st[r][kt][e] = __builtin_amdgcn_exp2f(st[r][kt][e] - ms);
-          ps += st[r][kt][e];
-        }
-      l[r] = l[r] * alpha + ps;
+      m[r] = -INFINITY;
+      l[r] = 0.f;
 #pragma unroll
       for (int b = 0; b < VB; ++b)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][b][c] *= alpha;
+        for (int c = 0; c < 4; ++c) acc[r][b][c] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
-    if (!odd) {
+  }
+};
+
+// Four columns of a row's result: a record, or the output itself.
+__device__ __forceinline__ void store(const MhaArgs& a, const Item& it, int row, int c, floatx4 o, float M, float L) {
+  const int t = row / a.G, h = it.hk * a.G + row - t * a.G;
+  const size_t token = (size_t)it.tok0 + t;
+  if (a.part_o) {
+    const size_t rec = ((size_t)it.part * a.b.n_tok + token) * a.H + h;
+    *reinterpret_cast<floatx4*>(a.part_o + rec * a.dh + c) = o;
+    if (c == 0) {
+      a.part_ml[2 * rec] = M;
+      a.part_ml[2 * rec + 1] = L;
+    }
+  } else {
+    *reinterpret_cast<floatx4*>(a.out + token * a.ld_o + (size_t)h * a.dh + c) =
+        L == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : o * (1.f / L);
+    if (c == 0 && a.lse) a.lse[token * a.H + h] = L == 0.f ? -INFINITY : (M + __log2f(L)) * LN2;
+  }
+}
+
+// ---------------------------------------------------------------- 32 keys in registers
+
+__device__ __forceinline__ floatx4 load4(const float* p) { return *reinterpret_cast<const floatx4*>(p); }
+
+// 32 keys as their loads left them.  K lies as the MFMA takes it (lane (g, l16): key l16 of 16, fp32
+// columns 16c + 4g …, bf16 columns 32c + 8g …), of V lane (g, l16) has columns 64b + 4·l16 … of the
+// keys 16kt + 4g + e.  `at`: the pool row of key lane % 32, or −1; such a key loads row 0, its score is
+// masked and its V taken as zero.  Columns past the head are its last ones again: of K they become
+// zeros before use, of V they end in output columns that nobody stores.
+template <class T, int DT>
+struct Keys32 {
+  static constexpr bool F32 = std::is_same<T, float>::value;
+  static constexpr int VB = (DT + 3) / 4, KC = F32 ? DT : (DT + 1) / 2;
+  using K4 = typename std::conditional<F32, floatx4, uint4v>::type;
+  using V4 = typename std::conditional<F32, floatx4, uint2v>::type;
+  K4 k[2][KC];
+  V4 v[2][4][VB];
+  template <bool STREAM>
+  __device__ __forceinline__ void load_k(const MhaArgs& a, int hk, int at, int g, int l16) {
+    const size_t ld = (size_t)a.Hkv * a.dh;
+    const T* kp = static_cast<const T*>(a.k) + (size_t)hk * a.dh;
+    constexpr int W = F32 ? 4 : 8;  // columns of a lane's piece
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
+    for (int kt = 0; kt < 2; ++kt) {
+      const T* p = kp + (size_t)max(__shfl(at, 16 * kt + l16, 64), 0) * ld;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+      for (int c = 0; c < KC; ++c) k[kt][c] = get<STREAM, K4>(p + min(4 * W * c + W * g, a.dh - W));
+    }
+  }
+  template <bool STREAM>
+  __device__ __forceinline__ void load_v(const MhaArgs& a, int hk, int at, int g, int l16) {
+    const size_t ld = (size_t)a.Hkv * a.dh;
+    const T* vp = static_cast<const T*>(a.v) + (size_t)hk * a.dh;
 #pragma unroll
-          for (int b = 0; b < VB; ++b)
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+      for (int e = 0; e < 4; ++e) {
+        const T* p = vp + (size_t)max(__shfl(at, 16 * kt + 4 * g + e, 64), 0) * ld;
 #pragma unroll
-              for (int r = 0; r < RT; ++r)
-                acc[r][b][c] = mfma16x16x4(vf[kt][e][b][c], st[r][kt][e], acc[r][b][c]);
-    } else {
-      // An infinity or NaN among values that not every row sees: each row adds only those it does.
+        for (int b = 0; b < VB; ++b) v[kt][e][b] = get<STREAM, V4>(p + min(64 * b + 4 * l16, a.dh - 4));
+      }
+  }
+  // STREAM: read once, past the caches.
+  template <bool STREAM, class V>
+  static __device__ __forceinline__ V get(const T* p) {
+    if (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    return *reinterpret_cast<const V*>(p);
+  }
+  __device__ __forceinline__ void drop_missing(unsigned there, int g) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+      for (int e = 0; e < 4; ++e)
+        if (!(there >> (16 * kt + 4 * g + e) & 1))
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int b = 0; b < VB; ++b) v[kt][e][b] = V4{};
+  }
+};
+
+// x as the sum of three bf16 numbers, exactly but for what lies 2^-24 below it and more (8 bits each,
+// with the range of fp32, so no scales are needed; an infinity becomes NaN).
+__device__ __forceinline__ void split3(float x0, float x1, bf16x2& h, bf16x2& m, bf16x2& l) {
+  h = __builtin_convertvector(float2v{x0, x1}, bf16x2);
+  const float r0 = x0 - (float)h[0], r1 = x1 - (float)h[1];
+  m = __builtin_convertvector(float2v{r0, r1}, bf16x2);
+  l = __builtin_convertvector(float2v{r0 - (float)m[0], r1 - (float)m[1]}, bf16x2);
+}
+struct Split8 {
+  bf16x8 h, m, l;
+  __device__ __forceinline__ void set(int i, float x0, float x1) {
+    bf16x2 a, b, c;
+    split3(x0, x1, a, b, c);
+    h[i] = a[0], h[i + 1] = a[1];
+    m[i] = b[0], m[i + 1] = b[1];
+    l[i] = c[0], l[i + 1] = c[1];
+  }
+};
+__device__ __forceinline__ floatx4 mfma_bf16(bf16x8 a, bf16x8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// A wave's queries as the MFMA's second operand, times log2(e)/√d_head: fp32 pieces of 4 columns, or
+// for bf16 keys three bf16 parts of 8 columns.
+template <class T, int DT, int RT>
+struct Queries;
+template <int DT, int RT>
+struct Queries<float, DT, RT> {
+  floatx4 q[RT][DT];
+  __device__ __forceinline__ void load(const Rows<RT>& r, int dh, int g, float sl2) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < DT; ++c) {
+        const int col = 16 * c + 4 * g;
+        q[i][c] = r.q[i] && col < dh ? load4(r.q[i] + col) * sl2 : floatx4{0.f, 0.f, 0.f, 0.f};
+      }
+  }
+};
+template <int DT, int RT>
+struct Queries<__bf16, DT, RT> {
+  static constexpr int KC = (DT + 1) / 2;
+  Split8 q[RT][KC];
+  __device__ __forceinline__ void load(const Rows<RT>& r, int dh, int g, float sl2) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const int col = 32 * c + 8 * g;
+        floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+        if (r.q[i] && col < dh) {
+          x = load4(r.q[i] + col) * sl2;
+          y = load4(r.q[i] + col + 4) * sl2;
+        }
+        q[i][c].set(0, x[0], x[1]);
+        q[i][c].set(2, x[2], x[3]);
+        q[i][c].set(4, y[0], y[1]);
+        q[i][c].set(6, y[2], y[3]);
+      }
+  }
+};
+
+// Sᵀ tiles of 32 keys: st[r][kt][e] is key 16kt + 4g + e against row l16 of tile r.
+template <int DT, int RT>
+__device__ __forceinline__ void scores(const Keys32<float, DT>& x, const Queries<float, DT, RT>& q, int dh, int g,
+                                       floatx4 (&st)[RT][2]) {
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) st[r][kt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < DT; ++c) {
+      floatx4 k = x.k[kt][c];
+      if (c >= DT - (DT > 4 ? 2 : 1) && 16 * c + 4 * g >= dh) k = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) st[r][kt] = mfma16x16x4(k[e], q.q[r][c][e], st[r][kt]);
+    }
+  }
+}
+template <int DT, int RT>
+__device__ __forceinline__ void scores(const Keys32<__bf16, DT>& x, const Queries<__bf16, DT, RT>& q, int dh, int g,
+                                       floatx4 (&st)[RT][2]) {
+  constexpr int KC = (DT + 1) / 2;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) st[r][kt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      uint4v u = x.k[kt][c];
+      if (32 * c + 8 * g >= dh) u = uint4v{0, 0, 0, 0};
+      const bf16x8 k = __builtin_bit_cast(bf16x8, u);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) st[r][kt] = mfma_bf16(k, q.q[r][c].l, st[r][kt]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) st[r][kt] = mfma_bf16(k, q.q[r][c].m, st[r][kt]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) st[r][kt] = mfma_bf16(k, q.q[r][c].h, st[r][kt]);
+    }
+  }
+}
+
+// acc += Vᵀ·Pᵀ.
+template <int DT, int RT>
+__device__ __forceinline__ void add_values(const Keys32<float, DT>& x, const floatx4 (&st)[RT][2], Sums<DT, RT>& s) {
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int b = 0; b < Sums<DT, RT>::VB; ++b)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) s.acc[r][b][c] = mfma16x16x4(x.v[kt][e][b][c], st[r][kt][e], s.acc[r][b][c]);
+}
+template <int DT, int RT>
+__device__ __forceinline__ void add_values(const Keys32<__bf16, DT>& x, const floatx4 (&st)[RT][2], Sums<DT, RT>& s) {
+  // the MFMA's 8 keys of a lane group: 4g … 4g + 3 of both tiles of 16
+  Split8 p[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      p[r].set(4 * kt, st[r][kt][0], st[r][kt][1]);
+      p[r].set(4 * kt + 2, st[r][kt][2], st[r][kt][3]);
+    }
+#pragma unroll
+  for (int b = 0; b < Sums<DT, RT>::VB; ++b)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint4v u;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          u[2 * kt + i] = __builtin_amdgcn_perm(x.v[kt][2 * i + 1][b][c >> 1], x.v[kt][2 * i][b][c >> 1],
+                                                c & 1 ? 0x07060302u : 0x05040100u);
+      const bf16x8 v = __builtin_bit_cast(bf16x8, u);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s.acc[r][b][c] = mfma_bf16(v, p[r].l, s.acc[r][b][c]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s.acc[r][b][c] = mfma_bf16(v, p[r].m, s.acc[r][b][c]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) s.acc[r][b][c] = mfma_bf16(v, p[r].h, s.acc[r][b][c]);
+    }
+}
+
+// Scores that a row does not see become −∞.
+template <int RT>
+__device__ __forceinline__ void mask(floatx4 (&st)[RT][2], const int (&vis)[RT], int x, unsigned there, int g) {
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = 16 * kt + 4 * g + e;
+        if (x + key >= vis[r] || !(there >> key & 1)) st[r][kt][e] = -INFINITY;
+      }
+}
+
+// The running softmax: scores to exp2(score − new maximum), sums rescaled.
+template <int DT, int RT>
+__device__ __forceinline__ void soften(floatx4 (&st)[RT][2], Sums<DT, RT>& s) {
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+      mx = fmaxf(mx, fmaxf(fmaxf(st[r][kt][0], st[r][kt][1]), fmaxf(st[r][kt][2], st[r][kt][3])));
+    const float m_new = fmaxf(s.m[r], rows4_max(mx));
+    const float at = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(s.m[r] - at);
+    s.m[r] = m_new;
+    float ps = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        st[r][kt][e] = __builtin_amdgcn_exp2f(st[r][kt][e] - at);
+        ps += st[r][kt][e];
+      }
+    s.l[r] = s.l[r] * alpha + ps;
+#pragma unroll
+    for (int b = 0; b < Sums<DT, RT>::VB; ++b)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s.acc[r][b][c] *= alpha;
+  }
+}
+
+template <int DT, int RT>
+__device__ __forceinline__ bool finite(const Sums<DT, RT>& s) {
+  float z = 0.f;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    z += 0.f * s.l[r];
+#pragma unroll
+    for (int b = 0; b < Sums<DT, RT>::VB; ++b)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z += 0.f * s.acc[r][b][c][i];
+  }
+  return __ballot(z != 0.f) == 0;  // 0 times an infinity or NaN is NaN
+}
+
+// The sums of a wave's rows over keys x, x + stride, … again, where they came out as infinity or NaN:
+// scores by the fp32 MFMA from whole operands, and every row adds the values of those keys alone that
+// it sees (0 times an infinity that it does not see would be NaN).
+template <class T, int DT, int RT>
+__device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, int stride, Sums<DT, RT>& s) {
+  constexpr int VB = Sums<DT, RT>::VB;
+  const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
+  Rows<RT> rows;
+  take_rows(a, it, row0, l16, rows);
+  const T* kp = static_cast<const T*>(a.k) + (size_t)it.hk * a.dh;
+  const T* vp = static_cast<const T*>(a.v) + (size_t)it.hk * a.dh;
+  const size_t ld = (size_t)a.Hkv * a.dh;
+  const float sl2 = a.scale * LOG2E;
+  s.clear();
 #pragma unroll 1
-            for (int kg = 0; kg < 4; ++kg) {
-              const float p = __shfl(st[r][kt][e], 16 * kg + l16, 64);
-              const int key = 16 * kt + 4 * kg + e;
-              const bool seen = x + key < vis[r] && (there >> key & 1);
+  for (; x < it.x1; x += stride) {
+    const int at = row_of(a, it, x + (lane & 31), page_of(a, it.s, it.pre, x + (lane & 31)));
+    const unsigned there = (unsigned)__ballot(at >= 0);
+    floatx4 st[RT][2] = {};
 #pragma unroll
-              for (int b = 0; b < VB; ++b)
+    for (int kt = 0; kt < 2; ++kt) {
+      const T* p = kp + (size_t)max(__shfl(at, 16 * kt + l16, 64), 0) * ld;
+#pragma unroll 1
+      for (int c = 0; c < a.dh; c += 16) {
+        const bool live = c + 4 * g < a.dh;
+        floatx4 k = {0.f, 0.f, 0.f, 0.f};
+        if (live) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+          for (int e = 0; e < 4; ++e) k[e] = (float)p[c + 4 * g + e];
+        }
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const float v = __shfl(vf[kt][e][b][c], 16 * kg + 4 * g + i, 64);
-                    if (seen) acc[r][b][c][i] += p * v;
-                  }
-            }
+        for (int r = 0; r < RT; ++r) {
+          floatx4 q = {0.f, 0.f, 0.f, 0.f};
+          if (live && rows.q[r]) q = load4(rows.q[r] + c + 4 * g) * sl2;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st[r][kt] = mfma16x16x4(k[e], q[e], st[r][kt]);
+        }
+      }
     }
+    mask<RT>(st, rows.vis, x, there, g);
+    soften<DT, RT>(st, s);
+#pragma unroll 1
+    for (int key = 0; key < 32; ++key) {
+      const int row = __shfl(at, key, 64), from = (key & 12) * 4 + l16;
+      if (row < 0) continue;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const floatx4 pv = key < 16 ? st[r][0] : st[r][1];
+        const float pe = (key & 2) ? ((key & 1) ? pv[3] : pv[2]) : ((key & 1) ? pv[1] : pv[0]);
+        const float p = __shfl(pe, from, 64);
+        const bool seen = x + key < rows.vis[r];
+#pragma unroll
+        for (int b = 0; b < VB; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int col = 64 * b + 16 * g + 4 * i + c;
+              if (seen && col < a.dh) s.acc[r][b][c][i] += p * (float)vp[(size_t)row * ld + col];
+            }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- few rows: keys through the registers
+
+// Up to 16·RT rows an item.
+template <class T, int DT, int RT>
+__global__ void __launch_bounds__(64 * NW) paged_mha_kernel(MhaArgs a) {
+  constexpr int VB = Sums<DT, RT>::VB;
+  constexpr int R = 16 * RT, OS = 64 * VB + 4, STRIDE = STEP * NW;  // also a multiple of the tile kernels' keys
+  __shared__ float sm[NW][R], sl[NW][R];
+  __shared__ __attribute__((aligned(16))) float so[R][OS];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int g = lane >> 4, l16 = lane & 15, k32 = lane & 31;
+
+  Item it;
+  int page;
+  if (!take_item<R>(a, it, STEP * w + k32, page)) return;
+  int x = it.x0 + STEP * w;
+  Sums<DT, RT> s;
+  s.clear();
+  if (x < it.x1) {
+    Keys32<T, DT> keys;
+    int at = row_of(a, it, x + k32, page);
+    keys.template load_k<true>(a, it.hk, at, g, l16);
+    keys.template load_v<true>(a, it.hk, at, g, l16);
+    page = page_of(a, it.s, it.pre, x + STRIDE + k32);
+    Rows<RT> rows;
+    take_rows(a, it, it.row0, l16, rows);
+    Queries<T, DT, RT> q;
+    q.load(rows, a.dh, g, a.scale * LOG2E);
+    for (; x < it.x1; x += STRIDE) {
+      // the next keys' loads go out as soon as this step has used the registers
+      const bool more = x + STRIDE < it.x1;
+      const unsigned there = (unsigned)__ballot(at >= 0);
+      floatx4 st[RT][2];
+      scores(keys, q, a.dh, g, st);
+      if (more) {
+        at = row_of(a, it, x + STRIDE + k32, page);
+        keys.template load_k<true>(a, it.hk, at, g, l16);
+        page = page_of(a, it.s, it.pre, x + 2 * STRIDE + k32);
+      }
+      if (there != ~0u || x + STEP > rows.vmin) mask<RT>(st, rows.vis, x, there, g);
+      soften(st, s);
+      if (there != ~0u) keys.drop_missing(there, g);
+      add_values(keys, st, s);
+      if (more) keys.template load_v<true>(a, it.hk, at, g, l16);
+    }
+    if (!finite(s)) exact_sums<T, DT, RT>(a, it, it.row0, it.x0 + STEP * w, STRIDE, s);
   }
 
   // Join the four waves: common maximum, then their sums added in wave order.
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    l[r] = rows4_sum(l[r]);
+    s.l[r] = rows4_sum(s.l[r]);
     if (g == 0) {
-      sm[w][16 * r + l16] = m[r];
-      sl[w][16 * r + l16] = l[r];
+      sm[w][16 * r + l16] = s.m[r];
+      sl[w][16 * r + l16] = s.l[r];
     }
   }
   __syncthreads();
@@ -298,11 +577,11 @@ __global__ void __launch_bounds__(64 * NW) paged_mha_kernel(MhaArgs a) {
     float M = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NW; ++i) M = fmaxf(M, sm[i][16 * r + l16]);
-    const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - M);
+    const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s.m[r] - M);
 #pragma unroll
     for (int b = 0; b < VB; ++b)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[r][b][c] *= f;
+      for (int c = 0; c < 4; ++c) s.acc[r][b][c] *= f;
   }
   for (int i = 0; i < NW; ++i) {
     if (w == i) {
@@ -313,7 +592,7 @@ __global__ void __launch_bounds__(64 * NW) paged_mha_kernel(MhaArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             floatx4* p = reinterpret_cast<floatx4*>(&so[16 * r + l16][64 * b + 16 * g + 4 * j]);
-            const floatx4 v = {acc[r][b][0][j], acc[r][b][1][j], acc[r][b][2][j], acc[r][b][3][j]};
+            const floatx4 v = {s.acc[r][b][0][j], s.acc[r][b][1][j], s.acc[r][b][2][j], s.acc[r][b][3][j]};
             *p = i == 0 ? v : *p + v;
           }
     }
@@ -321,26 +600,293 @@ __global__ void __launch_bounds__(64 * NW) paged_mha_kernel(MhaArgs a) {
   }
   const int n4 = a.dh / 4;
   for (int i = tid; i < R * n4; i += 64 * NW) {
-    const int r = i / n4, c = 4 * (i - r * n4), row = row0 + r;
-    if (row >= n_rows) break;
-    const int t = row / a.G, h = hk * a.G + row - t * a.G;
+    const int r = i / n4, c = 4 * (i - r * n4);
+    if (it.row0 + r >= it.n_rows) break;
     float M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int j = 0; j < NW; ++j) M = fmaxf(M, sm[j][r]);
 #pragma unroll
     for (int j = 0; j < NW; ++j) L += (M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[j][r] - M)) * sl[j][r];
-    const floatx4 o = *reinterpret_cast<const floatx4*>(&so[r][c]);
-    const size_t token = (size_t)tok0 + t;
-    if (a.part_o) {
-      const size_t rec = ((size_t)part * a.b.n_tok + token) * a.H + h;
-      *reinterpret_cast<floatx4*>(a.part_o + rec * a.dh + c) = o;
-      if (c == 0) {
-        a.part_ml[2 * rec] = M;
-        a.part_ml[2 * rec + 1] = L;
+    store(a, it, it.row0 + r, c, *reinterpret_cast<const floatx4*>(&so[r][c]), M, L);
+  }
+}
+
+// ---------------------------------------------------------------- many rows: keys through LDS
+
+// 64·NR rows an item, 16·NR of a wave.  The block lays KT keys down in LDS as bf16 parts (fp32: three,
+// whose six products above 2^-24 of the largest the MFMA sums; bf16 keys are one part, Q and P three),
+// K as [key][column], V as [column][key], while the next keys' loads are under way.
+template <class T, int DT>
+struct TileGeo {
+  static constexpr bool F32 = std::is_same<T, float>::value;
+  static constexpr int PARTS = F32 ? 3 : 1;
+  static constexpr int KT = DT > 4 ? 32 : 64;      // keys of a tile
+  static constexpr int KC = (DT + 1) / 2;          // 32-column steps of a score
+  static constexpr int KROW = KC == 1 ? 64 : KC == 2 ? 128 : 256;
+  static constexpr int KPLANE = KT * KROW, VPLANE = DT * 16 * KT * 2;
+  static constexpr int TPR = 256 / KT, NI = (4 * KC + TPR - 1) / TPR;  // threads of a K row, octets of a thread
+  static constexpr int PAIRS = 8 * DT;             // V: a thread has 2 columns of 8 keys
+};
+// Granule q (16 bytes) of row r in rows of ROW bytes: every phase of 16 lanes covers the 64 banks once.
+template <int ROW>
+__device__ __forceinline__ int tile_granule(int r, int q) {
+  return ROW == 64 ? split_granule(r, q) : ROW == 128 ? granule128(r, q) : r * 256 + ((q ^ r) & 15) * 16;
+}
+
+template <class T, int DT, int NR>
+__global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
+  using G = TileGeo<T, DT>;
+  constexpr bool F32 = G::F32;
+  constexpr int KT = G::KT, KC = G::KC, NI = G::NI, NK = KT / 16;
+  __shared__ __attribute__((aligned(1024))) char ks[G::PARTS * G::KPLANE];
+  __shared__ __attribute__((aligned(1024))) char vs[G::PARTS * G::VPLANE];
+  __shared__ int places[3][KT];  // pool rows of the keys of this tile and the next two
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int g = lane >> 4, l16 = lane & 15;
+
+  Item it;
+  int page;
+  if (!take_item<64 * NR>(a, it, tid % KT, page)) return;
+  const int row0 = it.row0 + 16 * NR * w;  // this wave's
+  Rows<NR> rows;
+  take_rows(a, it, row0, l16, rows);
+  int vmax = 0;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) vmax = max(vmax, rows.vis[r]);
+#pragma unroll
+  for (int m = 1; m < 16; m *= 2) vmax = max(vmax, __shfl_xor(vmax, m, 64));
+
+  // Pool rows of a tile's keys; the pages' numbers are asked for a tile before they are needed.
+  int xp = it.x0 + tid % KT;  // the key whose page is under way
+  auto place = [&](int slot) {
+    if (tid < KT) places[slot][tid] = row_of(a, it, xp, page);
+    xp += KT;
+    page = page_of(a, it.s, it.pre, xp);
+  };
+  place(0);
+  place(1);
+  __syncthreads();
+
+  const size_t ld = (size_t)a.Hkv * a.dh;
+  const T* kp = static_cast<const T*>(a.k) + (size_t)it.hk * a.dh;
+  const T* vp = static_cast<const T*>(a.v) + (size_t)it.hk * a.dh;
+  const int kr = tid / G::TPR, ko = tid % G::TPR;  // K: row kr, octets ko + TPR·i
+  const int vc = tid % G::PAIRS, vg = tid / G::PAIRS;  // V: columns 2vc, 2vc + 1 of granule vg
+  const bool v_on = vg < KT / 8;
+  const int vkey = 32 * (vg >> 2) + 4 * (vg & 3);  // … the keys vkey + 16·(i/4) + i%4
+  floatx4 kx[NI][F32 ? 2 : 1];  // as loaded
+  float2v vx[8];
+  auto load = [&](int slot) {
+    const int at = places[slot][kr];
+    const T* p = kp + (size_t)max(at, 0) * ld;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = min(8 * (ko + G::TPR * i), a.dh - 8);
+      kx[i][0] = *reinterpret_cast<const floatx4*>(p + c);
+      if (F32) kx[i][F32] = *reinterpret_cast<const floatx4*>(p + c + 4);
+    }
+    const int c = min(2 * vc, a.dh - 2);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = v_on ? places[slot][vkey + 16 * (i >> 2) + (i & 3)] : -1;
+      vx[i] = float2v{0.f, 0.f};
+      if (row >= 0) {
+        const T* q = vp + (size_t)row * ld + c;
+        if (F32)
+          vx[i] = *reinterpret_cast<const float2v*>(q);
+        else
+          vx[i][0] = *reinterpret_cast<const float*>(q);
+      }
+    }
+  };
+  auto lay_down = [&] {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int q = ko + G::TPR * i;
+      if (4 * KC % G::TPR != 0 && q >= 4 * KC) continue;
+      const bool live = 8 * q < a.dh;
+      char* p = ks + tile_granule<G::KROW>(kr, q);
+      const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+      if (F32) {
+        const floatx4 x = live ? kx[i][0] : zero, y = live ? kx[i][F32] : zero;
+        Split8 s;
+        s.set(0, x[0], x[1]);
+        s.set(2, x[2], x[3]);
+        s.set(4, y[0], y[1]);
+        s.set(6, y[2], y[3]);
+        *reinterpret_cast<bf16x8*>(p) = s.h;
+        *reinterpret_cast<bf16x8*>(p + G::KPLANE) = s.m;
+        *reinterpret_cast<bf16x8*>(p + 2 * G::KPLANE) = s.l;
+      } else {
+        *reinterpret_cast<floatx4*>(p) = live ? kx[i][0] : zero;
+      }
+    }
+    if (!v_on) return;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      char* p = vs + tile_granule<2 * KT>(2 * vc + c, vg);
+      if (F32) {
+        Split8 s;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) s.set(i, vx[i][c], vx[i + 1][c]);
+        *reinterpret_cast<bf16x8*>(p) = s.h;
+        *reinterpret_cast<bf16x8*>(p + G::VPLANE) = s.m;
+        *reinterpret_cast<bf16x8*>(p + 2 * G::VPLANE) = s.l;
+      } else {
+        uint4v u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          u[i] = __builtin_amdgcn_perm(__float_as_uint(vx[2 * i + 1][0]), __float_as_uint(vx[2 * i][0]),
+                                       c ? 0x07060302u : 0x05040100u);
+        *reinterpret_cast<uint4v*>(p) = u;
+      }
+    }
+  };
+  load(0);
+
+  Queries<__bf16, DT, NR> q;
+  q.load(rows, a.dh, g, a.scale * LOG2E);
+  const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+  floatx4 acc[NR][DT];
+  float m[NR], l[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[r][d] = zero;
+  }
+
+  int slot = 0;
+  for (int x = it.x0; x < it.x1; x += KT) {
+    if (x > it.x0) __syncthreads();  // every wave is done with the last tile
+    lay_down();
+    const int next = slot == 2 ? 0 : slot + 1;
+    place(next == 2 ? 0 : next + 1);
+    __syncthreads();
+    if (x + KT < it.x1) load(next);
+    const unsigned long long there = __ballot(places[slot][lane % KT] >= 0);
+    slot = next;
+    if (x >= vmax) continue;  // none of the wave's rows sees this tile
+    floatx4 st[NR][NK];
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      bf16x8 kf[G::PARTS][KC];
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int i = 0; i < G::PARTS; ++i)
+          kf[i][c] = *reinterpret_cast<const bf16x8*>(ks + i * G::KPLANE + tile_granule<G::KROW>(16 * j + l16, 4 * c + g));
+#pragma unroll
+      for (int r = 0; r < NR; ++r) st[r][j] = zero;
+      // products in ascending size
+      auto add = [&](int part, auto of) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int r = 0; r < NR; ++r) st[r][j] = mfma_bf16(kf[part][c], of(q.q[r][c]), st[r][j]);
+      };
+      if (F32) add(F32 * 2, [](const Split8& s) { return s.h; });
+      add(0, [](const Split8& s) { return s.l; });
+      if (F32) {
+        add(F32, [](const Split8& s) { return s.m; });
+        add(F32, [](const Split8& s) { return s.h; });
+      }
+      add(0, [](const Split8& s) { return s.m; });
+      add(0, [](const Split8& s) { return s.h; });
+    }
+    if (there != ~0ull || x + KT > rows.vmin) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = 16 * j + 4 * g + e;
+            if (x + key >= rows.vis[r] || !(there >> key & 1)) st[r][j][e] = -INFINITY;
+          }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) mx = fmaxf(mx, fmaxf(fmaxf(st[r][j][0], st[r][j][1]), fmaxf(st[r][j][2], st[r][j][3])));
+      const float m_new = fmaxf(m[r], rows4_max(mx));
+      const float at = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m[r] - at);
+      m[r] = m_new;
+      float ps = 0.f;
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          st[r][j][e] = __builtin_amdgcn_exp2f(st[r][j][e] - at);
+          ps += st[r][j][e];
+        }
+      l[r] = l[r] * alpha + ps;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[r][d] *= alpha;
+    }
+#pragma unroll
+    for (int kk = 0; kk < KT / 32; ++kk) {
+      Split8 pf[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) pf[r].set(i, st[r][2 * kk + i / 4][i & 3], st[r][2 * kk + i / 4][(i & 3) + 1]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        bf16x8 vf[G::PARTS];
+#pragma unroll
+        for (int i = 0; i < G::PARTS; ++i)
+          vf[i] = *reinterpret_cast<const bf16x8*>(vs + i * G::VPLANE + tile_granule<2 * KT>(16 * d + l16, 4 * kk + g));
+        auto add = [&](int part, auto of) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) acc[r][d] = mfma_bf16(vf[part], of(pf[r]), acc[r][d]);
+        };
+        if (F32) add(F32 * 2, [](const Split8& s) { return s.h; });
+        add(0, [](const Split8& s) { return s.l; });
+        if (F32) {
+          add(F32, [](const Split8& s) { return s.m; });
+          add(F32, [](const Split8& s) { return s.h; });
+        }
+        add(0, [](const Split8& s) { return s.m; });
+        add(0, [](const Split8& s) { return s.h; });
+      }
+    }
+  }
+
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    float z = 0.f * l[r];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (DT * 16 == a.dh || 16 * d + 4 * g + i < a.dh) z += 0.f * acc[r][d][i];
+    const int row = row0 + 16 * r + l16;
+    if (__ballot(z != 0.f) == 0) {
+      const float L = rows4_sum(l[r]);
+      if (row < it.n_rows) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          if (DT * 16 == a.dh || 16 * d + 4 * g < a.dh) store(a, it, row, 16 * d + 4 * g, acc[r][d], m[r], L);
       }
     } else {
-      *reinterpret_cast<floatx4*>(a.out + token * a.ld_o + (size_t)h * a.dh + c) = L == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : o * (1.f / L);
-      if (c == 0 && a.lse) a.lse[token * a.H + h] = L == 0.f ? -INFINITY : (M + __log2f(L)) * LN2;
+      Sums<DT, 1> e;
+      exact_sums<T, DT, 1>(a, it, row0 + 16 * r, it.x0, STEP, e);
+      const float L = rows4_sum(e.l[0]);
+      if (row < it.n_rows) {
+#pragma unroll
+        for (int b = 0; b < Sums<DT, 1>::VB; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int col = 64 * b + 16 * g + 4 * j;
+            if (col < a.dh)
+              store(a, it, row, col, floatx4{e.acc[0][b][0][j], e.acc[0][b][1][j], e.acc[0][b][2][j], e.acc[0][b][3][j]},
+                    e.m[0], L);
+          }
+      }
     }
   }
 }
@@ -380,14 +926,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(MhaArgs a) {
 
 // How a call is cut into items, from what the host knows; the scratch's size follows from it.
 struct Plan {
-  int pooled, p_rt, o_rt, p_tiles, p_splits, p_keys, o_tiles, o_splits, o_keys;
+  int pooled, p_tile, o_tile, p_tiles, p_splits, p_keys, o_tiles, o_splits, o_keys;
   int parts() const { return p_splits + o_splits; }
 };
 
-int tiles_of(long long rows, int* rt) {
-  *rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  return (int)((rows + 16 * *rt - 1) / (16 * *rt));
-}
+// Rows of an item: 16 and 32 keep their keys in registers, 64 and 128 lay them down in LDS.
+int tile_of(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 constexpr uint32_t kMaxRows = 0x7fffff00u;  // query rows of a call, and a tile more, are ints
 constexpr int kItems = 1024;  // blocks that a launch aims at: 4 of each CU
@@ -396,11 +940,13 @@ Plan make_plan(const Batch& b, int Hkv, int G) {
   Plan p{};
   const int P = b.prefix_len;
   p.pooled = P > 0 && b.b > 1 && (long long)b.max_tok * G < 64;
-  p.o_tiles = tiles_of((long long)b.max_tok * G, &p.o_rt);
-  p.p_rt = 1;
-  if (p.pooled) p.p_tiles = tiles_of((long long)b.n_tok * G, &p.p_rt);
+  const long long o_rows = (long long)b.max_tok * G, p_rows = (long long)b.n_tok * G;
+  p.o_tile = tile_of(o_rows);
+  p.o_tiles = (int)((o_rows + p.o_tile - 1) / p.o_tile);
+  p.p_tile = tile_of(p_rows);
+  p.p_tiles = p.pooled ? (int)((p_rows + p.p_tile - 1) / p.p_tile) : 0;
   const int axis = b.max_own + (p.pooled ? 0 : P);
-  const int block = STEP * NW;
+  const int block = STEP * NW;  // also a multiple of the tile kernels' keys
   const double work = (double)Hkv * ((double)p.p_tiles * P + (double)b.b * p.o_tiles * axis);
   const double want = work / kItems;
   int keys = want > 1e9 ? 1000000000 : ((int)want + block - 1) / block * block;
@@ -416,29 +962,31 @@ size_t ws_floats(const Plan& p, const Batch& b, int H, int dh) {
 }
 
 template <class T, int DT>
-void launch_rt(const MhaArgs& a, int rt, unsigned items, hipStream_t st) {
-  const dim3 g(items), b(64 * NW);
-  if (rt == 1)
+void launch_rt(const MhaArgs& a, int tile, unsigned items, hipStream_t st) {
+  const dim3 g(items), b(256);
+  if (tile == 16)
     hipLaunchKernelGGL((paged_mha_kernel<T, DT, 1>), g, b, 0, st, a);
-  else if (rt == 2)
+  else if (tile == 32)
     hipLaunchKernelGGL((paged_mha_kernel<T, DT, 2>), g, b, 0, st, a);
+  else if (tile == 64)
+    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1>), g, b, 0, st, a);
   else
-    hipLaunchKernelGGL((paged_mha_kernel<T, DT, 4>), g, b, 0, st, a);
+    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 2>), g, b, 0, st, a);
 }
 
 template <class T>
-void launch_dt(const MhaArgs& a, int rt, unsigned items, hipStream_t st) {
+void launch_dt(const MhaArgs& a, int tile, unsigned items, hipStream_t st) {
   const int dt = (a.dh + 15) / 16;
-  if (dt == 1) launch_rt<T, 1>(a, rt, items, st);
-  else if (dt == 2) launch_rt<T, 2>(a, rt, items, st);
-  else if (dt == 3) launch_rt<T, 3>(a, rt, items, st);
-  else if (dt == 4) launch_rt<T, 4>(a, rt, items, st);
-  else if (dt <= 6) launch_rt<T, 6>(a, rt, items, st);
-  else launch_rt<T, 8>(a, rt, items, st);
+  if (dt == 1) launch_rt<T, 1>(a, tile, items, st);
+  else if (dt == 2) launch_rt<T, 2>(a, tile, items, st);
+  else if (dt == 3) launch_rt<T, 3>(a, tile, items, st);
+  else if (dt == 4) launch_rt<T, 4>(a, tile, items, st);
+  else if (dt <= 6) launch_rt<T, 6>(a, tile, items, st);
+  else launch_rt<T, 8>(a, tile, items, st);
 }
 
-void launch_items(const MhaArgs& a, bool f32, int rt, unsigned items, hipStream_t st) {
-  f32 ? launch_dt<float>(a, rt, items, st) : launch_dt<__bf16>(a, rt, items, st);
+void launch_items(const MhaArgs& a, bool f32, int tile, unsigned items, hipStream_t st) {
+  f32 ? launch_dt<float>(a, tile, items, st) : launch_dt<__bf16>(a, tile, items, st);
 }
 
 }  // namespace
@@ -496,11 +1044,11 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
   const bool f32 = cache->dtype == AUR_PAGED_F32;
   if (p.pooled) {
     a.p_items = (int)p_items;
-    launch_items(a, f32, p.p_rt, (unsigned)p_items, ctx->stream);
+    launch_items(a, f32, p.p_tile, (unsigned)p_items, ctx->stream);
     AUR_LAUNCH_CHECK(ctx, "paged_mha_kernel (prefix)");
     a.p_items = 0;
   }
-  launch_items(a, f32, p.o_rt, (unsigned)o_items, ctx->stream);
+  launch_items(a, f32, p.o_tile, (unsigned)o_items, ctx->stream);
   AUR_LAUNCH_CHECK(ctx, "paged_mha_kernel");
   if (floats) {
     hipLaunchKernelGGL(paged_join_kernel, dim3(a.b.n_tok), dim3(256), 0, ctx->stream, a);
