@@ -516,13 +516,19 @@ __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, in
 
 // ---------------------------------------------------------------- few rows: keys through the registers
 
-// Up to 16·RT rows an item.
-template <class T, int DT, int RT>
-__global__ void __launch_bounds__(64 * NW) paged_mha_kernel(MhaArgs a) {
-  constexpr int VB = Sums<DT, RT>::VB;
-  constexpr int R = 16 * RT, OS = 64 * VB + 4, STRIDE = STEP * NW;  // also a multiple of the tile kernels' keys
-  __shared__ float sm[NW][R], sl[NW][R];
-  __shared__ __attribute__((aligned(16))) float so[R][OS];
+// Up to 16 rows an item.
+template <int DT>
+struct RowsLds {
+  static constexpr int R = 16, OS = 64 * ((DT + 3) / 4) + 4;
+  float m[NW][R], l[NW][R];
+  __attribute__((aligned(16))) float o[R][OS];
+};
+template <class T, int DT>
+__device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
+  constexpr int VB = Sums<DT, 1>::VB, RT = 1, R = RowsLds<DT>::R, STRIDE = STEP * NW;
+  auto& sm = lds.m;
+  auto& sl = lds.l;
+  auto& so = lds.o;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = lane >> 4, l16 = lane & 15, k32 = lane & 31;
 
@@ -613,10 +619,11 @@ __global__ void __launch_bounds__(64 * NW) paged_mha_kernel(MhaArgs a) {
 
 // ---------------------------------------------------------------- many rows: keys through LDS
 
-// 64·NR rows an item, 16·NR of a wave.  The block lays KT keys down in LDS as bf16 parts (fp32: three,
-// whose six products above 2^-24 of the largest the MFMA sums; bf16 keys are one part, Q and P three),
-// K as [key][column], V as [column][key], while the next keys' loads are under way.
-template <class T, int DT>
+// 16·NR·W rows an item, 16·NR of each of the block's W waves.  The block lays KT keys down in LDS as
+// bf16 parts (fp32: three, whose six products above 2^-24 of the largest the MFMA sums; bf16 keys are
+// one part, Q and P three), K as [key][column], V as [column][key], while the next keys' loads are
+// under way.
+template <class T, int DT, int W>
 struct TileGeo {
   static constexpr bool F32 = std::is_same<T, float>::value;
   static constexpr int PARTS = F32 ? 3 : 1;
@@ -624,29 +631,38 @@ struct TileGeo {
   static constexpr int KC = (DT + 1) / 2;          // 32-column steps of a score
   static constexpr int KROW = KC == 1 ? 64 : KC == 2 ? 128 : 256;
   static constexpr int KPLANE = KT * KROW, VPLANE = DT * 16 * KT * 2;
-  static constexpr int TPR = 256 / KT, NI = (4 * KC + TPR - 1) / TPR;  // threads of a K row, octets of a thread
-  static constexpr int PAIRS = 8 * DT;             // V: a thread has 2 columns of 8 keys
+  static constexpr int TPR = 64 * W / KT, NI = (4 * KC + TPR - 1) / TPR;  // K: threads of a row, octets of a thread
+  static constexpr int VC = F32 && W == 8 ? 1 : 2, VN = 16 * DT / VC;      // V: a thread has VC columns of 8 keys
 };
 // Granule q (16 bytes) of row r in rows of ROW bytes: every phase of 16 lanes covers the 64 banks once.
 template <int ROW>
 __device__ __forceinline__ int tile_granule(int r, int q) {
   return ROW == 64 ? split_granule(r, q) : ROW == 128 ? granule128(r, q) : r * 256 + ((q ^ r) & 15) * 16;
 }
+__device__ __forceinline__ float max3(float x, float y, float z) {  // one instruction; NaN if one is
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x, y), z);
+}
 
-template <class T, int DT, int NR>
-__global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
-  using G = TileGeo<T, DT>;
+template <class T, int DT, int W>
+struct TileLds {
+  using G = TileGeo<T, DT, W>;
+  char k[G::PARTS * G::KPLANE], v[G::PARTS * G::VPLANE];
+  int places[3][G::KT];  // pool rows of the keys of this tile and the next two
+};
+template <class T, int DT, int NR, int W>
+__device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& lds) {
+  using G = TileGeo<T, DT, W>;
   constexpr bool F32 = G::F32;
-  constexpr int KT = G::KT, KC = G::KC, NI = G::NI, NK = KT / 16;
-  __shared__ __attribute__((aligned(1024))) char ks[G::PARTS * G::KPLANE];
-  __shared__ __attribute__((aligned(1024))) char vs[G::PARTS * G::VPLANE];
-  __shared__ int places[3][KT];  // pool rows of the keys of this tile and the next two
+  constexpr int KT = G::KT, KC = G::KC, NI = G::NI, NK = KT / 16, VC = G::VC;
+  char* const ks = lds.k;
+  char* const vs = lds.v;
+  auto& places = lds.places;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = lane >> 4, l16 = lane & 15;
 
   Item it;
   int page;
-  if (!take_item<64 * NR>(a, it, tid % KT, page)) return;
+  if (!take_item<16 * NR * W>(a, it, tid % KT, page)) return;
   const int row0 = it.row0 + 16 * NR * w;  // this wave's
   Rows<NR> rows;
   take_rows(a, it, row0, l16, rows);
@@ -671,11 +687,11 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
   const T* kp = static_cast<const T*>(a.k) + (size_t)it.hk * a.dh;
   const T* vp = static_cast<const T*>(a.v) + (size_t)it.hk * a.dh;
   const int kr = tid / G::TPR, ko = tid % G::TPR;  // K: row kr, octets ko + TPR·i
-  const int vc = tid % G::PAIRS, vg = tid / G::PAIRS;  // V: columns 2vc, 2vc + 1 of granule vg
+  const int vc = tid % G::VN * VC, vg = tid / G::VN;  // V: columns vc … of granule vg
   const bool v_on = vg < KT / 8;
   const int vkey = 32 * (vg >> 2) + 4 * (vg & 3);  // … the keys vkey + 16·(i/4) + i%4
   floatx4 kx[NI][F32 ? 2 : 1];  // as loaded
-  float2v vx[8];
+  float vx[8][F32 ? VC : 1];
   auto load = [&](int slot) {
     const int at = places[slot][kr];
     const T* p = kp + (size_t)max(at, 0) * ld;
@@ -685,17 +701,21 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
       kx[i][0] = *reinterpret_cast<const floatx4*>(p + c);
       if (F32) kx[i][F32] = *reinterpret_cast<const floatx4*>(p + c + 4);
     }
-    const int c = min(2 * vc, a.dh - 2);
+    const int c = min(vc, a.dh - VC);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int row = v_on ? places[slot][vkey + 16 * (i >> 2) + (i & 3)] : -1;
-      vx[i] = float2v{0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < (F32 ? VC : 1); ++j) vx[i][j] = 0.f;
       if (row >= 0) {
         const T* q = vp + (size_t)row * ld + c;
-        if (F32)
-          vx[i] = *reinterpret_cast<const float2v*>(q);
-        else
-          vx[i][0] = *reinterpret_cast<const float*>(q);
+        if (F32 && VC == 2) {
+          const float2v x = *reinterpret_cast<const float2v*>(q);
+          vx[i][0] = x[0];
+          vx[i][F32 ? VC - 1 : 0] = x[1];
+        } else {
+          vx[i][0] = *reinterpret_cast<const float*>(q);  // or a pair of bf16
+        }
       }
     }
   };
@@ -704,7 +724,7 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
     for (int i = 0; i < NI; ++i) {
       const int q = ko + G::TPR * i;
       if (4 * KC % G::TPR != 0 && q >= 4 * KC) continue;
-      const bool live = 8 * q < a.dh;
+      const bool live = DT * 16 == 32 * KC || 8 * q < a.dh;
       char* p = ks + tile_granule<G::KROW>(kr, q);
       const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
       if (F32) {
@@ -723,12 +743,12 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
     }
     if (!v_on) return;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      char* p = vs + tile_granule<2 * KT>(2 * vc + c, vg);
+    for (int c = 0; c < VC; ++c) {
+      char* p = vs + tile_granule<2 * KT>(vc + c, vg);
       if (F32) {
         Split8 s;
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) s.set(i, vx[i][c], vx[i + 1][c]);
+        for (int i = 0; i < 8; i += 2) s.set(i, vx[i][F32 ? c : 0], vx[i + 1][F32 ? c : 0]);
         *reinterpret_cast<bf16x8*>(p) = s.h;
         *reinterpret_cast<bf16x8*>(p + G::VPLANE) = s.m;
         *reinterpret_cast<bf16x8*>(p + 2 * G::VPLANE) = s.l;
@@ -757,17 +777,7 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
     for (int d = 0; d < DT; ++d) acc[r][d] = zero;
   }
 
-  int slot = 0;
-  for (int x = it.x0; x < it.x1; x += KT) {
-    if (x > it.x0) __syncthreads();  // every wave is done with the last tile
-    lay_down();
-    const int next = slot == 2 ? 0 : slot + 1;
-    place(next == 2 ? 0 : next + 1);
-    __syncthreads();
-    if (x + KT < it.x1) load(next);
-    const unsigned long long there = __ballot(places[slot][lane % KT] >= 0);
-    slot = next;
-    if (x >= vmax) continue;  // none of the wave's rows sees this tile
+  auto compute = [&](int x, unsigned long long there, auto some) {
     floatx4 st[NR][NK];
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
@@ -795,7 +805,7 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
       add(0, [](const Split8& s) { return s.m; });
       add(0, [](const Split8& s) { return s.h; });
     }
-    if (there != ~0ull || x + KT > rows.vmin) {
+    if (decltype(some)::value) {  // keys that some row does not see
 #pragma unroll
       for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -808,12 +818,17 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
     }
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      float mx = -INFINITY;
+      float mx = m[r];
 #pragma unroll
-      for (int j = 0; j < NK; ++j) mx = fmaxf(mx, fmaxf(fmaxf(st[r][j][0], st[r][j][1]), fmaxf(st[r][j][2], st[r][j][3])));
-      const float m_new = fmaxf(m[r], rows4_max(mx));
+      for (int j = 0; j < NK; ++j) mx = max3(max3(mx, st[r][j][0], st[r][j][1]), st[r][j][2], st[r][j][3]);
+      const float m_new = rows4_max(mx);
       const float at = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m[r] - at);
+      if (__ballot(m_new != m[r])) {  // a maximum grew: rarely, after the first tiles
+        const float alpha = __builtin_amdgcn_exp2f(m[r] - at);
+        l[r] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[r][d] *= alpha;
+      }
       m[r] = m_new;
       float ps = 0.f;
 #pragma unroll
@@ -823,9 +838,7 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
           st[r][j][e] = __builtin_amdgcn_exp2f(st[r][j][e] - at);
           ps += st[r][j][e];
         }
-      l[r] = l[r] * alpha + ps;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) acc[r][d] *= alpha;
+      l[r] += ps;
     }
 #pragma unroll
     for (int kk = 0; kk < KT / 32; ++kk) {
@@ -854,6 +867,23 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
         add(0, [](const Split8& s) { return s.h; });
       }
     }
+  };
+
+  int slot = 0;
+  for (int x = it.x0; x < it.x1; x += KT) {
+    if (x > it.x0) __syncthreads();  // every wave is done with the last tile
+    lay_down();
+    const int next = slot == 2 ? 0 : slot + 1;
+    place(next == 2 ? 0 : next + 1);
+    __syncthreads();
+    if (x + KT < it.x1) load(next);
+    const unsigned long long there = __ballot(places[slot][lane % KT] >= 0);
+    slot = next;
+    if (x >= vmax) continue;  // none of the wave's rows sees this tile
+    if (there != ~0ull || x + KT > rows.vmin)
+      compute(x, there, std::true_type{});
+    else
+      compute(x, there, std::false_type{});
   }
 
 #pragma unroll
@@ -891,66 +921,111 @@ __global__ void __launch_bounds__(256) paged_mha_tile_kernel(MhaArgs a) {
   }
 }
 
-// out and lse of a token's rows from the records of their ranges, in the ranges' order.
-__global__ void __launch_bounds__(256) paged_join_kernel(MhaArgs a) {
-  const int t = blockIdx.x;
-  const int s = sequence_of(a.b, t);
+// ---------------------------------------------------------------- launches
+
+template <class T, int DT>
+__global__ void __launch_bounds__(64 * NW, 2) paged_mha_rows_kernel(MhaArgs a) {
+  __shared__ RowsLds<DT> lds;
+  rows_item<T, DT>(a, lds);
+}
+
+template <class T, int DT, int NR, int W>
+__global__ void __launch_bounds__(64 * W, 2) paged_mha_tile_kernel(MhaArgs a) {
+  __shared__ __attribute__((aligned(1024))) TileLds<T, DT, W> lds;
+  tile_item<T, DT, NR, W>(a, lds);
+}
+
+// A decode step of many sequences in one launch: the prefix's items, bound by their products, beside the
+// own ones, bound by memory.
+template <class T, int DT>
+__global__ void __launch_bounds__(64 * NW, 2) paged_mha_step_kernel(MhaArgs a) {
+  __shared__ __attribute__((aligned(1024))) union {
+    TileLds<T, DT, NW> tile;
+    RowsLds<DT> rows;
+  } lds;
+  if ((int)blockIdx.x < a.p_items)
+    tile_item<T, DT, 1, NW>(a, lds.tile);
+  else
+    rows_item<T, DT>(a, lds.rows);
+}
+
+// out and lse of a row from the records of its ranges: one wave a row.  The lanes of a group have 4
+// columns each, the groups take every other range in turn and are added as a tree, so the order is fixed.
+__global__ void __launch_bounds__(256) paged_join_kernel(MhaArgs a, int lanes) {
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int t = (int)(row / a.H), h = (int)(row - (long long)t * a.H);
+  if (t >= a.b.n_tok) return;
+  int s = 0;
+  for (int i0 = 0; i0 < a.b.b; i0 += 64) {
+    const int i = i0 + lane;
+    s += __popcll(__ballot(i < a.b.b && a.b.tok_off[i + 1] <= t));
+  }
   if (s >= a.b.b) return;  // a row behind the last sequence
   const Seq q = sequence(a.b, s);
   if (t < q.lo || t - q.lo >= q.n) return;
   const int axis = q.len + (a.pooled ? 0 : a.b.prefix_len);
   const int np = a.p_splits + max((axis + a.o_keys - 1) / a.o_keys, 1);  // range 0 is always written
-  const int n4 = a.dh / 4;
-  const size_t step = (size_t)a.b.n_tok * a.H;
-  for (int i = threadIdx.x; i < a.H * n4; i += 256) {
-    const int h = i / n4, c = 4 * (i - h * n4);
-    size_t rec = (size_t)t * a.H + h;
-    float M = -INFINITY, L = 0.f;
-    floatx4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < np; ++p, rec += step) {
-      const float m = a.part_ml[2 * rec], l = a.part_ml[2 * rec + 1];
-      const floatx4 v = load4(a.part_o + rec * a.dh + c);
-      const float M1 = fmaxf(M, m), ms = M1 == -INFINITY ? 0.f : M1;
-      // a record without a maximum was summed against 0
-      const float f = M == -INFINITY ? (M1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(-ms)) : __builtin_amdgcn_exp2f(M - ms);
-      const float e = m == -INFINITY ? (M1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(-ms)) : __builtin_amdgcn_exp2f(m - ms);
-      L = L * f + l * e;
-      o = o * f + v * e;
-      M = M1;
-    }
-    *reinterpret_cast<floatx4*>(a.out + (size_t)t * a.ld_o + (size_t)h * a.dh + c) =
-        L == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : o * (1.f / L);
-    if (c == 0 && a.lse) a.lse[(size_t)t * a.H + h] = L == 0.f ? -INFINITY : (M + __log2f(L)) * LN2;
+  const size_t step = (size_t)a.b.n_tok * a.H, rec = (size_t)t * a.H + h;
+  const float* ml = a.part_ml + 2 * rec;
+  float M = -INFINITY;
+  for (int p = lane; p < np; p += 64) M = fmaxf(M, ml[2 * p * step]);
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) M = fmaxf(M, __shfl_xor(M, i, 64));
+  auto factor = [&](int p) { return M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[2 * p * step] - M); };
+  float L = 0.f;
+  for (int p = lane; p < np; p += 64) L += factor(p) * ml[2 * p * step + 1];
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) L += __shfl_xor(L, i, 64);
+  const int c = 4 * (lane % lanes), groups = 64 / lanes;
+  const float* o = a.part_o + rec * a.dh + min(c, a.dh - 4);
+  floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = lane / lanes; p < np; p += groups) v += load4(o + (size_t)p * step * a.dh) * factor(p);
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) {
+    if (i < lanes) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], i, 64);
   }
+  if (lane < lanes && c < a.dh)
+    *reinterpret_cast<floatx4*>(a.out + (size_t)t * a.ld_o + (size_t)h * a.dh + c) =
+        L == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v * (1.f / L);
+  if (lane == 0 && a.lse) a.lse[(size_t)t * a.H + h] = L == 0.f ? -INFINITY : (M + __log2f(L)) * LN2;
 }
 
 // How a call is cut into items, from what the host knows; the scratch's size follows from it.
 struct Plan {
   int pooled, p_tile, o_tile, p_tiles, p_splits, p_keys, o_tiles, o_splits, o_keys;
   int parts() const { return p_splits + o_splits; }
+  // One launch serves both kinds of items, unless the prefix has the larger tiles.
+  bool together() const { return p_tile <= 64; }
 };
 
-// Rows of an item: 16 and 32 keep their keys in registers, 64 and 128 lay them down in LDS.
-int tile_of(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Rows of an item: 16 keep their keys in registers, more lay them down in LDS.
+int tile_of(long long rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
 
 constexpr uint32_t kMaxRows = 0x7fffff00u;  // query rows of a call, and a tile more, are ints
-constexpr int kItems = 1024;  // blocks that a launch aims at: 4 of each CU
+constexpr int kItems = 2048;     // items that a launch aims at, two rounds of four blocks a CU
+constexpr int kLeastKeys = 256;  // of an item: two rounds of its waves
+constexpr int kPoolFrom = 32768;  // keys times heads that pooling saves, and from where it pays its join
 
 Plan make_plan(const Batch& b, int Hkv, int G) {
   Plan p{};
   const int P = b.prefix_len;
-  p.pooled = P > 0 && b.b > 1 && (long long)b.max_tok * G < 64;
   const long long o_rows = (long long)b.max_tok * G, p_rows = (long long)b.n_tok * G;
   p.o_tile = tile_of(o_rows);
   p.o_tiles = (int)((o_rows + p.o_tile - 1) / p.o_tile);
-  p.p_tile = tile_of(p_rows);
+  p.p_tile = p_rows <= 32 ? 16 : p_rows <= 256 ? 64 : 256;
+  const int p_tiles = (int)((p_rows + p.p_tile - 1) / p.p_tile);
+  p.pooled = o_rows < 64 && ((double)b.b * p.o_tiles - p_tiles) * Hkv * P >= kPoolFrom;
+  if (p.pooled && p.p_tile == 16 && p.o_tile > 16) p.p_tile = 64;
   p.p_tiles = p.pooled ? (int)((p_rows + p.p_tile - 1) / p.p_tile) : 0;
   const int axis = b.max_own + (p.pooled ? 0 : P);
-  const int block = STEP * NW;  // also a multiple of the tile kernels' keys
   const double work = (double)Hkv * ((double)p.p_tiles * P + (double)b.b * p.o_tiles * axis);
   const double want = work / kItems;
-  int keys = want > 1e9 ? 1000000000 : ((int)want + block - 1) / block * block;
-  if (keys < block) keys = block;
+  int keys = want > 1e9 ? 1000000000 : ((int)want + 127) / 128 * 128;
+  if (keys < kLeastKeys) keys = kLeastKeys;
   p.p_keys = p.o_keys = keys;
   p.p_splits = p.pooled ? (P + keys - 1) / keys : 0;
   p.o_splits = axis > keys ? (axis + keys - 1) / keys : 1;
@@ -961,32 +1036,35 @@ size_t ws_floats(const Plan& p, const Batch& b, int H, int dh) {
   return p.parts() > 1 ? (size_t)p.parts() * b.n_tok * H * (dh + 2) : 0;
 }
 
+// p_tile 0: items of one kind (or of one tile).
 template <class T, int DT>
-void launch_rt(const MhaArgs& a, int tile, unsigned items, hipStream_t st) {
-  const dim3 g(items), b(256);
-  if (tile == 16)
-    hipLaunchKernelGGL((paged_mha_kernel<T, DT, 1>), g, b, 0, st, a);
-  else if (tile == 32)
-    hipLaunchKernelGGL((paged_mha_kernel<T, DT, 2>), g, b, 0, st, a);
+void launch_tile(const MhaArgs& a, int p_tile, int tile, unsigned items, hipStream_t st) {
+  const dim3 g(items);
+  if (p_tile == 64 && tile == 16)
+    hipLaunchKernelGGL((paged_mha_step_kernel<T, DT>), g, dim3(256), 0, st, a);
+  else if (tile == 16)
+    hipLaunchKernelGGL((paged_mha_rows_kernel<T, DT>), g, dim3(256), 0, st, a);
   else if (tile == 64)
-    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1>), g, b, 0, st, a);
+    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 4>), g, dim3(256), 0, st, a);
+  else if (tile == 128)
+    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 8>), g, dim3(512), 0, st, a);
   else
-    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 2>), g, b, 0, st, a);
+    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 2, 8>), g, dim3(512), 0, st, a);
 }
 
 template <class T>
-void launch_dt(const MhaArgs& a, int tile, unsigned items, hipStream_t st) {
+void launch_head(const MhaArgs& a, int p_tile, int tile, unsigned items, hipStream_t st) {
   const int dt = (a.dh + 15) / 16;
-  if (dt == 1) launch_rt<T, 1>(a, tile, items, st);
-  else if (dt == 2) launch_rt<T, 2>(a, tile, items, st);
-  else if (dt == 3) launch_rt<T, 3>(a, tile, items, st);
-  else if (dt == 4) launch_rt<T, 4>(a, tile, items, st);
-  else if (dt <= 6) launch_rt<T, 6>(a, tile, items, st);
-  else launch_rt<T, 8>(a, tile, items, st);
+  if (dt == 1) launch_tile<T, 1>(a, p_tile, tile, items, st);
+  else if (dt == 2) launch_tile<T, 2>(a, p_tile, tile, items, st);
+  else if (dt == 3) launch_tile<T, 3>(a, p_tile, tile, items, st);
+  else if (dt == 4) launch_tile<T, 4>(a, p_tile, tile, items, st);
+  else if (dt <= 6) launch_tile<T, 6>(a, p_tile, tile, items, st);
+  else launch_tile<T, 8>(a, p_tile, tile, items, st);
 }
 
-void launch_items(const MhaArgs& a, bool f32, int tile, unsigned items, hipStream_t st) {
-  f32 ? launch_dt<float>(a, tile, items, st) : launch_dt<__bf16>(a, tile, items, st);
+void launch_items(const MhaArgs& a, bool f32, int p_tile, int tile, unsigned items, hipStream_t st) {
+  f32 ? launch_head<float>(a, p_tile, tile, items, st) : launch_head<__bf16>(a, p_tile, tile, items, st);
 }
 
 }  // namespace
@@ -1038,20 +1116,27 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
   }
   const uint64_t p_items = (uint64_t)a.Hkv * p.p_tiles * p.p_splits;
   const uint64_t o_items = (uint64_t)a.Hkv * p.o_tiles * a.b.b * p.o_splits;
-  if (p_items > kMaxBlocks || o_items > kMaxBlocks)
+  const uint64_t rows4 = ((uint64_t)a.b.n_tok * n_head + 3) / 4;  // blocks of the join
+  if (p_items + o_items > kMaxBlocks / 2 || rows4 > kMaxBlocks)
     return aur::set_error(ctx, AUR_ELIMIT, "%s: %llu + %llu blocks", who, (unsigned long long)p_items,
                           (unsigned long long)o_items);
   const bool f32 = cache->dtype == AUR_PAGED_F32;
-  if (p.pooled) {
+  if (p.pooled && !p.together()) {
     a.p_items = (int)p_items;
-    launch_items(a, f32, p.p_tile, (unsigned)p_items, ctx->stream);
-    AUR_LAUNCH_CHECK(ctx, "paged_mha_kernel (prefix)");
+    launch_items(a, f32, 0, p.p_tile, (unsigned)p_items, ctx->stream);
+    AUR_LAUNCH_CHECK(ctx, "paged_mha kernels (prefix)");
     a.p_items = 0;
+    launch_items(a, f32, 0, p.o_tile, (unsigned)o_items, ctx->stream);
+  } else {
+    a.p_items = (int)p_items;
+    launch_items(a, f32, p.pooled ? p.p_tile : 0, p.o_tile, (unsigned)(p_items + o_items), ctx->stream);
   }
-  launch_items(a, f32, p.o_tile, (unsigned)o_items, ctx->stream);
-  AUR_LAUNCH_CHECK(ctx, "paged_mha_kernel");
+  AUR_LAUNCH_CHECK(ctx, "paged_mha kernels");
   if (floats) {
-    hipLaunchKernelGGL(paged_join_kernel, dim3(a.b.n_tok), dim3(256), 0, ctx->stream, a);
+    int lanes = 2;  // of a row: a power of two of them, 4 columns each
+    while (4 * lanes < a.dh) lanes *= 2;
+    hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)(((uint64_t)a.b.n_tok * a.H + 3) / 4)), dim3(256), 0,
+                       ctx->stream, a, lanes);
     AUR_LAUNCH_CHECK(ctx, "paged_join_kernel");
   }
   return 0;
