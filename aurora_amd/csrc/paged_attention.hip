@@ -632,7 +632,8 @@ struct TileGeo {
   static constexpr int KROW = KC == 1 ? 64 : KC == 2 ? 128 : 256;
   static constexpr int KPLANE = KT * KROW, VPLANE = DT * 16 * KT * 2;
   static constexpr int TPR = 64 * W / KT, NI = (4 * KC + TPR - 1) / TPR;  // K: threads of a row, octets of a thread
-  static constexpr int VC = F32 && W == 8 ? 1 : 2, VN = 16 * DT / VC;      // V: a thread has VC columns of 8 keys
+  static constexpr int VC = F32 && 2 * DT * KT <= 64 * W ? 1 : 2, VN = 16 * DT / VC;  // V: VC columns of 8 keys a thread
+  static_assert(VN * (KT / 8) <= 64 * W, "every piece of V has its thread");
 };
 // Granule q (16 bytes) of row r in rows of ROW bytes: every phase of 16 lanes covers the 64 banks once.
 template <int ROW>
@@ -647,7 +648,8 @@ template <class T, int DT, int W>
 struct TileLds {
   using G = TileGeo<T, DT, W>;
   char k[G::PARTS * G::KPLANE], v[G::PARTS * G::VPLANE];
-  int places[3][G::KT];  // pool rows of the keys of this tile and the next two
+  long long offset[3][G::KT];  // in bytes, of the keys of this tile and the next two in the pools
+  unsigned long long have[3];  // which of them are there
 };
 template <class T, int DT, int NR, int W>
 __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& lds) {
@@ -656,7 +658,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
   constexpr int KT = G::KT, KC = G::KC, NI = G::NI, NK = KT / 16, VC = G::VC;
   char* const ks = lds.k;
   char* const vs = lds.v;
-  auto& places = lds.places;
+  constexpr unsigned long long ALL = KT == 64 ? ~0ull : 0xffffffffull;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = lane >> 4, l16 = lane & 15;
 
@@ -672,50 +674,51 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
 #pragma unroll
   for (int m = 1; m < 16; m *= 2) vmax = max(vmax, __shfl_xor(vmax, m, 64));
 
-  // Pool rows of a tile's keys; the pages' numbers are asked for a tile before they are needed.
-  int xp = it.x0 + tid % KT;  // the key whose page is under way
+  // Where a tile's keys lie; the first KT threads ask for the pages' numbers a tile before they are needed.
+  const long long ld = (long long)a.Hkv * a.dh * sizeof(T);
+  int xp = it.x0 + tid;  // the key whose page is under way
   auto place = [&](int slot) {
-    if (tid < KT) places[slot][tid] = row_of(a, it, xp, page);
-    xp += KT;
-    page = page_of(a, it.s, it.pre, xp);
+    if (tid < KT) {
+      const int at = row_of(a, it, xp, page);
+      lds.offset[slot][tid] = at < 0 ? 0 : at * ld;
+      const unsigned long long have = __ballot(at >= 0);
+      if (tid == 0) lds.have[slot] = have;
+      xp += KT;
+      page = page_of(a, it.s, it.pre, xp);
+    }
   };
   place(0);
   place(1);
   __syncthreads();
 
-  const size_t ld = (size_t)a.Hkv * a.dh;
-  const T* kp = static_cast<const T*>(a.k) + (size_t)it.hk * a.dh;
-  const T* vp = static_cast<const T*>(a.v) + (size_t)it.hk * a.dh;
   const int kr = tid / G::TPR, ko = tid % G::TPR;  // K: row kr, octets ko + TPR·i
   const int vc = tid % G::VN * VC, vg = tid / G::VN;  // V: columns vc … of granule vg
   const bool v_on = vg < KT / 8;
-  const int vkey = 32 * (vg >> 2) + 4 * (vg & 3);  // … the keys vkey + 16·(i/4) + i%4
+  const int vkey = v_on ? 32 * (vg >> 2) + 4 * (vg & 3) : 0;  // … the keys vkey + 16·(i/4) + i%4
+  const char* const kp = static_cast<const char*>(a.k) + (size_t)it.hk * a.dh * sizeof(T);
+  const char* const vp = static_cast<const char*>(a.v) + ((size_t)it.hk * a.dh + min(vc, a.dh - VC)) * sizeof(T);
   floatx4 kx[NI][F32 ? 2 : 1];  // as loaded
-  float vx[8][F32 ? VC : 1];
+  float vx[8][F32 ? VC : 1];    // bf16: a pair
+  unsigned long long have = 0;  // of the keys in them
   auto load = [&](int slot) {
-    const int at = places[slot][kr];
-    const T* p = kp + (size_t)max(at, 0) * ld;
+    have = lds.have[slot];
+    const char* p = kp + lds.offset[slot][kr];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int c = min(8 * (ko + G::TPR * i), a.dh - 8);
-      kx[i][0] = *reinterpret_cast<const floatx4*>(p + c);
-      if (F32) kx[i][F32] = *reinterpret_cast<const floatx4*>(p + c + 4);
+      const char* q = p + min(8 * (ko + G::TPR * i), a.dh - 8) * (int)sizeof(T);
+      kx[i][0] = *reinterpret_cast<const floatx4*>(q);
+      if (F32) kx[i][F32] = *reinterpret_cast<const floatx4*>(q + 16);
     }
-    const int c = min(vc, a.dh - VC);
+    if (G::VN * (KT / 8) < 64 * W && !v_on) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int row = v_on ? places[slot][vkey + 16 * (i >> 2) + (i & 3)] : -1;
-#pragma unroll
-      for (int j = 0; j < (F32 ? VC : 1); ++j) vx[i][j] = 0.f;
-      if (row >= 0) {
-        const T* q = vp + (size_t)row * ld + c;
-        if (F32 && VC == 2) {
-          const float2v x = *reinterpret_cast<const float2v*>(q);
-          vx[i][0] = x[0];
-          vx[i][F32 ? VC - 1 : 0] = x[1];
-        } else {
-          vx[i][0] = *reinterpret_cast<const float*>(q);  // or a pair of bf16
-        }
+      const char* q = vp + lds.offset[slot][vkey + 16 * (i >> 2) + (i & 3)];
+      if (F32 && VC == 2) {
+        const float2v x = *reinterpret_cast<const float2v*>(q);
+        vx[i][0] = x[0];
+        vx[i][F32 ? VC - 1 : 0] = x[1];
+      } else {
+        vx[i][0] = *reinterpret_cast<const float*>(q);
       }
     }
   };
@@ -741,7 +744,14 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
         *reinterpret_cast<floatx4*>(p) = live ? kx[i][0] : zero;
       }
     }
-    if (!v_on) return;
+    if (G::VN * (KT / 8) < 64 * W && !v_on) return;
+    if (have != ALL) {  // a key that is not there adds nothing, whatever lies in its place
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(have >> (vkey + 16 * (i >> 2) + (i & 3)) & 1))
+#pragma unroll
+          for (int c = 0; c < (F32 ? VC : 1); ++c) vx[i][c] = 0.f;
+    }
 #pragma unroll
     for (int c = 0; c < VC; ++c) {
       char* p = vs + tile_granule<2 * KT>(vc + c, vg);
@@ -873,14 +883,14 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
   for (int x = it.x0; x < it.x1; x += KT) {
     if (x > it.x0) __syncthreads();  // every wave is done with the last tile
     lay_down();
+    const unsigned long long there = have;
     const int next = slot == 2 ? 0 : slot + 1;
     place(next == 2 ? 0 : next + 1);
     __syncthreads();
     if (x + KT < it.x1) load(next);
-    const unsigned long long there = __ballot(places[slot][lane % KT] >= 0);
     slot = next;
     if (x >= vmax) continue;  // none of the wave's rows sees this tile
-    if (there != ~0ull || x + KT > rows.vmin)
+    if (there != ALL || x + KT > rows.vmin)
       compute(x, there, std::true_type{});
     else
       compute(x, there, std::false_type{});
@@ -929,8 +939,12 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_mha_rows_kernel(MhaArgs a) {
   rows_item<T, DT>(a, lds);
 }
 
+// Waves a SIMD should hold: bf16 keys leave registers for three.
+template <class T, int DT, int NR>
+constexpr int kWaves = sizeof(T) == 2 && DT <= 4 && NR == 1 ? 3 : 2;
+
 template <class T, int DT, int NR, int W>
-__global__ void __launch_bounds__(64 * W, 2) paged_mha_tile_kernel(MhaArgs a) {
+__global__ void __launch_bounds__(64 * W, (kWaves<T, DT, NR>)) paged_mha_tile_kernel(MhaArgs a) {
   __shared__ __attribute__((aligned(1024))) TileLds<T, DT, W> lds;
   tile_item<T, DT, NR, W>(a, lds);
 }
@@ -938,7 +952,7 @@ __global__ void __launch_bounds__(64 * W, 2) paged_mha_tile_kernel(MhaArgs a) {
 // A decode step of many sequences in one launch: the prefix's items, bound by their products, beside the
 // own ones, bound by memory.
 template <class T, int DT>
-__global__ void __launch_bounds__(64 * NW, 2) paged_mha_step_kernel(MhaArgs a) {
+__global__ void __launch_bounds__(64 * NW, (kWaves<T, DT, 1>)) paged_mha_step_kernel(MhaArgs a) {
   __shared__ __attribute__((aligned(1024))) union {
     TileLds<T, DT, NW> tile;
     RowsLds<DT> rows;
@@ -1003,29 +1017,30 @@ struct Plan {
 };
 
 // Rows of an item: 16 keep their keys in registers, more lay them down in LDS.
-int tile_of(long long rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+int tile_of(long long rows, int dh) { return rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 || dh > 64 ? 128 : 256; }
 
 constexpr uint32_t kMaxRows = 0x7fffff00u;  // query rows of a call, and a tile more, are ints
-constexpr int kItems = 2048;     // items that a launch aims at, two rounds of four blocks a CU
-constexpr int kLeastKeys = 256;  // of an item: two rounds of its waves
+constexpr int kItems = 1024;     // items that a launch aims at: 4 of a CU, of 256 rows 2
+constexpr int kLeastKeys = 256;  // of an item of 16 rows, two rounds of its waves; of more rows 128
 constexpr int kPoolFrom = 32768;  // keys times heads that pooling saves, and from where it pays its join
 
-Plan make_plan(const Batch& b, int Hkv, int G) {
+Plan make_plan(const Batch& b, int Hkv, int G, int dh) {
   Plan p{};
   const int P = b.prefix_len;
   const long long o_rows = (long long)b.max_tok * G, p_rows = (long long)b.n_tok * G;
-  p.o_tile = tile_of(o_rows);
+  p.o_tile = tile_of(o_rows, dh);
   p.o_tiles = (int)((o_rows + p.o_tile - 1) / p.o_tile);
-  p.p_tile = p_rows <= 32 ? 16 : p_rows <= 256 ? 64 : 256;
+  p.p_tile = p_rows <= 32 ? 16 : p_rows <= 256 ? 64 : dh > 64 ? 128 : 256;
   const int p_tiles = (int)((p_rows + p.p_tile - 1) / p.p_tile);
   p.pooled = o_rows < 64 && ((double)b.b * p.o_tiles - p_tiles) * Hkv * P >= kPoolFrom;
   if (p.pooled && p.p_tile == 16 && p.o_tile > 16) p.p_tile = 64;
   p.p_tiles = p.pooled ? (int)((p_rows + p.p_tile - 1) / p.p_tile) : 0;
   const int axis = b.max_own + (p.pooled ? 0 : P);
   const double work = (double)Hkv * ((double)p.p_tiles * P + (double)b.b * p.o_tiles * axis);
-  const double want = work / kItems;
+  const double want = work / (p.o_tile == 256 ? kItems / 2 : kItems);
   int keys = want > 1e9 ? 1000000000 : ((int)want + 127) / 128 * 128;
-  if (keys < kLeastKeys) keys = kLeastKeys;
+  const int least = p.o_tile == 16 ? kLeastKeys : kLeastKeys / 2;
+  if (keys < least) keys = least;
   p.p_keys = p.o_keys = keys;
   p.p_splits = p.pooled ? (P + keys - 1) / keys : 0;
   p.o_splits = axis > keys ? (axis + keys - 1) / keys : 1;
@@ -1046,8 +1061,10 @@ void launch_tile(const MhaArgs& a, int p_tile, int tile, unsigned items, hipStre
     hipLaunchKernelGGL((paged_mha_rows_kernel<T, DT>), g, dim3(256), 0, st, a);
   else if (tile == 64)
     hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 4>), g, dim3(256), 0, st, a);
-  else if (tile == 128)
+  else if constexpr (DT > 4)
     hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 8>), g, dim3(512), 0, st, a);
+  else if (tile == 128)
+    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 2, 4>), g, dim3(256), 0, st, a);
   else
     hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 2, 8>), g, dim3(512), 0, st, a);
 }
@@ -1076,7 +1093,7 @@ size_t aur_mha_paged_ws_bytes(const aur_paged_cache* cache, const aur_paged_batc
   if (check_paged(nullptr, "aur_mha_paged_ws_bytes", cache, batch, &b) != 0 || n_head == 0 || n_head > 4096 ||
       (uint64_t)b.n_tok * n_head > kMaxRows || n_head % cache->n_kv_head != 0 || b.b == 0 || b.n_tok == 0)
     return 0;
-  return 4 * ws_floats(make_plan(b, (int)cache->n_kv_head, (int)(n_head / cache->n_kv_head)), b, (int)n_head,
+  return 4 * ws_floats(make_plan(b, (int)cache->n_kv_head, (int)(n_head / cache->n_kv_head), (int)cache->d_head), b, (int)n_head,
                        (int)cache->d_head);
 }
 
@@ -1102,7 +1119,7 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
   a.H = (int)n_head; a.Hkv = (int)cache->n_kv_head; a.G = a.H / a.Hkv; a.dh = (int)cache->d_head;
   a.n_pages = (int)cache->n_pages; a.sh = log2_of(cache->page_len);
   a.scale = 1.0f / sqrtf((float)a.dh);
-  const Plan p = make_plan(a.b, a.Hkv, a.G);
+  const Plan p = make_plan(a.b, a.Hkv, a.G, a.dh);
   a.pooled = p.pooled;
   a.p_tiles = p.p_tiles; a.p_splits = p.p_splits; a.p_keys = p.p_keys;
   a.o_tiles = p.o_tiles; a.o_splits = p.o_splits; a.o_keys = p.o_keys;
