@@ -964,12 +964,30 @@ __global__ void __launch_bounds__(64 * NW, (kWaves<T, DT, 1>)) paged_mha_step_ke
 }
 
 // out and lse of a row from the records of its ranges: one wave a row.  The lanes of a group have 4
-// columns each, the groups take every other range in turn and are added as a tree, so the order is fixed.
+// columns each, the groups take the ranges in turn and are added as a tree, so the order is fixed.
+// Which ranges were written depends on the sequence's length; the loads do not wait for it (what lies in
+// a range that was not is masked).  Of up to six dependent loads three remain: 7.2 → 4.7 µs for 16 rows of 17
+// ranges, 3.8 → 3.0 µs for 512 rows of 2, 16 → 13 µs for 25,000 rows of 5.
+// JOIN: ranges of a group that are under way at once.
+template <int JOIN>
 __global__ void __launch_bounds__(256) paged_join_kernel(MhaArgs a, int lanes) {
   const int lane = threadIdx.x & 63;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int t = (int)(row / a.H), h = (int)(row - (long long)t * a.H);
   if (t >= a.b.n_tok) return;
+  const int all = a.p_splits + a.o_splits, c = 4 * (lane % lanes), groups = 64 / lanes, g = lane / lanes;
+  const size_t step = (size_t)a.b.n_tok * a.H, rec = (size_t)t * a.H + h;
+  const float* ml = a.part_ml + 2 * rec;
+  const float* o = a.part_o + rec * a.dh + min(c, a.dh - 4);
+  auto pair = [&](int p) { return *reinterpret_cast<const float2v*>(ml + 2 * (size_t)min(p, all - 1) * step); };
+  floatx4 v[JOIN];
+  float2v w[JOIN];
+#pragma unroll
+  for (int i = 0; i < JOIN; ++i) {
+    v[i] = load4(o + (size_t)min(g + i * groups, all - 1) * step * a.dh);
+    w[i] = pair(g + i * groups);
+  }
+  const float2v first = pair(lane);
   int s = 0;
   for (int i0 = 0; i0 < a.b.b; i0 += 64) {
     const int i = i0 + lane;
@@ -980,31 +998,32 @@ __global__ void __launch_bounds__(256) paged_join_kernel(MhaArgs a, int lanes) {
   if (t < q.lo || t - q.lo >= q.n) return;
   const int axis = q.len + (a.pooled ? 0 : a.b.prefix_len);
   const int np = a.p_splits + max((axis + a.o_keys - 1) / a.o_keys, 1);  // range 0 is always written
-  const size_t step = (size_t)a.b.n_tok * a.H, rec = (size_t)t * a.H + h;
-  const float* ml = a.part_ml + 2 * rec;
-  float M = -INFINITY;
-  for (int p = lane; p < np; p += 64) M = fmaxf(M, ml[2 * p * step]);
+  float M = lane < np ? first[0] : -INFINITY;
+  for (int p = lane + 64; p < np; p += 64) M = fmaxf(M, pair(p)[0]);
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) M = fmaxf(M, __shfl_xor(M, i, 64));
-  auto factor = [&](int p) { return M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[2 * p * step] - M); };
-  float L = 0.f;
-  for (int p = lane; p < np; p += 64) L += factor(p) * ml[2 * p * step + 1];
+  auto factor = [&](float m) { return M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - M); };
+  float L = lane < np ? factor(first[0]) * first[1] : 0.f;
+  for (int p = lane + 64; p < np; p += 64) {
+    const float2v x = pair(p);
+    L += factor(x[0]) * x[1];
+  }
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) L += __shfl_xor(L, i, 64);
-  const int c = 4 * (lane % lanes), groups = 64 / lanes;
-  const float* o = a.part_o + rec * a.dh + min(c, a.dh - 4);
-  floatx4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int p = lane / lanes; p < np; p += groups) v += load4(o + (size_t)p * step * a.dh) * factor(p);
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < JOIN; ++i)
+    if (g + i * groups < np) sum += v[i] * factor(w[i][0]);
+  for (int p = g + JOIN * groups; p < np; p += groups) sum += load4(o + (size_t)p * step * a.dh) * factor(pair(p)[0]);
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) {
     if (i < lanes) continue;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], i, 64);
+    for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], i, 64);
   }
   if (lane < lanes && c < a.dh)
     *reinterpret_cast<floatx4*>(a.out + (size_t)t * a.ld_o + (size_t)h * a.dh + c) =
-        L == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : v * (1.f / L);
+        L == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : sum * (1.f / L);
   if (lane == 0 && a.lse) a.lse[(size_t)t * a.H + h] = L == 0.f ? -INFINITY : (M + __log2f(L)) * LN2;
 }
 
@@ -1152,8 +1171,10 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
   if (floats) {
     int lanes = 2;  // of a row: a power of two of them, 4 columns each
     while (4 * lanes < a.dh) lanes *= 2;
-    hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)(((uint64_t)a.b.n_tok * a.H + 3) / 4)), dim3(256), 0,
-                       ctx->stream, a, lanes);
+    const int turns = (p.parts() * lanes + 63) / 64;
+    auto* join = turns <= 1 ? paged_join_kernel<1> : turns <= 2 ? paged_join_kernel<2>
+                 : turns <= 4 ? paged_join_kernel<4> : paged_join_kernel<8>;
+    hipLaunchKernelGGL(join, dim3((unsigned)rows4), dim3(256), 0, ctx->stream, a, lanes);
     AUR_LAUNCH_CHECK(ctx, "paged_join_kernel");
   }
   return 0;
