@@ -521,14 +521,11 @@ template <int DT>
 struct RowsLds {
   static constexpr int R = 16, OS = 64 * ((DT + 3) / 4) + 4;
   float m[NW][R], l[NW][R];
-  __attribute__((aligned(16))) float o[R][OS];
+  __attribute__((aligned(16))) float o[NW][R][OS];
 };
 template <class T, int DT>
 __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
   constexpr int VB = Sums<DT, 1>::VB, RT = 1, R = RowsLds<DT>::R, STRIDE = STEP * NW;
-  auto& sm = lds.m;
-  auto& sl = lds.l;
-  auto& so = lds.o;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = lane >> 4, l16 = lane & 15, k32 = lane & 31;
 
@@ -542,12 +539,12 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
     Keys32<T, DT> keys;
     int at = row_of(a, it, x + k32, page);
     keys.template load_k<true>(a, it.hk, at, g, l16);
-    keys.template load_v<true>(a, it.hk, at, g, l16);
-    page = page_of(a, it.s, it.pre, x + STRIDE + k32);
     Rows<RT> rows;
     take_rows(a, it, it.row0, l16, rows);
     Queries<T, DT, RT> q;
     q.load(rows, a.dh, g, a.scale * LOG2E);
+    keys.template load_v<true>(a, it.hk, at, g, l16);
+    page = page_of(a, it.s, it.pre, x + STRIDE + k32);
     for (; x < it.x1; x += STRIDE) {
       // the next keys' loads go out as soon as this step has used the registers
       const bool more = x + STRIDE < it.x1;
@@ -568,52 +565,36 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
     if (!finite(s)) exact_sums<T, DT, RT>(a, it, it.row0, it.x0 + STEP * w, STRIDE, s);
   }
 
-  // Join the four waves: common maximum, then their sums added in wave order.
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    s.l[r] = rows4_sum(s.l[r]);
+  // Join the four waves in their order.
+  s.l[0] = rows4_sum(s.l[0]);
+  if (it.row0 + l16 < it.n_rows) {
     if (g == 0) {
-      sm[w][16 * r + l16] = s.m[r];
-      sl[w][16 * r + l16] = s.l[r];
+      lds.m[w][l16] = s.m[0];
+      lds.l[w][l16] = s.l[0];
     }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    float M = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) M = fmaxf(M, sm[i][16 * r + l16]);
-    const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s.m[r] - M);
 #pragma unroll
     for (int b = 0; b < VB; ++b)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s.acc[r][b][c] *= f;
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<floatx4*>(&lds.o[w][l16][64 * b + 16 * g + 4 * j]) =
+            floatx4{s.acc[0][b][0][j], s.acc[0][b][1][j], s.acc[0][b][2][j], s.acc[0][b][3][j]};
   }
-  for (int i = 0; i < NW; ++i) {
-    if (w == i) {
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int b = 0; b < VB; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            floatx4* p = reinterpret_cast<floatx4*>(&so[16 * r + l16][64 * b + 16 * g + 4 * j]);
-            const floatx4 v = {s.acc[r][b][0][j], s.acc[r][b][1][j], s.acc[r][b][2][j], s.acc[r][b][3][j]};
-            *p = i == 0 ? v : *p + v;
-          }
-    }
-    __syncthreads();
-  }
+  __syncthreads();
   const int n4 = a.dh / 4;
   for (int i = tid; i < R * n4; i += 64 * NW) {
     const int r = i / n4, c = 4 * (i - r * n4);
     if (it.row0 + r >= it.n_rows) break;
     float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int j = 0; j < NW; ++j) M = fmaxf(M, sm[j][r]);
+    for (int j = 0; j < NW; ++j) M = fmaxf(M, lds.m[j][r]);
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NW; ++j) L += (M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[j][r] - M)) * sl[j][r];
-    store(a, it, it.row0 + r, c, *reinterpret_cast<const floatx4*>(&so[r][c]), M, L);
+    for (int j = 0; j < NW; ++j) {
+      const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(lds.m[j][r] - M);
+      L += f * lds.l[j][r];
+      o += f * *reinterpret_cast<const floatx4*>(&lds.o[j][r][c]);
+    }
+    store(a, it, it.row0 + r, c, o, M, L);
   }
 }
 

@@ -342,13 +342,15 @@ class PagedKvAppendKernel(_Kernel):
 
     def dispatch_into(self, ctx, cache, batch, q, ld_q, k, v, ld_kv, q_out, ld_qo, table, n_pos, rot_dim,
                       n_head, pairs=False):
-        n, row = batch.n_tok, cache.n_kv_head * cache.d_head
-        _need("PagedKvAppendKernel q", _rows(n, ld_q, n_head * cache.d_head), q)
-        _need("PagedKvAppendKernel q_out", _rows(n, ld_qo, n_head * cache.d_head), q_out)
-        _need("PagedKvAppendKernel k/v", _rows(n, ld_kv, row), k, v)
-        _need("PagedKvAppendKernel table", n_pos * rot_dim, table)
-        ctx.call("aur_kv_append_paged", cache.ref, batch.ref, _p(q), ld_q, _p(k), _p(v), ld_kv, _p(q_out), ld_qo,
-                 _p(table), n_pos, rot_dim, n_head, 1 if pairs else 0)
+        if GpuBuffer in (type(q), type(k), type(v), type(q_out), type(table)):  # a step's raw pointers pass at once
+            n, row = batch.n_tok, cache.n_kv_head * cache.d_head
+            _need("PagedKvAppendKernel q", _rows(n, ld_q, n_head * cache.d_head), q)
+            _need("PagedKvAppendKernel q_out", _rows(n, ld_qo, n_head * cache.d_head), q_out)
+            _need("PagedKvAppendKernel k/v", _rows(n, ld_kv, row), k, v)
+            _need("PagedKvAppendKernel table", n_pos * rot_dim, table)
+            q, k, v, q_out, table = _p(q), _p(k), _p(v), _p(q_out), _p(table)
+        ctx.call("aur_kv_append_paged", cache.ref, batch.ref, q, ld_q, k, v, ld_kv, q_out, ld_qo, table, n_pos,
+                 rot_dim, n_head, 1 if pairs else 0)
 
 
 class PagedMhaKernel(_Kernel):
@@ -359,11 +361,11 @@ class PagedMhaKernel(_Kernel):
         return (_lib.load().aur_mha_paged_ws_bytes(cache.ref, batch.ref, n_head) + 3) // 4
 
     def dispatch_into(self, ctx, cache, batch, q, ld_q, out, ld_o, lse, scratch, scratch_len, n_head):
-        d = n_head * cache.d_head
-        _need("PagedMhaKernel q", _rows(batch.n_tok, ld_q, d), q)
-        _need("PagedMhaKernel out", _rows(batch.n_tok, ld_o, d), out)
-        if lse:
+        if GpuBuffer in (type(q), type(out), type(lse), type(scratch)):
+            d = n_head * cache.d_head
+            _need("PagedMhaKernel q", _rows(batch.n_tok, ld_q, d), q)
+            _need("PagedMhaKernel out", _rows(batch.n_tok, ld_o, d), out)
             _need("PagedMhaKernel lse", batch.n_tok * n_head, lse)
-        _need("PagedMhaKernel scratch", scratch_len, scratch)
-        ctx.call("aur_mha_paged", cache.ref, batch.ref, _p(q), ld_q, _p(out), ld_o, _p(lse), _p(scratch),
-                 4 * scratch_len, n_head)
+            _need("PagedMhaKernel scratch", scratch_len, scratch)
+            q, out, lse, scratch = _p(q), _p(out), _p(lse), _p(scratch)
+        ctx.call("aur_mha_paged", cache.ref, batch.ref, q, ld_q, out, ld_o, lse, scratch, 4 * scratch_len, n_head)
