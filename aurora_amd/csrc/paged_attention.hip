@@ -1020,8 +1020,13 @@ struct Plan {
 int tile_of(long long rows, int dh) { return rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 || dh > 64 ? 128 : 256; }
 
 constexpr uint32_t kMaxRows = 0x7fffff00u;  // query rows of a call, and a tile more, are ints
-constexpr int kItems = 1024;     // items that a launch aims at: 4 of a CU, of 256 rows 2
-constexpr int kLeastKeys = 256;  // of an item of 16 rows, two rounds of its waves; of more rows 128
+// Items that a launch aims at, measured at 128 to 4096 of them: with 16-row own items 3 of a CU (64
+// sequences on a prefix of 32768 in bf16: 86 µs, with 256 items 140, with 2048 97), with larger ones 4
+// (tails of 128 on 2048: 113 µs, with 768 items 120), of 8 waves one (512 sequences on a prefix of 16384:
+// 240 µs, with 1024 items 303).
+constexpr int kItems16 = 768, kItems = 1024, kItems8 = 256;
+// The fewest keys of an item: of 16 rows two rounds of its waves, of more rows half of that.
+constexpr int kLeastKeys = 256;
 constexpr int kPoolFrom = 32768;  // keys times heads that pooling saves, and from where it pays its join
 
 Plan make_plan(const Batch& b, int Hkv, int G, int dh) {
@@ -1030,20 +1035,25 @@ Plan make_plan(const Batch& b, int Hkv, int G, int dh) {
   const long long o_rows = (long long)b.max_tok * G, p_rows = (long long)b.n_tok * G;
   p.o_tile = tile_of(o_rows, dh);
   p.o_tiles = (int)((o_rows + p.o_tile - 1) / p.o_tile);
-  p.p_tile = p_rows <= 32 ? 16 : p_rows <= 256 ? 64 : dh > 64 ? 128 : 256;
+  p.p_tile = p_rows <= 32 ? 16 : p_rows <= (dh > 64 ? 256 : 128) ? 64 : dh > 64 ? 128 : 256;
   const int p_tiles = (int)((p_rows + p.p_tile - 1) / p.p_tile);
   p.pooled = o_rows < 64 && ((double)b.b * p.o_tiles - p_tiles) * Hkv * P >= kPoolFrom;
   if (p.pooled && p.p_tile == 16 && p.o_tile > 16) p.p_tile = 64;
   p.p_tiles = p.pooled ? (int)((p_rows + p.p_tile - 1) / p.p_tile) : 0;
   const int axis = b.max_own + (p.pooled ? 0 : P);
-  const double work = (double)Hkv * ((double)p.p_tiles * P + (double)b.b * p.o_tiles * axis);
-  const double want = work / (p.o_tile == 256 ? kItems / 2 : kItems);
-  int keys = want > 1e9 ? 1000000000 : ((int)want + 127) / 128 * 128;
-  const int least = p.o_tile == 16 ? kLeastKeys : kLeastKeys / 2;
-  if (keys < least) keys = least;
-  p.p_keys = p.o_keys = keys;
-  p.p_splits = p.pooled ? (P + keys - 1) / keys : 0;
-  p.o_splits = axis > keys ? (axis + keys - 1) / keys : 1;
+  auto range = [dh](double work, int tile) {  // keys of an item
+    const bool eight = tile == 256 || (tile == 128 && dh > 64);
+    const double want = work / (eight ? kItems8 : tile > 16 ? kItems : kItems16);
+    const int keys = want > 1e9 ? 1000000000 : ((int)want + 127) / 128 * 128;
+    const int least = tile == 16 ? kLeastKeys : kLeastKeys / 2;
+    return keys < least ? least : keys;
+  };
+  const double p_work = (double)Hkv * p.p_tiles * P, o_work = (double)Hkv * b.b * p.o_tiles * axis;
+  const bool one = !p.pooled || p.together();
+  p.o_keys = range(one ? p_work + o_work : o_work, p.o_tile);
+  p.p_keys = one ? p.o_keys : range(p_work, p.p_tile);
+  p.p_splits = p.pooled ? (P + p.p_keys - 1) / p.p_keys : 0;
+  p.o_splits = axis > p.o_keys ? (axis + p.o_keys - 1) / p.o_keys : 1;
   return p;
 }
 
