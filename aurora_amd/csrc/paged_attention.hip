@@ -27,6 +27,8 @@
 #include "common.hpp"
 #include "paged.hpp"
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 using namespace aurattn;
@@ -1025,9 +1027,13 @@ constexpr uint32_t kMaxRows = 0x7fffff00u;  // query rows of a call, and a tile 
 // (tails of 128 on 2048: 113 µs, with 768 items 120), of 8 waves one (512 sequences on a prefix of 16384:
 // 240 µs, with 1024 items 303).
 constexpr int kItems16 = 768, kItems = 1024, kItems8 = 256;
-// The fewest keys of an item: of 16 rows two rounds of its waves, of more rows half of that.
-constexpr int kLeastKeys = 256;
-constexpr int kPoolFrom = 32768;  // keys times heads that pooling saves, and from where it pays its join
+// An axis up to so many keys is one range: a join costs 4 µs, 128 keys of a 16-row item (a round of its
+// waves) 1.5 µs.  Longer ones are cut into ranges of 128 keys or more, 48 at most.
+constexpr int kWhole16 = 384, kWhole = 256;
+constexpr int kLeastKeys = 128, kMostRanges = 48;
+// Keys times heads that pooling saves, from where it pays its records and its join (8 sequences of 12 heads
+// on a prefix of 1294, 108,000: 13 against 33 µs; 53 sequences of 5 heads on 139, 35,000: 22 against 10).
+constexpr int kPoolFrom = 65536;
 
 Plan make_plan(const Batch& b, int Hkv, int G, int dh) {
   Plan p{};
@@ -1041,19 +1047,25 @@ Plan make_plan(const Batch& b, int Hkv, int G, int dh) {
   if (p.pooled && p.p_tile == 16 && p.o_tile > 16) p.p_tile = 64;
   p.p_tiles = p.pooled ? (int)((p_rows + p.p_tile - 1) / p.p_tile) : 0;
   const int axis = b.max_own + (p.pooled ? 0 : P);
-  auto range = [dh](double work, int tile) {  // keys of an item
-    const bool eight = tile == 256 || (tile == 128 && dh > 64);
-    const double want = work / (eight ? kItems8 : tile > 16 ? kItems : kItems16);
-    const int keys = want > 1e9 ? 1000000000 : ((int)want + 127) / 128 * 128;
-    const int least = tile == 16 ? kLeastKeys : kLeastKeys / 2;
-    return keys < least ? least : keys;
+  // Ranges of one length, so that no item is left with a few keys.
+  // (A CU holds one block of 8 waves: more of them than CUs would be a second round.)
+  auto eight = [dh](int tile) { return tile == 256 || (tile == 128 && dh > 64); };
+  auto items = [&](int tile) { return eight(tile) ? kItems8 : tile > 16 ? kItems : kItems16; };
+  auto cut = [&](int n, double want, int tile, int* keys) {
+    int splits = 1;
+    if (n > (tile == 16 ? kWhole16 : kWhole)) {
+      const int most = std::min(kMostRanges, (n + kLeastKeys - 1) / kLeastKeys);
+      const double parts = n / want;
+      splits = (int)std::min((double)most, std::max(1.0, eight(tile) ? parts : std::ceil(parts)));
+    }
+    *keys = n > 0 ? ((n + splits - 1) / splits + 31) / 32 * 32 : 32;
+    return n > 0 ? (n + *keys - 1) / *keys : 1;
   };
   const double p_work = (double)Hkv * p.p_tiles * P, o_work = (double)Hkv * b.b * p.o_tiles * axis;
   const bool one = !p.pooled || p.together();
-  p.o_keys = range(one ? p_work + o_work : o_work, p.o_tile);
-  p.p_keys = one ? p.o_keys : range(p_work, p.p_tile);
-  p.p_splits = p.pooled ? (P + p.p_keys - 1) / p.p_keys : 0;
-  p.o_splits = axis > p.o_keys ? (axis + p.o_keys - 1) / p.o_keys : 1;
+  const double o_want = (one ? p_work + o_work : o_work) / items(p.o_tile);
+  p.o_splits = cut(axis, o_want, p.o_tile, &p.o_keys);
+  p.p_splits = p.pooled ? cut(P, one ? o_want : p_work / items(p.p_tile), p.p_tile, &p.p_keys) : 0;
   return p;
 }
 
