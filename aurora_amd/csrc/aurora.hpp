@@ -11,6 +11,8 @@
 //   MhaKvCacheKernel           src/gpu/kv_cache.rs:366-466
 //   DecoderTransformerGpu      src/gpu/transformer.rs:32-116 (train step, KV decode)
 //   KvCacheGpu                 src/gpu/kv_cache.rs:21-92
+//   PagedKvCache, PagedBatch, RotaryTableKernel, PagedKvAppendKernel, PagedMhaKernel
+//                              (no counterpart: a paged K/V cache with a shared prefix)
 //
 // Kernel structs keep the reference's argument order and its contract:
 // `dispatch_into` only enqueues on the context's stream, buffers belong to
@@ -191,6 +193,91 @@ struct MhaKvCacheKernel {
           aur_mha_kv_step(c.raw(), q_new.ptr(), k_history.ptr(), v_history.ptr(), out.ptr(), scratch.ptr(),
                           t_total, n_head, d_head, max_len),
           "MhaKvCacheKernel");
+  }
+};
+
+// ------------------------------------------------------------ paged K/V cache
+
+// Two pools [n_pages, page_len, n_kv_head * d_head] of T: float, or uint16_t holding bf16.
+template <class T>
+struct PagedKvCache {
+  GpuBuffer<T> k, v;
+  aur_paged_cache raw;
+  PagedKvCache(const GpuContext& c, uint32_t n_pages, uint32_t page_len, uint32_t n_kv_head, uint32_t d_head)
+      : k(GpuBuffer<T>::zeros(c, (size_t)n_pages * page_len * n_kv_head * d_head)),
+        v(GpuBuffer<T>::zeros(c, (size_t)n_pages * page_len * n_kv_head * d_head)),
+        raw{k.ptr(),   v.ptr(), n_pages, page_len, n_kv_head, d_head,
+            sizeof(T) == 4 ? AUR_PAGED_F32 : AUR_PAGED_BF16} {
+    static_assert(sizeof(T) == 4 || sizeof(T) == 2, "fp32 or bf16");
+  }
+};
+
+// Sequences with new tokens on a paged cache: device arrays, and the host's bounds on what they hold
+// (aur_paged_batch).
+struct PagedBatch {
+  aur_paged_batch raw;
+  PagedBatch(const GpuBuffer<int32_t>& tok_off, const GpuBuffer<int32_t>& own_len, const GpuBuffer<int32_t>& pages,
+             uint32_t b, uint32_t max_pages, uint32_t n_tok, uint32_t max_tok, uint32_t max_own)
+      : raw{tok_off.ptr(), own_len.ptr(), pages.ptr(), nullptr, b, max_pages, n_tok, max_tok, max_own, 0, 0} {
+    if (tok_off.len() < (size_t)b + 1 || own_len.len() < b || pages.len() < (size_t)b * max_pages)
+      throw Error("PagedBatch: array too short", AUR_EINVAL);
+  }
+  // … behind a prefix that they share.
+  PagedBatch& behind(const GpuBuffer<int32_t>& prefix_pages, uint32_t prefix_len) {
+    raw.prefix_pages = prefix_pages.ptr();
+    raw.n_prefix_pages = (uint32_t)prefix_pages.len();
+    raw.prefix_len = prefix_len;
+    return *this;
+  }
+};
+
+struct RotaryTableKernel {
+  void dispatch_into(const GpuContext& c, const GpuBuffer<float>& table, uint32_t n_pos, uint32_t rot_dim,
+                     float theta = 10000.f) const {
+    need(table, (size_t)n_pos * rot_dim, "RotaryTableKernel table");
+    check(c.raw(), aur_rotary_table(c.raw(), table.ptr(), n_pos, rot_dim, theta), "RotaryTableKernel");
+  }
+};
+
+// Rows of the token tensors lie densely here; aur_kv_append_paged and aur_mha_paged take strides.
+struct PagedKvAppendKernel {
+  template <class T>
+  void dispatch_into(const GpuContext& c, const PagedKvCache<T>& cache, const PagedBatch& batch,
+                     const GpuBuffer<float>& q, const GpuBuffer<float>& k, const GpuBuffer<float>& v,
+                     const GpuBuffer<float>& q_out, const GpuBuffer<float>& table, uint32_t n_pos, uint32_t rot_dim,
+                     uint32_t n_head, bool pairs = false) const {
+    const size_t n = batch.raw.n_tok;
+    const uint32_t d = n_head * cache.raw.d_head, row = cache.raw.n_kv_head * cache.raw.d_head;
+    need(q, n * d, "PagedKvAppendKernel q");
+    need(q_out, n * d, "PagedKvAppendKernel q_out");
+    need(k, n * row, "PagedKvAppendKernel k");
+    need(v, n * row, "PagedKvAppendKernel v");
+    need(table, (size_t)n_pos * rot_dim, "PagedKvAppendKernel table");
+    check(c.raw(),
+          aur_kv_append_paged(c.raw(), &cache.raw, &batch.raw, q.ptr(), d, k.ptr(), v.ptr(), row, q_out.ptr(), d,
+                              table.ptr(), n_pos, rot_dim, n_head, pairs),
+          "PagedKvAppendKernel");
+  }
+};
+
+struct PagedMhaKernel {
+  template <class T>
+  static size_t scratch_len(const PagedKvCache<T>& cache, const PagedBatch& batch, uint32_t n_head) {
+    return (aur_mha_paged_ws_bytes(&cache.raw, &batch.raw, n_head) + 3) / 4;
+  }
+  template <class T>
+  void dispatch_into(const GpuContext& c, const PagedKvCache<T>& cache, const PagedBatch& batch,
+                     const GpuBuffer<float>& q, const GpuBuffer<float>& out, const GpuBuffer<float>& lse,
+                     const GpuBuffer<float>& scratch, uint32_t n_head) const {
+    const size_t n = batch.raw.n_tok;
+    const uint32_t d = n_head * cache.raw.d_head;
+    need(q, n * d, "PagedMhaKernel q");
+    need(out, n * d, "PagedMhaKernel out");
+    need(lse, n * n_head, "PagedMhaKernel lse");
+    check(c.raw(),
+          aur_mha_paged(c.raw(), &cache.raw, &batch.raw, q.ptr(), d, out.ptr(), d, lse.ptr(), scratch.ptr(),
+                        4 * scratch.len(), n_head),
+          "PagedMhaKernel");
   }
 };
 
