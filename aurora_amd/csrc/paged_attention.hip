@@ -97,7 +97,8 @@ __device__ __forceinline__ bool take_item(const MhaArgs& a, Item& it, int lead, 
     item /= a.Hkv;
     it.row0 = item % a.p_tiles * R;
     it.part = item / a.p_tiles;
-    it.n_rows = a.b.n_tok * a.G;
+    it.n_rows = min(max(a.b.tok_off[a.b.b], 0), a.b.n_tok) * a.G;  // rows behind the last sequence are none
+    if (it.row0 >= it.n_rows) return false;
     it.pre = a.b.prefix_len;
     it.x0 = it.part * a.p_keys;
     it.x1 = min(it.x0 + a.p_keys, it.pre);
@@ -435,8 +436,9 @@ __device__ __forceinline__ void soften(floatx4 (&st)[RT][2], Sums<DT, RT>& s) {
   }
 }
 
+// Of the lanes that have a row.
 template <int DT, int RT>
-__device__ __forceinline__ bool finite(const Sums<DT, RT>& s) {
+__device__ __forceinline__ bool finite(const Sums<DT, RT>& s, bool live) {
   float z = 0.f;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
@@ -448,7 +450,7 @@ __device__ __forceinline__ bool finite(const Sums<DT, RT>& s) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) z += 0.f * s.acc[r][b][c][i];
   }
-  return __ballot(z != 0.f) == 0;  // 0 times an infinity or NaN is NaN
+  return __ballot(live && z != 0.f) == 0;  // 0 times an infinity or NaN is NaN
 }
 
 // The sums of a wave's rows over keys x, x + stride, … again, where they came out as infinity or NaN:
@@ -564,7 +566,7 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
       add_values(keys, st, s);
       if (more) keys.template load_v<true>(a, it.hk, at, g, l16);
     }
-    if (!finite(s)) exact_sums<T, DT, RT>(a, it, it.row0, it.x0 + STEP * w, STRIDE, s);
+    if (!finite(s, it.row0 + l16 < it.n_rows)) exact_sums<T, DT, RT>(a, it, it.row0, it.x0 + STEP * w, STRIDE, s);
   }
 
   // Join the four waves in their order.
@@ -888,7 +890,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
       for (int i = 0; i < 4; ++i)
         if (DT * 16 == a.dh || 16 * d + 4 * g + i < a.dh) z += 0.f * acc[r][d][i];
     const int row = row0 + 16 * r + l16;
-    if (__ballot(z != 0.f) == 0) {
+    if (__ballot(row < it.n_rows && z != 0.f) == 0) {
       const float L = rows4_sum(l[r]);
       if (row < it.n_rows) {
 #pragma unroll

@@ -233,7 +233,8 @@ int aur_mha_kv_step_batched(aur_ctx* ctx, const float* q_new,
  * own_len <= max_own <= max_pages*page_len, tok_off[b] <= n_tok, tok_off
  * ascending.  Values beyond the bounds are cut to them, so that nothing out of
  * range is touched (results then mean nothing); page numbers outside
- * [0, n_pages) read and write nothing: the keys count as not there. */
+ * [0, n_pages) read and write nothing: the keys count as not there.  Sequences
+ * that are appended to in one call share no page. */
 #define AUR_PAGED_F32 0u
 #define AUR_PAGED_BF16 1u
 typedef struct {
@@ -259,7 +260,7 @@ int aur_rotary_table(aur_ctx* ctx, float* table, uint32_t n_pos, uint32_t rot_di
  * or with pairs != 0 columns (2u, 2u + 1); columns from rot_dim on are copied.
  * rot_dim is a multiple of 8 up to d_head, 0 for no rotation (table may be NULL
  * then); the table holds n_pos >= prefix_len + max_own positions.  q and q_out
- * may be one buffer, or both NULL.  bf16 pools take the nearest value, ties to
+ * may be one buffer of one stride, or both NULL.  bf16 pools take the nearest value, ties to
  * even.  Rows 16-byte aligned, strides multiples of 4.  A token with j < 0
  * (own_len below n_s) is skipped, q_out included. */
 int aur_kv_append_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,
@@ -277,7 +278,10 @@ int aur_kv_append_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_pa
  * `scratch` is caller-owned, 16-byte aligned, of scratch_bytes >=
  * aur_mha_paged_ws_bytes(cache, batch, n_head) (0: it may be NULL), which goes
  * by the host's fields alone; calls that overlap in time need a scratch each.
- * Sums are fp32 and joined in a fixed order: the same call gives the same bits. */
+ * Sums are fp32 and joined in a fixed order: the same call gives the same bits.
+ * (With more than 16 query rows to a K/V head, fp32 values of V below 2^-110 are
+ * exact to 2^-126 only: the matrix cores take no subnormal bf16.)  `out` may not
+ * overlap q. */
 size_t aur_mha_paged_ws_bytes(const aur_paged_cache* cache, const aur_paged_batch* batch,
                               uint32_t n_head);
 int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,

@@ -30,7 +30,7 @@ class Device:
         self.off, self.len = up(c.off), up(c.length.astype(np.int32))
         self.pages, self.prefix = up(c.pages.ravel()), up(c.prefix_pages if c.prefix else np.zeros(1, np.int32))
         qs = np.full((c.n_tok, self.ld_q), np.nan, np.float32)
-        qs[:, :d] = c.q
+        qs[:c.off[-1], :d] = c.q[:c.off[-1]]  # rows behind the last sequence hold NaN, like the padding of the others
         self.q = up(qs.ravel())
         self.out = GpuBuffer.from_slice(ctx, np.full(c.n_tok * self.ld_o, 7.5, np.float32))
         self.lse = GpuBuffer.from_slice(ctx, np.full(c.n_tok * c.h, 7.5, np.float32)) if lse else 0
@@ -218,6 +218,23 @@ def test_large_scores_and_small_ones(ctx):
     dev.attend()
     out, lse = dev.result()
     assert np.all(out == 0) and np.all(np.isneginf(lse))
+    dev.free()
+
+
+@pytest.mark.parametrize("n,prefix,dtype", [([1, 1, 1], 400, "f32"), ([1] * 40, 300, "f32"), ([1] * 40, 300, "bf16"),
+                                            ([90, 70], 60, "f32"), ([90, 70], 60, "bf16"), ([300], 0, "f32")])
+@pytest.mark.parametrize("vs,ks", [(2.0**-100, 1.0), (2.0**100, 1.0), (1.0, 2.0**40), (1.0, 2.0**-40)])
+def test_values_of_any_size(ctx, n, prefix, dtype, vs, ks):
+    """V of any size, and columns of K far larger or smaller than the others whose queries make up for
+    it: nothing is lost beside a larger neighbour."""
+    rng = np.random.default_rng(16)
+    c = Case(rng, n, [x + 20 for x in n], prefix, 16, 1, 1, 64, dtype)
+    c.vp[:, ::2] *= np.float32(vs)
+    c.kp[:, 1::3] *= np.float32(ks)
+    c.q[:, 1::3] /= np.float32(ks)
+    dev = Device(ctx, c)
+    dev.attend()
+    _check(c, *dev.result())
     dev.free()
 
 
