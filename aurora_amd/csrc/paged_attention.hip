@@ -25,6 +25,7 @@
 #include "attention.hpp"
 #include "attention_split.hpp"
 #include "common.hpp"
+#include "lanes.hpp"
 #include "paged.hpp"
 
 #include <algorithm>
@@ -602,6 +603,155 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
   }
 }
 
+// ---------------------------------------------------------------- one row: no matrix products
+
+// A single row (one new token, a head of its own).  Its items are bound by reading K and V; the MFMA of
+// rows_item works on 16 rows whatever there are, and its cycles stand between the loads: 64 sequences of
+// 1024 keys, 16 heads of 64, take 85 µs there and 67 here (5.9 TB/s), bf16 keys 53 and 40.  LP lanes have a
+// key's head, 16 bytes each, so that a load brings 64/LP whole keys; a score is added up over the LP lanes,
+// l and the columns over the key groups once at the end.  All of it is fp32 arithmetic.  While one half of
+// the registers is in use, the loads of the other are under way, and the page of the step after them.
+template <class T, int DT>
+struct OneRow {
+  static constexpr int E = 16 / sizeof(T);                // columns of a lane
+  static constexpr int N = (16 * DT + E - 1) / E;         // lanes of a head
+  static constexpr int LP = N <= 2 ? 2 : N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : 32;
+  static constexpr int KPI = 64 / LP;                     // keys of a load
+  static constexpr int U = KPI > 16 ? 64 / KPI : 4;       // loads of K, and of V, under way; as many are in use
+  static constexpr int KEYS = U * KPI;                    // of a step; a lane finds the row of one
+  static_assert(KEYS <= 64 && N <= 32, "a wave finds the rows of a step");
+};
+template <class T>
+struct OneLds {
+  float m[NW], l[NW];
+  __attribute__((aligned(16))) float o[NW][128];
+};
+__device__ __forceinline__ void unpack(floatx4 x, float (&y)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = x[i];
+}
+__device__ __forceinline__ void unpack(floatx4 x, float (&y)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    y[2 * i] = __uint_as_float(__float_as_uint(x[i]) << 16);
+    y[2 * i + 1] = __uint_as_float(__float_as_uint(x[i]) & 0xffff0000u);
+  }
+}
+
+template <class T, int DT>
+__device__ __forceinline__ void one_item(const MhaArgs& a, OneLds<T>& lds) {
+  using G = OneRow<T, DT>;
+  constexpr int E = G::E, LP = G::LP, U = G::U, KPI = G::KPI, KEYS = G::KEYS, STRIDE = NW * KEYS;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int part = lane % LP, kg = lane / LP;
+  const bool live = E * part < a.dh;  // a lane of the group past the head is idle; its loads stay in range
+  const int col = live ? E * part : a.dh - E;
+
+  Item it;
+  int page;
+  if (!take_item<1>(a, it, KEYS * w + lane % KEYS, page)) return;
+  const char* const kp = static_cast<const char*>(a.k) + ((size_t)it.hk * a.dh + col) * sizeof(T);
+  const char* const vp = static_cast<const char*>(a.v) + ((size_t)it.hk * a.dh + col) * sizeof(T);
+  const long long ld = (long long)a.Hkv * a.dh * sizeof(T);
+  const float* qp = a.q + (size_t)it.tok0 * a.ld_q + (size_t)it.hk * a.dh + col;
+  int x = it.x0 + KEYS * w;
+  float m = -INFINITY, l = 0.f, acc[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) acc[i] = 0.f;
+  if (x < it.x1) {
+    floatx4 k[2][U], v[2][U];
+    unsigned long long there[2];
+    auto load = [&](int b, int at) {
+      there[b] = __ballot(at >= 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long o = max(__shfl(at, u * KPI + kg, 64), 0) * ld;
+        k[b][u] = __builtin_nontemporal_load(reinterpret_cast<const floatx4*>(kp + o));
+        v[b][u] = __builtin_nontemporal_load(reinterpret_cast<const floatx4*>(vp + o));
+      }
+    };
+    load(0, row_of(a, it, x + lane % KEYS, page));
+    float q[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) q[i] = qp[i] * (a.scale * LOG2E);
+    page = page_of(a, it.s, it.pre, x + STRIDE + lane % KEYS);
+    // the keys of one half of the registers, while those of the other come
+    auto step = [&](auto b) {
+      constexpr int B = decltype(b)::value;
+      if (x + STRIDE < it.x1) {
+        load(1 - B, row_of(a, it, x + STRIDE + lane % KEYS, page));
+        page = page_of(a, it.s, it.pre, x + 2 * STRIDE + lane % KEYS);
+      }
+      float s[U], mx = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float y[E];
+        unpack(k[B][u], y);
+        float d = q[0] * y[0];
+#pragma unroll
+        for (int i = 1; i < E; ++i) d += q[i] * y[i];
+        s[u] = aurlanes::group_reduce<1, LP, false>(live ? d : 0.f);
+      }
+      if (there[B] != ~0ull) {  // keys that are not there: no score, and no value whatever lies in the row
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (!(there[B] >> (u * KPI + kg) & 1)) {
+            s[u] = -INFINITY;
+            v[B][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u]);
+      mx = aurlanes::group_reduce<LP, 64, true>(mx);
+      const float at = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m - at);
+      m = mx;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[i] *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float p = __builtin_amdgcn_exp2f(s[u] - at);
+        l += p;
+        float y[E];
+        unpack(v[B][u], y);
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[i] += p * y[i];
+      }
+      x += STRIDE;
+    };
+    for (;;) {
+      step(std::integral_constant<int, 0>{});
+      if (x >= it.x1) break;
+      step(std::integral_constant<int, 1>{});
+      if (x >= it.x1) break;
+    }
+  }
+  l = aurlanes::group_reduce<LP, 64, false>(l);
+#pragma unroll
+  for (int i = 0; i < E; ++i) acc[i] = aurlanes::group_sum_lanes<LP>(acc[i]);
+  if (kg == 0 && live) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) *reinterpret_cast<floatx4*>(&lds.o[w][col + i]) = floatx4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
+  }
+  if (lane == 0) {
+    lds.m[w] = m;
+    lds.l[w] = l;
+  }
+  __syncthreads();
+  if (4 * tid >= a.dh) return;
+  float M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int j = 0; j < NW; ++j) M = fmaxf(M, lds.m[j]);
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < NW; ++j) {
+    const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(lds.m[j] - M);
+    L += f * lds.l[j];
+    o += f * *reinterpret_cast<const floatx4*>(&lds.o[j][4 * tid]);
+  }
+  store(a, it, 0, 4 * tid, o, M, L);
+}
+
 // ---------------------------------------------------------------- many rows: keys through LDS
 
 // 16·NR·W rows an item, 16·NR of each of the block's W waves.  The block lays KT keys down in LDS as
@@ -918,11 +1068,14 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
 
 // ---------------------------------------------------------------- launches
 
-template <class T, int DT>
-__global__ void __launch_bounds__(64 * NW, 2) paged_mha_rows_kernel(MhaArgs a) {
-  __shared__ RowsLds<DT> lds;
-  rows_item<T, DT>(a, lds);
-}
+// What a launch of 256-thread blocks holds: own items of 16 rows (ONE: of one), prefix items of none, 16
+// or 64 rows.
+template <class T, int DT, bool ONE, int PRE>
+union StepLds {
+  typename std::conditional<(PRE == 16 || !ONE), RowsLds<DT>, OneLds<T>>::type rows;
+  typename std::conditional<ONE, OneLds<T>, RowsLds<DT>>::type own;
+  typename std::conditional<PRE == 64, TileLds<T, DT, NW>, OneLds<T>>::type tile;
+};
 
 // Waves a SIMD should hold: bf16 keys leave registers for three.
 template <class T, int DT, int NR>
@@ -936,16 +1089,18 @@ __global__ void __launch_bounds__(64 * W, (kWaves<T, DT, NR>)) paged_mha_tile_ke
 
 // A decode step of many sequences in one launch: the prefix's items, bound by their products, beside the
 // own ones, bound by memory.
-template <class T, int DT>
-__global__ void __launch_bounds__(64 * NW, (kWaves<T, DT, 1>)) paged_mha_step_kernel(MhaArgs a) {
-  __shared__ __attribute__((aligned(1024))) union {
-    TileLds<T, DT, NW> tile;
-    RowsLds<DT> rows;
-  } lds;
-  if ((int)blockIdx.x < a.p_items)
-    tile_item<T, DT, 1, NW>(a, lds.tile);
+template <class T, int DT, bool ONE, int PRE>
+__global__ void __launch_bounds__(64 * NW, (PRE == 64 ? kWaves<T, DT, 1> : 2)) paged_mha_step_kernel(MhaArgs a) {
+  __shared__ __attribute__((aligned(1024))) StepLds<T, DT, ONE, PRE> lds;
+  if (PRE > 0 && (int)blockIdx.x < a.p_items) {
+    if constexpr (PRE == 64) tile_item<T, DT, 1, NW>(a, lds.tile);
+    if constexpr (PRE == 16) rows_item<T, DT>(a, lds.rows);
+    return;
+  }
+  if constexpr (ONE)
+    one_item<T, DT>(a, lds.own);
   else
-    rows_item<T, DT>(a, lds.rows);
+    rows_item<T, DT>(a, lds.own);
 }
 
 // out and lse of a row from the records of its ranges: one wave a row.  The lanes of a group have 4
@@ -1079,18 +1234,23 @@ size_t ws_floats(const Plan& p, const Batch& b, int H, int dh) {
 template <class T, int DT>
 void launch_tile(const MhaArgs& a, int p_tile, int tile, unsigned items, hipStream_t st) {
   const dim3 g(items);
-  if (p_tile == 64 && tile == 16)
-    hipLaunchKernelGGL((paged_mha_step_kernel<T, DT>), g, dim3(256), 0, st, a);
-  else if (tile == 16)
-    hipLaunchKernelGGL((paged_mha_rows_kernel<T, DT>), g, dim3(256), 0, st, a);
-  else if (tile == 64)
-    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 4>), g, dim3(256), 0, st, a);
-  else if constexpr (DT > 4)
+  const dim3 four(256);
+  if (tile == 16 && a.b.max_tok == 1 && a.G == 1) {
+    auto* step = p_tile == 64 ? paged_mha_step_kernel<T, DT, true, 64> : p_tile == 16 ? paged_mha_step_kernel<T, DT, true, 16>
+                 : paged_mha_step_kernel<T, DT, true, 0>;
+    hipLaunchKernelGGL(step, g, four, 0, st, a);
+  } else if (tile == 16) {  // (prefix items of 16 rows are the same code)
+    auto* step = p_tile == 64 ? paged_mha_step_kernel<T, DT, false, 64> : paged_mha_step_kernel<T, DT, false, 0>;
+    hipLaunchKernelGGL(step, g, four, 0, st, a);
+  } else if (tile == 64) {
+    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 4>), g, four, 0, st, a);
+  } else if constexpr (DT > 4) {
     hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 8>), g, dim3(512), 0, st, a);
-  else if (tile == 128)
-    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 2, 4>), g, dim3(256), 0, st, a);
-  else
+  } else if (tile == 128) {
+    hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 2, 4>), g, four, 0, st, a);
+  } else {
     hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 2, 8>), g, dim3(512), 0, st, a);
+  }
 }
 
 template <class T>
