@@ -603,16 +603,19 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
   }
 }
 
-// ---------------------------------------------------------------- one row: no matrix products
+// ---------------------------------------------------------------- single tokens: no matrix products
 
-// A single row (one new token, a head of its own).  Its items are bound by reading K and V; the MFMA of
-// rows_item works on 16 rows whatever there are, and its cycles stand between the loads: 64 sequences of
-// 1024 keys, 16 heads of 64, take 85 µs there and 67 here (5.9 TB/s), bf16 keys 53 and 40.  LP lanes have a
-// key's head, 16 bytes each, so that a load brings 64/LP whole keys; a score is added up over the LP lanes,
-// l and the columns over the key groups once at the end.  All of it is fp32 arithmetic.  While one half of
-// the registers is in use, the loads of the other are under way, and the page of the step after them.
+// The rows of one token: the query heads of a K/V head, all of which see the same keys.  Such items are
+// bound by reading K and V; the MFMA of rows_item works on 16 rows whatever there are, and its cycles stand
+// between the loads.  Vector instructions cost by the row.  64 sequences of 1024 keys, 16 K/V heads of 64,
+// µs by vectors and by the MFMA: 1 row 67 and 85 (5.9 TB/s), 2 rows 73 and 84, 4 rows 83 and 92; bf16 keys
+// 1 row 40 and 53, 2 rows 43 and 54, 4 rows 55 and 56 (with a prefix of 2048 beside it 40 and 38): so 4
+// rows in fp32, 2 in bf16.  LP lanes have a key's head, 16 bytes each, so that a load brings 64/LP whole
+// keys; a score is added up over the LP lanes, l and the columns over the key groups once at the end, all
+// of it in fp32.  While one half of the registers is in use, the loads of the other are under way, and the
+// page of the step after them.
 template <class T, int DT>
-struct OneRow {
+struct FewRows {
   static constexpr int E = 16 / sizeof(T);                // columns of a lane
   static constexpr int N = (16 * DT + E - 1) / E;         // lanes of a head
   static constexpr int LP = N <= 2 ? 2 : N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : 32;
@@ -621,10 +624,10 @@ struct OneRow {
   static constexpr int KEYS = U * KPI;                    // of a step; a lane finds the row of one
   static_assert(KEYS <= 64 && N <= 32, "a wave finds the rows of a step");
 };
-template <class T>
-struct OneLds {
-  float m[NW], l[NW];
-  __attribute__((aligned(16))) float o[NW][128];
+template <int R>
+struct FewLds {
+  float m[NW][R], l[NW][R];
+  __attribute__((aligned(16))) float o[NW][R][128];
 };
 __device__ __forceinline__ void unpack(floatx4 x, float (&y)[4]) {
 #pragma unroll
@@ -638,9 +641,9 @@ __device__ __forceinline__ void unpack(floatx4 x, float (&y)[8]) {
   }
 }
 
-template <class T, int DT>
-__device__ __forceinline__ void one_item(const MhaArgs& a, OneLds<T>& lds) {
-  using G = OneRow<T, DT>;
+template <class T, int DT, int R>
+__device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
+  using G = FewRows<T, DT>;
   constexpr int E = G::E, LP = G::LP, U = G::U, KPI = G::KPI, KEYS = G::KEYS, STRIDE = NW * KEYS;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int part = lane % LP, kg = lane / LP;
@@ -649,15 +652,20 @@ __device__ __forceinline__ void one_item(const MhaArgs& a, OneLds<T>& lds) {
 
   Item it;
   int page;
-  if (!take_item<1>(a, it, KEYS * w + lane % KEYS, page)) return;
+  if (!take_item<R>(a, it, KEYS * w + lane % KEYS, page)) return;
   const char* const kp = static_cast<const char*>(a.k) + ((size_t)it.hk * a.dh + col) * sizeof(T);
   const char* const vp = static_cast<const char*>(a.v) + ((size_t)it.hk * a.dh + col) * sizeof(T);
   const long long ld = (long long)a.Hkv * a.dh * sizeof(T);
-  const float* qp = a.q + (size_t)it.tok0 * a.ld_q + (size_t)it.hk * a.dh + col;
+  const float* qp = a.q + (size_t)it.tok0 * a.ld_q + (size_t)it.hk * a.G * a.dh + col;
   int x = it.x0 + KEYS * w;
-  float m = -INFINITY, l = 0.f, acc[E];
+  float m[R], l[R], acc[R][E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) acc[i] = 0.f;
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[r][i] = 0.f;
+  }
   if (x < it.x1) {
     floatx4 k[2][U], v[2][U];
     unsigned long long there[2];
@@ -671,9 +679,11 @@ __device__ __forceinline__ void one_item(const MhaArgs& a, OneLds<T>& lds) {
       }
     };
     load(0, row_of(a, it, x + lane % KEYS, page));
-    float q[E];
+    float q[R][E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) q[i] = qp[i] * (a.scale * LOG2E);
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < E; ++i) q[r][i] = qp[(size_t)min(r, a.G - 1) * a.dh + i] * (a.scale * LOG2E);
     page = page_of(a, it.s, it.pre, x + STRIDE + lane % KEYS);
     // the keys of one half of the registers, while those of the other come
     auto step = [&](auto b) {
@@ -682,40 +692,53 @@ __device__ __forceinline__ void one_item(const MhaArgs& a, OneLds<T>& lds) {
         load(1 - B, row_of(a, it, x + STRIDE + lane % KEYS, page));
         page = page_of(a, it.s, it.pre, x + 2 * STRIDE + lane % KEYS);
       }
-      float s[U], mx = m;
+      float s[R][U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float y[E];
         unpack(k[B][u], y);
-        float d = q[0] * y[0];
 #pragma unroll
-        for (int i = 1; i < E; ++i) d += q[i] * y[i];
-        s[u] = aurlanes::group_reduce<1, LP, false>(live ? d : 0.f);
+        for (int r = 0; r < R; ++r) {
+          float d = q[r][0] * y[0];
+#pragma unroll
+          for (int i = 1; i < E; ++i) d += q[r][i] * y[i];
+          s[r][u] = aurlanes::group_reduce<1, LP, false>(live ? d : 0.f);
+        }
       }
       if (there[B] != ~0ull) {  // keys that are not there: no score, and no value whatever lies in the row
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (!(there[B] >> (u * KPI + kg) & 1)) {
-            s[u] = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[r][u] = -INFINITY;
             v[B][u] = floatx4{0.f, 0.f, 0.f, 0.f};
           }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u]);
-      mx = aurlanes::group_reduce<LP, 64, true>(mx);
-      const float at = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m - at);
-      m = mx;
-      l *= alpha;
+      for (int r = 0; r < R; ++r) {
+        float mx = m[r];
 #pragma unroll
-      for (int i = 0; i < E; ++i) acc[i] *= alpha;
+        for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[r][u]);
+        mx = aurlanes::group_reduce<LP, 64, true>(mx);
+        const float at = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m[r] - at);
+        m[r] = mx;
+        l[r] *= alpha;
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[r][i] *= alpha;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          s[r][u] = __builtin_amdgcn_exp2f(s[r][u] - at);
+          l[r] += s[r][u];
+        }
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float p = __builtin_amdgcn_exp2f(s[u] - at);
-        l += p;
         float y[E];
         unpack(v[B][u], y);
 #pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] += p * y[i];
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < E; ++i) acc[r][i] += s[r][u] * y[i];
       }
       x += STRIDE;
     };
@@ -726,30 +749,35 @@ __device__ __forceinline__ void one_item(const MhaArgs& a, OneLds<T>& lds) {
       if (x >= it.x1) break;
     }
   }
-  l = aurlanes::group_reduce<LP, 64, false>(l);
 #pragma unroll
-  for (int i = 0; i < E; ++i) acc[i] = aurlanes::group_sum_lanes<LP>(acc[i]);
-  if (kg == 0 && live) {
+  for (int r = 0; r < R; ++r) {
+    l[r] = aurlanes::group_reduce<LP, 64, false>(l[r]);
 #pragma unroll
-    for (int i = 0; i < E; i += 4) *reinterpret_cast<floatx4*>(&lds.o[w][col + i]) = floatx4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
-  }
-  if (lane == 0) {
-    lds.m[w] = m;
-    lds.l[w] = l;
+    for (int i = 0; i < E; ++i) acc[r][i] = aurlanes::group_sum_lanes<LP>(acc[r][i]);
+    if (kg == 0 && live) {
+#pragma unroll
+      for (int i = 0; i < E; i += 4)
+        *reinterpret_cast<floatx4*>(&lds.o[w][r][col + i]) = floatx4{acc[r][i], acc[r][i + 1], acc[r][i + 2], acc[r][i + 3]};
+    }
+    if (lane == 0) {
+      lds.m[w][r] = m[r];
+      lds.l[w][r] = l[r];
+    }
   }
   __syncthreads();
-  if (4 * tid >= a.dh) return;
+  const int r = tid / 32, c = 4 * (tid % 32);
+  if (r >= min(R, it.n_rows) || c >= a.dh) return;
   float M = -INFINITY, L = 0.f;
 #pragma unroll
-  for (int j = 0; j < NW; ++j) M = fmaxf(M, lds.m[j]);
+  for (int j = 0; j < NW; ++j) M = fmaxf(M, lds.m[j][r]);
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < NW; ++j) {
-    const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(lds.m[j] - M);
-    L += f * lds.l[j];
-    o += f * *reinterpret_cast<const floatx4*>(&lds.o[j][4 * tid]);
+    const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(lds.m[j][r] - M);
+    L += f * lds.l[j][r];
+    o += f * *reinterpret_cast<const floatx4*>(&lds.o[j][r][c]);
   }
-  store(a, it, 0, 4 * tid, o, M, L);
+  store(a, it, r, c, o, M, L);
 }
 
 // ---------------------------------------------------------------- many rows: keys through LDS
@@ -1068,13 +1096,11 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
 
 // ---------------------------------------------------------------- launches
 
-// What a launch of 256-thread blocks holds: own items of 16 rows (ONE: of one), prefix items of none, 16
-// or 64 rows.
-template <class T, int DT, bool ONE, int PRE>
+// What a launch of 256-thread blocks holds: own items of 1, 4 or 16 rows, prefix items of none, 16 or 64.
+template <class T, int DT, int R, int PRE>
 union StepLds {
-  typename std::conditional<(PRE == 16 || !ONE), RowsLds<DT>, OneLds<T>>::type rows;
-  typename std::conditional<ONE, OneLds<T>, RowsLds<DT>>::type own;
-  typename std::conditional<PRE == 64, TileLds<T, DT, NW>, OneLds<T>>::type tile;
+  typename std::conditional<R == 16, RowsLds<DT>, FewLds<R>>::type own;
+  typename std::conditional<PRE == 64, TileLds<T, DT, NW>, typename std::conditional<PRE == 16, RowsLds<DT>, char>::type>::type pre;
 };
 
 // Waves a SIMD should hold: bf16 keys leave registers for three.
@@ -1089,16 +1115,16 @@ __global__ void __launch_bounds__(64 * W, (kWaves<T, DT, NR>)) paged_mha_tile_ke
 
 // A decode step of many sequences in one launch: the prefix's items, bound by their products, beside the
 // own ones, bound by memory.
-template <class T, int DT, bool ONE, int PRE>
+template <class T, int DT, int R, int PRE>
 __global__ void __launch_bounds__(64 * NW, (PRE == 64 ? kWaves<T, DT, 1> : 2)) paged_mha_step_kernel(MhaArgs a) {
-  __shared__ __attribute__((aligned(1024))) StepLds<T, DT, ONE, PRE> lds;
+  __shared__ __attribute__((aligned(1024))) StepLds<T, DT, R, PRE> lds;
   if (PRE > 0 && (int)blockIdx.x < a.p_items) {
-    if constexpr (PRE == 64) tile_item<T, DT, 1, NW>(a, lds.tile);
-    if constexpr (PRE == 16) rows_item<T, DT>(a, lds.rows);
+    if constexpr (PRE == 64) tile_item<T, DT, 1, NW>(a, lds.pre);
+    if constexpr (PRE == 16) rows_item<T, DT>(a, lds.pre);
     return;
   }
-  if constexpr (ONE)
-    one_item<T, DT>(a, lds.own);
+  if constexpr (R < 16)
+    few_item<T, DT, R>(a, lds.own);
   else
     rows_item<T, DT>(a, lds.own);
 }
@@ -1230,18 +1256,27 @@ size_t ws_floats(const Plan& p, const Batch& b, int H, int dh) {
   return p.parts() > 1 ? (size_t)p.parts() * b.n_tok * H * (dh + 2) : 0;
 }
 
+// Own items of R rows, prefix items of 16, 64 or none.
+template <class T, int DT, int R>
+void launch_step(const MhaArgs& a, int p_tile, unsigned items, hipStream_t st) {
+  auto* step = p_tile == 64 ? paged_mha_step_kernel<T, DT, R, 64> : paged_mha_step_kernel<T, DT, R, 0>;
+  if constexpr (R < 16)
+    if (p_tile == 16) step = paged_mha_step_kernel<T, DT, R, 16>;
+  hipLaunchKernelGGL(step, dim3(items), dim3(256), 0, st, a);
+}
+
 // p_tile 0: items of one kind (or of one tile).
 template <class T, int DT>
 void launch_tile(const MhaArgs& a, int p_tile, int tile, unsigned items, hipStream_t st) {
   const dim3 g(items);
   const dim3 four(256);
-  if (tile == 16 && a.b.max_tok == 1 && a.G == 1) {
-    auto* step = p_tile == 64 ? paged_mha_step_kernel<T, DT, true, 64> : p_tile == 16 ? paged_mha_step_kernel<T, DT, true, 16>
-                 : paged_mha_step_kernel<T, DT, true, 0>;
-    hipLaunchKernelGGL(step, g, four, 0, st, a);
-  } else if (tile == 16) {  // (prefix items of 16 rows are the same code)
-    auto* step = p_tile == 64 ? paged_mha_step_kernel<T, DT, false, 64> : paged_mha_step_kernel<T, DT, false, 0>;
-    hipLaunchKernelGGL(step, g, four, 0, st, a);
+  if (tile == 16) {
+    const int rows = a.b.max_tok == 1 ? a.G : 16;
+    if (rows == 1) return launch_step<T, DT, 1>(a, p_tile, items, st);
+    if (rows == 2) return launch_step<T, DT, 2>(a, p_tile, items, st);
+    if constexpr (std::is_same<T, float>::value)
+      if (rows <= 4) return launch_step<T, DT, 4>(a, p_tile, items, st);
+    launch_step<T, DT, 16>(a, p_tile, items, st);
   } else if (tile == 64) {
     hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 4>), g, four, 0, st, a);
   } else if constexpr (DT > 4) {

@@ -121,13 +121,14 @@ def test_attention_matches_float64(ctx, b, n, past, prefix, page, kv, group, dh,
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("group", [1, 2, 3])
 @pytest.mark.parametrize("dh", [8, 16, 24, 40, 64, 72, 96, 120, 128])
 @pytest.mark.parametrize("n,past,prefix", [([1, 0, 1, 1], [0, 9, 62, 500], 0), ([1], [129], 65), ([1, 1, 1], [63, 64, 0], 257),
                                            ([1] * 35, [7 * i % 90 for i in range(35)], 300)])
-def test_steps_of_single_rows(ctx, n, past, prefix, dh, dtype):
-    """One new token a sequence, every head with keys of its own: the lengths around a wave's step."""
+def test_steps_of_few_rows(ctx, n, past, prefix, dh, group, dtype):
+    """One new token a sequence, few heads on the same keys: the lengths around a wave's step."""
     rng = np.random.default_rng(dh + len(n))
-    c = Case(rng, n, [x + y for x, y in zip(n, past)], prefix, 16, 3, 1, dh, dtype, behind=1)
+    c = Case(rng, n, [x + y for x, y in zip(n, past)], prefix, 16, 3, group, dh, dtype, behind=1)
     dev = Device(ctx, c, ld_q=c.h * dh + 4)
     dev.attend()
     _check(c, *dev.result())
