@@ -1209,7 +1209,10 @@ constexpr uint32_t kMaxRows = 0x7fffff00u;  // query rows of a call, and a tile 
 // sequences on a prefix of 32768 in bf16: 86 µs, with 256 items 140, with 2048 97), with larger ones 4
 // (tails of 128 on 2048: 113 µs, with 768 items 120), of 8 waves one (512 sequences on a prefix of 16384:
 // 240 µs, with 1024 items 303).
-constexpr int kItems16 = 768, kItems = 1024, kItems8 = 256;
+// fp32 keys of more than 64 columns fill the registers, and keys without a prefix's items beside them the
+// memory, with 2 a CU (64 sequences of 1024 keys, 8 heads of 128, 4 rows each: 77 µs, with 768 items 85; one
+// sequence of 16884 keys, 16 heads of 64: 28, with 768 items 30).
+constexpr int kItems16 = 768, kItemsWide = 512, kItems = 1024, kItems8 = 256;
 // An axis up to so many keys is one range: a join costs 4 µs, 128 keys of a 16-row item (a round of its
 // waves) 1.5 µs.  Longer ones are cut into ranges of 128 keys or more, 48 at most.
 constexpr int kWhole16 = 384, kWhole = 256;
@@ -1218,7 +1221,7 @@ constexpr int kLeastKeys = 128, kMostRanges = 48;
 // on a prefix of 1294, 108,000: 13 against 33 µs; 53 sequences of 5 heads on 139, 35,000: 22 against 10).
 constexpr int kPoolFrom = 65536;
 
-Plan make_plan(const Batch& b, int Hkv, int G, int dh) {
+Plan make_plan(const Batch& b, int Hkv, int G, int dh, bool f32) {
   Plan p{};
   const int P = b.prefix_len;
   const long long o_rows = (long long)b.max_tok * G, p_rows = (long long)b.n_tok * G;
@@ -1233,7 +1236,8 @@ Plan make_plan(const Batch& b, int Hkv, int G, int dh) {
   // Ranges of one length, so that no item is left with a few keys.
   // (A CU holds one block of 8 waves: more of them than CUs would be a second round.)
   auto eight = [dh](int tile) { return tile == 256 || (tile == 128 && dh > 64); };
-  auto items = [&](int tile) { return eight(tile) ? kItems8 : tile > 16 ? kItems : kItems16; };
+  const int items16 = f32 && (dh > 64 || !p.pooled) ? kItemsWide : kItems16;
+  auto items = [&](int tile) { return eight(tile) ? kItems8 : tile > 16 ? kItems : items16; };
   auto cut = [&](int n, double want, int tile, int* keys) {
     int splits = 1;
     if (n > (tile == 16 ? kWhole16 : kWhole)) {
@@ -1312,7 +1316,8 @@ size_t aur_mha_paged_ws_bytes(const aur_paged_cache* cache, const aur_paged_batc
   if (check_paged(nullptr, "aur_mha_paged_ws_bytes", cache, batch, &b) != 0 || n_head == 0 || n_head > 4096 ||
       (uint64_t)b.n_tok * n_head > kMaxRows || n_head % cache->n_kv_head != 0 || b.b == 0 || b.n_tok == 0)
     return 0;
-  return 4 * ws_floats(make_plan(b, (int)cache->n_kv_head, (int)(n_head / cache->n_kv_head), (int)cache->d_head), b, (int)n_head,
+  return 4 * ws_floats(make_plan(b, (int)cache->n_kv_head, (int)(n_head / cache->n_kv_head), (int)cache->d_head,
+                                  cache->dtype == AUR_PAGED_F32), b, (int)n_head,
                        (int)cache->d_head);
 }
 
@@ -1338,7 +1343,7 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
   a.H = (int)n_head; a.Hkv = (int)cache->n_kv_head; a.G = a.H / a.Hkv; a.dh = (int)cache->d_head;
   a.n_pages = (int)cache->n_pages; a.sh = log2_of(cache->page_len);
   a.scale = 1.0f / sqrtf((float)a.dh);
-  const Plan p = make_plan(a.b, a.Hkv, a.G, a.dh);
+  const Plan p = make_plan(a.b, a.Hkv, a.G, a.dh, cache->dtype == AUR_PAGED_F32);
   a.pooled = p.pooled;
   a.p_tiles = p.p_tiles; a.p_splits = p.p_splits; a.p_keys = p.p_keys;
   a.o_tiles = p.o_tiles; a.o_splits = p.o_splits; a.o_keys = p.o_keys;
