@@ -2,26 +2,24 @@
 // prefix.  Query row (token (s, i), head h) sees the P keys of the prefix and
 // its sequence's own keys 0 .. j, j = L − n + i:
 //   out = Σ softmax(q·k / √d_head) v,   lse = log Σ exp(q·k / √d_head);
-// a row that sees no key gets out 0, lse −∞.
+// a row that sees no key gets out 0, lse −∞.  Scores carry log2(e) from the
+// queries on, so that every exponential is an exp2.
 //
-// Work is cut into items (one block each): up to 16·RT query rows that read the
-// same keys, and a range of those keys.
+// Work is cut into items (one block each): query rows that read the same keys,
+// and a range of those keys.
 //   * Pooled (few rows a sequence, as in decode): the rows of ALL sequences of one
 //     K/V head against a range of the prefix, so the prefix is read once for all,
 //     and the rows of one sequence against a range of its own keys.
 //   * Otherwise the rows of one sequence against prefix and own keys as one axis.
-// Where a row's keys are cut into several ranges, items leave (m, l, Σ p v) and a
-// second launch joins them in the order of the ranges: the result does not
-// depend on which block ends first.
+// Where a row's keys are cut into several ranges, items leave (m, l, Σ p v) in the
+// caller's scratch and a second launch joins them in the order of the ranges: the
+// result does not depend on which block ends first.
 //
-// In an item each of the block's 4 waves takes every fourth group of 32 keys and
-// keeps its own running maximum and sum; the waves are joined through LDS in
-// their order.  K and V go from the pools straight into the registers that feed
-// the MFMA, both as 16-byte loads: Sᵀ = K·Qᵀ takes 4 consecutive columns of a key
-// per lane (the four MFMAs that they feed use them as k = 0 … 3 of 4 lane groups),
-// its result is, as it lies, the B operand of Oᵀ += Vᵀ·Pᵀ, and there a lane's 4
-// consecutive columns of V are rows of four MFMAs (row r of MFMA c is column
-// 4r + c), so V needs no transposition.
+// Three kinds of items, by their rows:
+//   few_item   one token, 1 to 4 rows: vector instructions, bound by reading the keys
+//   rows_item  up to 16 rows: keys from the pools straight into the registers that
+//              feed the MFMA, bound by reading them and by the MFMA's cycles
+//   tile_item  64, 128 or 256 rows: keys laid down in LDS, bound by the MFMA
 #include "attention.hpp"
 #include "attention_split.hpp"
 #include "common.hpp"
@@ -454,7 +452,8 @@ __device__ __forceinline__ bool finite(const Sums<DT, RT>& s, bool live) {
   return __ballot(live && z != 0.f) == 0;  // 0 times an infinity or NaN is NaN
 }
 
-// The sums of a wave's rows over keys x, x + stride, … again, where they came out as infinity or NaN:
+// The sums of a wave's rows over keys x, x + stride, … again, where they came out as infinity or NaN (from
+// such operands, or from a split into parts, which has no infinities):
 // scores by the fp32 MFMA from whole operands, and every row adds the values of those keys alone that
 // it sees (0 times an infinity that it does not see would be NaN).
 template <class T, int DT, int RT>
@@ -521,7 +520,16 @@ __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, in
 
 // ---------------------------------------------------------------- few rows: keys through the registers
 
-// Up to 16 rows an item.
+// Up to 16 rows an item.  Each of the block's 4 waves takes every fourth group of 32 keys and keeps its own
+// running maximum and sum; the waves are joined through LDS in their order.  K and V are 16-byte loads into
+// the registers that feed the MFMA: Sᵀ = K·Qᵀ takes consecutive columns of a key per lane, its result is, as
+// it lies, the other operand of Oᵀ += Vᵀ·Pᵀ, and there a lane's 4 consecutive columns of V are rows of four
+// MFMAs (row r of MFMA c is column 4r + c), so V needs no transposition and nothing passes through LDS on
+// the way.  fp32 keys go into the fp32 MFMA; bf16 keys into the bf16 one with Q and P as three bf16 parts,
+// which keep 2^-24 of each.  A wave's next K is under way while it works, its V from the scores on.  Bound
+// by the reading with the MFMA's cycles in between: 64 sequences of 1024 keys, 16 K/V heads of 64, 4 rows
+// each: 56 µs in bf16 (3.6 TB/s), 92 in fp32 (4.3 TB/s); on widened keys the fp32 MFMA took bf16's own
+// keys of 64 such sequences 160 µs in a first version, the bf16 one 60.
 template <int DT>
 struct RowsLds {
   static constexpr int R = 16, OS = 64 * ((DT + 3) / 4) + 4;
@@ -785,7 +793,12 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
 // 16·NR·W rows an item, 16·NR of each of the block's W waves.  The block lays KT keys down in LDS as
 // bf16 parts (fp32: three, whose six products above 2^-24 of the largest the MFMA sums; bf16 keys are
 // one part, Q and P three), K as [key][column], V as [column][key], while the next keys' loads are
-// under way.
+// under way: six bf16 products cost 6/16 of the fp32 MFMA's time for one.  Bound by the MFMA and by what
+// lies between its issues, the conversion of the next tile and the softmax: 16 sequences of 512 tokens on a
+// prefix of 4096, 16 heads of 64, fp32: 667 µs, 161 TFLOP/s of the 210 that a bf16 product of 1262 leaves
+// for six.  The more rows, the less often K and V are loaded, converted and read from LDS: 16 rows a wave
+// of 4 waves 1191 µs, of 8 waves 804, 32 rows a wave with the keys' places in LDS 667.  Tiles of 32x32 took
+// 656 at d_head 64 and spilled at 128.
 template <class T, int DT, int W>
 struct TileGeo {
   static constexpr bool F32 = std::is_same<T, float>::value;
@@ -1096,7 +1109,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
 
 // ---------------------------------------------------------------- launches
 
-// What a launch of 256-thread blocks holds: own items of 1, 4 or 16 rows, prefix items of none, 16 or 64.
+// What a launch of 256-thread blocks holds: own items of 1, 2, 4 or 16 rows, prefix items of none, 16 or 64.
 template <class T, int DT, int R, int PRE>
 union StepLds {
   typename std::conditional<R == 16, RowsLds<DT>, FewLds<R>>::type own;
@@ -1114,7 +1127,8 @@ __global__ void __launch_bounds__(64 * W, (kWaves<T, DT, NR>)) paged_mha_tile_ke
 }
 
 // A decode step of many sequences in one launch: the prefix's items, bound by their products, beside the
-// own ones, bound by memory.
+// own ones, bound by memory (64 sequences of 1024 keys on a prefix of 32768, 16 heads of 64, bf16: 80 µs
+// with the join, 91 in two launches; 48 sequences of 4 heads of 128 on 4999: 46 and 58).
 template <class T, int DT, int R, int PRE>
 __global__ void __launch_bounds__(64 * NW, (PRE == 64 ? kWaves<T, DT, 1> : 2)) paged_mha_step_kernel(MhaArgs a) {
   __shared__ __attribute__((aligned(1024))) StepLds<T, DT, R, PRE> lds;
