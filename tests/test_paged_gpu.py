@@ -135,6 +135,33 @@ def test_steps_of_few_rows(ctx, n, past, prefix, dh, group, dtype):
     dev.free()
 
 
+POOLED = [  # sequences, tokens of each, prefix, kv heads, group: enough of them that the prefix is read once for all
+    (20, 1, 1300, 3, 1),   # 20 rows on the prefix
+    (9, 1, 2500, 4, 3),
+    (40, 1, 900, 2, 1),    # 40
+    (40, 1, 900, 2, 2),
+    (23, 1, 1601, 2, 4),
+    (30, 1, 1201, 2, 5),   # 150
+    (90, 1, 401, 2, 3),    # 270: prefix items of their own launch
+    (21, 3, 1177, 3, 2),   # several tokens
+    (12, 9, 2001, 3, 3),   # 27 own rows
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dh", [16, 48, 64, 88, 128])
+@pytest.mark.parametrize("b,n,prefix,kv,group", POOLED)
+def test_prefix_read_once_for_all(ctx, b, n, prefix, kv, group, dh, dtype):
+    rng = np.random.default_rng(b + dh)
+    toks = [n] * b
+    toks[b // 2] = 0  # a sequence that waits
+    c = Case(rng, toks, [x + (5 * i) % 37 for i, x in enumerate(toks)], prefix, 16, kv, group, dh, dtype, behind=1)
+    dev = Device(ctx, c, ld_o=c.h * dh + 4)
+    dev.attend()
+    _check(c, *dev.result())
+    dev.free()
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_attention_random_batches(ctx, seed):
     rng = np.random.default_rng(seed)
