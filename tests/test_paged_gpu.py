@@ -245,6 +245,30 @@ def test_infinities_stay_behind_the_mask(ctx, dtype, n, prefix, group):
     dev.free()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("group", [1, 2, 4])
+def test_infinities_that_single_tokens_see(ctx, dtype, group):
+    """Infinities and NaN among the keys of a step give what the formula gives, and only where they are seen."""
+    c = Case(np.random.default_rng(15), [1] * 5, [90, 40, 130, 70, 20], 40, 8, 2, group, 64, dtype)
+    own = [c.rows(c.pages[s], c.length[s]) for s in range(5)]
+    c.vp[own[0][5], 3], c.vp[own[0][80], 70] = np.inf, -np.inf
+    c.vp[own[1][39], 9] = np.nan
+    c.kp[own[2][100], 2] = np.inf  # the query's sign decides: NaN, or a key without weight
+    c.kp[own[3][0], 64:] = np.nan
+    dev = Device(ctx, c)
+    dev.attend()
+    out, lse = dev.result()
+    with np.errstate(all="ignore"):
+        want, _, tol, _ = attention(c)
+    fine = np.isfinite(want)
+    assert np.array_equal(fine, np.isfinite(out)) and np.array_equal(np.isnan(want), np.isnan(out))
+    assert np.array_equal(out[np.isinf(want)], want[np.isinf(want)])
+    bounded = fine & np.isfinite(tol)  # (an infinite key without weight leaves its row no bound)
+    assert bounded[4].all() and bounded[0].sum() == c.h * 64 - 2 * group
+    assert np.all(np.abs(out[bounded] - want[bounded]) <= tol[bounded])
+    dev.free()
+
+
 def test_large_scores_and_small_ones(ctx):
     """Scores far apart (±10^3, where the softmax is a single key) and all −∞."""
     rng = np.random.default_rng(8)
@@ -405,6 +429,39 @@ def test_pool_beyond_32_bit_offsets(ctx):
     c.pages, c.n_pages = np.array([[0, 1]], np.int32), 2
     want, _, tol, _ = attention(c)
     assert np.all(np.abs(got - want) <= tol)
+    for x in bufs + [ws]:
+        x.free()
+    cache.free()
+
+
+@pytest.mark.parametrize("n,group", [(1, 1), (1, 2), (1, 16), (3, 4)])
+def test_step_beyond_32_bit_offsets(ctx, n, group):
+    """The same for items of few rows."""
+    from aurora_amd.gpu import GpuBuffer, PagedBatch, PagedKvAppendKernel, PagedKvCache, PagedMhaKernel
+
+    kv, dh, page, own = 16, 128, 256, 300
+    row, d = kv * dh, kv * dh * group
+    n_pages = (2**31 + 2**28) // (page * row)
+    rng = np.random.default_rng(16)
+    c = Case(rng, [n], [own], 0, page, kv, group, dh, "bf16")
+    cache = PagedKvCache(GpuBuffer.empty(ctx, n_pages * page * row, np.uint16),
+                         GpuBuffer.empty(ctx, n_pages * page * row, np.uint16), n_pages, page, kv, dh, "bf16")
+    up = lambda x: GpuBuffer.from_slice(ctx, x)  # noqa: E731
+    k, v = rng.standard_normal((2, own, row)).astype(np.float32)
+    bufs = [up(np.array([0, own, 0, n], np.int32)), up(np.array([own], np.int32)),
+            up(np.array([n_pages - 1, n_pages - 3], np.int32)), up(k.ravel()), up(v.ravel()), up(c.q.ravel()),
+            GpuBuffer.empty(ctx, n * d)]
+    off, length, pg, bk, bv, bq, out = bufs
+    PagedKvAppendKernel.new().dispatch_into(ctx, cache, PagedBatch(off, length, pg, 1, 2, own, own, own), 0, 0, bk, bv,
+                                            row, 0, 0, 0, 0, 0, kv)
+    batch = PagedBatch(off.ptr + 8, length, pg, 1, 2, n, n, own)
+    ws_len = PagedMhaKernel.scratch_len(cache, batch, c.h)
+    ws = GpuBuffer.empty(ctx, max(1, ws_len))
+    PagedMhaKernel.new().dispatch_into(ctx, cache, batch, bq, d, out, d, 0, ws, ws_len, c.h)
+    c.kp, c.vp = (from_bf16_bits(to_bf16_bits(x)) for x in (k, v))
+    c.pages, c.n_pages = np.array([[0, 1]], np.int32), 2
+    want, _, tol, _ = attention(c)
+    assert np.all(np.abs(out.download().reshape(n, d) - want) <= tol)
     for x in bufs + [ws]:
         x.free()
     cache.free()
