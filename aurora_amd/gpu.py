@@ -342,7 +342,7 @@ class PagedKvAppendKernel(_Kernel):
 
     def dispatch_into(self, ctx, cache, batch, q, ld_q, k, v, ld_kv, q_out, ld_qo, table, n_pos, rot_dim,
                       n_head, pairs=False):
-        if GpuBuffer in (type(q), type(k), type(v), type(q_out), type(table)):  # a step's raw pointers pass at once
+        if not (int is type(q) is type(k) is type(v) is type(q_out) is type(table)):  # a step's raw pointers pass at once
             n, row = batch.n_tok, cache.n_kv_head * cache.d_head
             _need("PagedKvAppendKernel q", _rows(n, ld_q, n_head * cache.d_head), q)
             _need("PagedKvAppendKernel q_out", _rows(n, ld_qo, n_head * cache.d_head), q_out)
@@ -361,7 +361,7 @@ class PagedMhaKernel(_Kernel):
         return (_lib.load().aur_mha_paged_ws_bytes(cache.ref, batch.ref, n_head) + 3) // 4
 
     def dispatch_into(self, ctx, cache, batch, q, ld_q, out, ld_o, lse, scratch, scratch_len, n_head):
-        if GpuBuffer in (type(q), type(out), type(lse), type(scratch)):
+        if not (int is type(q) is type(out) is type(lse) is type(scratch)):
             d = n_head * cache.d_head
             _need("PagedMhaKernel q", _rows(batch.n_tok, ld_q, d), q)
             _need("PagedMhaKernel out", _rows(batch.n_tok, ld_o, d), out)
