@@ -331,6 +331,13 @@ class RotaryTableKernel(_Kernel):
         ctx.call("aur_rotary_table", _p(table), n_pos, rot_dim, theta)
 
 
+def _any_buffer(*args) -> bool:
+    for x in args:
+        if isinstance(x, GpuBuffer):
+            return True
+    return False
+
+
 def _rows(n, ld, d) -> int:
     """Elements from the first row's start to the last one's end."""
     return (n - 1) * ld + d if n > 0 else 0
@@ -342,7 +349,7 @@ class PagedKvAppendKernel(_Kernel):
 
     def dispatch_into(self, ctx, cache, batch, q, ld_q, k, v, ld_kv, q_out, ld_qo, table, n_pos, rot_dim,
                       n_head, pairs=False):
-        if not (int is type(q) is type(k) is type(v) is type(q_out) is type(table)):  # a step's raw pointers pass at once
+        if _any_buffer(q, k, v, q_out, table):  # a step's raw pointers pass as they are
             n, row = batch.n_tok, cache.n_kv_head * cache.d_head
             _need("PagedKvAppendKernel q", _rows(n, ld_q, n_head * cache.d_head), q)
             _need("PagedKvAppendKernel q_out", _rows(n, ld_qo, n_head * cache.d_head), q_out)
@@ -361,7 +368,7 @@ class PagedMhaKernel(_Kernel):
         return (_lib.load().aur_mha_paged_ws_bytes(cache.ref, batch.ref, n_head) + 3) // 4
 
     def dispatch_into(self, ctx, cache, batch, q, ld_q, out, ld_o, lse, scratch, scratch_len, n_head):
-        if not (int is type(q) is type(out) is type(lse) is type(scratch)):
+        if _any_buffer(q, out, lse, scratch):
             d = n_head * cache.d_head
             _need("PagedMhaKernel q", _rows(batch.n_tok, ld_q, d), q)
             _need("PagedMhaKernel out", _rows(batch.n_tok, ld_o, d), out)

@@ -1,4 +1,6 @@
 """CPU checks of what the paged kernels' Python calls hand to the library."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -61,3 +63,13 @@ def test_any_kind_of_buffer_is_checked_by_the_append(buffer, which, what):
     with pytest.raises(ValueError, match=what):
         PagedKvAppendKernel().dispatch_into(Recorder(), cache, batch, x[0], 128, x[1], x[2], 64, x[3], 128, x[4], 32, 32,
                                             4)
+
+
+def test_raw_pointers_pass_as_they_are():
+    """Addresses, ctypes pointers and None (no q, no lse) reach the library as they came."""
+    cache, batch = _set_up()
+    ctx, void = Recorder(), C.c_void_p(PTR)
+    PagedKvAppendKernel().dispatch_into(ctx, cache, batch, None, 0, void, PTR, 64, None, 0, None, 0, 0, 0)
+    assert ctx.args[2:4] == (None, 0) and ctx.args[4] is void and ctx.args[7] is None
+    PagedMhaKernel().dispatch_into(ctx, cache, batch, void, 128, PTR, 128, None, None, 0, 4)
+    assert ctx.args[2] is void and ctx.args[6] is None
