@@ -25,8 +25,8 @@
 #include "common.hpp"
 #include "lanes.hpp"
 #include "paged.hpp"
+#include "paged_plan.hpp"
 
-#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -1207,88 +1207,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(MhaArgs a, int lanes) {
   if (lane == 0 && a.lse) a.lse[(size_t)t * a.H + h] = L == 0.f ? -INFINITY : (M + __log2f(L)) * LN2;
 }
 
-// How a call is cut into items, from what the host knows; the scratch's size follows from it.
-struct Plan {
-  int pooled, p_tile, o_tile, p_tiles, p_splits, p_keys, o_tiles, o_splits, o_keys;
-  int parts() const { return p_splits + o_splits; }
-  // One launch serves both kinds of items, unless the prefix has the larger tiles.
-  bool together() const { return p_tile <= 64; }
-};
-
-// Rows of an item: 16 keep their keys in registers, more lay them down in LDS.
-int tile_of(long long rows, int dh) { return rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 || dh > 64 ? 128 : 256; }
-
 constexpr uint32_t kMaxRows = 0x7fffff00u;  // query rows of a call, and a tile more, are ints
-// Items that a launch aims at, measured at 128 to 4096 of them: with 16-row own items 3 of a CU (64
-// sequences on a prefix of 32768 in bf16: 86 µs, with 256 items 140, with 2048 97), with larger ones 4
-// (tails of 128 on 2048: 113 µs, with 768 items 120), of 8 waves one (512 sequences on a prefix of 16384:
-// 240 µs, with 1024 items 303).
-// fp32 keys of more than 64 columns fill the registers, and keys without a prefix's items beside them the
-// memory, with 2 a CU (64 sequences of 1024 keys, 8 heads of 128, 4 rows each: 77 µs, with 768 items 85; one
-// sequence of 16884 keys, 16 heads of 64: 28, with 768 items 30).
-constexpr int kItems16 = 768, kItemsWide = 512, kItems = 1024, kItems8 = 256;
-// An axis up to so many keys is one range: a join costs 4 µs, 128 keys of a 16-row item (a round of its
-// waves) 1.5 µs.  Longer ones are cut into ranges of 128 keys or more, 48 at most.  Larger items of so many
-// axes that they fill the chip uncut are not cut up to twice that length (23 sequences of 72 rows on 506
-// keys, 15 heads of 48, bf16: 31 µs, cut 40; uncut with fewer than 256 axes cost a batch's block its chain
-// of tiles: 6 of 185 rows on 465, one head, 36 µs against 20).
-constexpr int kWhole16 = 384, kWhole = 256, kWholeFull = 512, kFill = 256;
-constexpr int kLeastKeys = 128, kMostRanges = 48;
-// With little work the time is a block's chain of tiles, not the products: smaller items then.  16 rows up
-// to so many items of 16 rows by 128 keys (5 sequences of 74 rows on 434 keys, 3 heads of 48, bf16, 300 of
-// them: 9.9 µs, in 128 rows 14, in 64 rows 11.7; at 1024 a batch took 15 instead of 11), 64 rows where items
-// times ranges of 128 keys come to less than kSmall (10 sequences of 315 rows on 763, 2 heads of 64, 1440:
-// 19 µs, in 256 rows 25; 30 of 85 rows on 721, 2160: 27 against 25; 6 of 355 rows on 392, 14 heads, 2688:
-// 43 against 30).
-constexpr int kSmall16 = 512, kSmall = 1536;
-// Keys times heads that pooling saves, from where it pays its records and its join (8 sequences of 12 heads
-// on a prefix of 1294, 108,000: 13 against 33 µs; 53 sequences of 5 heads on 139, 35,000: 22 against 10).
-constexpr int kPoolFrom = 65536;
-
-Plan make_plan(const Batch& b, int Hkv, int G, int dh, bool f32) {
-  Plan p{};
-  const int P = b.prefix_len;
-  const long long o_rows = (long long)b.max_tok * G, p_rows = (long long)b.n_tok * G;
-  p.o_tile = tile_of(o_rows, dh);
-  p.o_tiles = (int)((o_rows + p.o_tile - 1) / p.o_tile);
-  p.p_tile = p_rows <= 32 ? 16 : p_rows <= (dh > 64 ? 256 : 128) ? 64 : dh > 64 ? 128 : 256;
-  const int p_tiles = (int)((p_rows + p.p_tile - 1) / p.p_tile);
-  p.pooled = o_rows < 64 && ((double)b.b * p.o_tiles - p_tiles) * Hkv * P >= kPoolFrom;
-  if (p.pooled && p.p_tile == 16 && p.o_tile > 16) p.p_tile = 64;
-  if (!p.pooled && p.o_tile > 16) {
-    const double ranges = (P + b.max_own + kLeastKeys - 1) / kLeastKeys;
-    auto items = [&](int tile) { return (double)Hkv * b.b * ((o_rows + tile - 1) / tile) * ranges; };
-    if (items(16) <= kSmall16)
-      p.o_tile = 16;
-    else if (items(p.o_tile) * ranges <= kSmall)
-      p.o_tile = 64;
-    p.o_tiles = (int)((o_rows + p.o_tile - 1) / p.o_tile);
-  }
-  p.p_tiles = p.pooled ? (int)((p_rows + p.p_tile - 1) / p.p_tile) : 0;
-  const int axis = b.max_own + (p.pooled ? 0 : P);
-  // Ranges of one length, so that no item is left with a few keys.
-  // (A CU holds one block of 8 waves: more of them than CUs would be a second round.)
-  auto eight = [dh](int tile) { return tile == 256 || (tile == 128 && dh > 64); };
-  const int items16 = f32 && (dh > 64 || !p.pooled) ? kItemsWide : kItems16;
-  auto items = [&](int tile) { return eight(tile) ? kItems8 : tile > 16 ? kItems : items16; };
-  auto cut = [&](int n, double axes, double want, int tile, int* keys) {
-    int splits = 1;
-    if (n > (tile == 16 ? kWhole16 : axes >= kFill ? kWholeFull : kWhole)) {
-      const int most = std::min(kMostRanges, (n + kLeastKeys - 1) / kLeastKeys);
-      const double parts = n / want;
-      splits = (int)std::min((double)most, std::max(1.0, eight(tile) ? parts : std::ceil(parts)));
-    }
-    *keys = n > 0 ? ((n + splits - 1) / splits + 31) / 32 * 32 : 32;
-    return n > 0 ? (n + *keys - 1) / *keys : 1;
-  };
-  const double p_axes = (double)Hkv * p.p_tiles, o_axes = (double)Hkv * b.b * p.o_tiles;
-  const double p_work = p_axes * P, o_work = o_axes * axis;
-  const bool one = !p.pooled || p.together();
-  const double o_want = (one ? p_work + o_work : o_work) / items(p.o_tile);
-  p.o_splits = cut(axis, o_axes, o_want, p.o_tile, &p.o_keys);
-  p.p_splits = p.pooled ? cut(P, p_axes, one ? o_want : p_work / items(p.p_tile), p.p_tile, &p.p_keys) : 0;
-  return p;
-}
 
 size_t ws_floats(const Plan& p, const Batch& b, int H, int dh) {
   return p.parts() > 1 ? (size_t)p.parts() * b.n_tok * H * (dh + 2) : 0;
@@ -1305,15 +1224,14 @@ void launch_step(const MhaArgs& a, int p_tile, unsigned items, hipStream_t st) {
 
 // p_tile 0: items of one kind (or of one tile).
 template <class T, int DT>
-void launch_tile(const MhaArgs& a, int p_tile, int tile, unsigned items, hipStream_t st) {
+void launch_tile(const MhaArgs& a, int p_tile, int tile, int rows, unsigned items, hipStream_t st) {
   const dim3 g(items);
   const dim3 four(256);
   if (tile == 16) {
-    const int rows = a.b.max_tok == 1 ? a.G : 16;
     if (rows == 1) return launch_step<T, DT, 1>(a, p_tile, items, st);
     if (rows == 2) return launch_step<T, DT, 2>(a, p_tile, items, st);
     if constexpr (std::is_same<T, float>::value)
-      if (rows <= 4) return launch_step<T, DT, 4>(a, p_tile, items, st);
+      if (rows == 4) return launch_step<T, DT, 4>(a, p_tile, items, st);
     launch_step<T, DT, 16>(a, p_tile, items, st);
   } else if (tile == 64) {
     hipLaunchKernelGGL((paged_mha_tile_kernel<T, DT, 1, 4>), g, four, 0, st, a);
@@ -1327,18 +1245,25 @@ void launch_tile(const MhaArgs& a, int p_tile, int tile, unsigned items, hipStre
 }
 
 template <class T>
-void launch_head(const MhaArgs& a, int p_tile, int tile, unsigned items, hipStream_t st) {
-  const int dt = (a.dh + 15) / 16;
-  if (dt == 1) launch_tile<T, 1>(a, p_tile, tile, items, st);
-  else if (dt == 2) launch_tile<T, 2>(a, p_tile, tile, items, st);
-  else if (dt == 3) launch_tile<T, 3>(a, p_tile, tile, items, st);
-  else if (dt == 4) launch_tile<T, 4>(a, p_tile, tile, items, st);
-  else if (dt <= 6) launch_tile<T, 6>(a, p_tile, tile, items, st);
-  else launch_tile<T, 8>(a, p_tile, tile, items, st);
+void launch_head(const MhaArgs& a, int p_tile, int tile, int rows, unsigned items, hipStream_t st) {
+  switch (head_tiles(a.dh)) {
+    case 1: return launch_tile<T, 1>(a, p_tile, tile, rows, items, st);
+    case 2: return launch_tile<T, 2>(a, p_tile, tile, rows, items, st);
+    case 3: return launch_tile<T, 3>(a, p_tile, tile, rows, items, st);
+    case 4: return launch_tile<T, 4>(a, p_tile, tile, rows, items, st);
+    case 6: return launch_tile<T, 6>(a, p_tile, tile, rows, items, st);
+    default: return launch_tile<T, 8>(a, p_tile, tile, rows, items, st);
+  }
 }
 
-void launch_items(const MhaArgs& a, bool f32, int p_tile, int tile, unsigned items, hipStream_t st) {
-  f32 ? launch_head<float>(a, p_tile, tile, items, st) : launch_head<__bf16>(a, p_tile, tile, items, st);
+Sizes sizes_of(const Batch& b, const aur_paged_cache& c, uint32_t n_head) {
+  return {b.b, b.n_tok, b.max_tok, b.max_own, b.prefix_len, (int)c.n_kv_head, (int)(n_head / c.n_kv_head), (int)c.d_head,
+          c.dtype == AUR_PAGED_F32};
+}
+
+void launch_items(const MhaArgs& a, const Sizes& z, int p_tile, int tile, unsigned items, hipStream_t st) {
+  const int rows = step_rows(z);
+  z.f32 ? launch_head<float>(a, p_tile, tile, rows, items, st) : launch_head<__bf16>(a, p_tile, tile, rows, items, st);
 }
 
 }  // namespace
@@ -1350,9 +1275,7 @@ size_t aur_mha_paged_ws_bytes(const aur_paged_cache* cache, const aur_paged_batc
   if (check_paged(nullptr, "aur_mha_paged_ws_bytes", cache, batch, &b) != 0 || n_head == 0 || n_head > 4096 ||
       (uint64_t)b.n_tok * n_head > kMaxRows || n_head % cache->n_kv_head != 0 || b.b == 0 || b.n_tok == 0)
     return 0;
-  return 4 * ws_floats(make_plan(b, (int)cache->n_kv_head, (int)(n_head / cache->n_kv_head), (int)cache->d_head,
-                                  cache->dtype == AUR_PAGED_F32), b, (int)n_head,
-                       (int)cache->d_head);
+  return 4 * ws_floats(make_plan(sizes_of(b, *cache, n_head)), b, (int)n_head, (int)cache->d_head);
 }
 
 int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch, const float* q,
@@ -1377,7 +1300,8 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
   a.H = (int)n_head; a.Hkv = (int)cache->n_kv_head; a.G = a.H / a.Hkv; a.dh = (int)cache->d_head;
   a.n_pages = (int)cache->n_pages; a.sh = log2_of(cache->page_len);
   a.scale = 1.0f / sqrtf((float)a.dh);
-  const Plan p = make_plan(a.b, a.Hkv, a.G, a.dh, cache->dtype == AUR_PAGED_F32);
+  const Sizes z = sizes_of(a.b, *cache, n_head);
+  const Plan p = make_plan(z);
   a.pooled = p.pooled;
   a.p_tiles = p.p_tiles; a.p_splits = p.p_splits; a.p_keys = p.p_keys;
   a.o_tiles = p.o_tiles; a.o_splits = p.o_splits; a.o_keys = p.o_keys;
@@ -1395,16 +1319,15 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
   if (p_items + o_items > kMaxBlocks / 2 || rows4 > kMaxBlocks)
     return aur::set_error(ctx, AUR_ELIMIT, "%s: %llu + %llu blocks", who, (unsigned long long)p_items,
                           (unsigned long long)o_items);
-  const bool f32 = cache->dtype == AUR_PAGED_F32;
   if (p.pooled && !p.together()) {
     a.p_items = (int)p_items;
-    launch_items(a, f32, 0, p.p_tile, (unsigned)p_items, ctx->stream);
+    launch_items(a, z, 0, p.p_tile, (unsigned)p_items, ctx->stream);
     AUR_LAUNCH_CHECK(ctx, "paged_mha kernels (prefix)");
     a.p_items = 0;
-    launch_items(a, f32, 0, p.o_tile, (unsigned)o_items, ctx->stream);
+    launch_items(a, z, 0, p.o_tile, (unsigned)o_items, ctx->stream);
   } else {
     a.p_items = (int)p_items;
-    launch_items(a, f32, p.pooled ? p.p_tile : 0, p.o_tile, (unsigned)(p_items + o_items), ctx->stream);
+    launch_items(a, z, p.pooled ? p.p_tile : 0, p.o_tile, (unsigned)(p_items + o_items), ctx->stream);
   }
   AUR_LAUNCH_CHECK(ctx, "paged_mha kernels");
   if (floats) {

@@ -1,0 +1,92 @@
+"""The paged attention's kernels, each by batches that the plan gives to it (tests/paged_tiles.py; which
+batch reaches what is held on the CPU by tests/test_paged_plan.py), against the definition in float64."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from tests.paged_tiles import ALL, D_HEADS, attention_blocks
+from tests.test_paged_gpu import Device, _hip
+
+pytestmark = pytest.mark.gpu
+
+
+def _compare(c, out, lse, loss=0.0, what=""):
+    """Every row against the definition: the same infinities and NaN, the rest within the bounds."""
+    want, want_lse, tol, tol_lse = attention_blocks(c, loss)
+    d, n = c.h * c.dh, int(c.off[-1])
+    assert np.all(out[n:] == 7.5) and np.all(out[:, d:] == 7.5), f"{what}: rows or columns that are none were written"
+    assert np.all(lse[n:] == 7.5)
+    worst = 0.0
+    for have, want, tol in ((out[:n, :d], want[:n], tol[:n]), (lse[:n], want_lse[:n], tol_lse[:n])):
+        fine = np.isfinite(want)
+        assert fine.any()
+        assert np.array_equal(np.isnan(have), np.isnan(want)), what
+        assert np.array_equal(have[np.isinf(want)], want[np.isinf(want)]), what
+        err = np.abs(have[fine] - want[fine])
+        worst = max(worst, float((err / np.maximum(tol[fine], 1e-300)).max()))
+        assert worst <= 1.0, f"{what}: {worst} of the bound"
+    return worst
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dh", D_HEADS)
+@pytest.mark.parametrize("name", ALL)
+def test_every_kernel_matches_float64(ctx, name, dh, dtype):
+    """Rows of other strides than their length, bounds above what the arrays hold, rows behind the last
+    sequence; and the same bits from a second call whose scratch holds the first one's records."""
+    b = ALL[name]
+    c = b.case(dh, dtype, behind=1)
+    dev = Device(ctx, c, ld_q=c.h * dh + 8, ld_o=c.h * dh + 4)
+    dev.attend()
+    out, lse = dev.result()
+    print(f"[paged] {_compare(c, out, lse):.3f} of the bound")
+    dev.attend()
+    for x, y in zip((out, lse), dev.result()):
+        assert np.array_equal(x, y)
+    dev.free()
+
+
+def test_tiles_captured_into_a_graph(ctx):
+    """Two batches, one with its prefix in a launch of its own, captured into one graph on one scratch;
+    every replay, with eager calls in between and other queries and lengths, equals the eager calls."""
+    from aurora_amd.gpu import GpuBuffer
+    from aurora_amd._lib import load
+
+    hip, stream = _hip(), load().aur_stream(ctx.ptr)
+    cases = [ALL["prefix 256, own 64"].case(64, "f32"), ALL["128 rows"].case(64, "bf16")]
+    eager, replayed = [[Device(ctx, c) for c in cases] for _ in range(2)]
+    ws = GpuBuffer.zeros(ctx, max(d.ws_len for d in replayed))
+    rng = np.random.default_rng(3)
+    graph, exe = ctypes.c_void_p(), ctypes.c_void_p()
+    ctx.sync()
+    assert hip.hipStreamBeginCapture(stream, 1) == 0  # hipStreamCaptureModeThreadLocal
+    try:
+        for d in replayed:
+            d.attend(ws=ws)
+    finally:
+        assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    try:
+        assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, 0) == 0
+        for step in range(4):
+            q = [rng.standard_normal(d.q.len).astype(np.float32) for d in eager]
+            for side in (eager, replayed):
+                for d, x in zip(side, q):
+                    d.q.upload(x)
+                    d.len.upload((d.c.length - min(step, 1) * (d.c.length > 3)).astype(np.int32))
+            for d in eager:
+                d.attend()
+            ctx.sync()
+            assert hip.hipGraphLaunch(exe, stream) == 0
+            ctx.sync()
+            for x, y in zip(eager, replayed):
+                for a, b in zip(x.result(), y.result()):
+                    assert np.array_equal(a, b), step
+    finally:
+        if exe.value:
+            hip.hipGraphExecDestroy(exe)
+        if graph.value:
+            hip.hipGraphDestroy(graph)
+        for d in eager + replayed:
+            d.free()
+        ws.free()
