@@ -47,6 +47,56 @@ def test_every_kernel_matches_float64(ctx, name, dh, dtype):
     dev.free()
 
 
+HARD = ["64 rows", "64 rows, group 4", "128 rows", "128 rows, group 2", "256 rows", "several tiles", "prefix 64, own 64",
+        "one prompt among steps", "prefix 64, own 16", "prefix 256, own 16", "prefix 256, own 64", "prefix 16, own 16"]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dh", [40, 64, 128])
+@pytest.mark.parametrize("name", HARD)
+@pytest.mark.parametrize("where", ["own", "prefix"])
+def test_infinities_of_many_rows(ctx, where, name, dh, dtype):
+    """Infinities and NaN among the keys and values of a batch: rows that see them get what the formula
+    gives, rows of the same item that do not are as if they were not there."""
+    c = ALL[name].case(dh, dtype)
+    if where == "own":
+        first, last = c.rows(c.pages[0], c.length[0]), c.rows(c.pages[-1], c.length[-1])
+        mid = first[c.length[0] - c.n[0] + c.n[0] // 2]  # a new token's, that the ones before it do not see
+        c.vp[mid, 3], c.vp[mid, dh + 6] = np.inf, np.nan
+        c.vp[first[-1], 5], c.kp[first[-1], dh + 1] = -np.inf, np.nan
+        c.kp[last[-1], 2] = np.inf  # the sign of the query's column decides: NaN, or a key without weight
+    else:
+        page = c.prefix_pages[c.prefix // c.page // 2] * c.page
+        c.vp[page, 1], c.vp[page, 2] = np.inf, -np.inf
+        c.vp[c.prefix_pages[0] * c.page, dh + 4] = np.nan
+        c.kp[page, dh + 7] = -np.inf
+    dev = Device(ctx, c)
+    dev.attend()
+    _compare(c, *dev.result())
+    dev.free()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("name", HARD)
+@pytest.mark.parametrize("vs,ks", [(2.0**-100, 1.0), (2.0**100, 1.0), (1.0, 2.0**40), (1.0, 2.0**-40)])
+def test_values_of_any_size_in_tiles(ctx, vs, ks, name, dtype):
+    """V of any size, and columns of K far larger or smaller than the others whose queries make up for it:
+    nothing is lost beside a larger neighbour."""
+    c = ALL[name].case(64, dtype)
+    c.vp[:, ::2] *= np.float32(vs)
+    _scale_columns(c, ks)
+    dev = Device(ctx, c)
+    dev.attend()
+    _compare(c, *dev.result())
+    dev.free()
+
+
+def _scale_columns(c, ks):
+    """Every third column of each head of K times ks, of the queries by 1/ks."""
+    c.kp.reshape(len(c.kp), c.kv, c.dh)[:, :, 1::3] *= np.float32(ks)
+    c.q.reshape(c.n_tok, c.h, c.dh)[:, :, 1::3] /= np.float32(ks)
+
+
 def test_tiles_captured_into_a_graph(ctx):
     """Two batches, one with its prefix in a launch of its own, captured into one graph on one scratch;
     every replay, with eager calls in between and other queries and lengths, equals the eager calls."""
