@@ -97,6 +97,32 @@ def _scale_columns(c, ks):
     c.q.reshape(c.n_tok, c.h, c.dh)[:, :, 1::3] /= np.float32(ks)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dh", [48, 128])
+@pytest.mark.parametrize("name", HARD)
+@pytest.mark.parametrize("own", ["some", "none"])
+def test_pages_that_are_not_there_in_tiles(ctx, own, name, dh, dtype):
+    """Page numbers outside the pool, the largest and smallest among them, take their keys out: single pages of
+    the prefix and of the sequences; a sequence that keeps its last pages only, or none of its own."""
+    c = ALL[name].case(dh, dtype)
+    odd = [-1, c.n_pages, 2**31 - 1, -2**31, c.n_pages + 7]
+    c.prefix_pages[[3, 7, 20, len(c.prefix_pages) // 2, -1]] = odd
+    used = -(-c.length // c.page)
+    for i, s in enumerate(np.flatnonzero(used > 0)):
+        if i == 1:
+            continue  # this one is whole
+        c.pages[s, used[s] // 2] = odd[i % 5]
+    longest = int(np.argmax(used))
+    if own == "some":
+        c.pages[longest, :(used[longest] + 1) // 2] = 2**31 - 1
+    else:
+        c.pages[longest] = -7
+    dev = Device(ctx, c)
+    dev.attend()
+    _compare(c, *dev.result())
+    dev.free()
+
+
 def test_tiles_captured_into_a_graph(ctx):
     """Two batches, one with its prefix in a launch of its own, captured into one graph on one scratch;
     every replay, with eager calls in between and other queries and lengths, equals the eager calls."""
