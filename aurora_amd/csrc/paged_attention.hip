@@ -243,7 +243,8 @@ struct Keys32 {
 };
 
 // x as the sum of three bf16 numbers, exactly but for what lies 2^-24 below it and more (8 bits each,
-// with the range of fp32, so no scales are needed; an infinity becomes NaN).
+// with the range of fp32, so no scales are needed; parts below 2^-126 the MFMA takes as zero; an infinity
+// becomes NaN).
 __device__ __forceinline__ void split3(float x0, float x1, bf16x2& h, bf16x2& m, bf16x2& l) {
   h = __builtin_convertvector(float2v{x0, x1}, bf16x2);
   const float r0 = x0 - (float)h[0], r1 = x1 - (float)h[1];

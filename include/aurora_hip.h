@@ -279,9 +279,15 @@ int aur_kv_append_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_pa
  * aur_mha_paged_ws_bytes(cache, batch, n_head) (0: it may be NULL), which goes
  * by the host's fields alone; calls that overlap in time need a scratch each.
  * Sums are fp32 and joined in a fixed order: the same call gives the same bits.
- * (With more than 16 query rows to a K/V head, fp32 values of V below 2^-110 are
- * exact to 2^-126 only: the matrix cores take no subnormal bf16.)  `out` may not
- * overlap q. */
+ * `out` may not overlap q.
+ * Smallest values: rows that pass through the matrix cores as bf16 parts lose
+ * what lies below 2^-126 of K, of the scaled queries, of V and of the softmax's
+ * weights, since those take no subnormal bf16.  V below 2^-110 then has an error
+ * of up to 2^-126, and a score one of 2^-126 * sum(|q|/sqrt(d_head) + |k|): 2^-14
+ * from a column of 2^-115 in a key of 64 and 2^115 in the query.  With fp32 pools
+ * these are items of more than 16 query rows of a K/V head (a prefix read once for
+ * all counts the rows of the whole batch), with bf16 pools all but single tokens of
+ * one or two rows. */
 size_t aur_mha_paged_ws_bytes(const aur_paged_cache* cache, const aur_paged_batch* batch,
                               uint32_t n_head);
 int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,

@@ -97,6 +97,25 @@ def _scale_columns(c, ks):
     c.q.reshape(c.n_tok, c.h, c.dh)[:, :, 1::3] /= np.float32(ks)
 
 
+LEAST = 2.0**-126  # the smallest normal number: the matrix cores take smaller bf16 operands as zero
+FEW = ["one row", "two rows", "three rows", "16 rows of one sequence", "prefix 16, own 16"]  # no item of more than 16 rows
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("name", HARD + [x for x in FEW if x not in HARD] + ["prefix 64, own 1"])
+@pytest.mark.parametrize("vs,ks", [(1.0, 2.0**-115), (1.0, 2.0**115), (2.0**-115, 1.0), (2.0**-130, 1.0), (2.0**-130, 2.0**-120)])
+def test_values_next_to_the_smallest(ctx, vs, ks, name, dtype):
+    """Keys, queries and values whose bf16 parts fall below 2^-126 are exact to 2^-126 (as is bf16's own
+    rounding of the pools here); fp32 ones in items of up to 16 rows to their roundings, as any others."""
+    c = ALL[name].case(64, dtype, seed=1)
+    c.vp[:, ::2] *= np.float32(vs)
+    _scale_columns(c, ks)
+    dev = Device(ctx, c)
+    dev.attend()
+    _compare(c, *dev.result(), loss=0.0 if dtype == "f32" and name in FEW else LEAST)
+    dev.free()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("dh", [48, 128])
 @pytest.mark.parametrize("name", HARD)
