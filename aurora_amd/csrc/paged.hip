@@ -194,6 +194,8 @@ int aur_kv_append_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_pa
                                                                ld_q > 0x7fffffffu || ld_qo > 0x7fffffffu)))
     return aur::set_error(ctx, AUR_EINVAL, "%s: ld_q=%u ld_kv=%u ld_qo=%u (multiples of 4, at least a row)", who, ld_q,
                           ld_kv, ld_qo);
+  if (q && q == q_out && ld_q != ld_qo && a.b.n_tok > 1)  // a row's result would lie on another's input
+    return aur::set_error(ctx, AUR_EINVAL, "%s: q and q_out one buffer with ld_q=%u, ld_qo=%u", who, ld_q, ld_qo);
   a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.kp = cache->k; a.vp = cache->v; a.table = table;
   a.ld_q = (int)ld_q; a.ld_kv = (int)ld_kv; a.ld_qo = (int)ld_qo;
   a.H = q ? (int)n_head : 0; a.Hkv = (int)cache->n_kv_head; a.dh = (int)dh; a.rot = (int)rot_dim;

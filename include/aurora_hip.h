@@ -260,8 +260,8 @@ int aur_rotary_table(aur_ctx* ctx, float* table, uint32_t n_pos, uint32_t rot_di
  * or with pairs != 0 columns (2u, 2u + 1); columns from rot_dim on are copied.
  * rot_dim is a multiple of 8 up to d_head, 0 for no rotation (table may be NULL
  * then); the table holds n_pos >= prefix_len + max_own positions.  q and q_out
- * may be one buffer of one stride, or both NULL.  bf16 pools take the nearest value, ties to
- * even.  Rows 16-byte aligned, strides multiples of 4.  A token with j < 0
+ * may be one buffer of one stride (AUR_EINVAL for two), or both NULL.  bf16 pools
+ * take the nearest value, ties to even.  Rows 16-byte aligned, strides multiples of 4.  A token with j < 0
  * (own_len below n_s) is skipped, q_out included. */
 int aur_kv_append_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,
                         const float* q, uint32_t ld_q, const float* k, const float* v,
