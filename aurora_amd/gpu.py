@@ -295,6 +295,8 @@ class PagedKvCache:
 
     @classmethod
     def zeros(cls, ctx: GpuContext, n_pages, page_len, n_kv_head, d_head, dtype="f32") -> "PagedKvCache":
+        if dtype not in cls.DTYPES:  # before there is anything to free
+            raise ValueError(f"PagedKvCache: dtype {dtype!r}, one of {sorted(cls.DTYPES)}")
         n = n_pages * page_len * n_kv_head * d_head
         np_type = np.float32 if dtype == "f32" else np.uint16
         return cls(GpuBuffer.zeros(ctx, n, np_type), GpuBuffer.zeros(ctx, n, np_type), n_pages, page_len,

@@ -73,3 +73,10 @@ def test_raw_pointers_pass_as_they_are():
     assert ctx.args[2:4] == (None, 0) and ctx.args[4] is void and ctx.args[7] is None
     PagedMhaKernel().dispatch_into(ctx, cache, batch, void, 128, PTR, 128, None, None, 0, 4)
     assert ctx.args[2] is void and ctx.args[6] is None
+
+
+def test_a_refused_type_allocates_nothing():
+    ctx = Recorder()
+    with pytest.raises(ValueError, match="f16"):
+        PagedKvCache.zeros(ctx, 4, 16, 2, 32, "f16")
+    assert ctx.args is None
