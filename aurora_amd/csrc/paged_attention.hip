@@ -528,9 +528,10 @@ __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, in
 // MFMAs (row r of MFMA c is column 4r + c), so V needs no transposition and nothing passes through LDS on
 // the way.  fp32 keys go into the fp32 MFMA; bf16 keys into the bf16 one with Q and P as three bf16 parts,
 // which keep 2^-24 of each.  A wave's next K is under way while it works, its V from the scores on.  Bound
-// by the reading with the MFMA's cycles in between: 64 sequences of 1024 keys, 16 K/V heads of 64, 4 rows
-// each: 56 µs in bf16 (3.6 TB/s), 92 in fp32 (4.3 TB/s); on widened keys the fp32 MFMA took bf16's own
-// keys of 64 such sequences 160 µs in a first version, the bf16 one 60.
+// by the reading with the MFMA's cycles in between: 64 sequences of 512 to 1024 keys (768 on average), 16
+// K/V heads of 64, 4 rows each: 56 µs in bf16 (3.7 TB/s), 92 in fp32 (4.5 TB/s); with 1024 keys each 62 µs
+// in bf16 (4.3 TB/s).  On widened keys the fp32 MFMA took bf16's own keys of 64 such sequences 160 µs in a
+// first version, the bf16 one 60.
 template <int DT>
 struct RowsLds {
   static constexpr int R = 16, OS = 64 * ((DT + 3) / 4) + 4;
@@ -616,10 +617,11 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
 
 // The rows of one token: the query heads of a K/V head, all of which see the same keys.  Such items are
 // bound by reading K and V; the MFMA of rows_item works on 16 rows whatever there are, and its cycles stand
-// between the loads.  Vector instructions cost by the row.  64 sequences of 1024 keys, 16 K/V heads of 64,
-// µs by vectors and by the MFMA: 1 row 67 and 85 (5.9 TB/s), 2 rows 73 and 84, 4 rows 83 and 92; bf16 keys
-// 1 row 40 and 53, 2 rows 43 and 54, 4 rows 55 and 56 (with a prefix of 2048 beside it 40 and 38): so 4
-// rows in fp32, 2 in bf16.  LP lanes have a key's head, 16 bytes each, so that a load brings 64/LP whole
+// between the loads.  Vector instructions cost by the row.  64 sequences of 512 to 1024 keys (768 on
+// average), 16 K/V heads of 64, µs by vectors and by the MFMA: 1 row 67 and 85 (5.9 TB/s), 2 rows 73 and 84,
+// 4 rows 83 and 92; bf16 keys 1 row 40 and 53 (5.0 TB/s), 2 rows 43 and 54, 4 rows 55 and 56 (with a prefix
+// of 2048 beside it 40 and 38): so 4 rows in fp32, 2 in bf16.  With 1024 keys each, by vectors: fp32 85 µs
+// (6.3 TB/s), 88 and 94, bf16 48 µs (5.6 TB/s) and 49.  LP lanes have a key's head, 16 bytes each, so that a load brings 64/LP whole
 // keys; a score is added up over the LP lanes, l and the columns over the key groups once at the end, all
 // of it in fp32.  While one half of the registers is in use, the loads of the other are under way, and the
 // page of the step after them.
@@ -795,11 +797,14 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
 // bf16 parts (fp32: three, whose six products above 2^-24 of the largest the MFMA sums; bf16 keys are
 // one part, Q and P three), K as [key][column], V as [column][key], while the next keys' loads are
 // under way: six bf16 products cost 6/16 of the fp32 MFMA's time for one.  Bound by the MFMA and by what
-// lies between its issues, the conversion of the next tile and the softmax: 16 sequences of 512 tokens on a
-// prefix of 4096, 16 heads of 64, fp32: 667 µs, 161 TFLOP/s of the 210 that a bf16 product of 1262 leaves
-// for six.  The more rows, the less often K and V are loaded, converted and read from LDS: 16 rows a wave
-// of 4 waves 1191 µs, of 8 waves 804, 32 rows a wave with the keys' places in LDS 667.  Tiles of 32x32 took
-// 656 at d_head 64 and spilled at 128.
+// lies between its issues, the conversion of the next tile and the softmax: 16 sequences of 259 to 503 tokens
+// on a prefix of 4096, 16 heads of 64, fp32: 667 µs, 161 TFLOP/s (rows behind a sequence's last fill a fourth
+// of its tiles; with 512 tokens each 696 µs, 210 TFLOP/s, the rate that a large library product of 1262 in
+// bf16 leaves for six, and bf16 454 µs, 321 of 421).  The more rows, the less often K and V are loaded,
+// converted and read from LDS: 16 rows a wave of 4 waves 1191 µs, of 8 waves 804, 32 rows a wave with the
+// keys' places in LDS 667.  Tiles of 32x32 took 656 at d_head 64 and spilled more at 128.  (Of those here some
+// spill at 256 registers too: fp32 keys of d_head 33 to 48 in 128 and 256 rows 18 and 9 registers, of d_head
+// above 96 in 64 rows 12, others up to 4.)
 template <class T, int DT, int W>
 struct TileGeo {
   static constexpr bool F32 = std::is_same<T, float>::value;
@@ -1117,7 +1122,10 @@ union StepLds {
   typename std::conditional<PRE == 64, TileLds<T, DT, NW>, typename std::conditional<PRE == 16, RowsLds<DT>, char>::type>::type pre;
 };
 
-// Waves a SIMD should hold: bf16 keys leave registers for three.
+// Waves a SIMD should hold.  bf16 keys leave registers for three, all but 2 to 19 that spill in 64-row items of
+// d_head 33 to 64.  µs with three and with two, 16 heads: 100 sequences on a prefix of 8192, d_head 64 39.6 and
+// 43.5; 30 of 32 heads on 8, prefix 4096 19.7 and 21.9; 64 on 32768 82 and 77.6, without own keys 48.6 and 51;
+// of d_head 48 on 16384 63.2 and 61.6; tails of 30 to 60 tokens on 2048 51.4 and 49.5.
 template <class T, int DT, int NR>
 constexpr int kWaves = sizeof(T) == 2 && DT <= 4 && NR == 1 ? 3 : 2;
 
@@ -1128,8 +1136,9 @@ __global__ void __launch_bounds__(64 * W, (kWaves<T, DT, NR>)) paged_mha_tile_ke
 }
 
 // A decode step of many sequences in one launch: the prefix's items, bound by their products, beside the
-// own ones, bound by memory (64 sequences of 1024 keys on a prefix of 32768, 16 heads of 64, bf16: 80 µs
-// with the join, 91 in two launches; 48 sequences of 4 heads of 128 on 4999: 46 and 58).
+// own ones, bound by memory (64 sequences of 516 to 1018 keys on a prefix of 32768, 16 heads of 64, bf16: 80
+// µs with the join, 91 in two launches; 48 sequences of 350 to 692, 4 heads of 128 on 4999: 46 and 58).  fp32
+// heads of more than 96 columns spill 13 to 17 of 256 registers in most forms of it.
 template <class T, int DT, int R, int PRE>
 __global__ void __launch_bounds__(64 * NW, (PRE == 64 ? kWaves<T, DT, 1> : 2)) paged_mha_step_kernel(MhaArgs a) {
   __shared__ __attribute__((aligned(1024))) StepLds<T, DT, R, PRE> lds;

@@ -27,11 +27,11 @@ inline int tile_of(long long rows, int dh) { return rows <= 16 ? 16 : rows <= 64
 
 // Items that a launch aims at, measured at 128 to 4096 of them: with 16-row own items 3 of a CU (64
 // sequences on a prefix of 32768 in bf16: 86 µs, with 256 items 140, with 2048 97), with larger ones 4
-// (tails of 128 on 2048: 113 µs, with 768 items 120), of 8 waves one (512 sequences on a prefix of 16384:
+// (tails of 66 to 122 on 2048: 113 µs, with 768 items 120), of 8 waves one (512 sequences on a prefix of 16384:
 // 240 µs, with 1024 items 303).
 // fp32 keys of more than 64 columns fill the registers, and keys without a prefix's items beside them the
-// memory, with 2 a CU (64 sequences of 1024 keys, 8 heads of 128, 4 rows each: 77 µs, with 768 items 85; one
-// sequence of 16884 keys, 16 heads of 64: 28, with 768 items 30).
+// memory, with 2 a CU (64 sequences of 512 to 1024 keys, 8 heads of 128, 4 rows each: 77 µs, with 768 items
+// 85; one sequence of 16757 keys, 16 heads of 64: 28, with 768 items 30).
 constexpr int kItems16 = 768, kItemsWide = 512, kItems = 1024, kItems8 = 256;
 // An axis up to so many keys is one range: a join costs 4 µs, 128 keys of a 16-row item (a round of its
 // waves) 1.5 µs.  Longer ones are cut into ranges of 128 keys or more, 48 at most.  Larger items of so many
@@ -50,6 +50,12 @@ constexpr int kSmall16 = 512, kSmall = 1536;
 // Keys times heads that pooling saves, from where it pays its records and its join (8 sequences of 12 heads
 // on a prefix of 1294, 108,000: 13 against 33 µs; 53 sequences of 5 heads on 139, 35,000: 22 against 10).
 constexpr int kPoolFrom = 65536;
+// Rows of all sequences up to which the prefix's items have 64, in the own ones' launch, instead of 256 (128
+// from d_head 65 on) in one of their own.  d_head 128 on a prefix of 4999, 16 heads on 4, µs with 64 and 128
+// rows: 144 rows of the batch fp32 43 and 53, 192 46 and 57, 256 56 and 63; bf16 32 and 43, 32 and 46, 40 and
+// 50.  d_head 64, with 64 and 256: 144 rows 27 and 35, 192 31 and 41, 256 36 and 45; bf16 20 and 28, 20 and 31,
+// 24 and 35: there too 64 rows are the faster up to 256, and its bound of 128 is short of that.
+constexpr int kPool64 = 128, kPool64Wide = 256;
 
 inline Plan make_plan(const Sizes& b) {
   Plan p{};
@@ -57,7 +63,7 @@ inline Plan make_plan(const Sizes& b) {
   const long long o_rows = (long long)b.max_tok * G, p_rows = (long long)b.n_tok * G;
   p.o_tile = tile_of(o_rows, dh);
   p.o_tiles = (int)((o_rows + p.o_tile - 1) / p.o_tile);
-  p.p_tile = p_rows <= 32 ? 16 : p_rows <= (dh > 64 ? 256 : 128) ? 64 : dh > 64 ? 128 : 256;
+  p.p_tile = p_rows <= 32 ? 16 : p_rows <= (dh > 64 ? kPool64Wide : kPool64) ? 64 : dh > 64 ? 128 : 256;
   const int p_tiles = (int)((p_rows + p.p_tile - 1) / p.p_tile);
   p.pooled = o_rows < 64 && ((double)b.b * p.o_tiles - p_tiles) * Hkv * P >= kPoolFrom;
   if (p.pooled && p.p_tile == 16 && p.o_tile > 16) p.p_tile = 64;
