@@ -33,8 +33,8 @@ def _compare(c, out, lse, loss=0.0, what=""):
 @pytest.mark.parametrize("dh", D_HEADS)
 @pytest.mark.parametrize("name", ALL)
 def test_every_kernel_matches_float64(ctx, name, dh, dtype):
-    """Rows of other strides than their length, bounds above what the arrays hold, rows behind the last
-    sequence; and the same bits from a second call whose scratch holds the first one's records."""
+    """Rows of other strides than their length and a row behind the last sequence; and the same bits from a
+    second call, whose scratch holds the first one's records."""
     b = ALL[name]
     c = b.case(dh, dtype, behind=1)
     dev = Device(ctx, c, ld_q=c.h * dh + 8, ld_o=c.h * dh + 4)
