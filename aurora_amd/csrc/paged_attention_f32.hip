@@ -1,0 +1,10 @@
+// The paged attention's kernels for pools of fp32.
+#include "paged_attention.hpp"
+
+namespace aurpaged {
+
+void launch_items_f32(const MhaArgs& a, const Sizes& z, int p_tile, int tile, unsigned items, hipStream_t st) {
+  launch_head<float>(a, p_tile, tile, step_rows(z), items, st);
+}
+
+}  // namespace aurpaged
