@@ -33,6 +33,8 @@ struct AppendArgs {
   int ld_q, ld_kv, ld_qo;
   int H, Hkv, dh, rot, n_pages, sh;
   bool pairs;
+  uint8_t *ks, *vs;  // scales of e4m3 pools, one for 2^ssh tokens of a head
+  int ssh;
 };
 
 // Rounded to the nearest bf16, ties to even.
@@ -65,9 +67,10 @@ __device__ __forceinline__ void move(const AppendArgs& a, const float* src, T* d
   put(dst + 4 * u + half, y * c + x * s);
 }
 
+// Block `block` of a grid of blocks_per_token of them for each row.
 template <class T>
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_per_token) {
-  const int t = blockIdx.x / blocks_per_token;
+__device__ __forceinline__ void append_rows(const AppendArgs& a, int block, int blocks_per_token) {
+  const int t = block / blocks_per_token;
   const int s = sequence_of(a.b, t);
   if (s >= a.b.b) return;  // a row behind the last sequence
   const Seq q = sequence(a.b, s);
@@ -77,7 +80,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_pe
   if (j < 0) return;  // fewer own tokens than new ones: this one has no place
   const float* tab = a.table + (size_t)(a.b.prefix_len + j) * a.rot;
   const int per_rot = a.dh / 4 - (a.pairs ? 0 : a.rot / 8);  // units of a rotated head
-  int u = (blockIdx.x % blocks_per_token) * 256 + threadIdx.x;
+  int u = (block % blocks_per_token) * 256 + threadIdx.x;
   if (u < a.H * per_rot) {
     if (a.q_out) {
       const int h = u / per_rot;
@@ -98,6 +101,161 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_pe
   const size_t dst = (row * a.Hkv + h) * a.dh;
   move(a, (is_k ? a.k : a.v) + (size_t)t * a.ld_kv + h * a.dh, static_cast<T*>(is_k ? a.kp : a.vp) + dst, u - h * per,
        tab, is_k && a.rot > 0);
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_per_token) {
+  append_rows<T>(a, blockIdx.x, blocks_per_token);
+}
+
+// ---------------------------------------------------------------- pools of e4m3
+
+// A unit is a block of 2^ssh tokens of one head of K or V.  Its new values' largest size m gives the least scale
+// 2^e, e from -117 to 119, with m <= 448·2^e: so all its numbers, subnormal ones too, are normal in bf16, and
+// finite.  Where the block holds older tokens e is no less than before; if it grew, they are rounded once more.
+// Elements are x·2^-e to the nearest e4m3, ties to even, and what lies beyond ±448·2^119 is that; an infinity or
+// NaN is held as NaN and has no part in m.
+//
+// A unit's new tokens lie in registers between its maximum and its rounding, so the rows are read once: one wave
+// holds up to 16 steps of 64 / LP tokens, LP lanes of 4 columns a head, and W = 4 waves share a unit that has
+// more.  Blocks walk over `chunk` rows of the batch each (no more than a block of tokens has, so that two of a
+// sequence's units at most begin there) and take the units that begin in them, their last rows may lie behind.
+struct UnitArgs {
+  int chunk, n_chunks, groups;  // rows of a chunk; blocks of a chunk, 4 / W units each
+  int q_blocks;                 // blocks of a row of q
+};
+
+constexpr int kUnitSteps = 16;
+
+// Four columns of a head, rotated: every product is rounded before the sum, so that a value next to the border
+// of two e4m3 numbers falls where plain 32-bit arithmetic lets it fall.
+__device__ __forceinline__ floatx4 rotated4(const AppendArgs& a, const float* src, int col, const float* tab) {
+#pragma clang fp contract(off)
+  const floatx4 x = *reinterpret_cast<const floatx4*>(src + col);
+  if (col >= a.rot) return x;
+  if (a.pairs) {
+    const floatx4 t = *reinterpret_cast<const floatx4*>(tab + col);
+    return floatx4{x[0] * t[0] - x[1] * t[1], x[1] * t[0] + x[0] * t[1], x[2] * t[2] - x[3] * t[3],
+                   x[3] * t[2] + x[2] * t[3]};
+  }
+  const int half = a.rot / 2, u = col < half ? col : col - half;
+  const floatx4 y = *reinterpret_cast<const floatx4*>(src + (col < half ? col + half : u));
+  const floatx4 t0 = *reinterpret_cast<const floatx4*>(tab + 2 * u), t1 = *reinterpret_cast<const floatx4*>(tab + 2 * u + 4);
+  const floatx4 c = {t0[0], t0[2], t1[0], t1[2]}, s = {t0[1], t0[3], t1[1], t1[3]};
+  return col < half ? x * c - y * s : x * c + y * s;
+}
+
+__device__ __forceinline__ unsigned round4(floatx4 x, int e) {  // of x·2^e
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[i] = fabsf(x[i]) <= 3.402823466e38f ? __builtin_amdgcn_fmed3f(ldexpf(x[i], e), -448.f, 448.f) : NAN;
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
+}
+
+// LP lanes of a head, W waves of a unit.
+template <int LP, int W>
+__device__ __forceinline__ void append_units(const AppendArgs& a, const UnitArgs& u, int block, float (&top)[4]) {
+  constexpr int PER = 64 / LP;  // tokens of a wave's step
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int r0 = block / u.groups * u.chunk, r1 = min(r0 + u.chunk, a.b.n_tok);
+  const int unit = block % u.groups * (4 / W) + w / W;
+  const bool is_k = unit < a.Hkv, on = unit < 2 * a.Hkv;
+  const int h = is_k ? unit : unit - a.Hkv, col = 4 * (lane % LP);
+  const bool live = on && col < a.dh;
+  const float* const src = (is_k ? a.k : a.v) + (size_t)h * a.dh;
+  uint8_t* const pool = static_cast<uint8_t*>(is_k ? a.kp : a.vp) + (size_t)h * a.dh;
+  const size_t ld = (size_t)a.Hkv * a.dh;
+  const int S = 1 << a.ssh;
+  for (int s = sequence_of(a.b, r0); s < a.b.b; ++s) {
+    const Seq q = sequence(a.b, s);
+    if (q.lo >= r1) break;
+    const int past = q.len - q.n, first = max(0, -past);  // tokens before `first` have no place
+    // the first unit that begins at row r0 or behind it
+    int i = max(first, r0 - q.lo);
+    if (i > first) i += -(past + i) & (S - 1);
+    for (; i < q.n && q.lo + i < r1; i += S - ((past + i) & (S - 1))) {
+      const int j = past + i, old = j & (S - 1), count = min(S - old, q.n - i);
+      const int page = a.b.pages[(size_t)s * a.b.max_pages + (j >> a.sh)];
+      if ((unsigned)page >= (unsigned)a.n_pages) continue;  // no page there: the rows are dropped
+      const int row = (page << a.sh) + (j & ((1 << a.sh) - 1));
+      uint8_t* const scale = (is_k ? a.ks : a.vs) + (on ? scale_index(row, h, a.Hkv, a.sh, a.ssh) : 0);
+      const int held = old && on ? *scale : 0;
+      floatx4 x[kUnitSteps];
+      float m = 0.f;
+#pragma unroll
+      for (int n = 0; n < kUnitSteps; ++n) {
+        const int k = (n * W + w % W) * PER + lane / LP;
+        x[n] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (n * PER * W < count && live && k < count) {
+          const float* p = src + (size_t)(q.lo + i + k) * a.ld_kv;
+          x[n] = is_k ? rotated4(a, p, col, a.table + (size_t)(a.b.prefix_len + j + k) * a.rot)
+                      : *reinterpret_cast<const floatx4*>(p + col);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[n][e]) <= 3.402823466e38f ? fabsf(x[n][e]) : 0.f);
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
+      if constexpr (W > 1) {
+        if (lane == 0) top[w] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        __syncthreads();
+      }
+      // m = f·2^x with f in [1, 2): e = x - 8, or x - 7 where f > 1.75
+      const int least = (int)((__float_as_uint(m) + 0x1fffffu) >> 23) - 8;
+      const int byte = max(min(max(least, 127 - 117), 127 + 119), held);
+      if (live && old && byte > held)
+        for (int k = (w % W) * PER + lane / LP; k < old; k += PER * W) {
+          unsigned* p = reinterpret_cast<unsigned*>(pool + (size_t)(row - old + k) * ld + col);
+          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(*p, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(*p, true);
+          *p = round4(floatx4{lo[0], lo[1], hi[0], hi[1]}, held - byte);
+        }
+#pragma unroll
+      for (int n = 0; n < kUnitSteps; ++n) {
+        const int k = (n * W + w % W) * PER + lane / LP;
+        if (n * PER * W < count && live && k < count) *reinterpret_cast<unsigned*>(pool + (size_t)(row + k) * ld + col) = round4(x[n], 127 - byte);
+      }
+      if (on && lane == 0 && w % W == 0 && (!old || byte > held)) *scale = (uint8_t)byte;
+    }
+  }
+}
+
+// Blocks of the chunks' units, then those of q's rows.
+template <int LP, int W>
+__global__ void __launch_bounds__(256) append_e4m3_kernel(AppendArgs a, UnitArgs u) {
+  __shared__ float top[4];
+  const int block = blockIdx.x, units = u.n_chunks * u.groups;
+  if (block < units) {
+    append_units<LP, W>(a, u, block, top);
+  } else {
+    AppendArgs q = a;
+    q.Hkv = 0;
+    append_rows<float>(q, block - units, u.q_blocks);
+  }
+}
+
+int launch_e4m3(aur_ctx* ctx, const char* who, const AppendArgs& a) {
+  int lp = 2;
+  while (4 * lp < a.dh) lp *= 2;
+  const int S = 1 << a.ssh, waves = S * lp > 64 * kUnitSteps ? 4 : 1;
+  UnitArgs u;
+  u.chunk = a.b.max_tok < S ? a.b.max_tok : S;
+  u.n_chunks = (a.b.n_tok + u.chunk - 1) / u.chunk;
+  u.groups = (2 * a.Hkv * waves + 3) / 4;
+  const int per_rot = a.dh / 4 - (a.pairs ? 0 : a.rot / 8);
+  u.q_blocks = (a.H * per_rot + 255) / 256;
+  const uint64_t blocks = (uint64_t)u.n_chunks * u.groups + (uint64_t)a.b.n_tok * u.q_blocks;
+  if (blocks > kMaxBlocks) return aur::set_error(ctx, AUR_ELIMIT, "%s: n_tok=%d rows of %d heads", who, a.b.n_tok, a.H);
+  auto* kernel = lp == 2    ? append_e4m3_kernel<2, 1>
+                 : lp == 4  ? append_e4m3_kernel<4, 1>
+                 : lp == 8  ? append_e4m3_kernel<8, 1>
+                 : lp == 16 ? (waves == 1 ? append_e4m3_kernel<16, 1> : append_e4m3_kernel<16, 4>)
+                            : (waves == 1 ? append_e4m3_kernel<32, 1> : append_e4m3_kernel<32, 4>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a, u);
+  AUR_LAUNCH_CHECK(ctx, "append_e4m3_kernel");
+  return 0;
 }
 
 // Angles in 64 bits: at position 10^6 a 32-bit product of position and frequency is off by
@@ -122,7 +280,7 @@ int check_paged(aur_ctx* ctx, const char* who, const aur_paged_cache* c, const a
   if (!c || !b) return set_error(ctx, AUR_EINVAL, "%s: null cache or batch", who);
   if (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v))
     return set_error(ctx, AUR_EINVAL, "%s: the pools must be there and 16-byte aligned", who);
-  if (c->dtype != AUR_PAGED_F32 && c->dtype != AUR_PAGED_BF16)
+  if (c->dtype != AUR_PAGED_F32 && c->dtype != AUR_PAGED_BF16 && c->dtype != AUR_PAGED_E4M3)
     return set_error(ctx, AUR_EINVAL, "%s: dtype %u", who, c->dtype);
   if (c->n_pages == 0 || c->page_len == 0 || (c->page_len & (c->page_len - 1)) || c->n_kv_head == 0 || c->d_head == 0)
     return set_error(ctx, AUR_EINVAL, "%s: n_pages=%u page_len=%u (a power of two) n_kv_head=%u d_head=%u", who,
@@ -132,6 +290,13 @@ int check_paged(aur_ctx* ctx, const char* who, const aur_paged_cache* c, const a
   if ((uint64_t)c->n_pages * c->page_len > 0x7fffffffu || c->n_kv_head > 4096)
     return set_error(ctx, AUR_ELIMIT, "%s: pool of %u pages of %u rows, n_kv_head=%u", who, c->n_pages, c->page_len,
                      c->n_kv_head);
+  if (c->dtype == AUR_PAGED_E4M3) {
+    if (!c->k_scale || !c->v_scale || c->scale_len == 0 || (c->scale_len & (c->scale_len - 1)) ||
+        c->scale_len > c->page_len)
+      return set_error(ctx, AUR_EINVAL, "%s: scale_len=%u (a power of two up to page_len=%u) with both scales", who,
+                       c->scale_len, c->page_len);
+    if (c->scale_len > 128) return set_error(ctx, AUR_ELIMIT, "%s: scale_len=%u (up to 128)", who, c->scale_len);
+  }
   if (b->n_tok > 0x00ffffffu || b->b > 0x00ffffffu)
     return set_error(ctx, AUR_ELIMIT, "%s: n_tok=%u b=%u", who, b->n_tok, b->b);
   if (b->b && b->n_tok) {
@@ -201,6 +366,10 @@ int aur_kv_append_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_pa
   a.ld_q = (int)ld_q; a.ld_kv = (int)ld_kv; a.ld_qo = (int)ld_qo;
   a.H = q ? (int)n_head : 0; a.Hkv = (int)cache->n_kv_head; a.dh = (int)dh; a.rot = (int)rot_dim;
   a.n_pages = (int)cache->n_pages; a.sh = log2_of(cache->page_len); a.pairs = pairs != 0;
+  if (cache->dtype == AUR_PAGED_E4M3) {
+    a.ks = cache->k_scale; a.vs = cache->v_scale; a.ssh = log2_of(cache->scale_len);
+    return launch_e4m3(ctx, who, a);
+  }
   const int per_rot = a.dh / 4 - (a.pairs ? 0 : a.rot / 8);
   const int units = (a.H + a.Hkv) * per_rot + a.Hkv * a.dh / 4;
   const int per_token = (units + 255) / 256;

@@ -40,6 +40,17 @@ __device__ __forceinline__ int sequence_of(const Batch& a, int t) {
   return s;
 }
 
+// Elements of a pool held in 8 bits: e4m3 numbers (sign, 4 bits of exponent, 3 of significand; up to 448 and down
+// to 2^-9, a NaN, no infinity) times a power of two of their own for every 2^ssh tokens of a head, held as the
+// byte e + 127 of 2^e.  A pool row's scales lie apart, [n_pages][n_kv_head][page_len >> ssh].
+struct e4m3 {
+  uint8_t bits;
+};
+__device__ __forceinline__ size_t scale_index(int row, int hk, int n_kv_head, int sh, int ssh) {
+  return (((size_t)(row >> sh) * n_kv_head + hk) << (sh - ssh)) + ((row & ((1 << sh) - 1)) >> ssh);
+}
+__device__ __forceinline__ float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }
+
 // Work items of a launch stay below 2^32: so many blocks of 256.
 constexpr uint32_t kMaxBlocks = 0x00ffffffu;
 

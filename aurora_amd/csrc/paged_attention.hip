@@ -80,7 +80,7 @@ Sizes sizes_of(const Batch& b, const aur_paged_cache& c, uint32_t n_head) {
 }
 
 void launch_items(const MhaArgs& a, const Sizes& z, int p_tile, int tile, unsigned items, hipStream_t st) {
-  (z.f32 ? launch_items_f32 : launch_items_bf16)(a, z, p_tile, tile, items, st);
+  (z.f32 ? launch_items_f32 : a.k_scale ? launch_items_e4m3 : launch_items_bf16)(a, z, p_tile, tile, items, st);
 }
 
 }  // namespace
@@ -117,6 +117,9 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
   a.H = (int)n_head; a.Hkv = (int)cache->n_kv_head; a.G = a.H / a.Hkv; a.dh = (int)cache->d_head;
   a.n_pages = (int)cache->n_pages; a.sh = log2_of(cache->page_len);
   a.scale = 1.0f / sqrtf((float)a.dh);
+  if (cache->dtype == AUR_PAGED_E4M3) {
+    a.k_scale = cache->k_scale; a.v_scale = cache->v_scale; a.ssh = log2_of(cache->scale_len);
+  }
   const Sizes z = sizes_of(a.b, *cache, n_head);
   const Plan p = make_plan(z);
   a.pooled = p.pooled;

@@ -45,6 +45,8 @@ struct MhaArgs {
   float *part_o, *part_ml;  // [part][token][H][dh], [part][token][H][2]; null: items write out and lse
   int ld_q, ld_o;
   int H, Hkv, G, dh, n_pages, sh;
+  const uint8_t *k_scale, *v_scale;  // of e4m3 pools
+  int ssh;
   float scale;
   // The plan: row tiles and key ranges of the prefix's items and the own ones.
   int pooled;
@@ -57,6 +59,7 @@ struct MhaArgs {
 // p_tile beside them (0: items of one kind).
 void launch_items_f32(const MhaArgs& a, const Sizes& z, int p_tile, int tile, unsigned items, hipStream_t st);
 void launch_items_bf16(const MhaArgs& a, const Sizes& z, int p_tile, int tile, unsigned items, hipStream_t st);
+void launch_items_e4m3(const MhaArgs& a, const Sizes& z, int p_tile, int tile, unsigned items, hipStream_t st);
 
 }  // namespace aurpaged
 
@@ -253,6 +256,98 @@ struct Keys32 {
   }
 };
 
+// Four e4m3 numbers times a scale, exactly but below 2^-126, as two pairs of bf16.
+__device__ __forceinline__ uint2v widen4(unsigned x, float scale) {
+  return uint2v{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, false)),
+                __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, true))};
+}
+// The scales of the key at pool row `at` (1 where there is none).
+__device__ __forceinline__ unsigned scale_byte(const MhaArgs& a, const uint8_t* scales, int hk, int at) {
+  return at < 0 ? 127u : scales[scale_index(at, hk, a.Hkv, a.sh, a.ssh)];
+}
+
+// The same of an e4m3 pool: 8 columns of K, 4 of V a lane, which the conversion to bf16 multiplies by the scale
+// of their key.  Lane l loads the scales of key l % 32; the others have them from there.
+template <int DT>
+struct Keys32<e4m3, DT> {
+  static constexpr int VB = (DT + 3) / 4, KC = (DT + 1) / 2;
+  uint2v k[2][KC];
+  unsigned v[2][4][VB], k_scale, v_scale;
+  template <bool STREAM>
+  __device__ __forceinline__ void load_k(const MhaArgs& a, int hk, int at, int g, int l16) {
+    const size_t ld = (size_t)a.Hkv * a.dh;
+    const uint8_t* kp = static_cast<const uint8_t*>(a.k) + (size_t)hk * a.dh;
+    k_scale = scale_byte(a, a.k_scale, hk, at);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const uint8_t* p = kp + (size_t)max(__shfl(at, 16 * kt + l16, 64), 0) * ld;
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+        k[kt][c] = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(p + min(32 * c + 8 * g, a.dh - 8)));
+    }
+  }
+  template <bool STREAM>
+  __device__ __forceinline__ void load_v(const MhaArgs& a, int hk, int at, int g, int l16) {
+    const size_t ld = (size_t)a.Hkv * a.dh;
+    const uint8_t* vp = static_cast<const uint8_t*>(a.v) + (size_t)hk * a.dh;
+    v_scale = scale_byte(a, a.v_scale, hk, at);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint8_t* p = vp + (size_t)max(__shfl(at, 16 * kt + 4 * g + e, 64), 0) * ld;
+#pragma unroll
+        for (int b = 0; b < VB; ++b)
+          v[kt][e][b] = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(p + min(64 * b + 4 * l16, a.dh - 4)));
+      }
+  }
+  __device__ __forceinline__ void drop_missing(unsigned there, int g) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!(there >> (16 * kt + 4 * g + e) & 1))
+#pragma unroll
+          for (int b = 0; b < VB; ++b) v[kt][e][b] = 0;
+  }
+};
+
+// As bf16 goes into the MFMA: K's piece c of tile kt, and V's pairs of columns (64b + 4·l16, + 1), (… + 2, + 3).
+template <int DT>
+__device__ __forceinline__ void keys_of(const Keys32<__bf16, DT>& x, int kt, int, uint4v (&k)[(DT + 1) / 2]) {
+#pragma unroll
+  for (int c = 0; c < (DT + 1) / 2; ++c) k[c] = x.k[kt][c];
+}
+template <int DT>
+__device__ __forceinline__ void keys_of(const Keys32<e4m3, DT>& x, int kt, int l16, uint4v (&k)[(DT + 1) / 2]) {
+  const float scale = scale_of(__shfl(x.k_scale, 16 * kt + l16, 64));
+#pragma unroll
+  for (int c = 0; c < (DT + 1) / 2; ++c) {
+    const uint2v lo = widen4(x.k[kt][c][0], scale), hi = widen4(x.k[kt][c][1], scale);
+    k[c] = uint4v{lo[0], lo[1], hi[0], hi[1]};
+  }
+}
+template <int DT>
+__device__ __forceinline__ void values_of(const Keys32<__bf16, DT>& x, int, uint2v (&v)[2][4][(DT + 3) / 4]) {
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int b = 0; b < (DT + 3) / 4; ++b) v[kt][e][b] = x.v[kt][e][b];
+}
+template <int DT>
+__device__ __forceinline__ void values_of(const Keys32<e4m3, DT>& x, int g, uint2v (&v)[2][4][(DT + 3) / 4]) {
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float scale = scale_of(__shfl(x.v_scale, 16 * kt + 4 * g + e, 64));
+#pragma unroll
+      for (int b = 0; b < (DT + 3) / 4; ++b) v[kt][e][b] = widen4(x.v[kt][e][b], scale);
+    }
+}
+
 // x as the sum of three bf16 numbers, exactly but for what lies 2^-24 below it and more (8 bits each,
 // with the range of fp32, so no scales are needed; parts below 2^-126 the MFMA takes as zero; an infinity
 // becomes NaN).
@@ -277,7 +372,7 @@ __device__ __forceinline__ floatx4 mfma_bf16(bf16x8 a, bf16x8 b, floatx4 c) {
 }
 
 // A wave's queries as the MFMA's second operand, times log2(e)/√d_head: fp32 pieces of 4 columns, or
-// for bf16 keys three bf16 parts of 8 columns.
+// for bf16 and e4m3 keys three bf16 parts of 8 columns.
 template <class T, int DT, int RT>
 struct Queries;
 template <int DT, int RT>
@@ -293,8 +388,8 @@ struct Queries<float, DT, RT> {
       }
   }
 };
-template <int DT, int RT>
-struct Queries<__bf16, DT, RT> {
+template <class T, int DT, int RT>
+struct Queries {
   static constexpr int KC = (DT + 1) / 2;
   Split8 q[RT][KC];
   __device__ __forceinline__ void load(const Rows<RT>& r, int dh, int g, float sl2) {
@@ -335,17 +430,19 @@ __device__ __forceinline__ void scores(const Keys32<float, DT>& x, const Queries
     }
   }
 }
-template <int DT, int RT>
-__device__ __forceinline__ void scores(const Keys32<__bf16, DT>& x, const Queries<__bf16, DT, RT>& q, int dh, int g,
+template <class T, int DT, int RT>
+__device__ __forceinline__ void scores(const Keys32<T, DT>& x, const Queries<T, DT, RT>& q, int dh, int g,
                                        floatx4 (&st)[RT][2]) {
   constexpr int KC = (DT + 1) / 2;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
+    uint4v kk[KC];
+    keys_of(x, kt, threadIdx.x & 15, kk);
 #pragma unroll
     for (int r = 0; r < RT; ++r) st[r][kt] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      uint4v u = x.k[kt][c];
+      uint4v u = kk[c];
       if (32 * c + 8 * g >= dh) u = uint4v{0, 0, 0, 0};
       const bf16x8 k = __builtin_bit_cast(bf16x8, u);
 #pragma unroll
@@ -372,8 +469,10 @@ __device__ __forceinline__ void add_values(const Keys32<float, DT>& x, const flo
 #pragma unroll
           for (int r = 0; r < RT; ++r) s.acc[r][b][c] = mfma16x16x4(x.v[kt][e][b][c], st[r][kt][e], s.acc[r][b][c]);
 }
-template <int DT, int RT>
-__device__ __forceinline__ void add_values(const Keys32<__bf16, DT>& x, const floatx4 (&st)[RT][2], Sums<DT, RT>& s) {
+template <class T, int DT, int RT>
+__device__ __forceinline__ void add_values(const Keys32<T, DT>& x, const floatx4 (&st)[RT][2], Sums<DT, RT>& s) {
+  uint2v vv[2][4][Sums<DT, RT>::VB];
+  values_of(x, (threadIdx.x & 63) >> 4, vv);
   // the MFMA's 8 keys of a lane group: 4g … 4g + 3 of both tiles of 16
   Split8 p[RT];
 #pragma unroll
@@ -392,7 +491,7 @@ __device__ __forceinline__ void add_values(const Keys32<__bf16, DT>& x, const fl
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          u[2 * kt + i] = __builtin_amdgcn_perm(x.v[kt][2 * i + 1][b][c >> 1], x.v[kt][2 * i][b][c >> 1],
+          u[2 * kt + i] = __builtin_amdgcn_perm(vv[kt][2 * i + 1][b][c >> 1], vv[kt][2 * i][b][c >> 1],
                                                 c & 1 ? 0x07060302u : 0x05040100u);
       const bf16x8 v = __builtin_bit_cast(bf16x8, u);
 #pragma unroll
@@ -468,6 +567,16 @@ __device__ __forceinline__ bool finite(const Sums<DT, RT>& s, bool live) {
 // such operands, or from a split into parts, which has no infinities):
 // scores by the fp32 MFMA from whole operands, and every row adds the values of those keys alone that
 // it sees (0 times an infinity that it does not see would be NaN).
+__device__ __forceinline__ float number(float x) { return x; }
+__device__ __forceinline__ float number(__bf16 x) { return (float)x; }
+__device__ __forceinline__ float number(e4m3 x) { return __builtin_amdgcn_cvt_f32_fp8(x.bits, 0); }
+// What an element of the key at pool row `at` is multiplied by.
+template <class T>
+__device__ __forceinline__ float key_scale(const MhaArgs& a, const uint8_t* scales, int hk, int at) {
+  if (!std::is_same<T, e4m3>::value) return 1.f;
+  const unsigned byte = scale_byte(a, scales, hk, at);
+  return byte == 255 ? NAN : ldexpf(1.f, (int)byte - 127);  // (the conversions to bf16 and fp32 do as much)
+}
 template <class T, int DT, int RT>
 __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, int stride, Sums<DT, RT>& s) {
   constexpr int VB = Sums<DT, RT>::VB;
@@ -486,14 +595,16 @@ __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, in
     floatx4 st[RT][2] = {};
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const T* p = kp + (size_t)max(__shfl(at, 16 * kt + l16, 64), 0) * ld;
+      const int key_at = __shfl(at, 16 * kt + l16, 64);
+      const T* p = kp + (size_t)max(key_at, 0) * ld;
+      const float ks = key_scale<T>(a, a.k_scale, it.hk, key_at);
 #pragma unroll 1
       for (int c = 0; c < a.dh; c += 16) {
         const bool live = c + 4 * g < a.dh;
         floatx4 k = {0.f, 0.f, 0.f, 0.f};
         if (live) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) k[e] = (float)p[c + 4 * g + e];
+          for (int e = 0; e < 4; ++e) k[e] = number(p[c + 4 * g + e]) * ks;
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -510,6 +621,7 @@ __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, in
     for (int key = 0; key < 32; ++key) {
       const int row = __shfl(at, key, 64), from = (key & 12) * 4 + l16;
       if (row < 0) continue;
+      const float vs = key_scale<T>(a, a.v_scale, it.hk, row);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         const floatx4 pv = key < 16 ? st[r][0] : st[r][1];
@@ -523,7 +635,7 @@ __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, in
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const int col = 64 * b + 16 * g + 4 * i + c;
-              if (seen && col < a.dh) s.acc[r][b][c][i] += p * (float)vp[(size_t)row * ld + col];
+              if (seen && col < a.dh) s.acc[r][b][c][i] += p * (number(vp[(size_t)row * ld + col]) * vs);
             }
       }
     }
@@ -638,11 +750,14 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
 // page of the step after them.
 template <class T, int DT>
 struct FewRows {
-  static constexpr int E = 16 / sizeof(T);                // columns of a lane
+  static constexpr bool B8 = sizeof(T) == 1;
+  static constexpr int E = B8 ? 8 : 16 / sizeof(T);       // columns of a lane
+  using Piece = typename std::conditional<B8, float2v, floatx4>::type;
   static constexpr int N = (16 * DT + E - 1) / E;         // lanes of a head
   static constexpr int LP = N <= 2 ? 2 : N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : 32;
   static constexpr int KPI = 64 / LP;                     // keys of a load
-  static constexpr int U = KPI > 16 ? 64 / KPI : 4;       // loads of K, and of V, under way; as many are in use
+  // loads of K, and of V, under way; as many are in use
+  static constexpr int U = KPI > 16 || (B8 && KPI > 8) ? 64 / KPI : B8 ? 8 : 4;
   static constexpr int KEYS = U * KPI;                    // of a step; a lane finds the row of one
   static_assert(KEYS <= 64 && N <= 32, "a wave finds the rows of a step");
 };
@@ -651,15 +766,25 @@ struct FewLds {
   float m[NW][R], l[NW][R];
   __attribute__((aligned(16))) float o[NW][R][128];
 };
-__device__ __forceinline__ void unpack(floatx4 x, float (&y)[4]) {
+__device__ __forceinline__ void unpack(floatx4 x, float (&y)[4], float) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = x[i];
 }
-__device__ __forceinline__ void unpack(floatx4 x, float (&y)[8]) {
+__device__ __forceinline__ void unpack(floatx4 x, float (&y)[8], float) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     y[2 * i] = __uint_as_float(__float_as_uint(x[i]) << 16);
     y[2 * i + 1] = __uint_as_float(__float_as_uint(x[i]) & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(float2v x, float (&y)[8], float scale) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2v p = __builtin_bit_cast(
+        float2v, i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(__float_as_uint(x[i / 2]), scale, true)
+                       : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(__float_as_uint(x[i / 2]), scale, false));
+    y[2 * i] = p[0];
+    y[2 * i + 1] = p[1];
   }
 }
 
@@ -689,15 +814,21 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
     for (int i = 0; i < E; ++i) acc[r][i] = 0.f;
   }
   if (x < it.x1) {
-    floatx4 k[2][U], v[2][U];
+    using Piece = typename G::Piece;
+    Piece k[2][U], v[2][U];
+    unsigned k_scale[2] = {}, v_scale[2] = {};  // of the key that this lane finds
     unsigned long long there[2];
     auto load = [&](int b, int at) {
       there[b] = __ballot(at >= 0);
+      if (G::B8) {
+        k_scale[b] = scale_byte(a, a.k_scale, it.hk, at);
+        v_scale[b] = scale_byte(a, a.v_scale, it.hk, at);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long long o = max(__shfl(at, u * KPI + kg, 64), 0) * ld;
-        k[b][u] = __builtin_nontemporal_load(reinterpret_cast<const floatx4*>(kp + o));
-        v[b][u] = __builtin_nontemporal_load(reinterpret_cast<const floatx4*>(vp + o));
+        k[b][u] = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(kp + o));
+        v[b][u] = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(vp + o));
       }
     };
     load(0, row_of(a, it, x + lane % KEYS, page));
@@ -718,7 +849,7 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float y[E];
-        unpack(k[B][u], y);
+        unpack(k[B][u], y, G::B8 ? scale_of(__shfl(k_scale[B], u * KPI + kg, 64)) : 1.f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           float d = q[r][0] * y[0];
@@ -733,7 +864,7 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
           if (!(there[B] >> (u * KPI + kg) & 1)) {
 #pragma unroll
             for (int r = 0; r < R; ++r) s[r][u] = -INFINITY;
-            v[B][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+            v[B][u] = Piece{};
           }
       }
 #pragma unroll
@@ -756,7 +887,7 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float y[E];
-        unpack(v[B][u], y);
+        unpack(v[B][u], y, G::B8 ? scale_of(__shfl(v_scale[B], u * KPI + kg, 64)) : 1.f);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -818,8 +949,9 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
 // above 96 in 64 rows 12, others up to 4.)
 template <class T, int DT, int W>
 struct TileGeo {
-  static constexpr bool F32 = std::is_same<T, float>::value;
+  static constexpr bool F32 = std::is_same<T, float>::value, B8 = sizeof(T) == 1;
   static constexpr int PARTS = F32 ? 3 : 1;
+  using KPiece = typename std::conditional<B8, uint2v, floatx4>::type;  // 8 columns of a key, or 4
   static constexpr int KT = DT > 4 ? 32 : 64;      // keys of a tile
   static constexpr int KC = (DT + 1) / 2;          // 32-column steps of a score
   static constexpr int KROW = KC == 1 ? 64 : KC == 2 ? 128 : 256;
@@ -843,11 +975,12 @@ struct TileLds {
   char k[G::PARTS * G::KPLANE], v[G::PARTS * G::VPLANE];
   long long offset[3][G::KT];  // in bytes, of the keys of this tile and the next two in the pools
   unsigned long long have[3];  // which of them are there
+  float scale[G::B8 ? 3 : 1][2][G::B8 ? G::KT : 1];  // of their K and V
 };
 template <class T, int DT, int NR, int W>
 __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& lds) {
   using G = TileGeo<T, DT, W>;
-  constexpr bool F32 = G::F32;
+  constexpr bool F32 = G::F32, B8 = G::B8;
   constexpr int KT = G::KT, KC = G::KC, NI = G::NI, NK = KT / 16, VC = G::VC;
   char* const ks = lds.k;
   char* const vs = lds.v;
@@ -870,9 +1003,17 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
   // Where a tile's keys lie; the first KT threads ask for the pages' numbers a tile before they are needed.
   const long long ld = (long long)a.Hkv * a.dh * sizeof(T);
   int xp = it.x0 + tid;  // the key whose page is under way
+  unsigned k_scale = 127, v_scale = 127;  // of the key placed last: they are laid down when the next one is
   auto place = [&](int slot) {
     if (tid < KT) {
       const int at = row_of(a, it, xp, page);
+      if constexpr (B8) {
+        const int last = slot == 0 ? 2 : slot - 1;
+        lds.scale[last][0][tid] = scale_of(k_scale);
+        lds.scale[last][1][tid] = scale_of(v_scale);
+        k_scale = scale_byte(a, a.k_scale, it.hk, at);
+        v_scale = scale_byte(a, a.v_scale, it.hk, at);
+      }
       lds.offset[slot][tid] = at < 0 ? 0 : at * ld;
       const unsigned long long have = __ballot(at >= 0);
       if (tid == 0) lds.have[slot] = have;
@@ -890,8 +1031,8 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
   const int vkey = v_on ? 32 * (vg >> 2) + 4 * (vg & 3) : 0;  // … the keys vkey + 16·(i/4) + i%4
   const char* const kp = static_cast<const char*>(a.k) + (size_t)it.hk * a.dh * sizeof(T);
   const char* const vp = static_cast<const char*>(a.v) + ((size_t)it.hk * a.dh + min(vc, a.dh - VC)) * sizeof(T);
-  floatx4 kx[NI][F32 ? 2 : 1];  // as loaded
-  float vx[8][F32 ? VC : 1];    // bf16: a pair
+  typename G::KPiece kx[NI][F32 ? 2 : 1];  // as loaded
+  float vx[8][F32 ? VC : 1];               // bf16, e4m3: a pair
   unsigned long long have = 0;  // of the keys in them
   auto load = [&](int slot) {
     have = lds.have[slot];
@@ -899,14 +1040,16 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const char* q = p + min(8 * (ko + G::TPR * i), a.dh - 8) * (int)sizeof(T);
-      kx[i][0] = *reinterpret_cast<const floatx4*>(q);
-      if (F32) kx[i][F32] = *reinterpret_cast<const floatx4*>(q + 16);
+      kx[i][0] = *reinterpret_cast<const typename G::KPiece*>(q);
+      if constexpr (F32) kx[i][1] = *reinterpret_cast<const floatx4*>(q + 16);
     }
     if (G::VN * (KT / 8) < 64 * W && !v_on) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const char* q = vp + lds.offset[slot][vkey + 16 * (i >> 2) + (i & 3)];
-      if (F32 && VC == 2) {
+      if (B8) {
+        vx[i][0] = __uint_as_float(*reinterpret_cast<const uint16_t*>(q));
+      } else if (F32 && VC == 2) {
         const float2v x = *reinterpret_cast<const float2v*>(q);
         vx[i][0] = x[0];
         vx[i][F32 ? VC - 1 : 0] = x[1];
@@ -915,7 +1058,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
       }
     }
   };
-  auto lay_down = [&] {
+  auto lay_down = [&](int slot) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int q = ko + G::TPR * i;
@@ -923,8 +1066,12 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
       const bool live = DT * 16 == 32 * KC || 8 * q < a.dh;
       char* p = ks + tile_granule<G::KROW>(kr, q);
       const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
-      if (F32) {
-        const floatx4 x = live ? kx[i][0] : zero, y = live ? kx[i][F32] : zero;
+      if constexpr (B8) {
+        const float scale = lds.scale[slot][0][kr];
+        const uint2v lo = widen4(kx[i][0][0], scale), hi = widen4(kx[i][0][1], scale);
+        *reinterpret_cast<uint4v*>(p) = live ? uint4v{lo[0], lo[1], hi[0], hi[1]} : uint4v{0, 0, 0, 0};
+      } else if constexpr (F32) {
+        const floatx4 x = live ? kx[i][0] : zero, y = live ? kx[i][1] : zero;
         Split8 s;
         s.set(0, x[0], x[1]);
         s.set(2, x[2], x[3]);
@@ -938,6 +1085,12 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
       }
     }
     if (G::VN * (KT / 8) < 64 * W && !v_on) return;
+    if constexpr (B8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        vx[i][0] = __builtin_bit_cast(float, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                                                 __float_as_uint(vx[i][0]), lds.scale[slot][1][vkey + 16 * (i >> 2) + (i & 3)], false));
+    }
     if (have != ALL) {  // a key that is not there adds nothing, whatever lies in its place
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -1075,7 +1228,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
   int slot = 0;
   for (int x = it.x0; x < it.x1; x += KT) {
     if (x > it.x0) __syncthreads();  // every wave is done with the last tile
-    lay_down();
+    lay_down(slot);
     const unsigned long long there = have;
     const int next = slot == 2 ? 0 : slot + 1;
     place(next == 2 ? 0 : next + 1);
@@ -1138,7 +1291,7 @@ union StepLds {
 // 43.5; 30 of 32 heads on 8, prefix 4096 19.7 and 21.9; 64 on 32768 82 and 77.6, without own keys 48.6 and 51;
 // of d_head 48 on 16384 63.2 and 61.6; tails of 30 to 60 tokens on 2048 51.4 and 49.5.
 template <class T, int DT, int NR>
-constexpr int kWaves = sizeof(T) == 2 && DT <= 4 && NR == 1 ? 3 : 2;
+constexpr int kWaves = sizeof(T) <= 2 && DT <= 4 && NR == 1 ? 3 : 2;
 
 template <class T, int DT, int NR, int W>
 __global__ void __launch_bounds__(64 * W, (kWaves<T, DT, NR>)) paged_mha_tile_kernel(MhaArgs a) {

@@ -24,7 +24,7 @@ __all__ = [
     "AuroraError", "GpuContext", "GpuBuffer", "GemmKernel", "GemmTransposeBKernel",
     "OuterProductAccumKernel", "CausalMhaForwardKernel", "CausalMhaBackwardKernel",
     "MhaKvCacheKernel", "PagedKvCache", "PagedBatch", "RotaryTableKernel", "PagedKvAppendKernel",
-    "PagedMhaKernel",
+    "PagedKvReadKernel", "PagedMhaKernel", "SampleKernel",
 ]
 
 
@@ -259,7 +259,8 @@ class MhaKvCacheKernel(_Kernel):
 class _PagedCacheStruct(C.Structure):
     """aur_paged_cache."""
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_uint32), ("page_len", C.c_uint32),
-                ("n_kv_head", C.c_uint32), ("d_head", C.c_uint32), ("dtype", C.c_uint32)]
+                ("n_kv_head", C.c_uint32), ("d_head", C.c_uint32), ("dtype", C.c_uint32),
+                ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("scale_len", C.c_uint32)]
 
 
 class _PagedBatchStruct(C.Structure):
@@ -271,39 +272,63 @@ class _PagedBatchStruct(C.Structure):
 
 
 class PagedKvCache:
-    """A paged K/V cache (aur_paged_cache): two pools [n_pages, page_len, n_kv_head*d_head] of "f32"
-    or "bf16" elements that the caller owns."""
+    """A paged K/V cache (aur_paged_cache): two pools [n_pages, page_len, n_kv_head*d_head] of "f32",
+    "bf16" or "e4m3" elements that the caller owns; e4m3 pools with scales [n_pages, n_kv_head,
+    page_len/scale_len], a byte each, for every `scale_len` tokens of a head."""
 
-    DTYPES = {"f32": 0, "bf16": 1}
+    DTYPES = {"f32": 0, "bf16": 1, "e4m3": 2}
+    _NUMPY = {"f32": np.float32, "bf16": np.uint16, "e4m3": np.uint8}
 
-    def __init__(self, k, v, n_pages, page_len, n_kv_head, d_head, dtype="f32"):
-        if dtype not in self.DTYPES:
-            raise ValueError(f"PagedKvCache: dtype {dtype!r}, one of {sorted(self.DTYPES)}")
+    def __init__(self, k, v, n_pages, page_len, n_kv_head, d_head, dtype="f32", k_scale=None, v_scale=None,
+                 scale_len=0):
+        self._check(dtype, page_len, scale_len)
+        if (dtype == "e4m3") != (k_scale is not None) or (dtype == "e4m3") != (v_scale is not None):
+            raise ValueError("PagedKvCache: k_scale and v_scale belong to e4m3 pools, and those need them")
         self.k, self.v, self.dtype = k, v, dtype
+        self.k_scale, self.v_scale, self.scale_len = k_scale, v_scale, scale_len
         self.n_pages, self.page_len, self.n_kv_head, self.d_head = n_pages, page_len, n_kv_head, d_head
-        size = 4 if dtype == "f32" else 2
+        size = np.dtype(self._NUMPY[dtype]).itemsize
         for b in (k, v):
             if isinstance(b, GpuBuffer) and b.nbytes < size * self.elements:
                 raise ValueError(f"PagedKvCache: pool of {b.nbytes} bytes, {size * self.elements} needed")
-        self._struct = _PagedCacheStruct(_p(k), _p(v), n_pages, page_len, n_kv_head, d_head, self.DTYPES[dtype])
+        for b in (k_scale, v_scale):
+            if isinstance(b, GpuBuffer) and b.nbytes < self.scales:
+                raise ValueError(f"PagedKvCache: {b.nbytes} bytes of scales, {self.scales} needed")
+        self._struct = _PagedCacheStruct(_p(k), _p(v), n_pages, page_len, n_kv_head, d_head, self.DTYPES[dtype],
+                                         0 if k_scale is None else _p(k_scale),
+                                         0 if v_scale is None else _p(v_scale), scale_len)
         self.ref = C.addressof(self._struct)
+
+    @classmethod
+    def _check(cls, dtype, page_len, scale_len) -> None:
+        if dtype not in cls.DTYPES:
+            raise ValueError(f"PagedKvCache: dtype {dtype!r}, one of {sorted(cls.DTYPES)}")
+        if dtype == "e4m3" and not (0 < scale_len <= page_len and scale_len & (scale_len - 1) == 0):
+            raise ValueError(f"PagedKvCache: scale_len {scale_len}, a power of two up to page_len {page_len}")
 
     @property
     def elements(self) -> int:
         """Elements of one pool."""
         return self.n_pages * self.page_len * self.n_kv_head * self.d_head
 
+    @property
+    def scales(self) -> int:
+        """Scales of one e4m3 pool."""
+        return self.n_pages * self.n_kv_head * (self.page_len // self.scale_len) if self.dtype == "e4m3" else 0
+
     @classmethod
-    def zeros(cls, ctx: GpuContext, n_pages, page_len, n_kv_head, d_head, dtype="f32") -> "PagedKvCache":
-        if dtype not in cls.DTYPES:  # before there is anything to free
-            raise ValueError(f"PagedKvCache: dtype {dtype!r}, one of {sorted(cls.DTYPES)}")
-        n = n_pages * page_len * n_kv_head * d_head
-        np_type = np.float32 if dtype == "f32" else np.uint16
-        return cls(GpuBuffer.zeros(ctx, n, np_type), GpuBuffer.zeros(ctx, n, np_type), n_pages, page_len,
-                   n_kv_head, d_head, dtype)
+    def zeros(cls, ctx: GpuContext, n_pages, page_len, n_kv_head, d_head, dtype="f32", scale_len=0) -> "PagedKvCache":
+        cls._check(dtype, page_len, scale_len)  # before there is anything to free
+        n, np_type = n_pages * page_len * n_kv_head * d_head, cls._NUMPY[dtype]
+        k, v = GpuBuffer.zeros(ctx, n, np_type), GpuBuffer.zeros(ctx, n, np_type)
+        if dtype != "e4m3":
+            return cls(k, v, n_pages, page_len, n_kv_head, d_head, dtype)
+        n = n_pages * n_kv_head * (page_len // scale_len)
+        return cls(k, v, n_pages, page_len, n_kv_head, d_head, dtype, GpuBuffer.zeros(ctx, n, np.uint8),
+                   GpuBuffer.zeros(ctx, n, np.uint8), scale_len)
 
     def free(self) -> None:
-        for b in (self.k, self.v):
+        for b in (self.k, self.v, self.k_scale, self.v_scale):
             if isinstance(b, GpuBuffer):
                 b.free()
 
@@ -362,6 +387,18 @@ class PagedKvAppendKernel(_Kernel):
                  rot_dim, n_head, 1 if pairs else 0)
 
 
+class PagedKvReadKernel(_Kernel):
+    """Keys [first, first + count) of every sequence's axis, prefix and then own keys, as dense fp32 rows
+    k_out, v_out [b*count, n_kv_head*d_head] (0: not wanted); zeros where there is no key."""
+
+    def dispatch_into(self, ctx, cache, batch, k_out, v_out, ld, first, count):
+        if _any_buffer(k_out, v_out):
+            n = _rows(batch.b * count, ld, cache.n_kv_head * cache.d_head)
+            _need("PagedKvReadKernel k_out/v_out", n, k_out, v_out)
+            k_out, v_out = _p(k_out), _p(v_out)
+        ctx.call("aur_kv_read_paged", cache.ref, batch.ref, k_out, v_out, ld, first, count)
+
+
 class PagedMhaKernel(_Kernel):
     """Attention of the batch's new tokens over the shared prefix and their own keys (lse = 0: none)."""
 
@@ -378,3 +415,17 @@ class PagedMhaKernel(_Kernel):
             _need("PagedMhaKernel scratch", scratch_len, scratch)
             q, out, lse, scratch = _p(q), _p(out), _p(lse), _p(scratch)
         ctx.call("aur_mha_paged", cache.ref, batch.ref, q, ld_q, out, ld_o, lse, scratch, 4 * scratch_len, n_head)
+
+
+class SampleKernel(_Kernel):
+    """The next token of each row of logits [b, vocab] from a random number u [b]: tokens [b] int32 and, unless
+    0, logprob [b].  temperature, top_k (int32), top_p and min_p are arrays of b values, 0 for none."""
+
+    def dispatch_into(self, ctx, logits, ld, u, tokens, logprob, b, vocab, temperature=0, top_k=0, top_p=0, min_p=0):
+        if _any_buffer(logits, u, tokens, logprob, temperature, top_k, top_p, min_p):
+            _need("SampleKernel logits", _rows(b, ld, vocab), logits)
+            _need("SampleKernel u/tokens/logprob", b, u, tokens, logprob)
+            _need("SampleKernel filters", b, temperature, top_k, top_p, min_p)
+            logits, u, tokens, logprob = _p(logits), _p(u), _p(tokens), _p(logprob)
+            temperature, top_k, top_p, min_p = _p(temperature), _p(top_k), _p(top_p), _p(min_p)
+        ctx.call("aur_sample", logits, ld, u, temperature, top_k, top_p, min_p, tokens, logprob, b, vocab)

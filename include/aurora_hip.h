@@ -237,10 +237,20 @@ int aur_mha_kv_step_batched(aur_ctx* ctx, const float* q_new,
  * that are appended to in one call share no page. */
 #define AUR_PAGED_F32 0u
 #define AUR_PAGED_BF16 1u
+/* Pools of e4m3 numbers (OCP 8-bit: 4 bits of exponent, 3 of significand, up to
+ * 448 and down to 2^-9, a NaN, no infinity), 1 byte each, with scales
+ * [n_pages, n_kv_head, page_len/scale_len] of bytes b (e8m0): an element stands
+ * for its number times 2^(b-127), for NaN where b is 255.  A scale serves scale_len tokens
+ * of a head, a power of two up to page_len and 128.  The other types have no
+ * scales and do not read these fields. */
+#define AUR_PAGED_E4M3 2u
 typedef struct {
   void* k;
   void* v;
   uint32_t n_pages, page_len, n_kv_head, d_head, dtype;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  uint32_t scale_len;
 } aur_paged_cache;
 typedef struct {
   const int32_t* tok_off;
@@ -262,11 +272,25 @@ int aur_rotary_table(aur_ctx* ctx, float* table, uint32_t n_pos, uint32_t rot_di
  * then); the table holds n_pos >= prefix_len + max_own positions.  q and q_out
  * may be one buffer of one stride (AUR_EINVAL for two), or both NULL.  bf16 pools
  * take the nearest value, ties to even.  Rows 16-byte aligned, strides multiples of 4.  A token with j < 0
- * (own_len below n_s) is skipped, q_out included. */
+ * (own_len below n_s) is skipped, q_out included.
+ * e4m3 pools: the new tokens of a block of scale_len take the least scale 2^e,
+ * e from -117 to 119, with |x| <= 448*2^e for all of them, a block that holds
+ * older tokens no less than it had; if its scale grew, those are rounded once
+ * more.  Elements are the nearest number, ties to even, beyond 448*2^119 that;
+ * an infinity or NaN is held as NaN and does not count for the scale. */
 int aur_kv_append_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,
                         const float* q, uint32_t ld_q, const float* k, const float* v,
                         uint32_t ld_kv, float* q_out, uint32_t ld_qo, const float* table,
                         uint32_t n_pos, uint32_t rot_dim, uint32_t n_head, int pairs);
+
+/* Reads keys [first, first + count) of every sequence's axis, its prefix and
+ * then its own keys, as fp32: key x of sequence s goes to row s*count + x - first
+ * of k_out and v_out [b*count, n_kv_head*d_head] (row stride ld, a multiple of 4;
+ * 16-byte aligned; either may be NULL).  Rows of keys behind a sequence's last,
+ * or in pages that are not there, become 0.  Of the batch own_len, pages and
+ * prefix_pages are read, tok_off is not and may be NULL.  Any type of pool. */
+int aur_kv_read_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,
+                      float* k_out, float* v_out, uint32_t ld, uint32_t first, uint32_t count);
 
 /* Attention of the new tokens over prefix and own keys: query token i of a
  * sequence sees the whole prefix and own keys 0 .. j.  q, out [n_tok,
@@ -293,6 +317,28 @@ size_t aur_mha_paged_ws_bytes(const aur_paged_cache* cache, const aur_paged_batc
 int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,
                   const float* q, uint32_t ld_q, float* out, uint32_t ld_o, float* lse,
                   float* scratch, size_t scratch_bytes, uint32_t n_head);
+
+/* ---- choosing the next token ------------------------------------------------
+ * The next token of each of b rows of logits [b, vocab] (row stride ld), from a
+ * random number u in [0, 1) for each.  With m the row's largest logit a token's
+ * weight is w = exp((x - m) / temperature).  In the order of falling logits,
+ * equal ones by rising index, the kept tokens are: the first top_k; of these the
+ * fewest whose weights reach top_p of the sum over the first top_k; of these the
+ * ones with w >= min_p; always the first.  tokens[r] is the least index at which
+ * the sum of the kept weights up to it, by rising index, exceeds u times their
+ * sum; logprob[r], if logprob is there, the log of its share of that sum.
+ * temperature, top_k, top_p and min_p are DEVICE arrays of b values, each may be
+ * NULL: temperature 1, no filter.  A filter is off where top_k <= 0 or >= vocab,
+ * top_p >= 1 or NaN, min_p <= 0 or NaN (above 1 it counts as 1).  temperature <= 0
+ * or NaN, top_k 1 and top_p <= 0 give the first largest logit, as greedy decoding
+ * does, with logprob 0.  u below 0 or NaN counts as 0, from 1 on as the last kept.
+ * A NaN logit counts as -inf; -inf is never chosen, and a row of nothing else gives
+ * token 0 and logprob -inf; logits of +inf share the row alone.
+ * Weights are whole multiples of 2^-F, F = 63 - ceil(log2 vocab) up to 50, so sums
+ * are exact and the same call gives the same tokens.  vocab up to 2^20 (AUR_ELIMIT). */
+int aur_sample(aur_ctx* ctx, const float* logits, uint32_t ld, const float* u,
+               const float* temperature, const int32_t* top_k, const float* top_p,
+               const float* min_p, int32_t* tokens, float* logprob, uint32_t b, uint32_t vocab);
 
 /* ---- model: DecoderTransformerGpu / KvCacheGpu ----------------------------
  * The caller of the hot path (src/gpu/transformer.rs:32-116, 949-2640),
