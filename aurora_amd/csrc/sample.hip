@@ -7,16 +7,18 @@
 // sum of the kept weights up to it, in the order of the indexes, exceeds u times their sum.
 //
 // Whether a token is kept, and which one is drawn, hangs on sums that pass a border, so these
-// have to come out the same in any order: a weight is computed in 64 bits (2^y = 2^n·2^(i/64)·e^r
-// with a table of 64 and five terms of e^r's series, |r| < 0.0055, to 2^-52) and held as a whole
-// number of units of 2^-F, F = 63 − ⌈log2 vocab⌉ up to 50, so that a row's sum stays below 2^63.
-// Whole numbers add up exactly, which lets threads and atomics add them as they come.
+// have to come out the same in any order: a weight is computed in 64 bits (2^y = 2^n·e^r, |r| <=
+// ln 2 / 2, twelve terms of e^r's series, to 2^-47) and held as a whole number of units of 2^-F,
+// F = 63 − ⌈log2 vocab⌉ up to 50, so that a row's sum stays below 2^63.  Whole numbers add up
+// exactly, which lets threads and atomics add them as they come.
 //
-// The border of top_k or top_p is found by one histogram over 1024 equal ranges of logits (each
-// range's count or weight), a scan over it, and the exact order among the tokens of the one range
-// that holds the border.  Where more than 1024 tokens lie in it, it is cut into 1024 again; a
-// range of one value alone is cut by index.
+// A block has one row, in LDS up to kStaged logits.  The border of top_k or top_p is found by one
+// histogram over 1024 equal ranges of logits below m (each range's count or weight), a scan over
+// it, and the exact order among the tokens of the one range that holds the border.  Where more
+// than kList tokens lie in it, it is cut into 1024 again; a range of one value alone is cut by index.
+// Where top_k leaves few tokens, those are compared with each other instead.
 #include "common.hpp"
+#include "lanes.hpp"
 
 #include <cmath>
 
@@ -35,57 +37,68 @@ struct SampleArgs {
 };
 
 constexpr int kBins = 1024, kList = 1024;
-constexpr int kSuper = 8;                 // chunks whose weights are added up together
+constexpr int kSuper = 8;          // chunks whose weights are added up together
 constexpr int kMaxVocab = 1 << 20;
+constexpr int kStaged = 32768;     // logits of a row in LDS
+
+struct Entry {
+  float x;
+  int i;
+  u64 w;
+};
 
 struct SampleLds {
   u64 hist[kBins];
-  u64 list_w[kList];
-  float list_x[kList];
-  int list_i[kList];
-  double pow2[64];                        // 2^(i/64)
+  __attribute__((aligned(16))) Entry list[kList];
   u64 wave[kSuper * 16];
   u64 super[kMaxVocab / (4 * 1024 * kSuper) + 1];
-  float red[2][16];
-  u64 before, total;
+  float red[16];
+  u64 before, upto;
   int bin, count, best, token;
 };
 
-__device__ __forceinline__ u64 shfl_up64(u64 x, int n) {
-  const uint32 lo = __shfl_up((uint32)x, n, 64), hi = __shfl_up((uint32)(x >> 32), n, 64);
+// Moves within a wave by DPP, 0 where there is no source lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp64(u64 x) {
+  const uint32 lo = __builtin_amdgcn_update_dpp(0, (int)(uint32)x, CTRL, ROWS, 0xf, false);
+  const uint32 hi = __builtin_amdgcn_update_dpp(0, (int)(uint32)(x >> 32), CTRL, ROWS, 0xf, false);
   return (u64)hi << 32 | lo;
 }
-__device__ __forceinline__ u64 shfl_xor64(u64 x, int n) {
-  const uint32 lo = __shfl_xor((uint32)x, n, 64), hi = __shfl_xor((uint32)(x >> 32), n, 64);
-  return (u64)hi << 32 | lo;
+__device__ __forceinline__ u64 lane64(u64 x, int lane) {
+  return (u64)(uint32)__builtin_amdgcn_readlane((int)(uint32)(x >> 32), lane) << 32 |
+         (uint32)__builtin_amdgcn_readlane((int)(uint32)x, lane);
 }
-__device__ __forceinline__ u64 wave_sum(u64 x) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) x += shfl_xor64(x, o);
+// The sum of the lanes up to this one: within rows of 16 lanes, then rows 0 and 2 to the next one, then the
+// first half to the second.
+__device__ __forceinline__ u64 wave_scan(u64 x) {
+  x += dpp64<0x111, 0xf>(x);
+  x += dpp64<0x112, 0xf>(x);
+  x += dpp64<0x114, 0xf>(x);
+  x += dpp64<0x118, 0xf>(x);
+  x += dpp64<0x142, 0xa>(x);
+  x += dpp64<0x143, 0xc>(x);
   return x;
 }
-__device__ __forceinline__ u64 wave_scan(u64 x) {  // of the lanes up to this one
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const u64 y = shfl_up64(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
+__device__ __forceinline__ u64 wave_sum(u64 x) { return lane64(wave_scan(x), 63); }
+__device__ __forceinline__ u64 quad_sum(u64 x) {  // of four neighbouring lanes
+  x += dpp64<0xb1, 0xf>(x);
+  return x + dpp64<0x4e, 0xf>(x);
 }
 
-// One row.  TH threads; the row lies in NCH chunks of 4 * TH logits in registers, or for NCH = 0 is read
-// again in each pass.
-template <int TH, int NCH>
+// The order of falling logits, equal ones by rising index.
+__device__ __forceinline__ bool before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
+
+// One row of TH threads, in chunks of 4 * TH logits: in LDS (ROW > 0), or read again in each pass.
+template <int TH, int ROW>
 struct Row {
+  static constexpr int NW = TH / 64;
   const SampleArgs& a;
   SampleLds& lds;
+  floatx4* held;  // the row in LDS
   const float* x;
   int n_chunks;
-  floatx4 held[NCH ? NCH : 1];
-  double scale;  // log2(e) / T
-  float m;
-  int frac;
+  double scale, inv_t;  // log2(e) / T, 1 / T
+  float m, T;
   bool infinite;  // the largest logit is +∞: such ones count as 0, all others as −∞
 
   __device__ __forceinline__ floatx4 ordinary(floatx4 v) const {
@@ -108,90 +121,105 @@ struct Row {
     for (int e = 0; e < 4; ++e) v[e] = v[e] == v[e] ? v[e] : -INFINITY;
     return infinite ? ordinary(v) : v;
   }
-  // f(index of the first, four logits) for every chunk from c0 on.
+  // f(chunk, index of the first, four logits) for the chunks from c0 up to c1.
   template <class F>
-  __device__ __forceinline__ void each(int c0, int c1, F f) {
-    if constexpr (NCH > 0) {
-#pragma unroll
-      for (int c = 0; c < NCH; ++c)
-        if (c >= c0 && c < c1) f(c, 4 * (c * TH + (int)threadIdx.x), held[c]);
-    } else {
-      for (int c = c0; c < c1; ++c) f(c, 4 * (c * TH + (int)threadIdx.x), load(c));
-    }
+  __device__ __forceinline__ void each(int c0, int c1, F f) const {
+    for (int c = c0; c < c1; ++c) f(c, 4 * (c * TH + (int)threadIdx.x), ROW ? held[c * TH + threadIdx.x] : load(c));
   }
 
   // The weight of logit v in units of 2^-frac, to the nearest.
   __device__ __forceinline__ u64 weight(float v) const {
-    if (v == -INFINITY) return 0;
-    if (v == m) return 1ull << frac;
-    const double y = ((double)v - (double)m) * (scale * 64.0);  // in 64ths
-    if (!(y > -64.0 * 64.0)) return 0;
-    const double n = __builtin_rint(y), r = (y - n) * 0.010830424696249145;  // ln 2 / 64
-    const int k = (int)n;
-    double p = 1.0 / 120.0;
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    const u64 bits = (u64)__double_as_longlong(p * lds.pow2[k & 63]);
-    const int shift = 52 - frac - (k >> 6) - ((int)(bits >> 52) - 1023);  // above 0: the weight is at most 1
-    const u64 mant = (bits & 0xfffffffffffffull) | 0x10000000000000ull;
-    return shift > 54 ? 0 : ((mant >> (shift - 1)) + 1) >> 1;
+    const double y = fmax(((double)v - (double)m) * scale, -2000.0);
+    const double n = __builtin_rint(y), r = (y - n) * 0.6931471805599453;
+    double p = 1.0 / 39916800.0;
+#define AUR_TERM(k) p = __builtin_fma(p, r, 1.0 / k)
+    AUR_TERM(3628800.0);
+    AUR_TERM(362880.0);
+    AUR_TERM(40320.0);
+    AUR_TERM(5040.0);
+    AUR_TERM(720.0);
+    AUR_TERM(120.0);
+    AUR_TERM(24.0);
+    AUR_TERM(6.0);
+    AUR_TERM(2.0);
+    AUR_TERM(1.0);
+    AUR_TERM(1.0);
+#undef AUR_TERM
+    p = __builtin_rint(ldexp(p, (int)n + a.frac));  // up to 2^50
+    const double hi = __builtin_floor(p * 0x1p-32);
+    return (u64)(uint32)hi << 32 | (uint32)__builtin_fma(hi, -0x1p32, p);
   }
 
   __device__ __forceinline__ float block_max(float v) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) v = fmaxf(v, __shfl_xor(v, o, 64));
+    v = aurlanes::group_reduce<1, 64, true>(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds.red[0][threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) lds.red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = lds.red[0][0];
+    v = lds.red[0];
 #pragma unroll
-    for (int w = 1; w < TH / 64; ++w) v = fmaxf(v, lds.red[0][w]);
+    for (int w = 1; w < NW; ++w) v = fmaxf(v, lds.red[w]);
     return v;
   }
 
-  // Weights f(index, logit) added up by groups of kSuper chunks; their sum.
-  template <class F>
-  __device__ __forceinline__ u64 add_up(F f) {
-    const int n = (n_chunks + kSuper - 1) / kSuper;
-    __syncthreads();
-    for (int s = threadIdx.x; s < n; s += TH) lds.super[s] = 0;
-    __syncthreads();
-    for (int s = 0; s < n; ++s) {
-      u64 sum = 0;
-      each(s * kSuper, min((s + 1) * kSuper, n_chunks), [&](int, int i, floatx4 v) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += f(i + e, v[e]);
-      });
-      sum = wave_sum(sum);
-      if ((threadIdx.x & 63) == 0) atomicAdd(&lds.super[s], sum);
-    }
-    __syncthreads();
-    u64 total = 0;
-    for (int s = 0; s < n; ++s) total += lds.super[s];
-    return total;
+  // The entry of sums[0 .. n), n <= 128, at which they exceed r; r becomes what is left of it there.  `all` is
+  // their sum.  Every wave finds it by itself.
+  __device__ __forceinline__ int locate(const u64* sums, int n, u64& r) const {
+    const int lane = threadIdx.x & 63;
+    const u64 s0 = 2 * lane < n ? sums[2 * lane] : 0, s1 = 2 * lane + 1 < n ? sums[2 * lane + 1] : 0;
+    const u64 up = wave_scan(s0 + s1) - s0 - s1;
+    const bool here = up <= r && r < up + s0 + s1, second = r >= up + s0;
+    const int at = __builtin_ctzll(__ballot(here));
+    const u64 rest = lane64(r - up - (second ? s0 : 0), at);
+    const int odd = (int)(__ballot(second) >> at & 1);
+    r = rest;
+    return 2 * at + odd;
   }
-  // The least index at which the sum of add_up's weights up to it exceeds r (r below their sum).
+  __device__ __forceinline__ u64 sum_of(const u64* sums, int n) const {
+    const int lane = threadIdx.x & 63;
+    return wave_sum((2 * lane < n ? sums[2 * lane] : 0) + (2 * lane + 1 < n ? sums[2 * lane + 1] : 0));
+  }
+  // The weights f(index, logit) of the chunks from c0 up to c1, kSuper at most, added up by waves.
   template <class F>
-  __device__ __forceinline__ int at_sum(u64 r, F f) {
-    constexpr int NW = TH / 64;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int s = 0;
-    while (lds.super[s] <= r) r -= lds.super[s++];
-    __syncthreads();
-    const int c0 = s * kSuper, c1 = min(c0 + kSuper, n_chunks);
+  __device__ __forceinline__ void sum_waves(int c0, int c1, F f) {
     each(c0, c1, [&](int c, int i, floatx4 v) {
       u64 sum = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum += f(i + e, v[e]);
       sum = wave_sum(sum);
-      if (lane == 0) lds.wave[(c - c0) * NW + w] = sum;
+      if ((threadIdx.x & 63) == 0) lds.wave[(c - c0) * NW + (threadIdx.x >> 6)] = sum;
     });
     __syncthreads();
-    int at = 0;
-    while (lds.wave[at] <= r) r -= lds.wave[at++];
+  }
+  // The least index at which the sum of the weights f(index, logit) up to it exceeds place(their sum).
+  template <class F, class G>
+  __device__ __forceinline__ int pick(F f, G place, u64& total) {
+    const int w = threadIdx.x >> 6, n = (n_chunks + kSuper - 1) / kSuper;
+    u64 r;
+    int c0 = 0;
+    __syncthreads();
+    if (n == 1) {
+      sum_waves(0, n_chunks, f);
+      total = sum_of(lds.wave, n_chunks * NW);
+      r = place(total);
+    } else {
+      for (int s = threadIdx.x; s < n; s += TH) lds.super[s] = 0;
+      __syncthreads();
+      for (int s = 0; s < n; ++s) {
+        u64 sum = 0;
+        each(s * kSuper, min((s + 1) * kSuper, n_chunks), [&](int, int i, floatx4 v) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum += f(i + e, v[e]);
+        });
+        sum = wave_sum(sum);
+        if ((threadIdx.x & 63) == 0) atomicAdd(&lds.super[s], sum);
+      }
+      __syncthreads();
+      total = sum_of(lds.super, n);
+      r = place(total);
+      c0 = locate(lds.super, n, r) * kSuper;
+      sum_waves(c0, min(c0 + kSuper, n_chunks), f);
+    }
+    const int at = locate(lds.wave, min(kSuper, n_chunks - c0) * NW, r);
     if (w == at % NW)
       each(c0 + at / NW, c0 + at / NW + 1, [&](int, int i, floatx4 v) {
         u64 t[4];
@@ -208,114 +236,191 @@ struct Row {
     return lds.token;
   }
 
-  // Of the order of falling logits, rising indexes: the place at which the sum of weights f(logit) reaches
-  // `target` (above 0), as its logit and index.  False: all of them come to less.
-  template <class F>
-  __device__ __forceinline__ bool reach(u64 target, float least, F f, float& at_x, int& at_i) {
+  // Of the order of falling logits, rising indexes: the place at which the sum of weights f(index, logit)
+  // reaches target(the sum of all), as its logit and index: 1.  There is none: 0.  f is the same for equal
+  // logits, but for a last part of them in the order that has none.
+  // few > 0: where that place's range and all above it hold no more than `few` tokens of a weight, these go
+  // into the list, lds.count of them: 2.
+  template <class F, class G>
+  __device__ __forceinline__ int reach(F f, G target_of, int few, float& at_x, int& at_i) {
+    using W = decltype(f(0, 0.f));
     constexpr int PER = kBins / TH;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    float lo = least, hi = m;
-    for (;;) {
-      // (in 64 bits, where no difference of two logits is lost: hi and lo never share a range)
-      const double inv = kBins / ((double)hi - (double)lo);
-      auto bin_of = [&](float v) { return min((int)(((double)hi - (double)v) * inv), kBins - 1); };
+    W* const hist = reinterpret_cast<W*>(lds.hist);
+    // the first ranges end where weights do; all below them share the last one
+    double hi = m, inv = kBins / (32.0 * (double)T);
+    float lo = -INFINITY;
+    u64 target = 0;
+    for (bool first = true;; first = false) {
+      auto bin_of = [&](float v) { return (int)fmin((hi - (double)v) * inv, kBins - 1.0); };
+      auto in = [&](float v) { return v > -INFINITY && v >= lo && (double)v <= hi; };
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < PER; ++i) lds.hist[tid + TH * i] = 0;
+      for (int i = 0; i < PER; ++i) hist[tid + TH * i] = 0;
       if (tid == 0) lds.bin = -1, lds.count = 0;
       __syncthreads();
-      each(0, n_chunks, [&](int, int, floatx4 v) {
+      each(0, n_chunks, [&](int, int i, floatx4 v) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (v[e] >= lo && v[e] <= hi) {
-            const u64 x = f(v[e]);
-            if (x) atomicAdd(&lds.hist[hi == lo ? 0 : bin_of(v[e])], x);
+          if (in(v[e])) {
+            const W x = f(i + e, v[e]);
+            if (x) atomicAdd(&hist[bin_of(v[e])], x);
           }
       });
       __syncthreads();
       u64 own[PER], sum = 0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sum += own[i] = lds.hist[PER * tid + i];
+      for (int i = 0; i < PER; ++i) sum += own[i] = hist[PER * tid + i];
       u64 up = wave_scan(sum);
       if (lane == 63) lds.wave[w] = up;
       __syncthreads();
       up -= sum;
-      for (int i = 0; i < w; ++i) up += lds.wave[i];
+      u64 all = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        if (i < w) up += lds.wave[i];
+        all += lds.wave[i];
+      }
+      if (first) target = target_of(all);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        if (up < target && target <= up + own[i]) lds.bin = PER * tid + i, lds.before = up;
+        if (up < target && target <= up + own[i]) lds.bin = PER * tid + i, lds.before = up, lds.upto = up + own[i];
         up += own[i];
       }
       __syncthreads();
       const int bin = lds.bin;
-      if (bin < 0) return false;
+      if (bin < 0) return 0;
       target -= lds.before;
+      if (first && lds.upto <= (u64)few) {  // (weights of one each: f counts)
+        each(0, n_chunks, [&](int, int i, floatx4 v) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (in(v[e]) && bin_of(v[e]) <= bin) lds.list[atomicAdd(&lds.count, 1)] = Entry{v[e], i + e, 0};
+        });
+        __syncthreads();
+        return 2;
+      }
       float most = -INFINITY, fewest = INFINITY;
       each(0, n_chunks, [&](int, int i, floatx4 v) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (v[e] >= lo && v[e] <= hi && (hi == lo || bin_of(v[e]) == bin)) {
+          if (in(v[e]) && bin_of(v[e]) == bin) {
             most = fmaxf(most, v[e]);
             fewest = fminf(fewest, v[e]);
             const int n = atomicAdd(&lds.count, 1);
-            if (n < kList) lds.list_x[n] = v[e], lds.list_i[n] = i + e;
+            if (n < kList) lds.list[n] = Entry{v[e], i + e, f(i + e, v[e])};
           }
       });
       __syncthreads();
       const int n = lds.count;
       if (n <= kList) {
-        for (int i = tid; i < n; i += TH) lds.list_w[i] = f(lds.list_x[i]);
-        __syncthreads();
         for (int i = tid; i < n; i += TH) {
-          const float v = lds.list_x[i];
-          const int index = lds.list_i[i];
-          u64 up = 0;
-          for (int j = 0; j < n; ++j)
-            if (lds.list_x[j] > v || (lds.list_x[j] == v && lds.list_i[j] < index)) up += lds.list_w[j];
-          if (up < target && target <= up + lds.list_w[i]) lds.best = i;
+          const Entry own_e = lds.list[i];
+          u64 sum_before = 0;
+#pragma unroll 4
+          for (int j = 0; j < n; ++j) {
+            const Entry o = lds.list[j];
+            sum_before += before(o.x, o.i, own_e.x, own_e.i) ? o.w : 0;
+          }
+          if (sum_before < target && target <= sum_before + own_e.w) lds.best = i;
         }
         __syncthreads();
-        at_x = lds.list_x[lds.best];
-        at_i = lds.list_i[lds.best];
-        return true;
+        at_x = lds.list[lds.best].x;
+        at_i = lds.list[lds.best].i;
+        return 1;
       }
-      hi = block_max(most);
+      const float top = block_max(most);
       lo = -block_max(-fewest);
-      if (lo == hi) {  // one value: its tokens in the order of their indexes
-        const u64 one = f(lo);
+      if (lo == top) {  // one value: its tokens in the order of their indexes
         const float v = lo;
-        auto same = [v](int, float y) { return (u64)(y == v); };
-        add_up(same);
+        const u64 one = f(0, v);
+        u64 none;
         at_x = v;
-        at_i = at_sum((target + one - 1) / one - 1, same);
-        return true;
+        at_i = pick([v](int, float y) { return (u64)(y == v); }, [&](u64) { return (target + one - 1) / one - 1; }, none);
+        return 1;
       }
+      // (in 64 bits, where no difference of two logits is lost: lo and hi never share a range)
+      hi = top;
+      inv = kBins / (hi - (double)lo);
+    }
+  }
+
+  // The choice among the n <= TH / 4 tokens in the list, the first k of which count.  Four threads have a token.
+  __device__ __forceinline__ void choose_few(int r, int n, int k, float p, double floor_y) {
+    const int e = threadIdx.x >> 2, part = threadIdx.x & 3;
+    const bool on = e < n;
+    Entry own{-INFINITY, 0x7fffffff, 0};
+    if (on) own = lds.list[e];
+    uint32 rank = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += 4) rank += before(lds.list[j].x, lds.list[j].i, own.x, own.i);
+    rank = (uint32)quad_sum(rank);
+    own.w = on && (int)rank < k ? weight(own.x) : 0;
+    if (on && part == 0) lds.list[e].w = own.w;
+    __syncthreads();
+    u64 sum = 0, ahead = 0;
+    if (p < 1.f) {
+#pragma unroll 4
+      for (int j = part; j < n; j += 4) {
+        const Entry o = lds.list[j];
+        sum += o.w;
+        ahead += before(o.x, o.i, own.x, own.i) ? o.w : 0;
+      }
+      sum = quad_sum(sum);
+      ahead = quad_sum(ahead);
+      if ((double)ahead >= (double)p * (double)sum && ahead > 0) own.w = 0;
+    }
+    if (own.x != m && !(((double)own.x - (double)m) * inv_t >= floor_y)) own.w = 0;
+    __syncthreads();
+    if (on && part == 0) lds.list[e].w = own.w;
+    __syncthreads();
+    sum = ahead = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += 4) {
+      const Entry o = lds.list[j];
+      sum += o.w;
+      ahead += o.i < own.i ? o.w : 0;
+    }
+    sum = quad_sum(sum);
+    ahead = quad_sum(ahead);
+    const u64 at = place(r, sum);
+    if (on && part == 0 && ahead <= at && at < ahead + own.w) result(r, own.i, own.x, sum);
+  }
+
+  // u times the sum, rounded down, below it.
+  __device__ __forceinline__ u64 place(int r, u64 total) const {
+    const float u = a.u[r];
+    const double want = (double)(u > 0.f ? u : 0.f) * (double)total;
+    const u64 at = want < (double)total ? (u64)want : total - 1;
+    return at < total ? at : total - 1;
+  }
+  __device__ __forceinline__ void result(int r, int token, float v, u64 total) const {
+    a.tokens[r] = token;
+    if (a.logprob) {
+      const double y = v == m ? 0.0 : ((double)v - (double)m) * inv_t;
+      a.logprob[r] = (float)(y - log(ldexp((double)total, -a.frac)));
     }
   }
 };
 
-template <int TH, int NCH>
+// ROW: 4-logit pieces of a row in LDS.
+template <int TH, int ROW>
 __global__ void __launch_bounds__(TH) sample_kernel(SampleArgs a) {
   __shared__ SampleLds lds;
+  __shared__ floatx4 held[ROW ? ROW : 1];
   const int r = blockIdx.x, tid = threadIdx.x;
-  Row<TH, NCH> row{a, lds, a.logits + (size_t)r * a.ld, (a.vocab + 4 * TH - 1) / (4 * TH)};
-  row.infinite = false;
-  if (tid < 64) lds.pow2[tid] = exp2(tid / 64.0);
+  Row<TH, ROW> row{a, lds, held, a.logits + (size_t)r * a.ld, (a.vocab + 4 * TH - 1) / (4 * TH)};
   const float T = a.temperature ? a.temperature[r] : 1.f, p = a.top_p ? a.top_p[r] : 1.f;
   const float least_p = a.min_p ? a.min_p[r] : 0.f;
-  const int k = a.top_k ? a.top_k[r] : 0;
-  float most = -INFINITY, least = INFINITY;
-  if constexpr (NCH > 0) {
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) row.held[c] = row.load(c);
+  int k = a.top_k ? a.top_k[r] : 0;
+  if (k >= a.vocab || k < 0) k = 0;
+  row.infinite = false;
+  float most = -INFINITY;
+  for (int c = 0; c < row.n_chunks; ++c) {
+    const floatx4 v = row.load(c);
+    if (ROW) held[c * TH + tid] = v;
+    most = fmaxf(fmaxf(most, fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));
   }
-  row.each(0, row.n_chunks, [&](int, int, floatx4 v) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      most = fmaxf(most, v[e]);
-      if (v[e] > -INFINITY) least = fminf(least, v[e]);
-    }
-  });
   row.m = row.block_max(most);
   if (row.m == -INFINITY) {  // nothing to choose from
     if (tid == 0) {
@@ -324,63 +429,57 @@ __global__ void __launch_bounds__(TH) sample_kernel(SampleArgs a) {
     }
     return;
   }
-  least = -row.block_max(-least);
   row.infinite = row.m == INFINITY;
   if (row.infinite) {
-    row.m = least = 0.f;
-    if constexpr (NCH > 0) {
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) row.held[c] = row.ordinary(row.held[c]);
-    }
+    row.m = 0.f;
+    if (ROW)
+      for (int c = 0; c < row.n_chunks; ++c) held[c * TH + tid] = row.ordinary(held[c * TH + tid]);
   }
-  row.frac = a.frac;
-  row.scale = 1.4426950408889634 / (double)T;
-  const bool greedy = !(T > 0.f) || k == 1 || p <= 0.f;
-
-  // The kept tokens: logits above cut_x, and at cut_x indexes up to cut_i.
-  float cut_x = -INFINITY;
-  int cut_i = 0x7fffffff;
-  auto one = [](float) { return (u64)1; };
-  if (greedy) {
+  if (!(T > 0.f) || k == 1 || p <= 0.f) {  // greedy: the first of the largest
+    int token = 0x7fffffff;
     const float m = row.m;
-    auto first = [m](int, float v) { return (u64)(v == m); };
-    row.add_up(first);
-    const int token = row.at_sum(0, first);
+    row.each(0, row.n_chunks, [&](int, int i, floatx4 v) {
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (v[e] == m) token = min(token, i + e);
+    });
+    if (tid == 0) lds.token = 0x7fffffff;
+    __syncthreads();
+    if (token != 0x7fffffff) atomicMin(&lds.token, token);
+    __syncthreads();
     if (tid == 0) {
-      a.tokens[r] = token;
+      a.tokens[r] = lds.token;
       if (a.logprob) a.logprob[r] = 0.f;
     }
     return;
   }
-  if (k > 0 && k < a.vocab) row.reach((u64)k, least, one, cut_x, cut_i);
+  row.T = T;
+  row.inv_t = 1.0 / (double)T;
+  row.scale = 1.4426950408889634 / (double)T;
+  const float m = row.m;
+  const double floor_y = least_p > 0.f ? log((double)fminf(least_p, 1.f)) : -INFINITY;
+
+  // The kept tokens: logits above cut_x, and at cut_x indexes up to cut_i.
+  float cut_x = -INFINITY;
+  int cut_i = 0x7fffffff;
+  if (k > 0 &&
+      row.reach([](int, float) { return 1u; }, [k](u64) { return (u64)k; }, TH / 4, cut_x, cut_i) == 2) {
+    row.choose_few(r, lds.count, k, p, floor_y);
+    return;
+  }
   if (p < 1.f) {
     const float kx = cut_x;
     const int ki = cut_i;
-    auto all = [&](int i, float v) { return v > kx || (v == kx && i <= ki) ? row.weight(v) : 0; };
-    const u64 mass = row.add_up(all);
-    const u64 target = (u64)fmax(ceil((double)p * (double)mass), 1.0);
-    row.reach(target, fmaxf(least, kx), [&](float v) { return row.weight(v); }, cut_x, cut_i);
+    auto all = [&](int i, float v) { return v > kx || (v == kx && i <= ki) ? row.weight(v) : (u64)0; };
+    row.reach(all, [p](u64 mass) { return (u64)fmax(ceil((double)p * (double)mass), 1.0); }, 0, cut_x, cut_i);
   }
-  // w >= min_p, of weights in 64 bits: the nearest unit's is a token's own
-  const double floor_y = least_p > 0.f ? log((double)fminf(least_p, 1.f)) : -INFINITY;
-  const double inv_t = 1.0 / (double)T;
-  const float m = row.m;
   auto kept = [&](int i, float v) {
-    const bool in = (v > cut_x || (v == cut_x && i <= cut_i)) && (v == m || ((double)v - (double)m) * inv_t >= floor_y);
-    return in ? row.weight(v) : 0;
+    const bool in = (v > cut_x || (v == cut_x && i <= cut_i)) && (v == m || ((double)v - (double)m) * row.inv_t >= floor_y);
+    return in ? row.weight(v) : (u64)0;
   };
-  const u64 total = row.add_up(kept);
-  const double want = (double)(a.u[r] > 0.f ? a.u[r] : 0.f) * (double)total;
-  const u64 at = want < (double)total ? (u64)want : total - 1;
-  const int token = row.at_sum(at < total ? at : total - 1, kept);
-  if (tid == 0) {
-    a.tokens[r] = token;
-    if (a.logprob) {
-      const float v = row.infinite ? 0.f : row.x[token];
-      const double y = v == m ? 0.0 : ((double)v - (double)m) * inv_t;
-      a.logprob[r] = (float)(y - log(ldexp((double)total, -a.frac)));
-    }
-  }
+  u64 total;
+  const int token = row.pick(kept, [&](u64 sum) { return row.place(r, sum); }, total);
+  if (tid == 0) row.result(r, token, row.infinite ? 0.f : row.x[token], total);
 }
 
 }  // namespace
@@ -400,8 +499,11 @@ extern "C" int aur_sample(aur_ctx* ctx, const float* logits, uint32_t ld, const 
   while ((1u << bits) < vocab) ++bits;
   SampleArgs a{logits, u, temperature, top_p, min_p, top_k, tokens, logprob, (int)vocab, (int)ld,
                63 - bits < 50 ? 63 - bits : 50, ld % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0};
-  auto* kernel = vocab <= 1024 ? sample_kernel<256, 1> : vocab <= 4096 ? sample_kernel<1024, 1> : sample_kernel<1024, 0>;
-  const dim3 threads(vocab <= 1024 ? 256 : 1024);
+  auto* kernel = vocab <= 256      ? sample_kernel<256, 256>
+                 : vocab <= 8192    ? sample_kernel<512, 2048>
+                 : vocab <= kStaged ? sample_kernel<1024, kStaged / 4>
+                                    : sample_kernel<1024, 0>;
+  const dim3 threads(vocab <= 256 ? 256 : vocab <= 8192 ? 512 : 1024);
   hipLaunchKernelGGL(kernel, dim3(b), threads, 0, ctx->stream, a);
   AUR_LAUNCH_CHECK(ctx, "sample_kernel");
   return 0;
