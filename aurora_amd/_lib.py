@@ -57,7 +57,8 @@ SIGNATURES: dict[str, tuple] = {
     "aur_mha_paged_ws_bytes": (C.c_size_t, [C.c_void_p, C.c_void_p, _u32]),
     "aur_mha_paged": (_i32, [_c_ctx, C.c_void_p, C.c_void_p, _f, _u32, _f, _u32, _f, _f, C.c_size_t, _u32]),
     "aur_kv_read_paged": (_i32, [_c_ctx, C.c_void_p, C.c_void_p, _f, _f, _u32, _u32, _u32]),
-    "aur_sample": (_i32, [_c_ctx, _f, _u32, _f, _f, _f, _f, _f, _f, _f, _u32, _u32]),
+    "aur_sample": (_i32, [_c_ctx, _f, _u32, _f, _f, _f, _f, _f, _f, _f, C.c_void_p, C.c_size_t, _u32, _u32]),
+    "aur_sample_ws_bytes": (C.c_size_t, [_u32, _u32]),
     "aur_model_create": (_i32, [_c_ctx, C.c_void_p, _u32, C.POINTER(C.c_void_p)]),
     "aur_model_destroy": (_i32, [C.c_void_p]),
     "aur_model_tensor": (_i32, [C.c_void_p, C.c_char_p, C.c_int32, C.c_int32,

@@ -33,13 +33,23 @@ struct SampleArgs {
   int32_t* tokens;
   float* logprob;
   int vocab, ld, frac;  // weights in units of 2^-frac
-  bool aligned;         // rows of whole 16-byte pieces
+  // Of rows that several blocks share, of each segment: the largest logit, the kept weight where no border has
+  // to be found, and the histograms.
+  int segments;
+  float* seg_max;
+  u64 *seg_mass, *mass;
+  uint32* count;
 };
 
-constexpr int kBins = 1024, kList = 1024;
+typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kBins = 1024, kList = 1024, kPairs = 64;
 constexpr int kSuper = 8;          // chunks whose weights are added up together
 constexpr int kMaxVocab = 1 << 20;
+constexpr float kLeastLogit = -3.402823466e38f;  // that can be chosen
 constexpr int kStaged = 32768;     // logits of a row in LDS
+constexpr int kSegment = 16384;    // … of a block, where several share a row
+constexpr int kMaxSegments = kMaxVocab / kSegment;
 
 struct Entry {
   float x;
@@ -49,9 +59,9 @@ struct Entry {
 
 struct SampleLds {
   u64 hist[kBins];
-  __attribute__((aligned(16))) Entry list[kList];
+  __attribute__((aligned(16))) Entry list[kList], pairs[kPairs];
   u64 wave[kSuper * 16];
-  u64 super[kMaxVocab / (4 * 1024 * kSuper) + 1];
+  u64 super[kMaxSegments];
   float red[16];
   u64 before, upto;
   int bin, count, best, token;
@@ -88,6 +98,81 @@ __device__ __forceinline__ u64 quad_sum(u64 x) {  // of four neighbouring lanes
 // The order of falling logits, equal ones by rising index.
 __device__ __forceinline__ bool before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
+// To the nearest whole number by adding 1.5·2^52, whose sum has it in its last bits.
+constexpr double kWhole = 6755399441055744.0;
+__device__ __forceinline__ int low32(double x) { return (int)(uint32)__double_as_longlong(x); }
+
+// The weight of logit v in units of 2^-frac, to the nearest; scale is log2(e) / T.  No instruction of it runs at
+// less than the rate of the others: conversions and powers of two are sums and moves of bits.
+__device__ __forceinline__ u64 weight_of(float v, float m, double scale, int frac) {
+  const double y = fmax(((double)v - (double)m) * scale, -2000.0);
+  const double t = y + kWhole, r = y - (t - kWhole);  // 2^y = 2^n·2^r, |r| <= 1/2
+  constexpr double l = 0.6931471805599453;
+  constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7,
+                   c8 = c7 * l / 8, c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
+  double p = c11;
+  p = __builtin_fma(p, r, c10);
+  p = __builtin_fma(p, r, c9);
+  p = __builtin_fma(p, r, c8);
+  p = __builtin_fma(p, r, c7);
+  p = __builtin_fma(p, r, c6);
+  p = __builtin_fma(p, r, c5);
+  p = __builtin_fma(p, r, c4);
+  p = __builtin_fma(p, r, c3);
+  p = __builtin_fma(p, r, c2);
+  p = __builtin_fma(p, r, l);
+  p = __builtin_fma(p, r, 1.0);
+  // times 2^(n + frac), at least 2^-2 (which rounds to nothing), to the nearest below 2^52
+  const u64 up = (u64)(uint32)max(low32(t) + frac, -2) << 52;
+  const double w = __longlong_as_double((long long)((u64)__double_as_longlong(p) + up)) + 0x1p52;
+  return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+}
+
+// The first ranges of a histogram: kBins of them down to where weights end; all below share the last one.
+struct Ranges {
+  double hi, inv;
+  __device__ __forceinline__ int of(float v) const { return low32(fmin((hi - (double)v) * inv, kBins - 1.0) + kWhole); }
+  // The least logit of the ranges 0 .. bin.
+  __device__ __forceinline__ float edge(int bin) const {
+    if (bin >= kBins - 1) return kLeastLogit;
+    const double c = hi - (bin + 0.5) / inv;
+    float v = c > kLeastLogit ? fminf((float)c, (float)hi) : kLeastLogit;
+    while (of(v) > bin) v = nextafterf(v, INFINITY);
+    while (v > kLeastLogit && of(nextafterf(v, -INFINITY)) <= bin) v = nextafterf(v, -INFINITY);
+    return v;
+  }
+};
+__device__ __forceinline__ Ranges first_ranges(float m, float T) { return {m, kBins / (32.0 * (double)T)}; }
+
+// A row's filters, those that do nothing as values that say so (k = 0, p = 1, floor_y = −∞).
+struct Filters {
+  float T, p;
+  int k;
+  double floor_y;  // log min_p: kept tokens have (x − m) / T >= floor_y
+  __device__ __forceinline__ Filters(const SampleArgs& a, int r) {
+    T = a.temperature ? a.temperature[r] : 1.f;
+    p = a.top_p ? a.top_p[r] : 1.f;
+    if (!(p < 1.f)) p = 1.f;
+    k = a.top_k ? a.top_k[r] : 0;
+    if (k >= a.vocab || k < 0) k = 0;
+    const float least_p = a.min_p ? a.min_p[r] : 0.f;
+    floor_y = least_p > 0.f ? log((double)fminf(least_p, 1.f)) : -INFINITY;
+  }
+  // The least logit that min_p keeps of a row with the largest one m.
+  __device__ __forceinline__ float least(float m) const {
+    if (floor_y == -INFINITY) return -INFINITY;
+    const double inv_t = 1.0 / (double)T, c = (double)m + (double)T * floor_y;
+    auto passes = [&](float v) { return v >= m || ((double)v - (double)m) * inv_t >= floor_y; };
+    float v = c > kLeastLogit ? fminf((float)c, m) : kLeastLogit;
+    while (!passes(v)) v = nextafterf(v, INFINITY);
+    while (v > kLeastLogit && passes(nextafterf(v, -INFINITY))) v = nextafterf(v, -INFINITY);
+    return v;
+  }
+  __device__ __forceinline__ bool greedy() const { return !(T > 0.f) || k == 1 || p <= 0.f; }
+};
+
+__device__ __forceinline__ u64 p_target(float p, u64 mass) { return (u64)fmax(ceil((double)p * (double)mass), 1.0); }
+
 // One row of TH threads, in chunks of 4 * TH logits: in LDS (ROW > 0), or read again in each pass.
 template <int TH, int ROW>
 struct Row {
@@ -101,22 +186,46 @@ struct Row {
   float m, T;
   bool infinite;  // the largest logit is +∞: such ones count as 0, all others as −∞
 
+  __device__ __forceinline__ Row(const SampleArgs& a, SampleLds& lds, floatx4* held, int r)
+      : a(a), lds(lds), held(held), x(a.logits + (size_t)r * a.ld), n_chunks((a.vocab + 4 * TH - 1) / (4 * TH)),
+        infinite(false) {}
+  __device__ __forceinline__ void take(float most, float t) {
+    infinite = most == INFINITY;
+    m = infinite ? 0.f : most;
+    T = t;
+    inv_t = 1.0 / (double)T;
+    scale = 1.4426950408889634 / (double)T;
+  }
+
   __device__ __forceinline__ floatx4 ordinary(floatx4 v) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = v[e] == INFINITY ? 0.f : -INFINITY;
     return v;
   }
-  // A logit that is NaN counts as −∞, and so does what lies behind the row.
-  __device__ __forceinline__ floatx4 load(int c) const {
+  // Chunk c as it lies in memory (rows need not be aligned); −∞ behind the row.
+  __device__ __forceinline__ floatx4 raw(int c) const {
     const int i = 4 * (c * TH + threadIdx.x);
+    if (4 * TH * (c + 1) <= a.vocab) return *reinterpret_cast<const floatx4_any*>(x + i);
     floatx4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    if (a.aligned && i + 3 < a.vocab) {
-      v = *reinterpret_cast<const floatx4*>(x + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < a.vocab) v[e] = x[i + e];
+    return v;
+  }
+  // N chunks from c on, their loads under way together.
+  template <int N>
+  __device__ __forceinline__ void raw(int c, floatx4 (&v)[N]) const {
+    if (4 * TH * (c + N) <= a.vocab) {
+      const floatx4_any* p = reinterpret_cast<const floatx4_any*>(x) + c * TH + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = p[i * TH];
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i + e < a.vocab) v[e] = x[i + e];
+      for (int i = 0; i < N; ++i) v[i] = raw(c + i);
     }
+  }
+  // A logit that is NaN counts as −∞.
+  __device__ __forceinline__ floatx4 clean(floatx4 v) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = v[e] == v[e] ? v[e] : -INFINITY;
     return infinite ? ordinary(v) : v;
@@ -124,31 +233,15 @@ struct Row {
   // f(chunk, index of the first, four logits) for the chunks from c0 up to c1.
   template <class F>
   __device__ __forceinline__ void each(int c0, int c1, F f) const {
-    for (int c = c0; c < c1; ++c) f(c, 4 * (c * TH + (int)threadIdx.x), ROW ? held[c * TH + threadIdx.x] : load(c));
+    floatx4 next = ROW ? floatx4{} : raw(c0);
+    for (int c = c0; c < c1; ++c) {
+      const floatx4 v = ROW ? held[c * TH + threadIdx.x] : clean(next);
+      if (!ROW && c + 1 < c1) next = raw(c + 1);
+      f(c, 4 * (c * TH + (int)threadIdx.x), v);
+    }
   }
 
-  // The weight of logit v in units of 2^-frac, to the nearest.
-  __device__ __forceinline__ u64 weight(float v) const {
-    const double y = fmax(((double)v - (double)m) * scale, -2000.0);
-    const double n = __builtin_rint(y), r = (y - n) * 0.6931471805599453;
-    double p = 1.0 / 39916800.0;
-#define AUR_TERM(k) p = __builtin_fma(p, r, 1.0 / k)
-    AUR_TERM(3628800.0);
-    AUR_TERM(362880.0);
-    AUR_TERM(40320.0);
-    AUR_TERM(5040.0);
-    AUR_TERM(720.0);
-    AUR_TERM(120.0);
-    AUR_TERM(24.0);
-    AUR_TERM(6.0);
-    AUR_TERM(2.0);
-    AUR_TERM(1.0);
-    AUR_TERM(1.0);
-#undef AUR_TERM
-    p = __builtin_rint(ldexp(p, (int)n + a.frac));  // up to 2^50
-    const double hi = __builtin_floor(p * 0x1p-32);
-    return (u64)(uint32)hi << 32 | (uint32)__builtin_fma(hi, -0x1p32, p);
-  }
+  __device__ __forceinline__ u64 weight(float v) const { return weight_of(v, m, scale, a.frac); }
 
   __device__ __forceinline__ float block_max(float v) {
     v = aurlanes::group_reduce<1, 64, true>(v);
@@ -159,6 +252,22 @@ struct Row {
 #pragma unroll
     for (int w = 1; w < NW; ++w) v = fmaxf(v, lds.red[w]);
     return v;
+  }
+
+  // The first index of logit v in the chunks from c0 up to c1.
+  __device__ __forceinline__ int first_of(float v, int c0, int c1) {
+    int token = 0x7fffffff;
+    each(c0, c1, [&](int, int i, floatx4 y) {
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (y[e] == v) token = min(token, i + e);
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) lds.token = 0x7fffffff;
+    __syncthreads();
+    if (token != 0x7fffffff) atomicMin(&lds.token, token);
+    __syncthreads();
+    return lds.token;
   }
 
   // The entry of sums[0 .. n), n <= 128, at which they exceed r; r becomes what is left of it there.  `all` is
@@ -193,7 +302,7 @@ struct Row {
   // The least index at which the sum of the weights f(index, logit) up to it exceeds place(their sum).
   template <class F, class G>
   __device__ __forceinline__ int pick(F f, G place, u64& total) {
-    const int w = threadIdx.x >> 6, n = (n_chunks + kSuper - 1) / kSuper;
+    const int n = (n_chunks + kSuper - 1) / kSuper;
     u64 r;
     int c0 = 0;
     __syncthreads();
@@ -219,7 +328,13 @@ struct Row {
       c0 = locate(lds.super, n, r) * kSuper;
       sum_waves(c0, min(c0 + kSuper, n_chunks), f);
     }
-    const int at = locate(lds.wave, min(kSuper, n_chunks - c0) * NW, r);
+    return pick_in(c0, min(c0 + kSuper, n_chunks), r, f);
+  }
+  // … at which what sum_waves added up from chunk c0 on exceeds r.
+  template <class F>
+  __device__ __forceinline__ int pick_in(int c0, int c1, u64 r, F f) {
+    const int w = threadIdx.x >> 6;
+    const int at = locate(lds.wave, (c1 - c0) * NW, r);
     if (w == at % NW)
       each(c0 + at / NW, c0 + at / NW + 1, [&](int, int i, floatx4 v) {
         u64 t[4];
@@ -236,6 +351,125 @@ struct Row {
     return lds.token;
   }
 
+  // Of the n <= kPairs entries in `list`, compared with each other, the one at which the sum of f(entry), in the
+  // order of falling logits, rising indexes, reaches the target (which it does).  Four threads have an entry.
+  template <class F>
+  __device__ __forceinline__ Entry reach_in_pairs(const Entry* list, int n, u64 target, F f) {
+    const int e = threadIdx.x >> 2;
+    const Entry own = list[min(e, n - 1)];
+    u64 ahead = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x & 3; j < n; j += 4) {
+      const Entry o = list[j];
+      ahead += before(o.x, o.i, own.x, own.i) ? f(o) : 0;
+    }
+    ahead = quad_sum(ahead);
+    if (e < n && ahead < target && target <= ahead + f(own)) lds.best = e;
+    __syncthreads();
+    return list[lds.best];
+  }
+  // The same of the n <= kList entries in lds.list, all of them in one range: by kBins parts of it, or where one
+  // part holds more than kPairs (many equal ones), all with each other.
+  template <class F>
+  __device__ __forceinline__ Entry reach_in_list(int n, u64 target, F f, const Ranges& ranges, int bin) {
+    constexpr int PER = kList / TH;
+    const int tid = threadIdx.x;
+    if (n <= kPairs) return reach_in_pairs(lds.list, n, target, f);
+    const Ranges part{ranges.hi - (bin - 0.5) / ranges.inv, ranges.inv * kBins};
+    clear();
+    int at[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      at[i] = -1;
+      if (tid + TH * i < n) {
+        const Entry e = lds.list[tid + TH * i];
+        at[i] = max(part.of(e.x), 0);
+        atomicAdd(&lds.hist[at[i]], f(e));
+      }
+    }
+    __syncthreads();
+    find(lds.hist, [&](u64) { return target; });
+    const int here = lds.bin;
+    const u64 rest = target - lds.before;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (at[i] == here) {
+        const int k = atomicAdd(&lds.count, 1);
+        if (k < kPairs) lds.pairs[k] = lds.list[tid + TH * i];
+      }
+    __syncthreads();
+    if (lds.count <= kPairs) return reach_in_pairs(lds.pairs, lds.count, rest, f);
+    for (int i = tid; i < n; i += TH) {
+      const Entry own = lds.list[i];
+      u64 ahead = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) ahead += before(lds.list[j].x, lds.list[j].i, own.x, own.i) ? f(lds.list[j]) : 0;
+      if (ahead < target && target <= ahead + f(own)) lds.best = i;
+    }
+    __syncthreads();
+    return lds.list[lds.best];
+  }
+  // An empty histogram, list and answer.
+  __device__ __forceinline__ void clear() {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBins / TH; ++i) lds.hist[threadIdx.x + TH * i] = 0;
+    if (threadIdx.x == 0) lds.bin = -1, lds.count = 0;
+    __syncthreads();
+  }
+  // The range at which the sum over the ranges reaches target(their sum), which is returned: lds.bin (left as it
+  // is where there is none), the sums before it and with it lds.before and lds.upto.
+  template <class W, class G>
+  __device__ __forceinline__ u64 find(const W* hist, G target_of) {
+    constexpr int PER = kBins / TH;
+    const int tid = threadIdx.x, w = tid >> 6;
+    u64 own[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += own[i] = hist[PER * tid + i];
+    u64 up = wave_scan(sum);
+    if ((tid & 63) == 63) lds.wave[w] = up;
+    __syncthreads();
+    up -= sum;
+    u64 all = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if (i < w) up += lds.wave[i];
+      all += lds.wave[i];
+    }
+    const u64 target = target_of(all);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (up < target && target <= up + own[i]) lds.bin = PER * tid + i, lds.before = up, lds.upto = up + own[i];
+      up += own[i];
+    }
+    __syncthreads();
+    return target;
+  }
+  // The tokens of least <= logit < end (of all from least on where end is −∞) in the list: their number,
+  // of which the list holds the first kList.
+  __device__ __forceinline__ int gather(float least, float end) {
+    constexpr int AT_ONCE = 8;
+    __syncthreads();
+    if (threadIdx.x == 0) lds.count = 0;
+    __syncthreads();
+    for (int c = 0; c < n_chunks; c += AT_ONCE) {
+      floatx4 v[AT_ONCE];
+      raw(c, v);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) v[i] = clean(v[i]);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v[i][e] >= least && (v[i][e] < end || end == -INFINITY)) {
+            const int n = atomicAdd(&lds.count, 1);
+            if (n < kList) lds.list[n] = Entry{v[i][e], 4 * ((c + i) * TH + (int)threadIdx.x) + e, weight(v[i][e])};
+          }
+    }
+    __syncthreads();
+    return lds.count;
+  }
+
   // Of the order of falling logits, rising indexes: the place at which the sum of weights f(index, logit)
   // reaches target(the sum of all), as its logit and index: 1.  There is none: 0.  f is the same for equal
   // logits, but for a last part of them in the order that has none.
@@ -244,21 +478,15 @@ struct Row {
   template <class F, class G>
   __device__ __forceinline__ int reach(F f, G target_of, int few, float& at_x, int& at_i) {
     using W = decltype(f(0, 0.f));
-    constexpr int PER = kBins / TH;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     W* const hist = reinterpret_cast<W*>(lds.hist);
     // the first ranges end where weights do; all below them share the last one
-    double hi = m, inv = kBins / (32.0 * (double)T);
+    Ranges ranges = first_ranges(m, T);
     float lo = -INFINITY;
     u64 target = 0;
     for (bool first = true;; first = false) {
-      auto bin_of = [&](float v) { return (int)fmin((hi - (double)v) * inv, kBins - 1.0); };
-      auto in = [&](float v) { return v > -INFINITY && v >= lo && (double)v <= hi; };
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < PER; ++i) hist[tid + TH * i] = 0;
-      if (tid == 0) lds.bin = -1, lds.count = 0;
-      __syncthreads();
+      auto bin_of = [&](float v) { return ranges.of(v); };
+      auto in = [&](float v) { return v > -INFINITY && v >= lo && (double)v <= ranges.hi; };
+      clear();
       each(0, n_chunks, [&](int, int i, floatx4 v) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -268,26 +496,7 @@ struct Row {
           }
       });
       __syncthreads();
-      u64 own[PER], sum = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) sum += own[i] = hist[PER * tid + i];
-      u64 up = wave_scan(sum);
-      if (lane == 63) lds.wave[w] = up;
-      __syncthreads();
-      up -= sum;
-      u64 all = 0;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        if (i < w) up += lds.wave[i];
-        all += lds.wave[i];
-      }
-      if (first) target = target_of(all);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (up < target && target <= up + own[i]) lds.bin = PER * tid + i, lds.before = up, lds.upto = up + own[i];
-        up += own[i];
-      }
-      __syncthreads();
+      target = find(hist, [&](u64 all) { return first ? target_of(all) : target; });
       const int bin = lds.bin;
       if (bin < 0) return 0;
       target -= lds.before;
@@ -314,19 +523,9 @@ struct Row {
       __syncthreads();
       const int n = lds.count;
       if (n <= kList) {
-        for (int i = tid; i < n; i += TH) {
-          const Entry own_e = lds.list[i];
-          u64 sum_before = 0;
-#pragma unroll 4
-          for (int j = 0; j < n; ++j) {
-            const Entry o = lds.list[j];
-            sum_before += before(o.x, o.i, own_e.x, own_e.i) ? o.w : 0;
-          }
-          if (sum_before < target && target <= sum_before + own_e.w) lds.best = i;
-        }
-        __syncthreads();
-        at_x = lds.list[lds.best].x;
-        at_i = lds.list[lds.best].i;
+        const Entry at = reach_in_list(n, target, [](const Entry& e) { return e.w; }, ranges, bin);
+        at_x = at.x;
+        at_i = at.i;
         return 1;
       }
       const float top = block_max(most);
@@ -340,13 +539,12 @@ struct Row {
         return 1;
       }
       // (in 64 bits, where no difference of two logits is lost: lo and hi never share a range)
-      hi = top;
-      inv = kBins / (hi - (double)lo);
+      ranges = {top, kBins / ((double)top - (double)lo)};
     }
   }
 
   // The choice among the n <= TH / 4 tokens in the list, the first k of which count.  Four threads have a token.
-  __device__ __forceinline__ void choose_few(int r, int n, int k, float p, double floor_y) {
+  __device__ __forceinline__ void choose_few(int r, int n, int k, float p, float least) {
     const int e = threadIdx.x >> 2, part = threadIdx.x & 3;
     const bool on = e < n;
     Entry own{-INFINITY, 0x7fffffff, 0};
@@ -370,7 +568,7 @@ struct Row {
       ahead = quad_sum(ahead);
       if ((double)ahead >= (double)p * (double)sum && ahead > 0) own.w = 0;
     }
-    if (own.x != m && !(((double)own.x - (double)m) * inv_t >= floor_y)) own.w = 0;
+    if (own.x < least) own.w = 0;
     __syncthreads();
     if (on && part == 0) lds.list[e].w = own.w;
     __syncthreads();
@@ -403,106 +601,323 @@ struct Row {
   }
 };
 
+// The row's logits from cut_x on, at cut_x those of indexes up to cut_i.
+struct Cut {
+  float x;
+  int i;
+  __device__ __forceinline__ bool keeps(float v, int at) const { return v > x || (v == x && at <= i); }
+  // Of all logits from v on as well.
+  __device__ __forceinline__ bool above(float v) {
+    if (!(x < v)) return false;
+    x = v;
+    i = 0x7fffffff;
+    return true;
+  }
+};
+
+// Borders and choice by passes over the whole row.
+template <int TH, int ROW>
+__device__ __forceinline__ void choose(Row<TH, ROW>& row, const Filters& f, int r) {
+  Cut cut{-INFINITY, 0x7fffffff};
+  if (f.k > 0 &&
+      row.reach([](int, float) { return 1u; }, [&](u64) { return (u64)f.k; }, TH / 4, cut.x, cut.i) == 2) {
+    row.choose_few(r, row.lds.count, f.k, f.p, f.least(row.m));
+    return;
+  }
+  if (f.p < 1.f) {
+    const Cut by_k = cut;
+    auto all = [&](int i, float v) { return by_k.keeps(v, i) ? row.weight(v) : (u64)0; };
+    row.reach(all, [&](u64 mass) { return p_target(f.p, mass); }, 0, cut.x, cut.i);
+  }
+  cut.above(f.least(row.m));
+  auto kept = [&](int i, float v) { return cut.keeps(v, i) ? row.weight(v) : (u64)0; };
+  u64 total;
+  const int token = row.pick(kept, [&](u64 sum) { return row.place(r, sum); }, total);
+  if (threadIdx.x == 0) row.result(r, token, row.infinite ? 0.f : row.x[token], total);
+}
+
+// A row without anything to choose from; nor with a choice to make: its first largest logit.
+__device__ __forceinline__ void certain(const SampleArgs& a, int r, int token, float logprob) {
+  a.tokens[r] = token;
+  if (a.logprob) a.logprob[r] = logprob;
+}
+
 // ROW: 4-logit pieces of a row in LDS.
 template <int TH, int ROW>
 __global__ void __launch_bounds__(TH) sample_kernel(SampleArgs a) {
   __shared__ SampleLds lds;
-  __shared__ floatx4 held[ROW ? ROW : 1];
+  __shared__ floatx4 held[ROW];
   const int r = blockIdx.x, tid = threadIdx.x;
-  Row<TH, ROW> row{a, lds, held, a.logits + (size_t)r * a.ld, (a.vocab + 4 * TH - 1) / (4 * TH)};
-  const float T = a.temperature ? a.temperature[r] : 1.f, p = a.top_p ? a.top_p[r] : 1.f;
-  const float least_p = a.min_p ? a.min_p[r] : 0.f;
-  int k = a.top_k ? a.top_k[r] : 0;
-  if (k >= a.vocab || k < 0) k = 0;
-  row.infinite = false;
+  Row<TH, ROW> row(a, lds, held, r);
+  const Filters f(a, r);
   float most = -INFINITY;
-  for (int c = 0; c < row.n_chunks; ++c) {
-    const floatx4 v = row.load(c);
-    if (ROW) held[c * TH + tid] = v;
-    most = fmaxf(fmaxf(most, fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));
-  }
-  row.m = row.block_max(most);
-  if (row.m == -INFINITY) {  // nothing to choose from
-    if (tid == 0) {
-      a.tokens[r] = 0;
-      if (a.logprob) a.logprob[r] = -INFINITY;
-    }
-    return;
-  }
-  row.infinite = row.m == INFINITY;
-  if (row.infinite) {
-    row.m = 0.f;
-    if (ROW)
-      for (int c = 0; c < row.n_chunks; ++c) held[c * TH + tid] = row.ordinary(held[c * TH + tid]);
-  }
-  if (!(T > 0.f) || k == 1 || p <= 0.f) {  // greedy: the first of the largest
-    int token = 0x7fffffff;
-    const float m = row.m;
-    row.each(0, row.n_chunks, [&](int, int i, floatx4 v) {
+  constexpr int AT_ONCE = ROW / TH < 4 ? ROW / TH : 4;
+  for (int c = 0; c < row.n_chunks; c += AT_ONCE) {
+    floatx4 v[AT_ONCE];
+    row.raw(c, v);
 #pragma unroll
-      for (int e = 3; e >= 0; --e)
-        if (v[e] == m) token = min(token, i + e);
-    });
-    if (tid == 0) lds.token = 0x7fffffff;
+    for (int i = 0; i < AT_ONCE; ++i) {
+      v[i] = row.clean(v[i]);
+      held[(c + i) * TH + tid] = v[i];
+      most = fmaxf(fmaxf(most, fmaxf(v[i][0], v[i][1])), fmaxf(v[i][2], v[i][3]));
+    }
+  }
+  row.take(row.block_max(most), f.T);
+  if (row.m == -INFINITY) {
+    if (tid == 0) certain(a, r, 0, -INFINITY);
+    return;
+  }
+  if (row.infinite)
+    for (int c = 0; c < row.n_chunks; ++c) held[c * TH + tid] = row.ordinary(held[c * TH + tid]);
+  if (f.greedy()) {
+    const int token = row.first_of(row.m, 0, row.n_chunks);
+    if (tid == 0) certain(a, r, token, 0.f);
+    return;
+  }
+  choose(row, f, r);
+}
+
+// ---------------------------------------------------------------- rows that several blocks share
+
+// Three launches: the segments' largest logits; with the row's largest their histograms of counts and weights; a
+// block a row, which adds these up, collects the tokens of the one or two ranges that hold its borders from the
+// row, and goes through the weights of the one segment that the random number falls into.
+
+__global__ void __launch_bounds__(512) sample_max_kernel(SampleArgs a) {
+  __shared__ SampleLds lds;
+  const int r = blockIdx.x / a.segments, g = blockIdx.x % a.segments;
+  Row<512, 0> row(a, lds, nullptr, r);
+  floatx4 v[kSegment / 2048];
+  float most = -INFINITY;
+  row.raw(g * (kSegment / 2048), v);
+#pragma unroll
+  for (int c = 0; c < kSegment / 2048; ++c) v[c] = row.clean(v[c]);
+#pragma unroll
+  for (int c = 0; c < kSegment / 2048; ++c) most = fmaxf(fmaxf(most, fmaxf(v[c][0], v[c][1])), fmaxf(v[c][2], v[c][3]));
+  most = row.block_max(most);
+  if (threadIdx.x == 0) a.seg_max[blockIdx.x] = most;
+}
+
+__device__ __forceinline__ float row_max(const SampleArgs& a, int r) {
+  const int lane = threadIdx.x & 63;
+  return aurlanes::group_reduce<1, 64, true>(lane < a.segments ? a.seg_max[(size_t)r * a.segments + lane] : -INFINITY);
+}
+
+__global__ void __launch_bounds__(512) sample_histogram_kernel(SampleArgs a) {
+  __shared__ SampleLds lds;
+  __shared__ uint32 counts[kBins];
+  const int r = blockIdx.x / a.segments, g = blockIdx.x % a.segments, tid = threadIdx.x;
+  Row<512, 0> row(a, lds, nullptr, r);
+  floatx4 v[kSegment / 2048];
+  row.raw(g * (kSegment / 2048), v);
+  const Filters f(a, r);
+  row.take(row_max(a, r), f.T);
+  if (row.m == -INFINITY || f.greedy()) return;
+  const bool borders = f.k > 0 || f.p < 1.f;
+  for (int i = tid; i < kBins; i += 512) lds.hist[i] = counts[i] = 0;
+  __syncthreads();
+  const Ranges ranges = first_ranges(row.m, f.T);
+  const float least = f.least(row.m);
+  u64 sum = 0;
+#pragma unroll 1
+  for (int c = 0; c < kSegment / 2048; ++c) {
+    const floatx4 x = row.clean(v[0]);
+#pragma unroll
+    for (int i = 0; i + 1 < kSegment / 2048; ++i) v[i] = v[i + 1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (!(x[e] > -INFINITY)) continue;
+      const u64 w = row.weight(x[e]);
+      if (borders) {
+        const int bin = ranges.of(x[e]);
+        atomicAdd(&counts[bin], 1u);
+        if (w) atomicAdd(&lds.hist[bin], w);
+      } else if (x[e] >= least) {
+        sum += w;
+      }
+    }
+  }
+  if (borders) {
     __syncthreads();
-    if (token != 0x7fffffff) atomicMin(&lds.token, token);
-    __syncthreads();
-    if (tid == 0) {
-      a.tokens[r] = lds.token;
-      if (a.logprob) a.logprob[r] = 0.f;
+    for (int i = tid; i < kBins; i += 512) {
+      a.mass[(size_t)blockIdx.x * kBins + i] = lds.hist[i];
+      a.count[(size_t)blockIdx.x * kBins + i] = counts[i];
     }
     return;
   }
-  row.T = T;
-  row.inv_t = 1.0 / (double)T;
-  row.scale = 1.4426950408889634 / (double)T;
-  const float m = row.m;
-  const double floor_y = least_p > 0.f ? log((double)fminf(least_p, 1.f)) : -INFINITY;
+  sum = wave_sum(sum);
+  if ((tid & 63) == 0) lds.wave[tid >> 6] = sum;
+  __syncthreads();
+  if (tid < 64) {
+    sum = row.sum_of(lds.wave, 8);
+    if (tid == 0) a.seg_mass[blockIdx.x] = sum;
+  }
+}
 
-  // The kept tokens: logits above cut_x, and at cut_x indexes up to cut_i.
-  float cut_x = -INFINITY;
-  int cut_i = 0x7fffffff;
-  if (k > 0 &&
-      row.reach([](int, float) { return 1u; }, [k](u64) { return (u64)k; }, TH / 4, cut_x, cut_i) == 2) {
-    row.choose_few(r, lds.count, k, p, floor_y);
+__global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
+  constexpr int TH = 1024, CHUNKS = kSegment / (4 * TH);
+  __shared__ SampleLds lds;
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, G = a.segments;
+  Row<TH, 0> row(a, lds, nullptr, r);
+  const Filters f(a, r);
+  row.take(row_max(a, r), f.T);
+  if (row.m == -INFINITY) {
+    if (tid == 0) certain(a, r, 0, -INFINITY);
     return;
   }
-  if (p < 1.f) {
-    const float kx = cut_x;
-    const int ki = cut_i;
-    auto all = [&](int i, float v) { return v > kx || (v == kx && i <= ki) ? row.weight(v) : (u64)0; };
-    row.reach(all, [p](u64 mass) { return (u64)fmax(ceil((double)p * (double)mass), 1.0); }, 0, cut_x, cut_i);
+  if (f.greedy()) {
+    const float top = row.infinite ? INFINITY : row.m;  // as the segments have it
+    const int g = __builtin_ctzll(__ballot(lane < G && a.seg_max[(size_t)r * G + lane] == top));
+    const int token = row.first_of(row.m, g * CHUNKS, min((g + 1) * CHUNKS, row.n_chunks));
+    if (tid == 0) certain(a, r, token, 0.f);
+    return;
   }
-  auto kept = [&](int i, float v) {
-    const bool in = (v > cut_x || (v == cut_x && i <= cut_i)) && (v == m || ((double)v - (double)m) * row.inv_t >= floor_y);
-    return in ? row.weight(v) : (u64)0;
-  };
-  u64 total;
-  const int token = row.pick(kept, [&](u64 sum) { return row.place(r, sum); }, total);
+  Cut cut{-INFINITY, 0x7fffffff};
+  if (f.k == 0 && f.p == 1.f) {
+    cut.above(f.least(row.m));
+    if (tid < G) lds.super[tid] = a.seg_mass[(size_t)r * G + tid];
+    __syncthreads();
+  } else {
+    // this thread's range over all segments
+    const u64* const mass = a.mass + (size_t)r * G * kBins;
+    const uint32* const count = a.count + (size_t)r * G * kBins;
+    u64 own_count = 0, own_mass = 0;
+#pragma unroll 8
+    for (int g = 0; g < G; ++g) {
+      own_count += count[(size_t)g * kBins + tid];
+      own_mass += mass[(size_t)g * kBins + tid];
+    }
+    const Ranges ranges = first_ranges(row.m, f.T);
+    auto list_of = [&](int bin) { return row.gather(ranges.edge(bin), bin > 0 ? ranges.edge(bin - 1) : -INFINITY); };
+    int listed = -1, n = 0;  // the range whose tokens are in the list
+    u64 kept_mass = 0;       // of the first top_k
+    bool crowded = false;    // more than the list holds: by passes over the row then
+    // The range where `own` reaches the target, and its tokens in the list; what is left of the target there.
+    auto search = [&](u64 own, auto target_of) {
+      row.clear();
+      lds.hist[tid] = own;
+      __syncthreads();
+      const u64 target = row.find(lds.hist, target_of);
+      const int bin = lds.bin;
+      const u64 rest = target - (bin < 0 ? 0 : lds.before);
+      __syncthreads();
+      if (bin >= 0 && bin != listed) {
+        if (tid == bin) lds.best = (int)own_count;
+        __syncthreads();
+        crowded = lds.best > kList;
+        if (!crowded) n = list_of(listed = bin);
+      }
+      return rest;
+    };
+    if (f.k > 0) {
+      const u64 rest = search(own_count, [&](u64) { return (u64)f.k; });
+      if (listed >= 0) {
+        const Entry at = row.reach_in_list(n, rest, [](const Entry&) { return (u64)1; }, ranges, listed);
+        cut = Cut{at.x, at.i};
+        if (f.p < 1.f) {  // the weight of all kept
+          __syncthreads();
+          if (tid == 0) lds.upto = 0;
+          __syncthreads();
+          u64 sum = tid < listed ? own_mass : 0;
+          for (int i = tid; i < n; i += TH) sum += cut.keeps(lds.list[i].x, lds.list[i].i) ? lds.list[i].w : 0;
+          sum = wave_sum(sum);
+          if (lane == 0) atomicAdd(&lds.upto, sum);
+          __syncthreads();
+          kept_mass = lds.upto;
+        }
+      }
+    }
+    if (f.p < 1.f && !crowded) {
+      const bool by_k = listed >= 0;
+      const u64 rest = search(own_mass, [&](u64 all) { return p_target(f.p, by_k ? kept_mass : all); });
+      if (!crowded) {
+        const Entry at = row.reach_in_list(n, rest, [](const Entry& e) { return e.w; }, ranges, listed);
+        cut = Cut{at.x, at.i};
+      }
+    }
+    if (!crowded && cut.above(f.least(row.m))) {
+      const int bin = ranges.of(cut.x);
+      if (bin != listed) n = list_of(listed = bin);
+      crowded = n > kList;
+    }
+    if (crowded) {
+      choose(row, f, r);
+      return;
+    }
+    // the segments' kept weights: of the ranges above the listed one, and the tokens in it; of all (k of as many
+    // tokens or more, nothing else) where none is
+    __syncthreads();
+    for (int g = w; g < G; g += TH / 64) {
+      u64 sum = 0;
+#pragma unroll
+      for (int i = 0; i < kBins / 64; ++i) {
+        const u64 x = mass[(size_t)g * kBins + 64 * i + lane];
+        sum += 64 * i + lane < (listed < 0 ? kBins : listed) ? x : 0;
+      }
+      sum = wave_sum(sum);
+      if (lane == 0) lds.super[g] = sum;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += TH)
+      if (cut.keeps(lds.list[i].x, lds.list[i].i)) atomicAdd(&lds.super[lds.list[i].i / kSegment], lds.list[i].w);
+    __syncthreads();
+  }
+  auto kept = [&](int i, float v) { return cut.keeps(v, i) ? row.weight(v) : (u64)0; };
+  const u64 total = row.sum_of(lds.super, G);
+  u64 at = row.place(r, total);
+  const int g = row.locate(lds.super, G, at), c1 = min((g + 1) * CHUNKS, row.n_chunks);
+  __syncthreads();
+  row.sum_waves(g * CHUNKS, c1, kept);
+  const int token = row.pick_in(g * CHUNKS, c1, at, kept);
   if (tid == 0) row.result(r, token, row.infinite ? 0.f : row.x[token], total);
 }
 
+int segments_of(uint32_t vocab) { return vocab > (uint32_t)kStaged ? (int)((vocab + kSegment - 1) / kSegment) : 0; }
+
 }  // namespace
+
+extern "C" size_t aur_sample_ws_bytes(uint32_t b, uint32_t vocab) {
+  if (vocab > (uint32_t)kMaxVocab || b > 0x000fffffu) return 0;
+  const size_t n = (size_t)b * segments_of(vocab);
+  return (n * (kBins * 12 + 8 + 4) + 15) / 16 * 16;
+}
 
 extern "C" int aur_sample(aur_ctx* ctx, const float* logits, uint32_t ld, const float* u, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens,
-                          float* logprob, uint32_t b, uint32_t vocab) {
+                          float* logprob, void* scratch, size_t scratch_bytes, uint32_t b, uint32_t vocab) {
   AUR_CHECK_CTX(ctx);
   const char* who = "aur_sample";
   if (vocab == 0 || ld < vocab)
     return aur::set_error(ctx, AUR_EINVAL, "%s: ld=%u of vocab=%u", who, ld, vocab);
-  if (vocab > kMaxVocab || b > 0x00ffffffu || ld > 0x7fffffffu)
+  if (vocab > kMaxVocab || b > 0x000fffffu || ld > 0x7fffffffu)
     return aur::set_error(ctx, AUR_ELIMIT, "%s: b=%u vocab=%u (up to %d) ld=%u", who, b, vocab, kMaxVocab, ld);
   if (b == 0) return 0;
   if (!logits || !u || !tokens) return aur::set_error(ctx, AUR_EINVAL, "%s: null logits, u or tokens", who);
   int bits = 0;
   while ((1u << bits) < vocab) ++bits;
   SampleArgs a{logits, u, temperature, top_p, min_p, top_k, tokens, logprob, (int)vocab, (int)ld,
-               63 - bits < 50 ? 63 - bits : 50, ld % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0};
-  auto* kernel = vocab <= 256      ? sample_kernel<256, 256>
-                 : vocab <= 8192    ? sample_kernel<512, 2048>
-                 : vocab <= kStaged ? sample_kernel<1024, kStaged / 4>
-                                    : sample_kernel<1024, 0>;
+               63 - bits < 50 ? 63 - bits : 50};
+  a.segments = segments_of(vocab);
+  if (a.segments) {
+    if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15) || scratch_bytes < aur_sample_ws_bytes(b, vocab))
+      return aur::set_error(ctx, AUR_EINVAL, "%s: scratch of %zu bytes (16-byte aligned), %zu needed", who,
+                            scratch ? scratch_bytes : (size_t)0, aur_sample_ws_bytes(b, vocab));
+    const size_t n = (size_t)b * a.segments;
+    a.mass = static_cast<u64*>(scratch);
+    a.seg_mass = a.mass + n * kBins;
+    a.count = reinterpret_cast<uint32*>(a.seg_mass + n);
+    a.seg_max = reinterpret_cast<float*>(a.count + n * kBins);
+    hipLaunchKernelGGL(sample_max_kernel, dim3((unsigned)n), dim3(512), 0, ctx->stream, a);
+    AUR_LAUNCH_CHECK(ctx, "sample_max_kernel");
+    hipLaunchKernelGGL(sample_histogram_kernel, dim3((unsigned)n), dim3(512), 0, ctx->stream, a);
+    AUR_LAUNCH_CHECK(ctx, "sample_histogram_kernel");
+    hipLaunchKernelGGL(sample_finish_kernel, dim3(b), dim3(1024), 0, ctx->stream, a);
+    AUR_LAUNCH_CHECK(ctx, "sample_finish_kernel");
+    return 0;
+  }
+  auto* kernel = vocab <= 256    ? sample_kernel<256, 256>
+                 : vocab <= 8192 ? sample_kernel<512, 2048>
+                                 : sample_kernel<1024, kStaged / 4>;
   const dim3 threads(vocab <= 256 ? 256 : vocab <= 8192 ? 512 : 1024);
   hipLaunchKernelGGL(kernel, dim3(b), threads, 0, ctx->stream, a);
   AUR_LAUNCH_CHECK(ctx, "sample_kernel");

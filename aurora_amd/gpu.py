@@ -419,7 +419,28 @@ class PagedMhaKernel(_Kernel):
 
 class SampleKernel(_Kernel):
     """The next token of each row of logits [b, vocab] from a random number u [b]: tokens [b] int32 and, unless
-    0, logprob [b].  temperature, top_k (int32), top_p and min_p are arrays of b values, 0 for none."""
+    0, logprob [b].  temperature, top_k (int32), top_p and min_p are arrays of b values, 0 for none.
+
+    For more than 32768 tokens the object keeps a scratch, allocated when a call needs a larger one (or ahead,
+    by `reserve`: a captured call cannot allocate); calls that overlap in time take an object each."""
+
+    def __init__(self):
+        self._scratch = None
+
+    @staticmethod
+    def scratch_bytes(b, vocab) -> int:
+        return _lib.load().aur_sample_ws_bytes(b, vocab)
+
+    def reserve(self, ctx, b, vocab) -> None:
+        n = self.scratch_bytes(b, vocab)
+        if n and (self._scratch is None or self._scratch.nbytes < n or self._scratch.ctx is not ctx):
+            self.free()
+            self._scratch = GpuBuffer.empty(ctx, n, np.uint8)
+
+    def free(self) -> None:
+        if self._scratch is not None:
+            self._scratch.free()
+            self._scratch = None
 
     def dispatch_into(self, ctx, logits, ld, u, tokens, logprob, b, vocab, temperature=0, top_k=0, top_p=0, min_p=0):
         if _any_buffer(logits, u, tokens, logprob, temperature, top_k, top_p, min_p):
@@ -428,4 +449,9 @@ class SampleKernel(_Kernel):
             _need("SampleKernel filters", b, temperature, top_k, top_p, min_p)
             logits, u, tokens, logprob = _p(logits), _p(u), _p(tokens), _p(logprob)
             temperature, top_k, top_p, min_p = _p(temperature), _p(top_k), _p(top_p), _p(min_p)
-        ctx.call("aur_sample", logits, ld, u, temperature, top_k, top_p, min_p, tokens, logprob, b, vocab)
+        scratch, nbytes = 0, 0
+        if vocab > 32768:
+            self.reserve(ctx, b, vocab)
+            if self._scratch is not None:
+                scratch, nbytes = self._scratch.ptr, self._scratch.nbytes
+        ctx.call("aur_sample", logits, ld, u, temperature, top_k, top_p, min_p, tokens, logprob, scratch, nbytes, b, vocab)

@@ -335,10 +335,15 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
  * A NaN logit counts as -inf; -inf is never chosen, and a row of nothing else gives
  * token 0 and logprob -inf; logits of +inf share the row alone.
  * Weights are whole multiples of 2^-F, F = 63 - ceil(log2 vocab) up to 50, so sums
- * are exact and the same call gives the same tokens.  vocab up to 2^20 (AUR_ELIMIT). */
+ * are exact and the same call gives the same tokens.  vocab up to 2^20 (AUR_ELIMIT).
+ * `scratch` is caller-owned, 16-byte aligned, of scratch_bytes >=
+ * aur_sample_ws_bytes(b, vocab) (0, and it may be NULL, up to 32768 tokens); calls
+ * that overlap in time need one each. */
+size_t aur_sample_ws_bytes(uint32_t b, uint32_t vocab);
 int aur_sample(aur_ctx* ctx, const float* logits, uint32_t ld, const float* u,
                const float* temperature, const int32_t* top_k, const float* top_p,
-               const float* min_p, int32_t* tokens, float* logprob, uint32_t b, uint32_t vocab);
+               const float* min_p, int32_t* tokens, float* logprob, void* scratch,
+               size_t scratch_bytes, uint32_t b, uint32_t vocab);
 
 /* ---- model: DecoderTransformerGpu / KvCacheGpu ----------------------------
  * The caller of the hot path (src/gpu/transformer.rs:32-116, 949-2640),

@@ -74,6 +74,13 @@ def test_python_structs_refuse():
         SampleKernel().dispatch_into(Nothing(), ok["logits"], 10, ok["u"], ok["tokens"], 0, 2, 10)
 
 
+def test_scratch_of_the_choice():
+    assert SampleKernel.scratch_bytes(64, 32768) == 0 and SampleKernel.scratch_bytes(0, 100000) == 0
+    n = SampleKernel.scratch_bytes(3, 32769)
+    assert n >= 3 * 3 * 1024 * 12 and n % 16 == 0
+    assert SampleKernel.scratch_bytes(64, 131072) < 8 << 20  # less than a fourth of the logits
+
+
 def test_numbers_and_rounding():
     import torch
 

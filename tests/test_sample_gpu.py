@@ -66,18 +66,19 @@ def test_matches_the_definition(ctx, vocab, top_k, top_p, min_p):
     _check(x, u, tokens, lp, **kw)
 
 
-def test_every_row_has_its_own_filters(ctx):
+@pytest.mark.parametrize("vocab", [300, 5000, 20000, 50000])
+def test_every_row_has_its_own_filters(ctx, vocab):
     rng = np.random.default_rng(1)
-    b, vocab = 64, 5000
+    b = 64
     x = (3 * rng.standard_normal((b, vocab))).astype(np.float32)
     u = rng.random(b).astype(np.float32)
-    kw = dict(temperature=rng.choice([0.0, 0.3, 1.0, 2.0, -1.0, np.nan], b), top_k=rng.choice([-1, 0, 1, 2, 100, 5000, 9999], b),
+    kw = dict(temperature=rng.choice([0.0, 0.3, 1.0, 2.0, -1.0, np.nan], b), top_k=rng.choice([-1, 0, 1, 2, 100, 5000, 9999, 60000], b),
               top_p=rng.choice([0.0, 0.1, 0.9, 1.0, 1.5, np.nan], b), min_p=rng.choice([-1.0, 0.0, 0.1, 1.0, 3.0, np.nan], b))
     tokens, lp = _run(ctx, x, u, **kw)
     _check(x, u, tokens, lp, **kw)
 
 
-@pytest.mark.parametrize("vocab", [7, 900, 3000, 9000])
+@pytest.mark.parametrize("vocab", [7, 900, 3000, 9000, 40001])
 def test_rows_that_are_not_16_byte_aligned(ctx, vocab):
     rng = np.random.default_rng(2)
     x = (2 * rng.standard_normal((4, vocab))).astype(np.float32)
@@ -112,7 +113,7 @@ def _exact(ctx, x, weights, u, top_k=0, top_p=1.0):
     return lp
 
 
-@pytest.mark.parametrize("vocab", [1, 5, 256, 1024, 3000, 20000])
+@pytest.mark.parametrize("vocab", [1, 5, 256, 1024, 3000, 20000, 33000])
 @pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (0, 0.5), (0, 0.25), (37, 1.0), (37, 0.5), (2048, 0.75)])
 def test_equal_logits_go_by_index(ctx, vocab, top_k, top_p):
     """One value throughout, where every border is met exactly and the lowest indexes are kept."""
@@ -137,9 +138,10 @@ def test_ties_at_the_borders(ctx):
 
 @pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (1500, 1.0), (0, 0.5), (2500, 0.9), (3, 1.0)])
 @pytest.mark.parametrize("what", ["band", "outlier", "subnormal", "far apart", "two bands"])
-def test_logits_that_crowd_one_range(ctx, what, top_k, top_p):
+@pytest.mark.parametrize("vocab", [5000, 40000])
+def test_logits_that_crowd_one_range(ctx, vocab, what, top_k, top_p):
     rng = np.random.default_rng(5)
-    b, vocab = 4, 5000
+    b = 4
     x = rng.permuted(np.tile(np.arange(vocab), (b, 1)), axis=1).astype(np.float64)
     if what == "band":
         x = 1 + x * 2.0**-23
@@ -161,7 +163,7 @@ def test_logits_that_crowd_one_range(ctx, what, top_k, top_p):
     _check(x, u, tokens, lp, **kw)
 
 
-@pytest.mark.parametrize("vocab", [4, 900, 2000, 5000])
+@pytest.mark.parametrize("vocab", [4, 900, 2000, 5000, 34000])
 @pytest.mark.parametrize("kw", [{}, dict(top_k=3), dict(top_p=0.5), dict(top_k=1500, top_p=0.7, min_p=0.1), dict(temperature=0.0)])
 def test_infinities_and_nan(ctx, vocab, kw):
     rng = np.random.default_rng(6)
@@ -180,9 +182,10 @@ def test_infinities_and_nan(ctx, vocab, kw):
     _check(x[2:], u[2:], tokens[2:], lp[2:], **kw)
 
 
-def test_temperatures_and_numbers_at_the_ends(ctx):
+@pytest.mark.parametrize("vocab", [3000, 36000])
+def test_temperatures_and_numbers_at_the_ends(ctx, vocab):
     rng = np.random.default_rng(7)
-    x = rng.standard_normal((8, 3000)).astype(np.float32)
+    x = rng.standard_normal((8, vocab)).astype(np.float32)
     t = np.array([1e-45, 1e-30, 1e30, 3.4e38, np.inf, 0.01, 100.0, 1.0], np.float32)
     u = np.full(8, 0.6, np.float32)
     tokens, lp = _run(ctx, x, u, temperature=t)
@@ -192,6 +195,67 @@ def test_temperatures_and_numbers_at_the_ends(ctx):
     for r in range(8):
         kept = np.sort(np.argsort(-x[r], kind="stable")[:20])
         assert tokens[r] == (kept[-1] if u[r] >= 1 else kept[0])
+    kw = dict(temperature=t, top_k=500, top_p=0.7, min_p=0.2)
+    u = np.full(8, 0.6, np.float32)
+    tokens, lp = _run(ctx, x, u, **kw)
+    _check(x, u, tokens, lp, **kw)
+
+
+@pytest.mark.parametrize("vocab", [33000, 49152, 131072, 200003])
+@pytest.mark.parametrize("kw", [{}, dict(min_p=0.3), dict(min_p=1e-4), dict(top_k=30000), dict(top_k=3), dict(top_k=20000, top_p=0.999),
+                                dict(top_p=0.01), dict(top_p=0.9999), dict(top_k=2000, top_p=0.999, min_p=0.001),
+                                dict(top_p=0.99, min_p=0.4), dict(top_k=500, min_p=0.0001)])
+def test_rows_that_several_blocks_share(ctx, vocab, kw):
+    rng = np.random.default_rng(vocab)
+    b = 9
+    x = (rng.choice([0.5, 2.5, 8.0], (b, 1)) * rng.standard_normal((b, vocab))).astype(np.float32)
+    x[1] = np.round(x[1] * 8) / 8  # equal logits in all segments
+    x[2, :20000] = -np.inf
+    x[3] = np.sort(x[3])
+    u = rng.random(b).astype(np.float32)
+    tokens, lp = _run(ctx, x, u, **kw)
+    _check(x, u, tokens, lp, **kw)
+
+
+def test_captured_into_a_graph(ctx):
+    """A call of each size captured once and replayed with new logits and numbers: as an eager call."""
+    import ctypes
+
+    from aurora_amd._lib import load
+    from aurora_amd.gpu import GpuBuffer, SampleKernel
+    from tests.test_paged_gpu import _hip
+
+    hip, stream = _hip(), load().aur_stream(ctx.ptr)
+    rng = np.random.default_rng(9)
+    for vocab in (200, 6000, 40000):
+        b = 5
+        logits, u = GpuBuffer.zeros(ctx, b * vocab), GpuBuffer.zeros(ctx, b)
+        t, p = GpuBuffer.from_slice(ctx, np.full(b, 0.8, np.float32)), GpuBuffer.from_slice(ctx, np.full(b, 0.9, np.float32))
+        out = [(GpuBuffer.zeros(ctx, b, np.int32), GpuBuffer.zeros(ctx, b)) for _ in range(2)]
+        kernels = SampleKernel.new(), SampleKernel.new()
+        for kernel in kernels:
+            kernel.reserve(ctx, b, vocab)
+        call = lambda i: kernels[i].dispatch_into(ctx, logits, vocab, u, *out[i], b, vocab, t, 0, p, 0)  # noqa: E731
+        graph, exe = ctypes.c_void_p(), ctypes.c_void_p()
+        ctx.sync()
+        assert hip.hipStreamBeginCapture(stream, 1) == 0  # hipStreamCaptureModeThreadLocal
+        try:
+            call(0)
+        finally:
+            assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, 0) == 0
+        for _ in range(4):
+            x, r = (3 * rng.standard_normal((b, vocab))).astype(np.float32), rng.random(b).astype(np.float32)
+            logits.upload(x.ravel()), u.upload(r)
+            assert hip.hipGraphLaunch(exe, stream) == 0
+            ctx.sync()
+            call(1)
+            for got, want in zip(*out):
+                assert np.array_equal(got.download(), want.download())
+            _check(x, r, out[0][0].download(), out[0][1].download(), temperature=0.8, top_p=0.9)
+        hip.hipGraphExecDestroy(exe), hip.hipGraphDestroy(graph)
+        for z in (logits, u, t, p, *out[0], *out[1], *kernels):
+            z.free()
 
 
 def test_without_logprob_and_twice_the_same(ctx):
