@@ -233,14 +233,39 @@ struct Row {
   // f(chunk, index of the first, four logits) for the chunks from c0 up to c1.
   template <class F>
   __device__ __forceinline__ void each(int c0, int c1, F f) const {
-    floatx4 next = ROW ? floatx4{} : raw(c0);
-    for (int c = c0; c < c1; ++c) {
-      const floatx4 v = ROW ? held[c * TH + threadIdx.x] : clean(next);
-      if (!ROW && c + 1 < c1) next = raw(c + 1);
-      f(c, 4 * (c * TH + (int)threadIdx.x), v);
+    if constexpr (ROW > 0) {
+      for (int c = c0; c < c1; ++c) f(c, 4 * (c * TH + (int)threadIdx.x), held[c * TH + threadIdx.x]);
+    } else {
+      for (int c = c0; c < c1;) {  // four under way together
+        floatx4 v[4];
+        raw(c, v);
+#pragma unroll 1
+        for (int i = 0; i < 4 && c < c1; ++i, ++c) {
+          f(c, 4 * (c * TH + (int)threadIdx.x), clean(v[0]));
+          v[0] = v[1];
+          v[1] = v[2];
+          v[2] = v[3];
+        }
+      }
     }
   }
 
+  // g(index, logit) of four logits.  A block that streams its row goes through much code once, and what it reads of
+  // code costs it more than a loop over one copy of g does (64 rows of 131072: 94 us, with four copies 124); a row
+  // in LDS is passed over by less (32 rows of 8192: 10.9 us by four copies, 11.7 by one).
+  template <class G>
+  static __device__ __forceinline__ void one_by_one(floatx4 v, int i, G g) {
+    if constexpr (ROW > 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g(i + e, v[e]);
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < 4; ++e) {
+        g(i + e, v[0]);
+        v = floatx4{v[1], v[2], v[3], v[0]};
+      }
+    }
+  }
   __device__ __forceinline__ u64 weight(float v) const { return weight_of(v, m, scale, a.frac); }
 
   __device__ __forceinline__ float block_max(float v) {
@@ -292,8 +317,7 @@ struct Row {
   __device__ __forceinline__ void sum_waves(int c0, int c1, F f) {
     each(c0, c1, [&](int c, int i, floatx4 v) {
       u64 sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += f(i + e, v[e]);
+      one_by_one(v, i, [&](int at, float x) { sum += f(at, x); });
       sum = wave_sum(sum);
       if ((threadIdx.x & 63) == 0) lds.wave[(c - c0) * NW + (threadIdx.x >> 6)] = sum;
     });
@@ -315,10 +339,8 @@ struct Row {
       __syncthreads();
       for (int s = 0; s < n; ++s) {
         u64 sum = 0;
-        each(s * kSuper, min((s + 1) * kSuper, n_chunks), [&](int, int i, floatx4 v) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum += f(i + e, v[e]);
-        });
+        each(s * kSuper, min((s + 1) * kSuper, n_chunks),
+             [&](int, int i, floatx4 v) { one_by_one(v, i, [&](int at, float x) { sum += f(at, x); }); });
         sum = wave_sum(sum);
         if ((threadIdx.x & 63) == 0) atomicAdd(&lds.super[s], sum);
       }
@@ -337,15 +359,15 @@ struct Row {
     const int at = locate(lds.wave, (c1 - c0) * NW, r);
     if (w == at % NW)
       each(c0 + at / NW, c0 + at / NW + 1, [&](int, int i, floatx4 v) {
-        u64 t[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = f(i + e, v[e]);
-        u64 up = wave_scan(t[0] + t[1] + t[2] + t[3]) - (t[0] + t[1] + t[2] + t[3]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (up <= r && r < up + t[e]) lds.token = i + e;
-          up += t[e];
-        }
+        u64 sum = 0;
+        one_by_one(v, i, [&](int at, float x) { sum += f(at, x); });
+        u64 up = wave_scan(sum) - sum;
+        if (up <= r && r < up + sum)
+          one_by_one(v, i, [&](int at, float x) {
+            const u64 t = f(at, x);
+            if (up <= r && r < up + t) lds.token = at;
+            up += t;
+          });
       });
     __syncthreads();
     return lds.token;
@@ -448,23 +470,33 @@ struct Row {
   // The tokens of least <= logit < end (of all from least on where end is −∞) in the list: their number,
   // of which the list holds the first kList.
   __device__ __forceinline__ int gather(float least, float end) {
-    constexpr int AT_ONCE = 8;
+    constexpr int AT_ONCE = 16;
     __syncthreads();
     if (threadIdx.x == 0) lds.count = 0;
     __syncthreads();
     for (int c = 0; c < n_chunks; c += AT_ONCE) {
       floatx4 v[AT_ONCE];
       raw(c, v);
+      u64 hits = 0;
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) v[i] = clean(v[i]);
+      for (int i = 0; i < AT_ONCE; ++i) {
+        v[i] = clean(v[i]);
+        uint32 four = 0;
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (v[i][e] >= least && (v[i][e] < end || end == -INFINITY)) {
-            const int n = atomicAdd(&lds.count, 1);
-            if (n < kList) lds.list[n] = Entry{v[i][e], 4 * ((c + i) * TH + (int)threadIdx.x) + e, weight(v[i][e])};
-          }
+        for (int e = 0; e < 4; ++e) four |= (uint32)(v[i][e] >= least && (v[i][e] < end || end == -INFINITY)) << e;
+        hits |= (u64)four << (4 * i);
+      }
+      for (; hits; hits &= hits - 1) {
+        const int bit = __builtin_ctzll(hits), at = 4 * ((c + (bit >> 2)) * TH + (int)threadIdx.x) + (bit & 3);
+        const int n = atomicAdd(&lds.count, 1);
+        if (n < kList) lds.list[n].i = at;
+      }
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < min(lds.count, kList); n += TH) {
+      const int at = lds.list[n].i;
+      const float v = infinite ? 0.f : x[at];
+      lds.list[n] = Entry{v, at, weight(v)};
     }
     __syncthreads();
     return lds.count;
@@ -488,12 +520,11 @@ struct Row {
       auto in = [&](float v) { return v > -INFINITY && v >= lo && (double)v <= ranges.hi; };
       clear();
       each(0, n_chunks, [&](int, int i, floatx4 v) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (in(v[e])) {
-            const W x = f(i + e, v[e]);
-            if (x) atomicAdd(&hist[bin_of(v[e])], x);
-          }
+        one_by_one(v, i, [&](int at, float y) {
+          if (!in(y)) return;
+          const W x = f(at, y);
+          if (x) atomicAdd(&hist[bin_of(y)], x);
+        });
       });
       __syncthreads();
       target = find(hist, [&](u64 all) { return first ? target_of(all) : target; });
@@ -502,23 +533,22 @@ struct Row {
       target -= lds.before;
       if (first && lds.upto <= (u64)few) {  // (weights of one each: f counts)
         each(0, n_chunks, [&](int, int i, floatx4 v) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (in(v[e]) && bin_of(v[e]) <= bin) lds.list[atomicAdd(&lds.count, 1)] = Entry{v[e], i + e, 0};
+          one_by_one(v, i, [&](int at, float y) {
+            if (in(y) && bin_of(y) <= bin) lds.list[atomicAdd(&lds.count, 1)] = Entry{y, at, 0};
+          });
         });
         __syncthreads();
         return 2;
       }
       float most = -INFINITY, fewest = INFINITY;
       each(0, n_chunks, [&](int, int i, floatx4 v) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (in(v[e]) && bin_of(v[e]) == bin) {
-            most = fmaxf(most, v[e]);
-            fewest = fminf(fewest, v[e]);
-            const int n = atomicAdd(&lds.count, 1);
-            if (n < kList) lds.list[n] = Entry{v[e], i + e, f(i + e, v[e])};
-          }
+        one_by_one(v, i, [&](int at, float y) {
+          if (!in(y) || bin_of(y) != bin) return;
+          most = fmaxf(most, y);
+          fewest = fminf(fewest, y);
+          const int n = atomicAdd(&lds.count, 1);
+          if (n < kList) lds.list[n] = Entry{y, at, f(at, y)};
+        });
       });
       __syncthreads();
       const int n = lds.count;
@@ -634,6 +664,12 @@ __device__ __forceinline__ void choose(Row<TH, ROW>& row, const Filters& f, int 
   u64 total;
   const int token = row.pick(kept, [&](u64 sum) { return row.place(r, sum); }, total);
   if (threadIdx.x == 0) row.result(r, token, row.infinite ? 0.f : row.x[token], total);
+}
+
+// The same out of line, for rows that hardly ever come.
+template <int TH, int ROW>
+__device__ __attribute__((noinline)) void choose_apart(Row<TH, ROW>& row, const Filters& f, int r) {
+  choose(row, f, r);
 }
 
 // A row without anything to choose from; nor with a choice to make: its first largest logit.
@@ -758,6 +794,15 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
   constexpr int TH = 1024, CHUNKS = kSegment / (4 * TH);
   __shared__ SampleLds lds;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, G = a.segments;
+  // this thread's range over all segments (what lies there where no histogram was made is not used)
+  const u64* const mass = a.mass + (size_t)r * G * kBins;
+  const uint32* const count = a.count + (size_t)r * G * kBins;
+  u64 own_count = 0, own_mass = 0;
+#pragma unroll 8
+  for (int g = 0; g < G; ++g) {
+    own_count += count[(size_t)g * kBins + tid];
+    own_mass += mass[(size_t)g * kBins + tid];
+  }
   Row<TH, 0> row(a, lds, nullptr, r);
   const Filters f(a, r);
   row.take(row_max(a, r), f.T);
@@ -778,15 +823,6 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
     if (tid < G) lds.super[tid] = a.seg_mass[(size_t)r * G + tid];
     __syncthreads();
   } else {
-    // this thread's range over all segments
-    const u64* const mass = a.mass + (size_t)r * G * kBins;
-    const uint32* const count = a.count + (size_t)r * G * kBins;
-    u64 own_count = 0, own_mass = 0;
-#pragma unroll 8
-    for (int g = 0; g < G; ++g) {
-      own_count += count[(size_t)g * kBins + tid];
-      own_mass += mass[(size_t)g * kBins + tid];
-    }
     const Ranges ranges = first_ranges(row.m, f.T);
     auto list_of = [&](int bin) { return row.gather(ranges.edge(bin), bin > 0 ? ranges.edge(bin - 1) : -INFINITY); };
     int listed = -1, n = 0;  // the range whose tokens are in the list
@@ -841,7 +877,7 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
       crowded = n > kList;
     }
     if (crowded) {
-      choose(row, f, r);
+      choose_apart(row, f, r);
       return;
     }
     // the segments' kept weights: of the ranges above the listed one, and the tokens in it; of all (k of as many
