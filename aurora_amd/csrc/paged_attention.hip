@@ -133,8 +133,9 @@ int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_ba
     a.part_o = scratch;
     a.part_ml = scratch + (size_t)p.parts() * a.b.n_tok * a.H * a.dh;
   }
-  const uint64_t p_items = (uint64_t)a.Hkv * p.p_tiles * p.p_splits;
-  const uint64_t o_items = (uint64_t)a.Hkv * p.o_tiles * a.b.b * p.o_splits;
+  const uint64_t p_groups = (uint64_t)p.p_tiles * p.p_splits, o_groups = (uint64_t)p.o_tiles * a.b.b * p.o_splits;
+  a.by_xcd = cache->dtype == AUR_PAGED_E4M3 && heads_by_xcd(a.dh, p_groups, o_groups);
+  const uint64_t p_items = items_of(a.by_xcd, p_groups, a.Hkv), o_items = items_of(a.by_xcd, o_groups, a.Hkv);
   const uint64_t rows4 = ((uint64_t)a.b.n_tok * n_head + 3) / 4;  // blocks of the join
   if (p_items + o_items > kMaxBlocks / 2 || rows4 > kMaxBlocks)
     return aur::set_error(ctx, AUR_ELIMIT, "%s: %llu + %llu blocks", who, (unsigned long long)p_items,

@@ -53,7 +53,21 @@ struct MhaArgs {
   int p_tiles, p_splits, p_keys;  // p_keys keys a range
   int o_tiles, o_splits, o_keys;
   int p_items;                    // items 0 .. p_items-1 are the prefix's
+  bool by_xcd;                    // the K/V heads of the same keys run on the same XCD
 };
+
+// The dice take blocks in turn, and each has an L2 of its own with lines of 128 bytes.  Where a head's row is
+// shorter than that, the items of all K/V heads on the same keys go to one die, one after the other, so that a
+// line is fetched once and not by every die that wants a part of it.  With fewer than kDice sets of such items
+// some dice would have none.
+constexpr int kDice = 8;
+inline bool heads_by_xcd(int row_bytes, uint64_t p_groups, uint64_t o_groups) {
+  return row_bytes < 128 && o_groups >= kDice && (p_groups == 0 || p_groups >= kDice);
+}
+// Blocks for `groups` sets of items, a K/V head each.
+inline uint64_t items_of(bool by_xcd, uint64_t groups, int n_kv_head) {
+  return (by_xcd ? (groups + kDice - 1) / kDice * kDice : groups) * n_kv_head;
+}
 
 // Launches a call's items for pools of each type: own items of z's rows where the tile is 16, prefix items of
 // p_tile beside them (0: items of one kind).
@@ -105,9 +119,17 @@ __device__ __forceinline__ bool take_item(const MhaArgs& a, Item& it, int lead, 
   it.s = 0;
   it.tok0 = 0;
   it.first = 0;
-  if (it.of_prefix) {
+  if (!it.of_prefix) item -= a.p_items;
+  if (a.by_xcd) {
+    const int i = item / kDice;
+    it.hk = i % a.Hkv;
+    item = i / a.Hkv * kDice + item % kDice;
+    if (item >= (it.of_prefix ? a.p_tiles * a.p_splits : a.o_tiles * a.b.b * a.o_splits)) return false;
+  } else {
     it.hk = item % a.Hkv;
     item /= a.Hkv;
+  }
+  if (it.of_prefix) {
     it.row0 = item % a.p_tiles * R;
     it.part = item / a.p_tiles;
     it.n_rows = min(max(a.b.tok_off[a.b.b], 0), a.b.n_tok) * a.G;  // rows behind the last sequence are none
@@ -118,9 +140,6 @@ __device__ __forceinline__ bool take_item(const MhaArgs& a, Item& it, int lead, 
     page = page_of(a, 0, it.pre, it.x0 + lead);
     return true;
   }
-  item -= a.p_items;
-  it.hk = item % a.Hkv;
-  item /= a.Hkv;
   it.row0 = item % a.o_tiles * R;
   item /= a.o_tiles;
   it.s = item % a.b.b;
@@ -256,96 +275,9 @@ struct Keys32 {
   }
 };
 
-// Four e4m3 numbers times a scale, exactly but below 2^-126, as two pairs of bf16.
-__device__ __forceinline__ uint2v widen4(unsigned x, float scale) {
-  return uint2v{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, false)),
-                __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, true))};
-}
 // The scales of the key at pool row `at` (1 where there is none).
 __device__ __forceinline__ unsigned scale_byte(const MhaArgs& a, const uint8_t* scales, int hk, int at) {
   return at < 0 ? 127u : scales[scale_index(at, hk, a.Hkv, a.sh, a.ssh)];
-}
-
-// The same of an e4m3 pool: 8 columns of K, 4 of V a lane, which the conversion to bf16 multiplies by the scale
-// of their key.  Lane l loads the scales of key l % 32; the others have them from there.
-template <int DT>
-struct Keys32<e4m3, DT> {
-  static constexpr int VB = (DT + 3) / 4, KC = (DT + 1) / 2;
-  uint2v k[2][KC];
-  unsigned v[2][4][VB], k_scale, v_scale;
-  template <bool STREAM>
-  __device__ __forceinline__ void load_k(const MhaArgs& a, int hk, int at, int g, int l16) {
-    const size_t ld = (size_t)a.Hkv * a.dh;
-    const uint8_t* kp = static_cast<const uint8_t*>(a.k) + (size_t)hk * a.dh;
-    k_scale = scale_byte(a, a.k_scale, hk, at);
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const uint8_t* p = kp + (size_t)max(__shfl(at, 16 * kt + l16, 64), 0) * ld;
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-        k[kt][c] = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(p + min(32 * c + 8 * g, a.dh - 8)));
-    }
-  }
-  template <bool STREAM>
-  __device__ __forceinline__ void load_v(const MhaArgs& a, int hk, int at, int g, int l16) {
-    const size_t ld = (size_t)a.Hkv * a.dh;
-    const uint8_t* vp = static_cast<const uint8_t*>(a.v) + (size_t)hk * a.dh;
-    v_scale = scale_byte(a, a.v_scale, hk, at);
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint8_t* p = vp + (size_t)max(__shfl(at, 16 * kt + 4 * g + e, 64), 0) * ld;
-#pragma unroll
-        for (int b = 0; b < VB; ++b)
-          v[kt][e][b] = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(p + min(64 * b + 4 * l16, a.dh - 4)));
-      }
-  }
-  __device__ __forceinline__ void drop_missing(unsigned there, int g) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (!(there >> (16 * kt + 4 * g + e) & 1))
-#pragma unroll
-          for (int b = 0; b < VB; ++b) v[kt][e][b] = 0;
-  }
-};
-
-// As bf16 goes into the MFMA: K's piece c of tile kt, and V's pairs of columns (64b + 4·l16, + 1), (… + 2, + 3).
-template <int DT>
-__device__ __forceinline__ void keys_of(const Keys32<__bf16, DT>& x, int kt, int, uint4v (&k)[(DT + 1) / 2]) {
-#pragma unroll
-  for (int c = 0; c < (DT + 1) / 2; ++c) k[c] = x.k[kt][c];
-}
-template <int DT>
-__device__ __forceinline__ void keys_of(const Keys32<e4m3, DT>& x, int kt, int l16, uint4v (&k)[(DT + 1) / 2]) {
-  const float scale = scale_of(__shfl(x.k_scale, 16 * kt + l16, 64));
-#pragma unroll
-  for (int c = 0; c < (DT + 1) / 2; ++c) {
-    const uint2v lo = widen4(x.k[kt][c][0], scale), hi = widen4(x.k[kt][c][1], scale);
-    k[c] = uint4v{lo[0], lo[1], hi[0], hi[1]};
-  }
-}
-template <int DT>
-__device__ __forceinline__ void values_of(const Keys32<__bf16, DT>& x, int, uint2v (&v)[2][4][(DT + 3) / 4]) {
-#pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int b = 0; b < (DT + 3) / 4; ++b) v[kt][e][b] = x.v[kt][e][b];
-}
-template <int DT>
-__device__ __forceinline__ void values_of(const Keys32<e4m3, DT>& x, int g, uint2v (&v)[2][4][(DT + 3) / 4]) {
-#pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float scale = scale_of(__shfl(x.v_scale, 16 * kt + 4 * g + e, 64));
-#pragma unroll
-      for (int b = 0; b < (DT + 3) / 4; ++b) v[kt][e][b] = widen4(x.v[kt][e][b], scale);
-    }
 }
 
 // x as the sum of three bf16 numbers, exactly but for what lies 2^-24 below it and more (8 bits each,
@@ -372,7 +304,7 @@ __device__ __forceinline__ floatx4 mfma_bf16(bf16x8 a, bf16x8 b, floatx4 c) {
 }
 
 // A wave's queries as the MFMA's second operand, times log2(e)/√d_head: fp32 pieces of 4 columns, or
-// for bf16 and e4m3 keys three bf16 parts of 8 columns.
+// for bf16 keys three bf16 parts of 8 columns.
 template <class T, int DT, int RT>
 struct Queries;
 template <int DT, int RT>
@@ -388,8 +320,8 @@ struct Queries<float, DT, RT> {
       }
   }
 };
-template <class T, int DT, int RT>
-struct Queries {
+template <int DT, int RT>
+struct Queries<__bf16, DT, RT> {
   static constexpr int KC = (DT + 1) / 2;
   Split8 q[RT][KC];
   __device__ __forceinline__ void load(const Rows<RT>& r, int dh, int g, float sl2) {
@@ -430,19 +362,17 @@ __device__ __forceinline__ void scores(const Keys32<float, DT>& x, const Queries
     }
   }
 }
-template <class T, int DT, int RT>
-__device__ __forceinline__ void scores(const Keys32<T, DT>& x, const Queries<T, DT, RT>& q, int dh, int g,
+template <int DT, int RT>
+__device__ __forceinline__ void scores(const Keys32<__bf16, DT>& x, const Queries<__bf16, DT, RT>& q, int dh, int g,
                                        floatx4 (&st)[RT][2]) {
   constexpr int KC = (DT + 1) / 2;
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    uint4v kk[KC];
-    keys_of(x, kt, threadIdx.x & 15, kk);
 #pragma unroll
     for (int r = 0; r < RT; ++r) st[r][kt] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      uint4v u = kk[c];
+      uint4v u = x.k[kt][c];
       if (32 * c + 8 * g >= dh) u = uint4v{0, 0, 0, 0};
       const bf16x8 k = __builtin_bit_cast(bf16x8, u);
 #pragma unroll
@@ -469,10 +399,8 @@ __device__ __forceinline__ void add_values(const Keys32<float, DT>& x, const flo
 #pragma unroll
           for (int r = 0; r < RT; ++r) s.acc[r][b][c] = mfma16x16x4(x.v[kt][e][b][c], st[r][kt][e], s.acc[r][b][c]);
 }
-template <class T, int DT, int RT>
-__device__ __forceinline__ void add_values(const Keys32<T, DT>& x, const floatx4 (&st)[RT][2], Sums<DT, RT>& s) {
-  uint2v vv[2][4][Sums<DT, RT>::VB];
-  values_of(x, (threadIdx.x & 63) >> 4, vv);
+template <int DT, int RT>
+__device__ __forceinline__ void add_values(const Keys32<__bf16, DT>& x, const floatx4 (&st)[RT][2], Sums<DT, RT>& s) {
   // the MFMA's 8 keys of a lane group: 4g … 4g + 3 of both tiles of 16
   Split8 p[RT];
 #pragma unroll
@@ -491,7 +419,7 @@ __device__ __forceinline__ void add_values(const Keys32<T, DT>& x, const floatx4
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          u[2 * kt + i] = __builtin_amdgcn_perm(vv[kt][2 * i + 1][b][c >> 1], vv[kt][2 * i][b][c >> 1],
+          u[2 * kt + i] = __builtin_amdgcn_perm(x.v[kt][2 * i + 1][b][c >> 1], x.v[kt][2 * i][b][c >> 1],
                                                 c & 1 ? 0x07060302u : 0x05040100u);
       const bf16x8 v = __builtin_bit_cast(bf16x8, u);
 #pragma unroll
@@ -642,6 +570,24 @@ __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, in
   }
 }
 
+// … of 16 rows from row0 on, each wave its own, over the item's keys; written out.
+template <class T, int DT>
+__device__ __forceinline__ void store_exact(const MhaArgs& a, const Item& it, int row0) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, row = row0 + (lane & 15);
+  Sums<DT, 1> e;
+  exact_sums<T, DT, 1>(a, it, row0, it.x0, STEP, e);
+  const float L = rows4_sum(e.l[0]);
+  if (row >= it.n_rows) return;
+#pragma unroll
+  for (int b = 0; b < Sums<DT, 1>::VB; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = 64 * b + 16 * g + 4 * j;
+      if (col < a.dh)
+        store(a, it, row, col, floatx4{e.acc[0][b][0][j], e.acc[0][b][1][j], e.acc[0][b][2][j], e.acc[0][b][3][j]}, e.m[0], L);
+    }
+}
+
 // ---------------------------------------------------------------- few rows: keys through the registers
 
 // Up to 16 rows an item.  Each of the block's 4 waves takes every fourth group of 32 keys and keeps its own
@@ -655,6 +601,9 @@ __device__ void exact_sums(const MhaArgs& a, const Item& it, int row0, int x, in
 // K/V heads of 64, 4 rows each: 56 µs in bf16 (3.7 TB/s), 92 in fp32 (4.5 TB/s); with 1024 keys each 62 µs
 // in bf16 (4.3 TB/s).  On widened keys the fp32 MFMA took bf16's own keys of 64 such sequences 160 µs in a
 // first version, the bf16 one 60.
+template <int DT>
+__device__ bool byte_sums(const MhaArgs& a, const Item& it, int x, int stride, int page, Sums<DT, 1>& s);  // e4m3 keys
+
 template <int DT>
 struct RowsLds {
   static constexpr int R = 16, OS = 64 * ((DT + 3) / 4) + 4;
@@ -673,7 +622,12 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
   int x = it.x0 + STEP * w;
   Sums<DT, RT> s;
   s.clear();
-  if (x < it.x1) {
+  if constexpr (sizeof(T) == 1) {
+    if (x < it.x1) {
+      const bool good = byte_sums<DT>(a, it, x, STRIDE, page, s);
+      if (!good || !finite(s, it.row0 + l16 < it.n_rows)) exact_sums<T, DT, RT>(a, it, it.row0, x, STRIDE, s);
+    }
+  } else if (x < it.x1) {
     Keys32<T, DT> keys;
     int at = row_of(a, it, x + k32, page);
     keys.template load_k<true>(a, it.hk, at, g, l16);
@@ -827,8 +781,13 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long long o = max(__shfl(at, u * KPI + kg, 64), 0) * ld;
-        k[b][u] = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(kp + o));
-        v[b][u] = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(vp + o));
+        if (G::B8 && a.by_xcd) {  // a line has other heads' parts
+          k[b][u] = *reinterpret_cast<const Piece*>(kp + o);
+          v[b][u] = *reinterpret_cast<const Piece*>(vp + o);
+        } else {
+          k[b][u] = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(kp + o));
+          v[b][u] = __builtin_nontemporal_load(reinterpret_cast<const Piece*>(vp + o));
+        }
       }
     };
     load(0, row_of(a, it, x + lane % KEYS, page));
@@ -949,9 +908,8 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
 // above 96 in 64 rows 12, others up to 4.)
 template <class T, int DT, int W>
 struct TileGeo {
-  static constexpr bool F32 = std::is_same<T, float>::value, B8 = sizeof(T) == 1;
+  static constexpr bool F32 = std::is_same<T, float>::value;
   static constexpr int PARTS = F32 ? 3 : 1;
-  using KPiece = typename std::conditional<B8, uint2v, floatx4>::type;  // 8 columns of a key, or 4
   static constexpr int KT = DT > 4 ? 32 : 64;      // keys of a tile
   static constexpr int KC = (DT + 1) / 2;          // 32-column steps of a score
   static constexpr int KROW = KC == 1 ? 64 : KC == 2 ? 128 : 256;
@@ -975,12 +933,11 @@ struct TileLds {
   char k[G::PARTS * G::KPLANE], v[G::PARTS * G::VPLANE];
   long long offset[3][G::KT];  // in bytes, of the keys of this tile and the next two in the pools
   unsigned long long have[3];  // which of them are there
-  float scale[G::B8 ? 3 : 1][2][G::B8 ? G::KT : 1];  // of their K and V
 };
 template <class T, int DT, int NR, int W>
 __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& lds) {
   using G = TileGeo<T, DT, W>;
-  constexpr bool F32 = G::F32, B8 = G::B8;
+  constexpr bool F32 = G::F32;
   constexpr int KT = G::KT, KC = G::KC, NI = G::NI, NK = KT / 16, VC = G::VC;
   char* const ks = lds.k;
   char* const vs = lds.v;
@@ -1003,17 +960,9 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
   // Where a tile's keys lie; the first KT threads ask for the pages' numbers a tile before they are needed.
   const long long ld = (long long)a.Hkv * a.dh * sizeof(T);
   int xp = it.x0 + tid;  // the key whose page is under way
-  unsigned k_scale = 127, v_scale = 127;  // of the key placed last: they are laid down when the next one is
   auto place = [&](int slot) {
     if (tid < KT) {
       const int at = row_of(a, it, xp, page);
-      if constexpr (B8) {
-        const int last = slot == 0 ? 2 : slot - 1;
-        lds.scale[last][0][tid] = scale_of(k_scale);
-        lds.scale[last][1][tid] = scale_of(v_scale);
-        k_scale = scale_byte(a, a.k_scale, it.hk, at);
-        v_scale = scale_byte(a, a.v_scale, it.hk, at);
-      }
       lds.offset[slot][tid] = at < 0 ? 0 : at * ld;
       const unsigned long long have = __ballot(at >= 0);
       if (tid == 0) lds.have[slot] = have;
@@ -1031,8 +980,8 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
   const int vkey = v_on ? 32 * (vg >> 2) + 4 * (vg & 3) : 0;  // … the keys vkey + 16·(i/4) + i%4
   const char* const kp = static_cast<const char*>(a.k) + (size_t)it.hk * a.dh * sizeof(T);
   const char* const vp = static_cast<const char*>(a.v) + ((size_t)it.hk * a.dh + min(vc, a.dh - VC)) * sizeof(T);
-  typename G::KPiece kx[NI][F32 ? 2 : 1];  // as loaded
-  float vx[8][F32 ? VC : 1];               // bf16, e4m3: a pair
+  floatx4 kx[NI][F32 ? 2 : 1];  // as loaded
+  float vx[8][F32 ? VC : 1];    // bf16: a pair
   unsigned long long have = 0;  // of the keys in them
   auto load = [&](int slot) {
     have = lds.have[slot];
@@ -1040,16 +989,14 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const char* q = p + min(8 * (ko + G::TPR * i), a.dh - 8) * (int)sizeof(T);
-      kx[i][0] = *reinterpret_cast<const typename G::KPiece*>(q);
-      if constexpr (F32) kx[i][1] = *reinterpret_cast<const floatx4*>(q + 16);
+      kx[i][0] = *reinterpret_cast<const floatx4*>(q);
+      if (F32) kx[i][F32] = *reinterpret_cast<const floatx4*>(q + 16);
     }
     if (G::VN * (KT / 8) < 64 * W && !v_on) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const char* q = vp + lds.offset[slot][vkey + 16 * (i >> 2) + (i & 3)];
-      if (B8) {
-        vx[i][0] = __uint_as_float(*reinterpret_cast<const uint16_t*>(q));
-      } else if (F32 && VC == 2) {
+      if (F32 && VC == 2) {
         const float2v x = *reinterpret_cast<const float2v*>(q);
         vx[i][0] = x[0];
         vx[i][F32 ? VC - 1 : 0] = x[1];
@@ -1058,7 +1005,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
       }
     }
   };
-  auto lay_down = [&](int slot) {
+  auto lay_down = [&] {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int q = ko + G::TPR * i;
@@ -1066,12 +1013,8 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
       const bool live = DT * 16 == 32 * KC || 8 * q < a.dh;
       char* p = ks + tile_granule<G::KROW>(kr, q);
       const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (B8) {
-        const float scale = lds.scale[slot][0][kr];
-        const uint2v lo = widen4(kx[i][0][0], scale), hi = widen4(kx[i][0][1], scale);
-        *reinterpret_cast<uint4v*>(p) = live ? uint4v{lo[0], lo[1], hi[0], hi[1]} : uint4v{0, 0, 0, 0};
-      } else if constexpr (F32) {
-        const floatx4 x = live ? kx[i][0] : zero, y = live ? kx[i][1] : zero;
+      if (F32) {
+        const floatx4 x = live ? kx[i][0] : zero, y = live ? kx[i][F32] : zero;
         Split8 s;
         s.set(0, x[0], x[1]);
         s.set(2, x[2], x[3]);
@@ -1085,12 +1028,6 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
       }
     }
     if (G::VN * (KT / 8) < 64 * W && !v_on) return;
-    if constexpr (B8) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        vx[i][0] = __builtin_bit_cast(float, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
-                                                 __float_as_uint(vx[i][0]), lds.scale[slot][1][vkey + 16 * (i >> 2) + (i & 3)], false));
-    }
     if (have != ALL) {  // a key that is not there adds nothing, whatever lies in its place
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -1228,7 +1165,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
   int slot = 0;
   for (int x = it.x0; x < it.x1; x += KT) {
     if (x > it.x0) __syncthreads();  // every wave is done with the last tile
-    lay_down(slot);
+    lay_down();
     const unsigned long long there = have;
     const int next = slot == 2 ? 0 : slot + 1;
     place(next == 2 ? 0 : next + 1);
@@ -1259,22 +1196,22 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
           if (DT * 16 == a.dh || 16 * d + 4 * g < a.dh) store(a, it, row, 16 * d + 4 * g, acc[r][d], m[r], L);
       }
     } else {
-      Sums<DT, 1> e;
-      exact_sums<T, DT, 1>(a, it, row0 + 16 * r, it.x0, STEP, e);
-      const float L = rows4_sum(e.l[0]);
-      if (row < it.n_rows) {
-#pragma unroll
-        for (int b = 0; b < Sums<DT, 1>::VB; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int col = 64 * b + 16 * g + 4 * j;
-            if (col < a.dh)
-              store(a, it, row, col, floatx4{e.acc[0][b][0][j], e.acc[0][b][1][j], e.acc[0][b][2][j], e.acc[0][b][3][j]},
-                    e.m[0], L);
-          }
-      }
+      store_exact<T, DT>(a, it, row0 + 16 * r);
     }
   }
+}
+
+#include "paged_attention_e4m3.hpp"
+
+// The item of many rows, by the type of the pools.
+template <class T, int DT, int W>
+using ManyLds = typename std::conditional<sizeof(T) == 1, ByteLds<DT, W>, TileLds<T, DT, W>>::type;
+template <class T, int DT, int NR, int W>
+__device__ __forceinline__ void many_item(const MhaArgs& a, ManyLds<T, DT, W>& lds) {
+  if constexpr (sizeof(T) == 1)
+    byte_tile_item<DT, NR, W>(a, lds);
+  else
+    tile_item<T, DT, NR, W>(a, lds);
 }
 
 // ---------------------------------------------------------------- launches
@@ -1283,7 +1220,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
 template <class T, int DT, int R, int PRE>
 union StepLds {
   typename std::conditional<R == 16, RowsLds<DT>, FewLds<R>>::type own;
-  typename std::conditional<PRE == 64, TileLds<T, DT, NW>, typename std::conditional<PRE == 16, RowsLds<DT>, char>::type>::type pre;
+  typename std::conditional<PRE == 64, ManyLds<T, DT, NW>, typename std::conditional<PRE == 16, RowsLds<DT>, char>::type>::type pre;
 };
 
 // Waves a SIMD should hold.  bf16 keys leave registers for three, all but 2 to 19 that spill in 64-row items of
@@ -1295,8 +1232,8 @@ constexpr int kWaves = sizeof(T) <= 2 && DT <= 4 && NR == 1 ? 3 : 2;
 
 template <class T, int DT, int NR, int W>
 __global__ void __launch_bounds__(64 * W, (kWaves<T, DT, NR>)) paged_mha_tile_kernel(MhaArgs a) {
-  __shared__ __attribute__((aligned(1024))) TileLds<T, DT, W> lds;
-  tile_item<T, DT, NR, W>(a, lds);
+  __shared__ __attribute__((aligned(1024))) ManyLds<T, DT, W> lds;
+  many_item<T, DT, NR, W>(a, lds);
 }
 
 // A decode step of many sequences in one launch: the prefix's items, bound by their products, beside the
@@ -1307,7 +1244,7 @@ template <class T, int DT, int R, int PRE>
 __global__ void __launch_bounds__(64 * NW, (PRE == 64 ? kWaves<T, DT, 1> : 2)) paged_mha_step_kernel(MhaArgs a) {
   __shared__ __attribute__((aligned(1024))) StepLds<T, DT, R, PRE> lds;
   if (PRE > 0 && (int)blockIdx.x < a.p_items) {
-    if constexpr (PRE == 64) tile_item<T, DT, 1, NW>(a, lds.pre);
+    if constexpr (PRE == 64) many_item<T, DT, 1, NW>(a, lds.pre);
     if constexpr (PRE == 16) rows_item<T, DT>(a, lds.pre);
     return;
   }
