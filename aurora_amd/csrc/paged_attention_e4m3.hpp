@@ -286,7 +286,7 @@ struct ByteGeo {
 template <int DT, int W>
 struct ByteLds {
   using G = ByteGeo<DT, W>;
-  char k[G::KT * G::KROW], v[DT * 16 * G::KT * 2];
+  char k[2][G::KT * G::KROW], v[2][DT * 16 * G::KT * 2];  // of this tile and the next
   long long offset[3][G::KT];  // in bytes, of the keys of this tile and the next two in the pools
   unsigned long long have[3];  // which of them are there
   __attribute__((aligned(16))) float scale[3][2][G::KT];  // K's and V's, relative to …
@@ -296,8 +296,6 @@ template <int DT, int NR, int W>
 __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>& lds) {
   using G = ByteGeo<DT, W>;
   constexpr int KT = G::KT, KC = G::KC, NI = G::NI, NK = KT / 16;
-  char* const ks = lds.k;
-  char* const vs = lds.v;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = lane >> 4, l16 = lane & 15;
 
@@ -390,7 +388,9 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
   HalfQueries<DT, NR> q;
   q.load(rows, a.dh, g, a.scale * LOG2E);
 
-  auto lay_down = [&](int slot) {
+  auto lay_down = [&](int slot, int buffer) {
+    char* const ks = lds.k[buffer];
+    char* const vs = lds.v[buffer];
     const Reference next{__builtin_amdgcn_readfirstlane(lds.ref[slot].k), __builtin_amdgcn_readfirstlane(lds.ref[slot].v)};
     if (next.k != ref.k) q.relative_to(next.k);
     if (next.v != ref.v && ref.v >= 0) {
@@ -436,7 +436,9 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
     }
   };
 
-  auto compute = [&](int x, unsigned long long there, auto some) {
+  auto compute = [&](int x, unsigned long long there, int buffer, auto some) {
+    const char* const ks = lds.k[buffer];
+    const char* const vs = lds.v[buffer];
     floatx4 st[NR][NK];
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
@@ -508,21 +510,29 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
     }
   };
 
-  int slot = 0;
+  // A tile is laid down by each wave as it is done with the last one: one barrier a tile, and the waves that
+  // still work on the last one use the matrix cores meanwhile.
+  lay_down(0, 0);
+  place(2);
+  __syncthreads();
+  int slot = 0, buffer = 0;
   for (int x = it.x0; x < it.x1; x += KT) {
-    if (x > it.x0) __syncthreads();  // every wave is done with the last tile
-    lay_down(slot);
     const unsigned long long there = have;
-    const int next = slot == 2 ? 0 : slot + 1;
-    place(next == 2 ? 0 : next + 1);
-    __syncthreads();
-    if (x + KT < it.x1) load(next);
-    slot = next;
-    if (x >= vmax) continue;  // none of the wave's rows sees this tile
-    if (there != ~0ull || x + KT > rows.vmin)
-      compute(x, there, std::true_type{});
-    else
-      compute(x, there, std::false_type{});
+    slot = slot == 2 ? 0 : slot + 1;
+    const bool more = x + KT < it.x1;
+    if (more) load(slot);
+    if (x < vmax) {  // else none of the wave's rows sees this tile
+      if (there != ~0ull || x + KT > rows.vmin)
+        compute(x, there, buffer, std::true_type{});
+      else
+        compute(x, there, buffer, std::false_type{});
+    }
+    if (more) {
+      buffer ^= 1;
+      lay_down(slot, buffer);
+      place(slot == 0 ? 2 : slot - 1);  // two tiles ahead: where the last one's places were
+      __syncthreads();
+    }
   }
   const bool exact = __syncthreads_or(!fits);
   const float back = ldexpf(1.f, ref.v - 127);
