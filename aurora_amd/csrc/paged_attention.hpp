@@ -1228,7 +1228,7 @@ union StepLds {
 // 43.5; 30 of 32 heads on 8, prefix 4096 19.7 and 21.9; 64 on 32768 82 and 77.6, without own keys 48.6 and 51;
 // of d_head 48 on 16384 63.2 and 61.6; tails of 30 to 60 tokens on 2048 51.4 and 49.5.
 template <class T, int DT, int NR>
-constexpr int kWaves = sizeof(T) <= 2 && DT <= 4 && NR == 1 ? 3 : 2;
+constexpr int kWaves = sizeof(T) == 2 && DT <= 4 && NR == 1 ? 3 : 2;
 
 template <class T, int DT, int NR, int W>
 __global__ void __launch_bounds__(64 * W, (kWaves<T, DT, NR>)) paged_mha_tile_kernel(MhaArgs a) {
