@@ -67,10 +67,9 @@ __device__ __forceinline__ void move(const AppendArgs& a, const float* src, T* d
   put(dst + 4 * u + half, y * c + x * s);
 }
 
-// Block `block` of a grid of blocks_per_token of them for each row.
 template <class T>
-__device__ __forceinline__ void append_rows(const AppendArgs& a, int block, int blocks_per_token) {
-  const int t = block / blocks_per_token;
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_per_token) {
+  const int t = blockIdx.x / blocks_per_token;
   const int s = sequence_of(a.b, t);
   if (s >= a.b.b) return;  // a row behind the last sequence
   const Seq q = sequence(a.b, s);
@@ -80,7 +79,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, int block, int 
   if (j < 0) return;  // fewer own tokens than new ones: this one has no place
   const float* tab = a.table + (size_t)(a.b.prefix_len + j) * a.rot;
   const int per_rot = a.dh / 4 - (a.pairs ? 0 : a.rot / 8);  // units of a rotated head
-  int u = (block % blocks_per_token) * 256 + threadIdx.x;
+  int u = (blockIdx.x % blocks_per_token) * 256 + threadIdx.x;
   if (u < a.H * per_rot) {
     if (a.q_out) {
       const int h = u / per_rot;
@@ -103,11 +102,6 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, int block, int 
        tab, is_k && a.rot > 0);
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_per_token) {
-  append_rows<T>(a, blockIdx.x, blocks_per_token);
-}
-
 // ---------------------------------------------------------------- pools of e4m3
 
 // A unit is a block of 2^ssh tokens of one head of K or V.  Its new values' largest size m gives the least scale
@@ -117,32 +111,27 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_pe
 // NaN is held as NaN and has no part in m.
 //
 // A unit's new tokens lie in registers between its maximum and its rounding, so the rows are read once: one wave
-// holds up to 16 steps of 64 / LP tokens, LP lanes of 4 columns a head, and W = 4 waves share a unit that has
-// more.  Blocks walk over `chunk` rows of the batch each (no more than a block of tokens has, so that two of a
+// holds up to 8 steps of 64 / LP tokens, LP lanes of 4 columns a head, and W = 4 waves share a unit that has
+// more (up to 16 steps each).  Blocks walk over `chunk` rows of the batch each (no more than a block of tokens has, so that two of a
 // sequence's units at most begin there) and take the units that begin in them, their last rows may lie behind.
 struct UnitArgs {
   int chunk, n_chunks, groups;  // rows of a chunk; blocks of a chunk, 4 / W units each
-  int q_blocks;                 // blocks of a row of q
 };
 
-constexpr int kUnitSteps = 16;
+constexpr int kUnitSteps = 8;   // more hold registers that others' loads want: prompts of 1024 tokens 45 µs, with 16 57
+constexpr int kAtOnce = 2;      // steps whose loads are under way together (4: 46.5 µs)
 
-// Four columns of a head, rotated: every product is rounded before the sum, so that a value next to the border
-// of two e4m3 numbers falls where plain 32-bit arithmetic lets it fall.
-__device__ __forceinline__ floatx4 rotated4(const AppendArgs& a, const float* src, int col, const float* tab) {
+// Four columns of a head, x, rotated with y, the ones that are their pairs' other halves, by t0 and t1, their (cos,
+// sin): every product is rounded before the sum, so that a value next to the border of two e4m3 numbers falls
+// where plain 32-bit arithmetic lets it fall.
+__device__ __forceinline__ floatx4 rotated4(const AppendArgs& a, int col, floatx4 x, floatx4 y, floatx4 t0, floatx4 t1) {
 #pragma clang fp contract(off)
-  const floatx4 x = *reinterpret_cast<const floatx4*>(src + col);
   if (col >= a.rot) return x;
-  if (a.pairs) {
-    const floatx4 t = *reinterpret_cast<const floatx4*>(tab + col);
-    return floatx4{x[0] * t[0] - x[1] * t[1], x[1] * t[0] + x[0] * t[1], x[2] * t[2] - x[3] * t[3],
-                   x[3] * t[2] + x[2] * t[3]};
-  }
-  const int half = a.rot / 2, u = col < half ? col : col - half;
-  const floatx4 y = *reinterpret_cast<const floatx4*>(src + (col < half ? col + half : u));
-  const floatx4 t0 = *reinterpret_cast<const floatx4*>(tab + 2 * u), t1 = *reinterpret_cast<const floatx4*>(tab + 2 * u + 4);
+  if (a.pairs)
+    return floatx4{x[0] * t0[0] - x[1] * t0[1], x[1] * t0[0] + x[0] * t0[1], x[2] * t0[2] - x[3] * t0[3],
+                   x[3] * t0[2] + x[2] * t0[3]};
   const floatx4 c = {t0[0], t0[2], t1[0], t1[2]}, s = {t0[1], t0[3], t1[1], t1[3]};
-  return col < half ? x * c - y * s : x * c + y * s;
+  return col < a.rot / 2 ? x * c - y * s : x * c + y * s;
 }
 
 __device__ __forceinline__ unsigned round4(floatx4 x, int e) {  // of x·2^e
@@ -153,8 +142,24 @@ __device__ __forceinline__ unsigned round4(floatx4 x, int e) {  // of x·2^e
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
 }
 
-// LP lanes of a head, W waves of a unit.
-template <int LP, int W>
+__device__ __forceinline__ unsigned again4(unsigned x, int e) {  // … of four e4m3 numbers
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(x, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
+  return round4(floatx4{lo[0], lo[1], hi[0], hi[1]}, e);
+}
+// The largest size of the finite ones.
+__device__ __forceinline__ float size4(floatx4 x) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[e]) <= 3.402823466e38f ? fabsf(x[e]) : 0.f);
+  return m;
+}
+// The byte of the least scale for sizes up to m = f·2^x, f in [1, 2): 2^(x − 8), or 2^(x − 7) where f > 1.75.
+__device__ __forceinline__ int scale_for(float m) {
+  return min(max((int)((__float_as_uint(m) + 0x1fffffu) >> 23) - 8, 127 - 117), 127 + 119);
+}
+
+// LP lanes of a head, W waves of a unit, STEPS of each.
+template <int LP, int W, int STEPS>
 __device__ __forceinline__ void append_units(const AppendArgs& a, const UnitArgs& u, int block, float (&top)[4]) {
   constexpr int PER = 64 / LP;  // tokens of a wave's step
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -181,19 +186,46 @@ __device__ __forceinline__ void append_units(const AppendArgs& a, const UnitArgs
       const int row = (page << a.sh) + (j & ((1 << a.sh) - 1));
       uint8_t* const scale = (is_k ? a.ks : a.vs) + (on ? scale_index(row, h, a.Hkv, a.sh, a.ssh) : 0);
       const int held = old && on ? *scale : 0;
-      floatx4 x[kUnitSteps];
+      floatx4 x[STEPS];
       float m = 0.f;
+      // Lanes behind the head or the last token hold another's values: no branch stands between the loads.
+      const int c = min(col, a.dh - 4), half = a.rot / 2;
+      // where column c's partners and angles are (those of column 0 for a column that is not rotated)
+      const bool turns = is_k && c < a.rot;
+      const int cy = !turns || a.pairs ? c : c < half ? c + half : c - half;
+      const int ct = !turns ? 0 : a.pairs ? c : 2 * (c < half ? c : c - half);
+      auto place = [&](int n) { return min((n * W + w % W) * PER + lane / LP, count - 1); };
+      auto take = [&](int n, floatx4 y) {
+        x[n] = y;
+        m = fmaxf(m, size4(y));
+      };
+      if (on) {
 #pragma unroll
-      for (int n = 0; n < kUnitSteps; ++n) {
-        const int k = (n * W + w % W) * PER + lane / LP;
-        x[n] = floatx4{0.f, 0.f, 0.f, 0.f};
-        if (n * PER * W < count && live && k < count) {
-          const float* p = src + (size_t)(q.lo + i + k) * a.ld_kv;
-          x[n] = is_k ? rotated4(a, p, col, a.table + (size_t)(a.b.prefix_len + j + k) * a.rot)
-                      : *reinterpret_cast<const floatx4*>(p + col);
-        }
+        for (int n0 = 0; n0 < STEPS; n0 += kAtOnce)
+          if (n0 * PER * W < count) {
+            if (is_k && a.rot > 0) {
+              floatx4 f[kAtOnce], y[kAtOnce], t0[kAtOnce], t1[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[n][e]) <= 3.402823466e38f ? fabsf(x[n][e]) : 0.f);
+              for (int n = 0; n < kAtOnce; ++n) {
+                const int k = place(n0 + n);
+                const float* p = src + (size_t)(q.lo + i + k) * a.ld_kv;
+                const float* tab = a.table + (size_t)(a.b.prefix_len + j + k) * a.rot + ct;
+                f[n] = *reinterpret_cast<const floatx4*>(p + c);
+                y[n] = *reinterpret_cast<const floatx4*>(p + cy);
+                t0[n] = *reinterpret_cast<const floatx4*>(tab);
+                t1[n] = *reinterpret_cast<const floatx4*>(a.pairs ? tab : tab + 4);
+              }
+#pragma unroll
+              for (int n = 0; n < kAtOnce; ++n) take(n0 + n, rotated4(a, c, f[n], y[n], t0[n], t1[n]));
+            } else {
+              floatx4 f[kAtOnce];
+#pragma unroll
+              for (int n = 0; n < kAtOnce; ++n)
+                f[n] = *reinterpret_cast<const floatx4*>(src + (size_t)(q.lo + i + place(n0 + n)) * a.ld_kv + c);
+#pragma unroll
+              for (int n = 0; n < kAtOnce; ++n) take(n0 + n, f[n]);
+            }
+          }
       }
 #pragma unroll
       for (int o = 1; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
@@ -203,17 +235,14 @@ __device__ __forceinline__ void append_units(const AppendArgs& a, const UnitArgs
         m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         __syncthreads();
       }
-      // m = f·2^x with f in [1, 2): e = x - 8, or x - 7 where f > 1.75
-      const int least = (int)((__float_as_uint(m) + 0x1fffffu) >> 23) - 8;
-      const int byte = max(min(max(least, 127 - 117), 127 + 119), held);
+      const int byte = max(scale_for(m), held);
       if (live && old && byte > held)
         for (int k = (w % W) * PER + lane / LP; k < old; k += PER * W) {
           unsigned* p = reinterpret_cast<unsigned*>(pool + (size_t)(row - old + k) * ld + col);
-          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(*p, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(*p, true);
-          *p = round4(floatx4{lo[0], lo[1], hi[0], hi[1]}, held - byte);
+          *p = again4(*p, held - byte);
         }
 #pragma unroll
-      for (int n = 0; n < kUnitSteps; ++n) {
+      for (int n = 0; n < STEPS; ++n) {
         const int k = (n * W + w % W) * PER + lane / LP;
         if (n * PER * W < count && live && k < count) *reinterpret_cast<unsigned*>(pool + (size_t)(row + k) * ld + col) = round4(x[n], 127 - byte);
       }
@@ -222,38 +251,143 @@ __device__ __forceinline__ void append_units(const AppendArgs& a, const UnitArgs
   }
 }
 
-// Blocks of the chunks' units, then those of q's rows.
-template <int LP, int W>
+// Blocks of fewer tokens than a step has (S·LP < 64): a wave takes STEPS whole steps of tokens, aligned to them,
+// and every S·LP of its lanes have a block.  Lanes of a block's older tokens round those again.
+template <int LP, int STEPS>
+__device__ __forceinline__ void append_spans(const AppendArgs& a, const UnitArgs& u, int block) {
+  constexpr int PER = 64 / LP, SPAN = PER * STEPS;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, S = 1 << a.ssh, group = LP << a.ssh;
+  const int r0 = block / u.groups * u.chunk, r1 = min(r0 + u.chunk, a.b.n_tok);
+  const int unit = block % u.groups * 4 + w;
+  const bool is_k = unit < a.Hkv, on = unit < 2 * a.Hkv;
+  const int h = is_k ? unit : unit - a.Hkv, col = 4 * (lane % LP), c = min(col, a.dh - 4);
+  const float* const src = (is_k ? a.k : a.v) + (size_t)h * a.dh;
+  uint8_t* const pool = static_cast<uint8_t*>(is_k ? a.kp : a.vp) + (size_t)h * a.dh;
+  const size_t ld = (size_t)a.Hkv * a.dh;
+  const int half = a.rot / 2;
+  const bool turns = is_k && c < a.rot;
+  const int cy = !turns || a.pairs ? c : c < half ? c + half : c - half;
+  const int ct = !turns ? 0 : a.pairs ? c : 2 * (c < half ? c : c - half);
+  for (int s = sequence_of(a.b, r0); s < a.b.b; ++s) {
+    const Seq q = sequence(a.b, s);
+    if (q.lo >= r1) break;
+    const int past = q.len - q.n, first = max(0, -past);
+    int i = max(first, r0 - q.lo);
+    if (i > first) i += -(past + i) & (SPAN - 1);
+    for (; i < q.n && q.lo + i < r1; i += SPAN - ((past + i) & (SPAN - 1))) {
+      if (!on) continue;
+      const int j = past + i, end = j + min(SPAN - (j & (SPAN - 1)), q.n - i), first_block = j >> a.ssh;
+      const int j0 = (j & ~(SPAN - 1)) + lane / LP;  // the lane's token of the first step
+#pragma unroll
+      for (int n0 = 0; n0 < STEPS; n0 += kAtOnce) {
+        if (j0 - lane / LP + n0 * PER >= end || j0 - lane / LP + (n0 + kAtOnce) * PER <= (first_block << a.ssh)) continue;
+        floatx4 f[kAtOnce], y[kAtOnce], t0[kAtOnce], t1[kAtOnce];
+        int page[kAtOnce];
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          const int at = min(max(j0 + (n0 + n) * PER, j), end - 1);  // (others' tokens where the lane has none)
+          const float* p = src + (size_t)(q.lo + i + at - j) * a.ld_kv;
+          f[n] = *reinterpret_cast<const floatx4*>(p + c);
+          if (is_k && a.rot > 0) {
+            const float* tab = a.table + (size_t)(a.b.prefix_len + at) * a.rot + ct;
+            y[n] = *reinterpret_cast<const floatx4*>(p + cy);
+            t0[n] = *reinterpret_cast<const floatx4*>(tab);
+            t1[n] = *reinterpret_cast<const floatx4*>(a.pairs ? tab : tab + 4);
+          }
+          page[n] = a.b.pages[(size_t)s * a.b.max_pages + (at >> a.sh)];
+        }
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          const int at = j0 + (n0 + n) * PER;
+          const floatx4 x = is_k && a.rot > 0 ? rotated4(a, c, f[n], y[n], t0[n], t1[n]) : f[n];
+          const bool fresh = at >= j && at < end;
+          float m = fresh ? size4(x) : 0.f;
+          for (int o = 1; o < group; o *= 2) m = fmaxf(m, __shfl_xor(m, o, 64));
+          // (a block lies in one page, that of its new tokens)
+          const bool there = at >> a.ssh >= first_block && at >> a.ssh <= (end - 1) >> a.ssh &&
+                             (unsigned)page[n] < (unsigned)a.n_pages;
+          if (!there) continue;
+          const int row = (page[n] << a.sh) + (at & ((1 << a.sh) - 1));
+          uint8_t* const scale = (is_k ? a.ks : a.vs) + scale_index(row, h, a.Hkv, a.sh, a.ssh);
+          const bool older = at >> a.ssh == first_block && (j & (S - 1));
+          const int held = older ? *scale : 0, byte = max(scale_for(m), held);
+          unsigned* const to = reinterpret_cast<unsigned*>(pool + (size_t)row * ld + c);
+          if (col < a.dh && fresh)
+            *to = round4(x, 127 - byte);
+          else if (col < a.dh && at < j && byte > held)
+            *to = again4(*to, held - byte);
+          if (lane % group == 0 && (!older || byte > held)) *scale = (uint8_t)byte;
+        }
+      }
+    }
+  }
+}
+
+// A piece of q to a thread: the units of move(), whatever rows a block's pieces lie in.
+__device__ __forceinline__ void rotate_q(const AppendArgs& a, int block) {
+  const int per_rot = a.dh / 4 - (a.pairs ? 0 : a.rot / 8), per_row = a.H * per_rot;
+  const long long first = (long long)block * 256;
+  int t = (int)(first / per_row), u = (int)(first - (long long)t * per_row) + threadIdx.x;
+  int s = sequence_of(a.b, t);  // of the block's first row
+  t += u / per_row;
+  u %= per_row;
+  if (t >= a.b.n_tok) return;
+  while (s < a.b.b && a.b.tok_off[s + 1] <= t) ++s;
+  if (s >= a.b.b) return;  // a row behind the last sequence
+  const Seq q = sequence(a.b, s);
+  const int i = t - q.lo, j = q.len - q.n + i;
+  if (i < 0 || i >= q.n || j < 0) return;
+  const int h = u / per_rot;
+  move(a, a.q + (size_t)t * a.ld_q + h * a.dh, a.q_out + (size_t)t * a.ld_qo + h * a.dh, u - h * per_rot,
+       a.table + (size_t)(a.b.prefix_len + j) * a.rot, a.rot > 0);
+}
+
+// Blocks of the chunks' units, then those of q's rows.  W = 0: spans of small blocks.
+template <int LP, int W, int STEPS>
 __global__ void __launch_bounds__(256) append_e4m3_kernel(AppendArgs a, UnitArgs u) {
   __shared__ float top[4];
   const int block = blockIdx.x, units = u.n_chunks * u.groups;
-  if (block < units) {
-    append_units<LP, W>(a, u, block, top);
-  } else {
-    AppendArgs q = a;
-    q.Hkv = 0;
-    append_rows<float>(q, block - units, u.q_blocks);
+  if (block >= units)
+    rotate_q(a, block - units);
+  else if constexpr (W > 0)
+    append_units<LP, W, STEPS>(a, u, block, top);
+  else
+    append_spans<LP, STEPS>(a, u, block);
+}
+
+template <int LP>
+void launch_e4m3_lanes(const AppendArgs& a, const UnitArgs& u, int waves, int steps, unsigned blocks, hipStream_t st) {
+  auto* kernel = append_e4m3_kernel<LP, 1, kUnitSteps>;
+  if constexpr (LP < 64) {
+    if (waves == 0) kernel = append_e4m3_kernel<LP, 0, kUnitSteps>;
   }
+  if constexpr (LP >= 8) {  // 128 tokens of a block: LP·128 > 64·kUnitSteps
+    if (waves == 4) kernel = append_e4m3_kernel<LP, 4, kUnitSteps>;
+  }
+  if constexpr (LP == 32) {
+    if (waves == 4 && steps > kUnitSteps) kernel = append_e4m3_kernel<LP, 4, 2 * kUnitSteps>;
+  }
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, st, a, u);
 }
 
 int launch_e4m3(aur_ctx* ctx, const char* who, const AppendArgs& a) {
   int lp = 2;
   while (4 * lp < a.dh) lp *= 2;
-  const int S = 1 << a.ssh, waves = S * lp > 64 * kUnitSteps ? 4 : 1;
+  const int S = 1 << a.ssh, waves = S * lp < 64 ? 0 : S * lp > 64 * kUnitSteps ? 4 : 1;
+  const int steps = waves ? S * lp / (64 * waves) : kUnitSteps, run = waves ? S : 64 / lp * kUnitSteps;
   UnitArgs u;
-  u.chunk = a.b.max_tok < S ? a.b.max_tok : S;
+  u.chunk = a.b.max_tok < run ? a.b.max_tok : run;
   u.n_chunks = (a.b.n_tok + u.chunk - 1) / u.chunk;
-  u.groups = (2 * a.Hkv * waves + 3) / 4;
+  u.groups = (2 * a.Hkv * (waves ? waves : 1) + 3) / 4;
   const int per_rot = a.dh / 4 - (a.pairs ? 0 : a.rot / 8);
-  u.q_blocks = (a.H * per_rot + 255) / 256;
-  const uint64_t blocks = (uint64_t)u.n_chunks * u.groups + (uint64_t)a.b.n_tok * u.q_blocks;
+  const uint64_t blocks = (uint64_t)u.n_chunks * u.groups + ((uint64_t)a.b.n_tok * a.H * per_rot + 255) / 256;
   if (blocks > kMaxBlocks) return aur::set_error(ctx, AUR_ELIMIT, "%s: n_tok=%d rows of %d heads", who, a.b.n_tok, a.H);
-  auto* kernel = lp == 2    ? append_e4m3_kernel<2, 1>
-                 : lp == 4  ? append_e4m3_kernel<4, 1>
-                 : lp == 8  ? append_e4m3_kernel<8, 1>
-                 : lp == 16 ? (waves == 1 ? append_e4m3_kernel<16, 1> : append_e4m3_kernel<16, 4>)
-                            : (waves == 1 ? append_e4m3_kernel<32, 1> : append_e4m3_kernel<32, 4>);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a, u);
+  auto* launch = lp == 2    ? launch_e4m3_lanes<2>
+                 : lp == 4  ? launch_e4m3_lanes<4>
+                 : lp == 8  ? launch_e4m3_lanes<8>
+                 : lp == 16 ? launch_e4m3_lanes<16>
+                            : launch_e4m3_lanes<32>;
+  launch(a, u, waves, steps, (unsigned)blocks, ctx->stream);
   AUR_LAUNCH_CHECK(ctx, "append_e4m3_kernel");
   return 0;
 }

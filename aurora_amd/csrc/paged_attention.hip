@@ -76,11 +76,11 @@ size_t ws_floats(const Plan& p, const Batch& b, int H, int dh) {
 
 Sizes sizes_of(const Batch& b, const aur_paged_cache& c, uint32_t n_head) {
   return {b.b, b.n_tok, b.max_tok, b.max_own, b.prefix_len, (int)c.n_kv_head, (int)(n_head / c.n_kv_head), (int)c.d_head,
-          c.dtype == AUR_PAGED_F32};
+          c.dtype == AUR_PAGED_F32, c.dtype == AUR_PAGED_E4M3};
 }
 
 void launch_items(const MhaArgs& a, const Sizes& z, int p_tile, int tile, unsigned items, hipStream_t st) {
-  (z.f32 ? launch_items_f32 : a.k_scale ? launch_items_e4m3 : launch_items_bf16)(a, z, p_tile, tile, items, st);
+  (z.f32 ? launch_items_f32 : z.e4m3 ? launch_items_e4m3 : launch_items_bf16)(a, z, p_tile, tile, items, st);
 }
 
 }  // namespace

@@ -12,6 +12,7 @@ struct Sizes {
   int b, n_tok, max_tok, max_own, prefix_len;  // of the batch (max_tok up to n_tok)
   int Hkv, G, dh;                              // K/V heads, query heads of each, columns
   bool f32;
+  bool e4m3 = false;
 };
 // How it is cut; the scratch's size follows from it.  Tiles are an item's rows, splits the ranges of an
 // axis, of so many keys each; p_ the prefix's items (pooled: 0 of them otherwise), o_ a sequence's own.
@@ -40,6 +41,10 @@ constexpr int kItems16 = 768, kItemsWide = 512, kItems = 1024, kItems8 = 256;
 // of tiles: 6 of 185 rows on 465, one head, 36 µs against 20).
 constexpr int kWhole16 = 384, kWhole = 256, kWholeFull = 512, kFill = 256;
 constexpr int kLeastKeys = 128, kMostRanges = 48;
+// e4m3 keys: a CU holds two of their larger items, which take their keys faster (tails of 66 to 122 on 2048, 16
+// heads of 64: 71 µs with 512 items, 78 with 1024), and ranges of 256 keys (the prefix of 4999 alone, 48
+// sequences of 16 heads on 4 of 128: 23 µs, with 128 keys 29; d_head 64 with their own keys 32.5 and 31.4).
+constexpr int kItemsE4m3 = 512, kLeastKeysE4m3 = 256;
 // With little work the time is a block's chain of tiles, not the products: smaller items then.  16 rows up
 // to so many items of 16 rows by 128 keys (5 sequences of 74 rows on 434 keys, 3 heads of 48, bf16, 300 of
 // them: 9.9 µs, in 128 rows 14, in 64 rows 11.7; at 1024 a batch took 15 instead of 11), 64 rows where items
@@ -82,11 +87,12 @@ inline Plan make_plan(const Sizes& b) {
   // (A CU holds one block of 8 waves: more of them than CUs would be a second round.)
   auto eight = [dh](int tile) { return tile == 256 || (tile == 128 && dh > 64); };
   const int items16 = b.f32 && (dh > 64 || !p.pooled) ? kItemsWide : kItems16;
-  auto items = [&](int tile) { return eight(tile) ? kItems8 : tile > 16 ? kItems : items16; };
+  const int four = b.e4m3 ? kItemsE4m3 : kItems, least = b.e4m3 ? kLeastKeysE4m3 : kLeastKeys;
+  auto items = [&](int tile) { return eight(tile) ? kItems8 : tile > 16 ? four : items16; };
   auto cut = [&](int n, double axes, double want, int tile, int* keys) {
     int splits = 1;
     if (n > (tile == 16 ? kWhole16 : axes >= kFill ? kWholeFull : kWhole)) {
-      const int most = std::min(kMostRanges, (n + kLeastKeys - 1) / kLeastKeys);
+      const int most = std::min(kMostRanges, (n + least - 1) / least);
       const double parts = n / want;
       splits = (int)std::min((double)most, std::max(1.0, eight(tile) ? parts : std::ceil(parts)));
     }

@@ -127,3 +127,22 @@ def test_sample_definitions_agree():
     # all of it: the token's share
     a, lp, _ = sample(np.log([1.0, 2.0, 5.0]), 0.3)
     assert a == 1 and abs(lp - np.log(2 / 8)) < 1e-12
+
+
+def test_every_kernel_is_reached(tmp_path):
+    """The batches that the GPU tests run on 8-bit pools reach all kernels, as the planner cuts them."""
+    import subprocess
+
+    from tests.paged_tiles import ALL, D_HEADS, ROOT, every_kernel, kernels
+    from tests.test_paged_plan import FIELDS
+
+    exe = tmp_path / "plan"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-o", str(exe),
+                    str(ROOT / "tests" / "cpp" / "paged_plan_e4m3.cpp")], check=True)
+    calls = [(len(b.n), sum(b.n), max(b.n), max(b.length), b.prefix, b.kv, b.group, dh) for b in ALL.values() for dh in D_HEADS]
+    res = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, c)) for c in calls), capture_output=True, text=True,
+                         check=True, timeout=60)
+    got = set()
+    for line in res.stdout.splitlines():
+        got |= kernels(dict(zip(FIELDS, map(int, line.split()))))
+    assert got == every_kernel(False), (every_kernel(False) - got, got - every_kernel(False))
