@@ -35,38 +35,58 @@ __device__ __forceinline__ floatx4 get(const e4m3* p, float scale) {
   return floatx4{lo[0], lo[1], hi[0], hi[1]};
 }
 
-// Rows blockIdx.y and every gridDim.y-th after it of one sequence; of a row the units of 4 columns that the
-// block's threads reach.
+// A block has ROWS rows to a thread of one sequence, units of 4 columns of them; their pages' numbers, then their
+// scales and elements, are under way together.
+constexpr int ROWS = 4;
 template <class T>
-__global__ void __launch_bounds__(256) read_kernel(ReadArgs a) {
-  const int s = blockIdx.x % a.b.b, d4 = a.Hkv * a.dh / 4;
+__global__ void __launch_bounds__(256) read_kernel(ReadArgs a, int lanes, int turns) {
+  const int s = blockIdx.x / turns, d4 = a.Hkv * a.dh / 4;
   const int len = min(max(a.b.own_len[s], 0), a.b.max_own);
-  const int u0 = threadIdx.x % min(d4, 256), lead = threadIdx.x / min(d4, 256), rows = 256 / min(d4, 256);
-  if (lead >= rows) return;
-  for (int i = (blockIdx.x / a.b.b) * rows + lead; i < a.count; i += gridDim.x / a.b.b * rows) {
-    const int x = a.first + i, own = x - a.b.prefix_len;
-    int page = -1;
-    if (own < 0)
-      page = a.b.prefix_pages[x >> a.sh];
-    else if (own < len)
-      page = a.b.pages[(size_t)s * a.b.max_pages + (own >> a.sh)];
-    const bool there = (unsigned)page < (unsigned)a.n_pages;
-    const int row = there ? (page << a.sh) + ((own < 0 ? x : own) & ((1 << a.sh) - 1)) : 0;
-    const size_t from = (size_t)row * a.Hkv * a.dh, to = ((size_t)s * a.count + i) * a.ld;
-    for (int u = u0; u < d4; u += 256) {
-      floatx4 k = {0.f, 0.f, 0.f, 0.f}, v = k;
-      if (there) {
-        float ks = 1.f, vs = 1.f;
-        if (sizeof(T) == 1) {
-          const size_t at = scale_index(row, 4 * u / a.dh, a.Hkv, a.sh, a.ssh);
-          ks = scale_of(a.ks[at]);
-          vs = scale_of(a.vs[at]);
-        }
-        if (a.k) k = get(static_cast<const T*>(a.kp) + from + 4 * u, ks);
-        if (a.v) v = get(static_cast<const T*>(a.vp) + from + 4 * u, vs);
+  const int u0 = threadIdx.x % lanes, per = 256 / lanes, lead = threadIdx.x / lanes;
+  if (lead >= per) return;
+  const int i0 = (blockIdx.x - s * turns) * ROWS * per + lead;
+  int row[ROWS];  // in the pools, −1: no key
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int x = a.first + i0 + r * per, own = x - a.b.prefix_len;
+    const bool is = i0 + r * per < a.count;
+    row[r] = -1;
+    if (is && own < 0)
+      row[r] = a.b.prefix_pages[x >> a.sh];
+    else if (is && own < len)
+      row[r] = a.b.pages[(size_t)s * a.b.max_pages + (own >> a.sh)];
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int x = a.first + i0 + r * per, own = x - a.b.prefix_len;
+    row[r] = (unsigned)row[r] < (unsigned)a.n_pages ? (row[r] << a.sh) + ((own < 0 ? x : own) & ((1 << a.sh) - 1)) : -1;
+  }
+  for (int u = u0; u < d4; u += lanes) {
+    const int head = sizeof(T) == 1 ? 4 * u / a.dh : 0;
+    floatx4 k[ROWS], v[ROWS];
+    float ks[ROWS], vs[ROWS];
+    if (sizeof(T) == 1) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const size_t at = scale_index(max(row[r], 0), head, a.Hkv, a.sh, a.ssh);
+        ks[r] = scale_of(a.ks[at]);
+        vs[r] = scale_of(a.vs[at]);
       }
-      if (a.k) *reinterpret_cast<floatx4*>(a.k + to + 4 * u) = k;
-      if (a.v) *reinterpret_cast<floatx4*>(a.v + to + 4 * u) = v;
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {  // (where no key is, row 0's, and not written)
+      const size_t from = (size_t)max(row[r], 0) * a.Hkv * a.dh + 4 * u;
+      k[r] = v[r] = floatx4{0.f, 0.f, 0.f, 0.f};
+      if (a.k) k[r] = get(static_cast<const T*>(a.kp) + from, ks[r]);
+      if (a.v) v[r] = get(static_cast<const T*>(a.vp) + from, vs[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int i = i0 + r * per;
+      if (i >= a.count) break;
+      const size_t to = ((size_t)s * a.count + i) * a.ld + 4 * u;
+      if (a.k) __builtin_nontemporal_store(row[r] < 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : k[r], reinterpret_cast<floatx4*>(a.k + to));
+      if (a.v) __builtin_nontemporal_store(row[r] < 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : v[r], reinterpret_cast<floatx4*>(a.v + to));
     }
   }
 }
@@ -96,18 +116,18 @@ extern "C" int aur_kv_read_paged(aur_ctx* ctx, const aur_paged_cache* cache, con
   a.kp = cache->k; a.vp = cache->v; a.k = k_out; a.v = v_out;
   a.Hkv = (int)cache->n_kv_head; a.dh = (int)cache->d_head; a.n_pages = (int)cache->n_pages;
   a.sh = log2_of(cache->page_len); a.ld = (int)ld; a.first = (int)first; a.count = (int)count;
-  const int d4 = (int)row / 4, rows = 256 / (d4 < 256 ? d4 : 256);
-  const uint32_t turns = (count + rows - 1) / rows;
-  if (a.b.b > (int)(kMaxBlocks / 2)) return aur::set_error(ctx, AUR_ELIMIT, "%s: b=%d", who, a.b.b);
-  const uint32_t most = kMaxBlocks / (uint32_t)a.b.b;
-  const dim3 grid((turns < most ? turns : most) * (uint32_t)a.b.b);
+  const int d4 = (int)row / 4, lanes = d4 < 256 ? d4 : 256, rows = ROWS * (256 / lanes);
+  const int turns = ((int)count + rows - 1) / rows;
+  if ((uint64_t)turns * a.b.b > kMaxBlocks)
+    return aur::set_error(ctx, AUR_ELIMIT, "%s: %u keys of %d sequences", who, count, a.b.b);
+  const dim3 grid((unsigned)(turns * a.b.b));
   if (cache->dtype == AUR_PAGED_F32) {
-    hipLaunchKernelGGL(read_kernel<float>, grid, dim3(256), 0, ctx->stream, a);
+    hipLaunchKernelGGL(read_kernel<float>, grid, dim3(256), 0, ctx->stream, a, lanes, turns);
   } else if (cache->dtype == AUR_PAGED_BF16) {
-    hipLaunchKernelGGL(read_kernel<__bf16>, grid, dim3(256), 0, ctx->stream, a);
+    hipLaunchKernelGGL(read_kernel<__bf16>, grid, dim3(256), 0, ctx->stream, a, lanes, turns);
   } else {
     a.ks = cache->k_scale; a.vs = cache->v_scale; a.ssh = log2_of(cache->scale_len);
-    hipLaunchKernelGGL(read_kernel<e4m3>, grid, dim3(256), 0, ctx->stream, a);
+    hipLaunchKernelGGL(read_kernel<e4m3>, grid, dim3(256), 0, ctx->stream, a, lanes, turns);
   }
   AUR_LAUNCH_CHECK(ctx, "read_kernel");
   return 0;
