@@ -99,6 +99,8 @@ SIGNATURES: dict[str, tuple] = {
     "aur_model_generate_step": (_i32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_void_p]),
     "aur_model_generate_greedy": (_i32, [C.c_void_p, C.c_void_p, _u32, C.c_void_p]),
+    "aur_model_generate_sampled": (_i32, [C.c_void_p, C.c_void_p, _u32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 
 

@@ -11,8 +11,9 @@
 //   MhaKvCacheKernel           src/gpu/kv_cache.rs:366-466
 //   DecoderTransformerGpu      src/gpu/transformer.rs:32-116 (train step, KV decode)
 //   KvCacheGpu                 src/gpu/kv_cache.rs:21-92
-//   PagedKvCache, PagedBatch, RotaryTableKernel, PagedKvAppendKernel, PagedMhaKernel
-//                              (no counterpart: a paged K/V cache with a shared prefix)
+//   PagedKvCache, PagedBatch, RotaryTableKernel, PagedKvAppendKernel, PagedKvReadKernel,
+//   PagedMhaKernel             (no counterpart: a paged K/V cache with a shared prefix)
+//   SampleKernel               (no counterpart: the next tokens from logits and random numbers)
 //
 // Kernel structs keep the reference's argument order and its contract:
 // `dispatch_into` only enqueues on the context's stream, buffers belong to
@@ -102,9 +103,10 @@ class GpuBuffer {
 // buffer shorter than that is refused here, where its length is known (the
 // reference's WGSL had wgpu's bounds-checked buffer access instead — an
 // out-of-range access on the GPU faults).
-inline void need(const GpuBuffer<float>& b, size_t n, const char* what) {
+template <class T>
+void need(const GpuBuffer<T>& b, size_t n, const char* what) {
   if (b.len() < n)
-    throw Error(std::string(what) + ": buffer of " + std::to_string(b.len()) + " floats, " +
+    throw Error(std::string(what) + ": buffer of " + std::to_string(b.len()) + " elements, " +
                     std::to_string(n) + " needed",
                 AUR_EINVAL);
 }
@@ -207,8 +209,28 @@ struct PagedKvCache {
       : k(GpuBuffer<T>::zeros(c, (size_t)n_pages * page_len * n_kv_head * d_head)),
         v(GpuBuffer<T>::zeros(c, (size_t)n_pages * page_len * n_kv_head * d_head)),
         raw{k.ptr(),   v.ptr(), n_pages, page_len, n_kv_head, d_head,
-            sizeof(T) == 4 ? AUR_PAGED_F32 : AUR_PAGED_BF16} {
+            sizeof(T) == 4 ? AUR_PAGED_F32 : AUR_PAGED_BF16, nullptr, nullptr, 0} {
     static_assert(sizeof(T) == 4 || sizeof(T) == 2, "fp32 or bf16");
+  }
+};
+
+// Pools of e4m3 bytes, with scales [n_pages, n_kv_head, page_len / scale_len].
+template <>
+struct PagedKvCache<uint8_t> {
+  GpuBuffer<uint8_t> k, v, k_scale, v_scale;
+  aur_paged_cache raw;
+  PagedKvCache(const GpuContext& c, uint32_t n_pages, uint32_t page_len, uint32_t n_kv_head, uint32_t d_head,
+               uint32_t scale_len)
+      : k(GpuBuffer<uint8_t>::zeros(c, (size_t)n_pages * page_len * n_kv_head * d_head)),
+        v(GpuBuffer<uint8_t>::zeros(c, (size_t)n_pages * page_len * n_kv_head * d_head)),
+        k_scale(GpuBuffer<uint8_t>::zeros(c, scales(n_pages, page_len, n_kv_head, scale_len))),
+        v_scale(GpuBuffer<uint8_t>::zeros(c, scales(n_pages, page_len, n_kv_head, scale_len))),
+        raw{k.ptr(), v.ptr(), n_pages, page_len, n_kv_head, d_head, AUR_PAGED_E4M3, k_scale.ptr(), v_scale.ptr(), scale_len} {}
+
+ private:
+  static size_t scales(uint32_t n_pages, uint32_t page_len, uint32_t n_kv_head, uint32_t scale_len) {
+    if (scale_len == 0 || page_len % scale_len != 0) throw Error("PagedKvCache: bad scale_len", AUR_EINVAL);
+    return (size_t)n_pages * n_kv_head * (page_len / scale_len);
   }
 };
 
@@ -260,6 +282,19 @@ struct PagedKvAppendKernel {
   }
 };
 
+// Keys [first, first + count) of every sequence's axis as dense rows [b * count, n_kv_head * d_head].
+struct PagedKvReadKernel {
+  template <class T>
+  void dispatch_into(const GpuContext& c, const PagedKvCache<T>& cache, const PagedBatch& batch,
+                     const GpuBuffer<float>& k_out, const GpuBuffer<float>& v_out, uint32_t first, uint32_t count) const {
+    const uint32_t row = cache.raw.n_kv_head * cache.raw.d_head;
+    need(k_out, (size_t)batch.raw.b * count * row, "PagedKvReadKernel k_out");
+    need(v_out, (size_t)batch.raw.b * count * row, "PagedKvReadKernel v_out");
+    check(c.raw(), aur_kv_read_paged(c.raw(), &cache.raw, &batch.raw, k_out.ptr(), v_out.ptr(), row, first, count),
+          "PagedKvReadKernel");
+  }
+};
+
 struct PagedMhaKernel {
   template <class T>
   static size_t scratch_len(const PagedKvCache<T>& cache, const PagedBatch& batch, uint32_t n_head) {
@@ -278,6 +313,32 @@ struct PagedMhaKernel {
           aur_mha_paged(c.raw(), &cache.raw, &batch.raw, q.ptr(), d, out.ptr(), d, lse.ptr(), scratch.ptr(),
                         4 * scratch.len(), n_head),
           "PagedMhaKernel");
+  }
+};
+
+// ------------------------------------------------------- choosing the next token
+
+// The next token of each of b rows of logits [b, vocab] from a random number u [b]; temperature, top_k, top_p and
+// min_p are arrays of b values or null (aur_sample).
+struct SampleKernel {
+  static size_t scratch_len(uint32_t b, uint32_t vocab) { return aur_sample_ws_bytes(b, vocab); }
+  void dispatch_into(const GpuContext& c, const GpuBuffer<float>& logits, const GpuBuffer<float>& u,
+                     const GpuBuffer<int32_t>& tokens, const GpuBuffer<float>& logprob, const GpuBuffer<uint8_t>& scratch,
+                     uint32_t b, uint32_t vocab, const GpuBuffer<float>* temperature = nullptr,
+                     const GpuBuffer<int32_t>* top_k = nullptr, const GpuBuffer<float>* top_p = nullptr,
+                     const GpuBuffer<float>* min_p = nullptr) const {
+    need(logits, (size_t)b * vocab, "SampleKernel logits");
+    need(u, b, "SampleKernel u");
+    need(tokens, b, "SampleKernel tokens");
+    need(logprob, b, "SampleKernel logprob");
+    for (const auto* f : {temperature, top_p, min_p})
+      if (f) need(*f, b, "SampleKernel filters");
+    if (top_k) need(*top_k, b, "SampleKernel top_k");
+    check(c.raw(),
+          aur_sample(c.raw(), logits.ptr(), vocab, u.ptr(), temperature ? temperature->ptr() : nullptr,
+                     top_k ? top_k->ptr() : nullptr, top_p ? top_p->ptr() : nullptr, min_p ? min_p->ptr() : nullptr,
+                     tokens.ptr(), logprob.ptr(), scratch.ptr(), scratch.len(), b, vocab),
+          "SampleKernel");
   }
 };
 
@@ -404,6 +465,11 @@ class DecoderTransformerGpu {
   void prefill_kv(KvCacheGpu& cache, const uint32_t* tokens, uint32_t b, uint32_t t, float* last_logits);
   void generate_step_kv(KvCacheGpu& cache, const uint32_t* tokens, float* logits_host,
                         uint32_t* next_tokens_host);
+  // n_steps tokens for every sequence, each drawn by aur_sample from the cache's last logits with u[n_steps, batch]
+  // and then fed; temperature, top_k, top_p, min_p [batch] or null; out_tokens, out_logprob [n_steps, batch] or null.
+  void generate_sampled(KvCacheGpu& cache, uint32_t n_steps, const float* u, const float* temperature,
+                        const int32_t* top_k, const float* top_p, const float* min_p, uint32_t* out_tokens,
+                        float* out_logprob);
 
  private:
   friend class KvCacheGpu;
@@ -476,6 +542,8 @@ class KvCacheGpu {
   bool split = false;
   size_t bytes_ = 0;
   void* graph_ = nullptr;       // hipGraphExec_t of one decode step, built on first use
+  void* sample_mem_ = nullptr;  // numbers, filters, results and scratch of generate_sampled, as many as it needed
+  size_t sample_bytes_ = 0;
 };
 
 }  // namespace aurora

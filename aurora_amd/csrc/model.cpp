@@ -780,6 +780,7 @@ KvCacheGpu::~KvCacheGpu() {
   }
   drop_graph();
   if (mem_) aur_free(ctx_, mem_);
+  if (sample_mem_) aur_free(ctx_, sample_mem_);
 }
 
 void KvCacheGpu::reset() {
@@ -861,6 +862,49 @@ void DecoderTransformerGpu::generate_step_kv(KvCacheGpu& cache, const uint32_t* 
   cache.current_len += 1;
   if (logits_host) ck(ctx_, aur_d2h(ctx_, logits_host, cache.logits_, (size_t)B * V * 4), "download logits");
   if (next_tokens_host) ck(ctx_, aur_d2h(ctx_, next_tokens_host, cache.tok_, (size_t)B * 4), "download tokens");
+}
+
+// The token that a step feeds is drawn from the logits that the last one (or the prefill) left, on the device: the
+// host sends the random numbers of all steps ahead and reads the tokens when all are done.
+void DecoderTransformerGpu::generate_sampled(KvCacheGpu& cache, uint32_t n_steps, const float* u,
+                                             const float* temperature, const int32_t* top_k, const float* top_p,
+                                             const float* min_p, uint32_t* out_tokens, float* out_logprob) {
+  check_cache(cache);
+  if (cache.current_len == 0) throw Error("generate_sampled: no logits to draw from (prefill first)", AUR_EINVAL);
+  if (n_steps > cache.max_len - cache.current_len) throw Error("generate_sampled: cache full", AUR_ELIMIT);
+  if (n_steps == 0) return;
+  const uint32_t B = cache.batch, V = cfg_.vocab;
+  const size_t n = (size_t)n_steps * B, ws = aur_sample_ws_bytes(B, V);
+  const size_t bytes = (3 * n + 4 * (size_t)B) * 4 + ws + 8 * 256;
+  if (bytes > cache.sample_bytes_) {
+    if (cache.sample_mem_) ck(ctx_, aur_free(ctx_, cache.sample_mem_), "generate_sampled buffers");
+    cache.sample_mem_ = nullptr;
+    cache.sample_bytes_ = 0;
+    ck(ctx_, aur_malloc(ctx_, bytes, &cache.sample_mem_), "generate_sampled buffers");
+    cache.sample_bytes_ = bytes;
+  }
+  Carver cv{static_cast<char*>(cache.sample_mem_)};
+  float* const du = cv.take<float>(n);
+  float* const lp = cv.take<float>(n);
+  int32_t* const tokens = cv.take<int32_t>(n);
+  auto up = [&](const auto* host, auto* dev) {
+    if (host) ck(ctx_, aur_h2d(ctx_, dev, host, (size_t)B * 4), "upload filters");
+    return host ? dev : nullptr;
+  };
+  const float* const dt = up(temperature, cv.take<float>(B));
+  const int32_t* const dk = up(top_k, cv.take<int32_t>(B));
+  const float* const dp = up(top_p, cv.take<float>(B));
+  const float* const dm = up(min_p, cv.take<float>(B));
+  void* const scratch = ws ? cv.take<char>(ws) : nullptr;
+  ck(ctx_, aur_h2d(ctx_, du, u, n * 4), "upload random numbers");
+  for (uint32_t s = 0; s < n_steps; ++s) {
+    const size_t at = (size_t)s * B;
+    ck(ctx_, aur_sample(ctx_, cache.logits_, V, du + at, dt, dk, dp, dm, tokens + at, lp + at, scratch, ws, B, V), "sample");
+    ck(ctx_, aur_d2d(ctx_, cache.tok_, tokens + at, (size_t)B * 4), "feed tokens");
+    generate_step_kv(cache, nullptr, nullptr, nullptr);
+  }
+  if (out_tokens) ck(ctx_, aur_d2h(ctx_, out_tokens, tokens, n * 4), "download tokens");
+  if (out_logprob) ck(ctx_, aur_d2h(ctx_, out_logprob, lp, n * 4), "download log-probabilities");
 }
 
 // Enqueues one decode step for every sequence of `cache`: it reads the input
@@ -1237,6 +1281,15 @@ int aur_model_generate_greedy(aur_model* m, aur_kv_cache* c, uint32_t n_steps, u
     const uint32_t B = c->c->batch;
     for (uint32_t s = 0; s < n_steps; ++s)
       m->m->generate_step_kv(*c->c, nullptr, nullptr, out_tokens ? out_tokens + (size_t)s * B : nullptr);
+  });
+}
+
+int aur_model_generate_sampled(aur_model* m, aur_kv_cache* c, uint32_t n_steps, const float* u, const float* temperature,
+                               const int32_t* top_k, const float* top_p, const float* min_p, uint32_t* out_tokens,
+                               float* out_logprob) {
+  if (!m || !c || (n_steps && !u)) return AUR_EINVAL;
+  return guard(m->m->ctx(), [&] {
+    m->m->generate_sampled(*c->c, n_steps, u, temperature, top_k, top_p, min_p, out_tokens, out_logprob);
   });
 }
 

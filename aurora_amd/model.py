@@ -243,6 +243,19 @@ class DecoderTransformerGpu:
                    out.ctypes.data if collect else None)
         return out
 
+    def generate_sampled(self, cache: "KvCacheGpu", u, temperature=None, top_k=None, top_p=None, min_p=None):
+        """A token for every row of u [n_steps, b], random numbers in [0, 1), drawn from the cache's last logits and
+        fed; the filters are single values or [b].  Returns (tokens [n_steps, b], log-probabilities [n_steps, b])."""
+        u = np.ascontiguousarray(u, np.float32)
+        if u.ndim != 2 or u.shape[1] != cache.batch:
+            raise ValueError(f"generate_sampled: u of shape {u.shape}, [n_steps, {cache.batch}] needed")
+        held = [None if x is None else np.ascontiguousarray(np.broadcast_to(np.asarray(x, t), (cache.batch,)))
+                for x, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        tokens, logprob = np.empty(u.shape, np.uint32), np.empty(u.shape, np.float32)
+        self._call("aur_model_generate_sampled", cache.ptr, u.shape[0], u.ctypes.data,
+                   *(None if x is None else x.ctypes.data for x in held), tokens.ctypes.data, logprob.ctypes.data)
+        return tokens, logprob
+
     def destroy(self) -> None:
         if self.ptr:
             _lib.load().aur_model_destroy(self.ptr)

@@ -485,6 +485,15 @@ int aur_model_generate_step(aur_model* m, aur_kv_cache* c, const uint32_t* token
                             uint32_t* next_tokens);
 /* n_steps greedy generate_step calls; out_tokens [n_steps, b] or NULL. */
 int aur_model_generate_greedy(aur_model* m, aur_kv_cache* c, uint32_t n_steps, uint32_t* out_tokens);
+/* n_steps tokens for every sequence, drawn by aur_sample: the first from the
+ * logits of the prefill (or of the last step), each then fed as a step, so the
+ * last one too is in the cache afterwards.  HOST arrays: u [n_steps, b] random
+ * numbers; temperature, top_k, top_p, min_p [b] or NULL; out_tokens, out_logprob
+ * [n_steps, b] or NULL.  AUR_EINVAL before a prefill, AUR_ELIMIT (and nothing is
+ * done) where the cache has no room for n_steps. */
+int aur_model_generate_sampled(aur_model* m, aur_kv_cache* c, uint32_t n_steps, const float* u,
+                               const float* temperature, const int32_t* top_k, const float* top_p,
+                               const float* min_p, uint32_t* out_tokens, float* out_logprob);
 
 #ifdef __cplusplus
 }
