@@ -33,8 +33,8 @@ struct SampleArgs {
   int32_t* tokens;
   float* logprob;
   int vocab, ld, frac;  // weights in units of 2^-frac
-  // Of rows that several blocks share, of each segment: the largest logit, the kept weight where no border has
-  // to be found, and the histograms.
+  // Of rows that several blocks share, of each segment: the largest logit, the weight of what min_p keeps, and
+  // the histograms (of counts for top_k).
   int segments;
   float* seg_max;
   u64 *seg_mass, *mass;
@@ -471,6 +471,10 @@ struct Row {
   // of which the list holds the first kList.
   __device__ __forceinline__ int gather(float least, float end) {
     constexpr int AT_ONCE = 16;
+    if (infinite) {  // logits as they lie in memory, of which only +∞ counts
+      end = (least <= 0.f && (0.f < end || end == -INFINITY)) ? -INFINITY : NAN;
+      least = INFINITY;
+    }
     __syncthreads();
     if (threadIdx.x == 0) lds.count = 0;
     __syncthreads();
@@ -480,7 +484,6 @@ struct Row {
       u64 hits = 0;
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) {
-        v[i] = clean(v[i]);
         uint32 four = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) four |= (uint32)(v[i][e] >= least && (v[i][e] < end || end == -INFINITY)) << e;
@@ -750,7 +753,8 @@ __global__ void __launch_bounds__(512) sample_histogram_kernel(SampleArgs a) {
   row.take(row_max(a, r), f.T);
   if (row.m == -INFINITY || f.greedy()) return;
   const bool borders = f.k > 0 || f.p < 1.f;
-  for (int i = tid; i < kBins; i += 512) lds.hist[i] = counts[i] = 0;
+  if (borders)
+    for (int i = tid; i < kBins; i += 512) lds.hist[i] = counts[i] = 0;
   __syncthreads();
   const Ranges ranges = first_ranges(row.m, f.T);
   const float least = f.least(row.m);
@@ -764,26 +768,21 @@ __global__ void __launch_bounds__(512) sample_histogram_kernel(SampleArgs a) {
     for (int e = 0; e < 4; ++e) {
       if (!(x[e] > -INFINITY)) continue;
       const u64 w = row.weight(x[e]);
-      if (borders) {
-        const int bin = ranges.of(x[e]);
-        atomicAdd(&counts[bin], 1u);
-        if (w) atomicAdd(&lds.hist[bin], w);
-      } else if (x[e] >= least) {
-        sum += w;
-      }
+      if (x[e] >= least) sum += w;
+      if (!borders) continue;
+      const int bin = ranges.of(x[e]);
+      if (f.k > 0) atomicAdd(&counts[bin], 1u);
+      if (w) atomicAdd(&lds.hist[bin], w);
     }
-  }
-  if (borders) {
-    __syncthreads();
-    for (int i = tid; i < kBins; i += 512) {
-      a.mass[(size_t)blockIdx.x * kBins + i] = lds.hist[i];
-      a.count[(size_t)blockIdx.x * kBins + i] = counts[i];
-    }
-    return;
   }
   sum = wave_sum(sum);
   if ((tid & 63) == 0) lds.wave[tid >> 6] = sum;
   __syncthreads();
+  if (borders)
+    for (int i = tid; i < kBins; i += 512) {
+      a.mass[(size_t)blockIdx.x * kBins + i] = lds.hist[i];
+      if (f.k > 0) a.count[(size_t)blockIdx.x * kBins + i] = counts[i];
+    }
   if (tid < 64) {
     sum = row.sum_of(lds.wave, 8);
     if (tid == 0) a.seg_mass[blockIdx.x] = sum;
@@ -799,12 +798,13 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
   const uint32* const count = a.count + (size_t)r * G * kBins;
   u64 own_count = 0, own_mass = 0;
 #pragma unroll 8
-  for (int g = 0; g < G; ++g) {
-    own_count += count[(size_t)g * kBins + tid];
-    own_mass += mass[(size_t)g * kBins + tid];
-  }
+  for (int g = 0; g < G; ++g) own_mass += mass[(size_t)g * kBins + tid];
   Row<TH, 0> row(a, lds, nullptr, r);
   const Filters f(a, r);
+  if (f.k > 0) {
+#pragma unroll 8
+    for (int g = 0; g < G; ++g) own_count += count[(size_t)g * kBins + tid];
+  }
   row.take(row_max(a, r), f.T);
   if (row.m == -INFINITY) {
     if (tid == 0) certain(a, r, 0, -INFINITY);
@@ -818,36 +818,33 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
     return;
   }
   Cut cut{-INFINITY, 0x7fffffff};
-  if (f.k == 0 && f.p == 1.f) {
-    cut.above(f.least(row.m));
-    if (tid < G) lds.super[tid] = a.seg_mass[(size_t)r * G + tid];
-    __syncthreads();
-  } else {
+  const float least = f.least(row.m);
+  int listed = -1, n = 0;  // the range whose tokens are in the list
+  if (f.k > 0 || f.p < 1.f) {
     const Ranges ranges = first_ranges(row.m, f.T);
-    auto list_of = [&](int bin) { return row.gather(ranges.edge(bin), bin > 0 ? ranges.edge(bin - 1) : -INFINITY); };
-    int listed = -1, n = 0;  // the range whose tokens are in the list
-    u64 kept_mass = 0;       // of the first top_k
-    bool crowded = false;    // more than the list holds: by passes over the row then
-    // The range where `own` reaches the target, and its tokens in the list; what is left of the target there.
-    auto search = [&](u64 own, auto target_of) {
+    const int least_bin = least > kLeastLogit ? ranges.of(least) : kBins;
+    u64 kept_mass = 0;  // of the first top_k
+    bool crowded = false, below = false;  // more than the list holds: by passes over the row then
+    // The range where `own` reaches the target, and its tokens in the list; what is left of the target there.  A
+    // border that only matters where it lies above min_p's is not looked for in a range below that one.
+    auto search = [&](u64 own, bool last, auto target_of) {
       row.clear();
       lds.hist[tid] = own;
       __syncthreads();
       const u64 target = row.find(lds.hist, target_of);
       const int bin = lds.bin;
       const u64 rest = target - (bin < 0 ? 0 : lds.before);
-      __syncthreads();
-      if (bin >= 0 && bin != listed) {
-        if (tid == bin) lds.best = (int)own_count;
-        __syncthreads();
-        crowded = lds.best > kList;
-        if (!crowded) n = list_of(listed = bin);
+      below = last && bin > least_bin;
+      if (bin >= 0 && bin != listed && !below) {
+        n = row.gather(ranges.edge(bin), bin > 0 ? ranges.edge(bin - 1) : -INFINITY);
+        listed = bin;
+        crowded = n > kList;
       }
       return rest;
     };
     if (f.k > 0) {
-      const u64 rest = search(own_count, [&](u64) { return (u64)f.k; });
-      if (listed >= 0) {
+      const u64 rest = search(own_count, f.p == 1.f, [&](u64) { return (u64)f.k; });
+      if (listed >= 0 && !crowded) {
         const Entry at = row.reach_in_list(n, rest, [](const Entry&) { return (u64)1; }, ranges, listed);
         cut = Cut{at.x, at.i};
         if (f.p < 1.f) {  // the weight of all kept
@@ -865,30 +862,31 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
     }
     if (f.p < 1.f && !crowded) {
       const bool by_k = listed >= 0;
-      const u64 rest = search(own_mass, [&](u64 all) { return p_target(f.p, by_k ? kept_mass : all); });
-      if (!crowded) {
+      const u64 rest = search(own_mass, true, [&](u64 all) { return p_target(f.p, by_k ? kept_mass : all); });
+      if (!crowded && !below) {
         const Entry at = row.reach_in_list(n, rest, [](const Entry& e) { return e.w; }, ranges, listed);
         cut = Cut{at.x, at.i};
       }
-    }
-    if (!crowded && cut.above(f.least(row.m))) {
-      const int bin = ranges.of(cut.x);
-      if (bin != listed) n = list_of(listed = bin);
-      crowded = n > kList;
     }
     if (crowded) {
       choose_apart(row, f, r);
       return;
     }
-    // the segments' kept weights: of the ranges above the listed one, and the tokens in it; of all (k of as many
-    // tokens or more, nothing else) where none is
+    if (below) listed = -1;
+  }
+  // The segments' kept weights: above min_p's border, or of the ranges above the listed one and of the tokens in it.
+  if (cut.above(least)) listed = -1;
+  __syncthreads();
+  if (listed < 0) {
+    if (tid < G) lds.super[tid] = a.seg_mass[(size_t)r * G + tid];
     __syncthreads();
+  } else {
     for (int g = w; g < G; g += TH / 64) {
       u64 sum = 0;
 #pragma unroll
       for (int i = 0; i < kBins / 64; ++i) {
         const u64 x = mass[(size_t)g * kBins + 64 * i + lane];
-        sum += 64 * i + lane < (listed < 0 ? kBins : listed) ? x : 0;
+        sum += 64 * i + lane < listed ? x : 0;
       }
       sum = wave_sum(sum);
       if (lane == 0) lds.super[g] = sum;
