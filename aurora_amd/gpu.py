@@ -422,10 +422,11 @@ class SampleKernel(_Kernel):
     0, logprob [b].  temperature, top_k (int32), top_p and min_p are arrays of b values, 0 for none.
 
     For more than 32768 tokens the object keeps a scratch, allocated when a call needs a larger one (or ahead,
-    by `reserve`: a captured call cannot allocate); calls that overlap in time take an object each."""
+    by `reserve`: a captured call cannot allocate); calls that overlap in time take an object each.  One that was
+    outgrown is kept until `free`, since a captured call may still use it."""
 
     def __init__(self):
-        self._scratch = None
+        self._scratch = []  # the last one is in use
 
     @staticmethod
     def scratch_bytes(b, vocab) -> int:
@@ -433,14 +434,12 @@ class SampleKernel(_Kernel):
 
     def reserve(self, ctx, b, vocab) -> None:
         n = self.scratch_bytes(b, vocab)
-        if n and (self._scratch is None or self._scratch.nbytes < n or self._scratch.ctx is not ctx):
-            self.free()
-            self._scratch = GpuBuffer.empty(ctx, n, np.uint8)
+        if n and not (self._scratch and self._scratch[-1].nbytes >= n and self._scratch[-1].ctx is ctx):
+            self._scratch.append(GpuBuffer.empty(ctx, n, np.uint8))
 
     def free(self) -> None:
-        if self._scratch is not None:
-            self._scratch.free()
-            self._scratch = None
+        while self._scratch:
+            self._scratch.pop().free()
 
     def dispatch_into(self, ctx, logits, ld, u, tokens, logprob, b, vocab, temperature=0, top_k=0, top_p=0, min_p=0):
         if _any_buffer(logits, u, tokens, logprob, temperature, top_k, top_p, min_p):
@@ -452,6 +451,6 @@ class SampleKernel(_Kernel):
         scratch, nbytes = 0, 0
         if vocab > 32768:
             self.reserve(ctx, b, vocab)
-            if self._scratch is not None:
-                scratch, nbytes = self._scratch.ptr, self._scratch.nbytes
+            if self._scratch:
+                scratch, nbytes = self._scratch[-1].ptr, self._scratch[-1].nbytes
         ctx.call("aur_sample", logits, ld, u, temperature, top_k, top_p, min_p, tokens, logprob, scratch, nbytes, b, vocab)
