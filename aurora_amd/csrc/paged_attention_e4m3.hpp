@@ -1,12 +1,14 @@
 // Items of 16 rows and more on pools of e4m3: what is included by paged_attention.hpp.
 //
 // An e4m3 number is an fp16 one, so K and V go into the fp16 MFMA as they are, and queries and weights as two
-// fp16 parts, which keep 2^-20 of them: two products where bf16 parts of the same accuracy take three (16
-// sequences of 259 to 503 tokens on a prefix of 4096, 16 heads of 64: KV_PROMPTS).
+// fp16 parts, which keep 2^-20 of them: two products where bf16 parts of the same accuracy take three.  Bound by
+// the MFMA and the softmax between its issues: 16 sequences of 512 tokens on a prefix of 4096, 16 heads of 64, 325
+// us, 330 TFLOP/s of the two products' 600 at a large library product's rate (the first form, of three bf16
+// products and two barriers a tile, 478); a step of 64 sequences of 1024 keys on 32768, 16 heads of 64, 60 us.
 //   * Scales.  Relative to the largest scale 2^E seen so far, of K and of V, a key's scale is 2^(e − E), which the
 //     conversion to fp16 multiplies by.  That is exact down to e − E = −kSpread, where the smallest e4m3 number
 //     is the smallest fp16 one.  E goes into the factor of the scores, and into the sums when it grows.  A smaller
-//     scale leaves the item to exact_sums; scales of 2^-117 and less (what zeros get) count as 0 there instead.
+//     scale leaves the item to exact_sums; but 2^-117 and less (what zeros get) counts as 0 beside 2^-67 and more.
 //   * Queries times 2^a with the row's largest between 2^12 and 2^13; a goes into the factor of the scores.
 //   * Weights are exp2(score − m) for a reference m 14 below the row's maximum, so up to 2^14: their second part is
 //     then 2^-38 of the largest or better.
@@ -17,6 +19,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kSpread = 15;       // of the powers of two of scales that items take in their stride
 constexpr int kLeastScale = 10;   // byte of 2^-117, the least that an append gives
+constexpr int kNothing = 60;      // byte of 2^-67: beside it such ones are 2^-30 of its smallest number at most
 constexpr float kAbove = 14.f;    // log2 of the largest weight
 
 struct Halves8 {  // eight numbers in two fp16 parts; the first is cut, the second has what that left
@@ -43,7 +46,7 @@ struct Reference {
 };
 // 2^(byte − of), and whether an item can go on with it.
 __device__ __forceinline__ float relative(int byte, int of, bool& fits) {
-  fits &= byte != 255 && (of - byte <= kSpread || byte <= kLeastScale);
+  fits &= byte != 255 && (of - byte <= kSpread || (byte <= kLeastScale && of >= kNothing));
   return scale_of((unsigned)max(127 + byte - of, 0));
 }
 // The larger of k and v bytes, each packed in 16 bits, over lanes 0 .. 63 (or of each half alike).

@@ -257,6 +257,24 @@ def test_scales_far_apart(ctx, n, prefix, group, dh, k_e, v_e):
     dev.free()
 
 
+@pytest.mark.parametrize("n,prefix,group", [([1, 1, 1], 400, 1), ([1] * 40, 300, 1), ([90, 70], 60, 2), ([5, 6], 30, 4)])
+@pytest.mark.parametrize("larger", [30, 26])
+def test_the_smallest_scale_beside_small_ones(ctx, n, prefix, group, larger):
+    """Values of the smallest scale beside ones 2^20 and 2^16 larger, which do not hide them."""
+    rng = np.random.default_rng(len(n))
+    c = Case8(rng, n, [x + 20 for x in n], prefix, 16, 1, group, 64, 4)
+    c.vs[...] = np.where(c.vs == 255, 255, rng.choice([10, larger], c.vs.shape, p=[0.9, 0.1]))
+    with np.errstate(invalid="ignore"):
+        c.refresh()
+    dev = Device8(ctx, c)
+    dev.attend()
+    out, _ = dev.result()
+    want, _, tol, _ = attention_blocks(c)
+    rows = int(c.off[-1])
+    assert np.all(np.abs(out[:rows] - want[:rows]) <= tol[:rows] + 2.0**-149 * (prefix + max(n) + 20))
+    dev.free()
+
+
 @pytest.mark.parametrize("change,what", [
     (dict(ld=124), "ld=124"), (dict(ld=130), "ld=130"), (dict(k="odd"), "16-byte"), (dict(v="odd"), "16-byte"),
     (dict(count=51), "keys 0 to 51"), (dict(first=2**32 - 1, count=2), "keys"), (dict(first=51, count=0), "keys 51"),
