@@ -599,7 +599,7 @@ __device__ __forceinline__ void store_exact(const MhaArgs& a, const Item& it, in
 // which keep 2^-24 of each.  A wave's next K is under way while it works, its V from the scores on.  Bound
 // by the reading with the MFMA's cycles in between: 64 sequences of 512 to 1024 keys (768 on average), 16
 // K/V heads of 64, 4 rows each: 56 µs in bf16 (3.7 TB/s), 92 in fp32 (4.5 TB/s); with 1024 keys each 62 µs
-// in bf16 (4.3 TB/s), 33 in e4m3 (4.1 TB/s).  On widened keys the fp32 MFMA took bf16's own keys of 64 such sequences 160 µs in a
+// in bf16 (4.3 TB/s), 38 in e4m3 (3.5 TB/s).  On widened keys the fp32 MFMA took bf16's own keys of 64 such sequences 160 µs in a
 // first version, the bf16 one 60.
 template <int DT>
 __device__ bool byte_sums(const MhaArgs& a, const Item& it, int x, int stride, int page, Sums<DT, 1>& s);  // e4m3 keys
@@ -698,11 +698,11 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
 // average), 16 K/V heads of 64, µs by vectors and by the MFMA: 1 row 67 and 85 (5.9 TB/s), 2 rows 73 and 84,
 // 4 rows 83 and 92; bf16 keys 1 row 40 and 53 (5.0 TB/s), 2 rows 43 and 54, 4 rows 55 and 56 (with a prefix
 // of 2048 beside it 40 and 38): so 4 rows in fp32, 2 in bf16.  With 1024 keys each, by vectors: fp32 85 µs
-// (6.3 TB/s), 88 and 94, bf16 48 µs (5.6 TB/s) and 49, e4m3 24 (5.6 TB/s) and 31, by the MFMA 32 and 32, and
-// 4 rows 43 against 33: so 2 rows in e4m3 as well.  LP lanes have a key's head, 16 bytes each, so that a load brings 64/LP whole
-// keys; a score is added up over the LP lanes, l and the columns over the key groups once at the end, all
-// of it in fp32.  While one half of the registers is in use, the loads of the other are under way, and the
-// page of the step after them.
+// (6.3 TB/s), 88 and 94, bf16 48 µs (5.6 TB/s) and 49, e4m3 (out of the chip's caches, which hold them) 24 and 31,
+// by the MFMA 32 and 32, and 4 rows 43 against 33: so 2 rows in e4m3 as well.  LP lanes have a key's head, 16
+// bytes each (8 of e4m3), so that a load brings 64/LP whole keys; a score is added up over the LP lanes, l and the
+// columns over the key groups once at the end, all of it in fp32.  While one half of the registers is in use, the
+// loads of the other are under way, and the page of the step after them.
 template <class T, int DT>
 struct FewRows {
   static constexpr bool B8 = sizeof(T) == 1;

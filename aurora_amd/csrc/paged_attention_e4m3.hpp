@@ -2,9 +2,10 @@
 //
 // An e4m3 number is an fp16 one, so K and V go into the fp16 MFMA as they are, and queries and weights as two
 // fp16 parts, which keep 2^-20 of them: two products where bf16 parts of the same accuracy take three.  Bound by
-// the MFMA and the softmax between its issues: 16 sequences of 512 tokens on a prefix of 4096, 16 heads of 64, 325
-// us, 330 TFLOP/s of the two products' 600 at a large library product's rate (the first form, of three bf16
-// products and two barriers a tile, 478); a step of 64 sequences of 1024 keys on 32768, 16 heads of 64, 60 us.
+// the softmax's instructions and the MFMA's between them: 16 sequences of 512 tokens on a prefix of 4096, 16 heads
+// of 64, 309 us, 350 TFLOP/s of the 600 that a large library product's rate leaves for two (the first form, of three
+// bf16 products and two barriers a tile, 478); a step of 64 sequences of 1024 keys on 32768, 16 heads of 64, 71 us,
+// 52 of them for the prefix.  The weights' sums as products with ones: 313 us, d_head 128 354 instead of 337.
 //   * Scales.  Relative to the largest scale 2^E seen so far, of K and of V, a key's scale is 2^(e − E), which the
 //     conversion to fp16 multiplies by.  That is exact down to e − E = −kSpread, where the smallest e4m3 number
 //     is the smallest fp16 one.  E goes into the factor of the scores, and into the sums when it grows.  A smaller
@@ -25,8 +26,13 @@ constexpr float kAbove = 14.f;    // log2 of the largest weight
 struct Halves8 {  // eight numbers in two fp16 parts; the first is cut, the second has what that left
   f16x8 h, l;
   __device__ __forceinline__ void set(int i, float x0, float x1) {
+    // A factor that the compiler does not know to be -1 leaves x - (float)h one instruction of mixed operands, where
+    // it would take two (16 sequences of 512 tokens on 4096, 16 heads of 64: 309 us, 326 without).
+    float minus;
+    asm("s_mov_b32 %0, -1.0" : "=s"(minus));
     const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0 - (float)a[0], x1 - (float)a[1]));
+    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)a[0], minus, x0),
+                                                                         __builtin_fmaf((float)a[1], minus, x1)));
     h[i] = a[0], h[i + 1] = a[1];
     l[i] = b[0], l[i + 1] = b[1];
   }
