@@ -114,14 +114,15 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_pe
 // holds up to 8 steps of 64 / LP tokens, LP lanes of 4 columns a head, and W = 4 waves share a unit that has
 // more (up to 16 steps each).  Blocks walk over `chunk` rows of the batch each (no more than a block of tokens has, so that two of a
 // sequence's units at most begin there) and take the units that begin in them, their last rows may lie behind.
-// 16 prompts of 1024 tokens, 16 heads of 64, blocks of 32, q rotated on the way: 45 us, 5.1 TB/s, the rate of a
-// large copy; blocks of one token 42 (312 while a wave took one block at a time); a step of 32 sequences 5 us.
+// 16 prompts of 512 to 1024 tokens, 16 heads of 64, blocks of 32, q rotated on the way: 55 us, 4.2 of the 5.1 TB/s
+// of a large copy; blocks of one token 54 (312 while a wave took one block at a time); a step of 32 sequences 5 us.
 struct UnitArgs {
   int chunk, n_chunks, groups;  // rows of a chunk; blocks of a chunk, 4 / W units each
 };
 
-constexpr int kUnitSteps = 8;   // more hold registers that others' loads want: prompts of 1024 tokens 45 µs, with 16 57
-constexpr int kAtOnce = 2;      // steps whose loads are under way together (4: 46.5 µs)
+// Those prompts: a unit's steps issued one by one 59 us, two by two 61, one by one with seven waves on a SIMD, which
+// spill 3 registers, 55; spans two by two 54, one by one 57.
+constexpr int kUnitSteps = 8, kUnitAtOnce = 1, kAtOnce = 2;
 
 // Four columns of a head, x, rotated with y, the ones that are their pairs' other halves, by t0 and t1, their (cos,
 // sin): every product is rounded before the sum, so that a value next to the border of two e4m3 numbers falls
@@ -203,12 +204,12 @@ __device__ __forceinline__ void append_units(const AppendArgs& a, const UnitArgs
       };
       if (on) {
 #pragma unroll
-        for (int n0 = 0; n0 < STEPS; n0 += kAtOnce)
+        for (int n0 = 0; n0 < STEPS; n0 += kUnitAtOnce)
           if (n0 * PER * W < count) {
             if (is_k && a.rot > 0) {
-              floatx4 f[kAtOnce], y[kAtOnce], t0[kAtOnce], t1[kAtOnce];
+              floatx4 f[kUnitAtOnce], y[kUnitAtOnce], t0[kUnitAtOnce], t1[kUnitAtOnce];
 #pragma unroll
-              for (int n = 0; n < kAtOnce; ++n) {
+              for (int n = 0; n < kUnitAtOnce; ++n) {
                 const int k = place(n0 + n);
                 const float* p = src + (size_t)(q.lo + i + k) * a.ld_kv;
                 const float* tab = a.table + (size_t)(a.b.prefix_len + j + k) * a.rot + ct;
@@ -218,14 +219,14 @@ __device__ __forceinline__ void append_units(const AppendArgs& a, const UnitArgs
                 t1[n] = *reinterpret_cast<const floatx4*>(a.pairs ? tab : tab + 4);
               }
 #pragma unroll
-              for (int n = 0; n < kAtOnce; ++n) take(n0 + n, rotated4(a, c, f[n], y[n], t0[n], t1[n]));
+              for (int n = 0; n < kUnitAtOnce; ++n) take(n0 + n, rotated4(a, c, f[n], y[n], t0[n], t1[n]));
             } else {
-              floatx4 f[kAtOnce];
+              floatx4 f[kUnitAtOnce];
 #pragma unroll
-              for (int n = 0; n < kAtOnce; ++n)
+              for (int n = 0; n < kUnitAtOnce; ++n)
                 f[n] = *reinterpret_cast<const floatx4*>(src + (size_t)(q.lo + i + place(n0 + n)) * a.ld_kv + c);
 #pragma unroll
-              for (int n = 0; n < kAtOnce; ++n) take(n0 + n, f[n]);
+              for (int n = 0; n < kUnitAtOnce; ++n) take(n0 + n, f[n]);
             }
           }
       }
@@ -346,7 +347,7 @@ __device__ __forceinline__ void rotate_q(const AppendArgs& a, int block) {
 
 // Blocks of the chunks' units, then those of q's rows.  W = 0: spans of small blocks.
 template <int LP, int W, int STEPS>
-__global__ void __launch_bounds__(256) append_e4m3_kernel(AppendArgs a, UnitArgs u) {
+__global__ void __launch_bounds__(256, STEPS > kUnitSteps ? 4 : 7) append_e4m3_kernel(AppendArgs a, UnitArgs u) {
   __shared__ float top[4];
   const int block = blockIdx.x, units = u.n_chunks * u.groups;
   if (block >= units)
