@@ -470,7 +470,7 @@ struct Row {
   // The tokens of least <= logit < end (of all from least on where end is −∞) in the list: their number,
   // of which the list holds the first kList.
   __device__ __forceinline__ int gather(float least, float end) {
-    constexpr int AT_ONCE = 16;
+    constexpr int AT_ONCE = 8;
     if (infinite) {  // logits as they lie in memory, of which only +∞ counts
       end = (least <= 0.f && (0.f < end || end == -INFINITY)) ? -INFINITY : NAN;
       least = INFINITY;
@@ -670,9 +670,12 @@ __device__ __forceinline__ void choose(Row<TH, ROW>& row, const Filters& f, int 
 }
 
 // The same out of line, for rows that hardly ever come.
+// They get a row of their own, for one whose address another function gets lies in memory wherever it is used.
 template <int TH, int ROW>
-__device__ __attribute__((noinline)) void choose_apart(Row<TH, ROW>& row, const Filters& f, int r) {
-  choose(row, f, r);
+__device__ __attribute__((noinline)) void choose_apart(const SampleArgs& a, SampleLds& lds, int r, float most, float T) {
+  Row<TH, ROW> row(a, lds, nullptr, r);
+  row.take(most, T);
+  choose(row, Filters(a, r), r);
 }
 
 // A row without anything to choose from; nor with a choice to make: its first largest logit.
@@ -721,8 +724,9 @@ __global__ void __launch_bounds__(TH) sample_kernel(SampleArgs a) {
 // Three launches: the segments' largest logits; with the row's largest their histograms of weights (and of counts
 // for top_k) and the weight of what min_p keeps; a block a row, which adds these up, collects the tokens of the one
 // or two ranges that hold its borders from the row, and goes through the weights of the one segment that the random
-// number falls into.  64 rows of 131072: 7, 17 and 30 us where min_p's border is the higher one, 50 for the last
-// where top_p's tokens are collected (one block reads its row at 30 GB/s); reading the logits once takes 7.
+// number falls into.  64 rows of 131072: 7, 19 and 28 us where min_p's border is the higher one, 44 for the last
+// where top_p's tokens are collected; reading the logits once takes 7.  The second is bound by its additions in
+// LDS, the last by how long one block takes for a row.
 
 __global__ void __launch_bounds__(512) sample_max_kernel(SampleArgs a) {
   __shared__ SampleLds lds;
@@ -871,7 +875,7 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
       }
     }
     if (crowded) {
-      choose_apart(row, f, r);
+      choose_apart<TH, 0>(a, lds, r, row.infinite ? INFINITY : row.m, f.T);
       return;
     }
     if (below) listed = -1;
