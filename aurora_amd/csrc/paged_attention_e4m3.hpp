@@ -6,10 +6,11 @@
 // of 64, 309 us, 350 TFLOP/s of the 600 that a large library product's rate leaves for two (the first form, of three
 // bf16 products and two barriers a tile, 478); a step of 64 sequences of 1024 keys on 32768, 16 heads of 64, 71 us,
 // 52 of them for the prefix.  The weights' sums as products with ones: 313 us, d_head 128 354 instead of 337.
-//   * Scales.  Relative to the largest scale 2^E seen so far, of K and of V, a key's scale is 2^(e − E), which the
-//     conversion to fp16 multiplies by.  That is exact down to e − E = −kSpread, where the smallest e4m3 number
-//     is the smallest fp16 one.  E goes into the factor of the scores, and into the sums when it grows.  A smaller
-//     scale leaves the item to exact_sums; but 2^-117 and less (what zeros get) counts as 0 beside 2^-67 and more.
+//   * Scales.  Relative to the largest scale 2^E seen so far, of K and of V, a key's scale is 2^(e − E + kUp), which
+//     the conversion to fp16 multiplies by: 448 times the largest one's is near fp16's end, and down to e − E =
+//     −kSpread, where the smallest e4m3 number is the smallest fp16 one, that is exact.  E goes into the factor of
+//     the scores, and into the sums when it grows.  A smaller scale leaves the item to exact_sums (50 times slower);
+//     but 2^-117 and less (what zeros get) counts as 0 beside 2^-67 and more.
 //   * Queries times 2^a with the row's largest between 2^12 and 2^13; a goes into the factor of the scores.
 //   * Weights are exp2(score − m) for a reference m 14 below the row's maximum, so up to 2^14: their second part is
 //     then 2^-38 of the largest or better.
@@ -18,7 +19,7 @@
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kSpread = 15;       // of the powers of two of scales that items take in their stride
+constexpr int kUp = 7, kSpread = 15 + kUp;
 constexpr int kLeastScale = 10;   // byte of 2^-117, the least that an append gives
 constexpr int kNothing = 60;      // byte of 2^-67: beside it such ones are 2^-30 of its smallest number at most
 constexpr float kAbove = 14.f;    // log2 of the largest weight
@@ -50,10 +51,10 @@ __device__ __forceinline__ uint2v widen4(unsigned x, float scale) {
 struct Reference {
   int k, v;
 };
-// 2^(byte − of), and whether an item can go on with it.
+// 2^(byte − of + kUp), and whether an item can go on with it.
 __device__ __forceinline__ float relative(int byte, int of, bool& fits) {
   fits &= byte != 255 && (of - byte <= kSpread || (byte <= kLeastScale && of >= kNothing));
-  return scale_of((unsigned)max(127 + byte - of, 0));
+  return scale_of((unsigned)max(127 + kUp + byte - of, 0));
 }
 // The larger of k and v bytes, each packed in 16 bits, over lanes 0 .. 63 (or of each half alike).
 __device__ __forceinline__ unsigned wave_top(unsigned x) {
@@ -109,7 +110,7 @@ struct HalfQueries {
   // The scores' factor for K relative to 2^(k − 127).
   __device__ __forceinline__ void relative_to(int k) {
 #pragma unroll
-    for (int i = 0; i < RT; ++i) factor[i] = fmaxf(ldexpf(1.f, back[i] + k - 127), 1.17549435e-38f);
+    for (int i = 0; i < RT; ++i) factor[i] = fmaxf(ldexpf(1.f, back[i] + k - 127 - kUp), 1.17549435e-38f);
   }
 };
 
@@ -269,7 +270,7 @@ __device__ __forceinline__ bool byte_sums(const MhaArgs& a, const Item& it, int 
       }
     if (more) keys.load_v(a, it.hk, at, g, l16);
   }
-  const float back = ldexpf(1.f, ref.v - 127);
+  const float back = ldexpf(1.f, ref.v - 127 - kUp);
 #pragma unroll
   for (int b = 0; b < VB; ++b)
 #pragma unroll
@@ -544,7 +545,7 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
     }
   }
   const bool exact = __syncthreads_or(!fits);
-  const float back = ldexpf(1.f, ref.v - 127);
+  const float back = ldexpf(1.f, ref.v - 127 - kUp);
 
 #pragma unroll
   for (int r = 0; r < NR; ++r) {

@@ -275,6 +275,31 @@ def test_the_smallest_scale_beside_small_ones(ctx, n, prefix, group, larger):
     dev.free()
 
 
+@pytest.mark.parametrize("n,prefix,group", [([1, 1, 1], 400, 1), ([1] * 40, 300, 1), ([90, 70], 60, 2), ([5, 6], 30, 4)])
+@pytest.mark.parametrize("apart", [15, 16, 21, 22, 23])
+@pytest.mark.parametrize("of_k", [False, True])
+def test_scales_at_the_border(ctx, n, prefix, group, apart, of_k):
+    """Largest and smallest numbers of scales about as far apart as the halves' products take."""
+    rng = np.random.default_rng(apart + len(n))
+    c = Case8(rng, n, [x + 20 for x in n], prefix, 16, 1, group, 64, 2)
+    byte, scale = (c.kb, c.ks) if of_k else (c.vb, c.vs)
+    scale[...] = np.where(scale == 255, 255, 127 - 8 * of_k - apart * rng.integers(0, 2, scale.shape))
+    ends = rng.choice(np.array([1, 126, 129, 254], np.uint8), byte.shape)  # ±2^-9, ±448
+    byte[...] = np.where(rng.random(byte.shape) < 0.5, ends, byte)
+    if of_k:  # scores of a few units for the larger ones
+        c.q *= np.float32(2.0**-8)
+    with np.errstate(invalid="ignore"):
+        c.refresh()
+    dev = Device8(ctx, c)
+    dev.attend()
+    out, lse = dev.result()
+    want, want_lse, tol, tol_lse = attention_blocks(c)
+    rows = int(c.off[-1])
+    assert np.all(np.abs(out[:rows] - want[:rows]) <= tol[:rows])
+    assert np.all(np.abs(lse[:rows] - want_lse[:rows]) <= tol_lse[:rows])
+    dev.free()
+
+
 @pytest.mark.parametrize("change,what", [
     (dict(ld=124), "ld=124"), (dict(ld=130), "ld=130"), (dict(k="odd"), "16-byte"), (dict(v="odd"), "16-byte"),
     (dict(count=51), "keys 0 to 51"), (dict(first=2**32 - 1, count=2), "keys"), (dict(first=51, count=0), "keys 51"),
