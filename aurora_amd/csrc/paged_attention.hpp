@@ -111,8 +111,9 @@ __device__ __forceinline__ int row_of(const MhaArgs& a, const Item& it, int x, i
   return x < it.x1 && (unsigned)page < (unsigned)a.n_pages ? (page << a.sh) + (i & ((1 << a.sh) - 1)) : -1;
 }
 
-// The block's item; `page` is the page of key x0 + lead.  False: nothing to do.
-template <int R>
+// The block's item; `page` is the page of key x0 + lead.  False: nothing to do.  T: by_xcd is looked at for e4m3
+// alone (the other types' steps took 3 % longer with a branch on it).
+template <class T, int R>
 __device__ __forceinline__ bool take_item(const MhaArgs& a, Item& it, int lead, int& page) {
   int item = blockIdx.x;
   it.of_prefix = item < a.p_items;
@@ -120,7 +121,7 @@ __device__ __forceinline__ bool take_item(const MhaArgs& a, Item& it, int lead, 
   it.tok0 = 0;
   it.first = 0;
   if (!it.of_prefix) item -= a.p_items;
-  if (a.by_xcd) {
+  if (sizeof(T) == 1 && a.by_xcd) {
     const int i = item / kDice;
     it.hk = i % a.Hkv;
     item = i / a.Hkv * kDice + item % kDice;
@@ -618,7 +619,7 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
 
   Item it;
   int page;
-  if (!take_item<R>(a, it, STEP * w + k32, page)) return;
+  if (!take_item<T, R>(a, it, STEP * w + k32, page)) return;
   int x = it.x0 + STEP * w;
   Sums<DT, RT> s;
   s.clear();
@@ -754,7 +755,7 @@ __device__ __forceinline__ void few_item(const MhaArgs& a, FewLds<R>& lds) {
 
   Item it;
   int page;
-  if (!take_item<R>(a, it, KEYS * w + lane % KEYS, page)) return;
+  if (!take_item<T, R>(a, it, KEYS * w + lane % KEYS, page)) return;
   const char* const kp = static_cast<const char*>(a.k) + ((size_t)it.hk * a.dh + col) * sizeof(T);
   const char* const vp = static_cast<const char*>(a.v) + ((size_t)it.hk * a.dh + col) * sizeof(T);
   const long long ld = (long long)a.Hkv * a.dh * sizeof(T);
@@ -948,7 +949,7 @@ __device__ __forceinline__ void tile_item(const MhaArgs& a, TileLds<T, DT, W>& l
 
   Item it;
   int page;
-  if (!take_item<16 * NR * W>(a, it, tid % KT, page)) return;
+  if (!take_item<T, 16 * NR * W>(a, it, tid % KT, page)) return;
   const int row0 = it.row0 + 16 * NR * w;  // this wave's
   Rows<NR> rows;
   take_rows(a, it, row0, l16, rows);

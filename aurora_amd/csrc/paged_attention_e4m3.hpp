@@ -311,7 +311,7 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
 
   Item it;
   int page;
-  if (!take_item<16 * NR * W>(a, it, tid % KT, page)) return;
+  if (!take_item<e4m3, 16 * NR * W>(a, it, tid % KT, page)) return;
   const int row0 = it.row0 + 16 * NR * w;  // this wave's
   Rows<NR> rows;
   take_rows(a, it, row0, l16, rows);
