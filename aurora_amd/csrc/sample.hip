@@ -33,8 +33,8 @@ struct SampleArgs {
   int32_t* tokens;
   float* logprob;
   int vocab, ld, frac;  // weights in units of 2^-frac
-  // Of rows that several blocks share, of each segment: the largest logit, the weight of what min_p keeps, and
-  // the histograms (of counts for top_k).
+  // Of rows that several blocks share, of each segment: the largest logit, the weight of what min_p keeps (for
+  // each of kParts parts of it), and the histograms (of counts for top_k).
   int segments;
   float* seg_max;
   u64 *seg_mass, *mass;
@@ -50,6 +50,7 @@ constexpr float kLeastLogit = -3.402823466e38f;  // that can be chosen
 constexpr int kStaged = 32768;     // logits of a row in LDS
 constexpr int kSegment = 16384;    // … of a block, where several share a row
 constexpr int kMaxSegments = kMaxVocab / kSegment;
+constexpr int kParts = 4;          // of a segment: chunks of the block that goes through the row at last
 
 struct Entry {
   float x;
@@ -102,25 +103,29 @@ __device__ __forceinline__ bool before(float x, int i, float y, int j) { return 
 constexpr double kWhole = 6755399441055744.0;
 __device__ __forceinline__ int low32(double x) { return (int)(uint32)__double_as_longlong(x); }
 
+// The coefficients of 2^r's series from r^11 down to r.
+struct Series {
+  double c[11];
+  __device__ __forceinline__ constexpr Series() : c{} {
+    constexpr double l = 0.6931471805599453;
+    double x = 1.0;
+    for (int i = 1; i <= 11; ++i) c[11 - i] = x *= l / i;
+  }
+  // In registers, where the compiler would copy each one there from a constant in every use: for loops of weights.
+  __device__ __forceinline__ void keep() {
+#pragma unroll
+    for (int i = 0; i < 11; ++i) asm("" : "+v"(c[i]));
+  }
+};
+
 // The weight of logit v in units of 2^-frac, to the nearest; scale is log2(e) / T.  No instruction of it runs at
 // less than the rate of the others: conversions and powers of two are sums and moves of bits.
-__device__ __forceinline__ u64 weight_of(float v, float m, double scale, int frac) {
+__device__ __forceinline__ u64 weight_of(float v, float m, double scale, int frac, const Series& s) {
   const double y = fmax(((double)v - (double)m) * scale, -2000.0);
   const double t = y + kWhole, r = y - (t - kWhole);  // 2^y = 2^n·2^r, |r| <= 1/2
-  constexpr double l = 0.6931471805599453;
-  constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7,
-                   c8 = c7 * l / 8, c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
-  double p = c11;
-  p = __builtin_fma(p, r, c10);
-  p = __builtin_fma(p, r, c9);
-  p = __builtin_fma(p, r, c8);
-  p = __builtin_fma(p, r, c7);
-  p = __builtin_fma(p, r, c6);
-  p = __builtin_fma(p, r, c5);
-  p = __builtin_fma(p, r, c4);
-  p = __builtin_fma(p, r, c3);
-  p = __builtin_fma(p, r, c2);
-  p = __builtin_fma(p, r, l);
+  double p = s.c[0];
+#pragma unroll
+  for (int i = 1; i < 11; ++i) p = __builtin_fma(p, r, s.c[i]);
   p = __builtin_fma(p, r, 1.0);
   // times 2^(n + frac), at least 2^-2 (which rounds to nothing), to the nearest below 2^52
   const u64 up = (u64)(uint32)max(low32(t) + frac, -2) << 52;
@@ -266,7 +271,7 @@ struct Row {
       }
     }
   }
-  __device__ __forceinline__ u64 weight(float v) const { return weight_of(v, m, scale, a.frac); }
+  __device__ __forceinline__ u64 weight(float v) const { return weight_of(v, m, scale, a.frac, Series()); }
 
   __device__ __forceinline__ float block_max(float v) {
     v = aurlanes::group_reduce<1, 64, true>(v);
@@ -723,10 +728,10 @@ __global__ void __launch_bounds__(TH) sample_kernel(SampleArgs a) {
 
 // Three launches: the segments' largest logits; with the row's largest their histograms of weights (and of counts
 // for top_k) and the weight of what min_p keeps; a block a row, which adds these up, collects the tokens of the one
-// or two ranges that hold its borders from the row, and goes through the weights of the one segment that the random
-// number falls into.  64 rows of 131072: 7, 19 and 28 us where min_p's border is the higher one, 44 for the last
-// where top_p's tokens are collected; reading the logits once takes 7.  The second is bound by its additions in
-// LDS, the last by how long one block takes for a row.
+// or two ranges that hold its borders from the row, and goes through the weights of the part of a segment that the
+// random number falls into (of the whole segment where a list decides which are kept).  64 rows of 131072: 7, 17 and
+// 23 us where min_p's border is the higher one, 43 for the last where top_p's tokens are collected; reading the
+// logits once takes 7.  The second is bound by its arithmetic in 64 bits, the last by how long one block takes.
 
 __global__ void __launch_bounds__(512) sample_max_kernel(SampleArgs a) {
   __shared__ SampleLds lds;
@@ -753,8 +758,19 @@ __global__ void __launch_bounds__(512) sample_histogram_kernel(SampleArgs a) {
   __shared__ uint32 counts[kBins];
   const int r = blockIdx.x / a.segments, g = blockIdx.x % a.segments, tid = threadIdx.x;
   Row<512, 0> row(a, lds, nullptr, r);
-  floatx4 v[kSegment / 2048];
-  row.raw(g * (kSegment / 2048), v);
+  // a wave has 2048 tokens that follow each other, so its sum is one of a part of the row
+  constexpr int N = kSegment / 2048;
+  const int first = g * kSegment + (tid >> 6) * 2048 + 4 * (tid & 63);
+  floatx4 v[N];
+  if ((g + 1) * kSegment <= a.vocab) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) v[c] = *reinterpret_cast<const floatx4_any*>(row.x + first + 256 * c);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[c][e] = first + 256 * c + e < a.vocab ? row.x[first + 256 * c + e] : -INFINITY;
+  }
   const Filters f(a, r);
   row.take(row_max(a, r), f.T);
   if (row.m == -INFINITY || f.greedy()) return;
@@ -765,15 +781,17 @@ __global__ void __launch_bounds__(512) sample_histogram_kernel(SampleArgs a) {
   const Ranges ranges = first_ranges(row.m, f.T);
   const float least = f.least(row.m);
   u64 sum = 0;
+  Series series;
+  series.keep();
 #pragma unroll 1
-  for (int c = 0; c < kSegment / 2048; ++c) {
+  for (int c = 0; c < N; ++c) {
     const floatx4 x = row.clean(v[0]);
 #pragma unroll
-    for (int i = 0; i + 1 < kSegment / 2048; ++i) v[i] = v[i + 1];
+    for (int i = 0; i + 1 < N; ++i) v[i] = v[i + 1];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (!(x[e] > -INFINITY)) continue;
-      const u64 w = row.weight(x[e]);
+      const u64 w = weight_of(x[e], row.m, row.scale, a.frac, series);
       if (x[e] >= least) sum += w;
       if (!borders) continue;
       const int bin = ranges.of(x[e]);
@@ -789,14 +807,12 @@ __global__ void __launch_bounds__(512) sample_histogram_kernel(SampleArgs a) {
       a.mass[(size_t)blockIdx.x * kBins + i] = lds.hist[i];
       if (f.k > 0) a.count[(size_t)blockIdx.x * kBins + i] = counts[i];
     }
-  if (tid < 64) {
-    sum = row.sum_of(lds.wave, 8);
-    if (tid == 0) a.seg_mass[blockIdx.x] = sum;
-  }
+  if (tid < kParts) a.seg_mass[(size_t)blockIdx.x * kParts + tid] = lds.wave[2 * tid] + lds.wave[2 * tid + 1];
 }
 
 __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
   constexpr int TH = 1024, CHUNKS = kSegment / (4 * TH);
+  static_assert(CHUNKS == kParts, "a part is a chunk");
   __shared__ SampleLds lds;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, G = a.segments;
   // this thread's range over all segments (what lies there where no histogram was made is not used)
@@ -884,7 +900,10 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
   if (cut.above(least)) listed = -1;
   __syncthreads();
   if (listed < 0) {
-    if (tid < G) lds.super[tid] = a.seg_mass[(size_t)r * G + tid];
+    if (tid < G) {
+      const u64* const m = a.seg_mass + ((size_t)r * G + tid) * kParts;
+      lds.super[tid] = m[0] + m[1] + m[2] + m[3];
+    }
     __syncthreads();
   } else {
     for (int g = w; g < G; g += TH / 64) {
@@ -905,10 +924,17 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
   auto kept = [&](int i, float v) { return cut.keeps(v, i) ? row.weight(v) : (u64)0; };
   const u64 total = row.sum_of(lds.super, G);
   u64 at = row.place(r, total);
-  const int g = row.locate(lds.super, G, at), c1 = min((g + 1) * CHUNKS, row.n_chunks);
+  const int g = row.locate(lds.super, G, at);
+  int c0 = g * CHUNKS, c1 = min(c0 + CHUNKS, row.n_chunks);
+  if (listed < 0) {
+    if (tid < kParts) lds.wave[tid] = a.seg_mass[((size_t)r * G + g) * kParts + tid];
+    __syncthreads();
+    c0 += row.locate(lds.wave, kParts, at);
+    c1 = c0 + 1;
+  }
   __syncthreads();
-  row.sum_waves(g * CHUNKS, c1, kept);
-  const int token = row.pick_in(g * CHUNKS, c1, at, kept);
+  row.sum_waves(c0, c1, kept);
+  const int token = row.pick_in(c0, c1, at, kept);
   if (tid == 0) row.result(r, token, row.infinite ? 0.f : row.x[token], total);
 }
 
@@ -921,7 +947,7 @@ int segments_of(uint32_t vocab) { return vocab > (uint32_t)kStaged ? (int)((voca
 extern "C" size_t aur_sample_ws_bytes(uint32_t b, uint32_t vocab) {
   if (vocab > (uint32_t)kMaxVocab || b > 0x000fffffu) return 0;
   const size_t n = (size_t)b * segments_of(vocab);
-  return (n * (kBins * 12 + 8 + 4) + 15) / 16 * 16;
+  return (n * (kBins * 12 + 8 * kParts + 4) + 15) / 16 * 16;
 }
 
 extern "C" int aur_sample(aur_ctx* ctx, const float* logits, uint32_t ld, const float* u, const float* temperature,
@@ -947,7 +973,7 @@ extern "C" int aur_sample(aur_ctx* ctx, const float* logits, uint32_t ld, const 
     const size_t n = (size_t)b * a.segments;
     a.mass = static_cast<u64*>(scratch);
     a.seg_mass = a.mass + n * kBins;
-    a.count = reinterpret_cast<uint32*>(a.seg_mass + n);
+    a.count = reinterpret_cast<uint32*>(a.seg_mass + n * kParts);
     a.seg_max = reinterpret_cast<float*>(a.count + n * kBins);
     hipLaunchKernelGGL(sample_max_kernel, dim3((unsigned)n), dim3(512), 0, ctx->stream, a);
     AUR_LAUNCH_CHECK(ctx, "sample_max_kernel");
