@@ -111,11 +111,12 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a, int blocks_pe
 // NaN is held as NaN and has no part in m.
 //
 // A unit's new tokens lie in registers between its maximum and its rounding, so the rows are read once: one wave
-// holds up to 8 steps of 64 / LP tokens, LP lanes of 4 columns a head, and W = 4 waves share a unit that has
-// more (up to 16 steps each).  Blocks walk over `chunk` rows of the batch each (no more than a block of tokens has, so that two of a
-// sequence's units at most begin there) and take the units that begin in them, their last rows may lie behind.
-// 16 prompts of 512 to 1024 tokens, 16 heads of 64, blocks of 32, q rotated on the way: 55 us, 4.2 of the 5.1 TB/s
-// of a large copy; blocks of one token 54 (312 while a wave took one block at a time); a step of 32 sequences 5 us.
+// holds up to 8 steps of 64 / LP tokens, LP lanes of 4 columns a head, and W = 4 waves share a unit that has more
+// (up to 16 steps each).  Blocks walk over `chunk` rows of the batch each (no more than a block of tokens has, so
+// that two of a sequence's units at most begin there) and take the units that begin in them, their last rows may lie
+// behind.  16 prompts of 512 to 1024 tokens, 16 heads of 64, q rotated on the way: blocks of 32 tokens 55 us, 4.2 of
+// the 5.1 TB/s of a large copy, of 64 and 128 62 and 58 (by two waves those of 64 59), of one 54 (312 while a wave
+// took one block at a time); 8 heads of 128 take 66 to 76.  A step of 32 sequences: 6.5 us.
 struct UnitArgs {
   int chunk, n_chunks, groups;  // rows of a chunk; blocks of a chunk, 4 / W units each
 };

@@ -378,3 +378,28 @@ def test_one_page_of_two_sequences(ctx):
     for z in (new, q, q_out):
         z.free()
     dev.free()
+
+
+@pytest.mark.parametrize("dh", [8, 16, 32, 48, 64, 88, 128])
+@pytest.mark.parametrize("block", [1, 2, 8, 16, 32, 64, 128])
+@pytest.mark.parametrize("kv", [1, 3])
+def test_append_of_every_block(ctx, dh, block, kv):
+    """Every number of waves that share a block: whole blocks, first and last parts of some, growing scales."""
+    from aurora_amd.gpu import GpuBuffer, PagedKvAppendKernel
+
+    rng = np.random.default_rng(dh + block)
+    n, past = [150, 1, 40, 128], [0, 70, 100, 3]
+    c = Case8(rng, n, [x + y for x, y in zip(n, past)], 0, 128, kv, 1, dh, block, behind=3)
+    dev = Device8(ctx, c)
+    row = kv * dh
+    x = [(rng.standard_normal((c.n_tok, row)) * 2.0 ** rng.integers(-3, 4, (c.n_tok, 1))).astype(np.float32) for _ in range(2)]
+    k, v = (GpuBuffer.from_slice(ctx, a.ravel()) for a in x)
+    PagedKvAppendKernel.new().dispatch_into(ctx, dev.cache, dev.batch, 0, 0, k, v, row, 0, 0, 0, 0, 0, 0)
+    with np.errstate(invalid="ignore"):
+        c.append(*(a.reshape(-1, kv, dh) for a in x))
+    got = dev.bytes()
+    for a, w in zip(got[:2], (c.kb, c.vb)):
+        nan = w & 127 == 127
+        assert np.array_equal(a & 127 == 127, nan) and np.array_equal(a[~nan], w[~nan])
+    assert np.array_equal(got[2], c.ks) and np.array_equal(got[3], c.vs)
+    dev.free(), k.free(), v.free()
