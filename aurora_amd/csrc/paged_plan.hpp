@@ -61,6 +61,11 @@ constexpr int kPoolFrom = 65536;
 // 50.  d_head 64, with 64 and 256: 144 rows 27 and 35, 192 31 and 41, 256 36 and 45; bf16 20 and 28, 20 and 31,
 // 24 and 35: there too 64 rows are the faster up to 256, and its bound of 128 is short of that.
 constexpr int kPool64 = 128, kPool64Wide = 256;
+// For e4m3 keys, whose launches are shorter, 64 rows up to so many rows times prefix keys times K/V columns too: on 4
+// heads of 64, µs with 64 and 256 rows: 192 rows on 4999 20 and 32, on 16384 34 and 39, on 30000 49 and 48, on 65536
+// 85 and 74; 384 rows on 4999 30 and 36; 2 heads of 128, with 64 and 128: 512 rows on 6000 32 and 38, on 24000 70
+// and 57; 1024 rows on 1500 24 and 35, on 6000 50 and 42.
+constexpr double kPoolWorkE4m3 = 1.1e9;
 
 inline Plan make_plan(const Sizes& b) {
   Plan p{};
@@ -68,7 +73,8 @@ inline Plan make_plan(const Sizes& b) {
   const long long o_rows = (long long)b.max_tok * G, p_rows = (long long)b.n_tok * G;
   p.o_tile = tile_of(o_rows, dh);
   p.o_tiles = (int)((o_rows + p.o_tile - 1) / p.o_tile);
-  p.p_tile = p_rows <= 32 ? 16 : p_rows <= (dh > 64 ? kPool64Wide : kPool64) ? 64 : dh > 64 ? 128 : 256;
+  const bool light = b.e4m3 && (double)p_rows * P * Hkv * dh <= kPoolWorkE4m3;
+  p.p_tile = p_rows <= 32 ? 16 : light || p_rows <= (dh > 64 ? kPool64Wide : kPool64) ? 64 : dh > 64 ? 128 : 256;
   const int p_tiles = (int)((p_rows + p.p_tile - 1) / p.p_tile);
   p.pooled = o_rows < 64 && ((double)b.b * p.o_tiles - p_tiles) * Hkv * P >= kPoolFrom;
   if (p.pooled && p.p_tile == 16 && p.o_tile > 16) p.p_tile = 64;

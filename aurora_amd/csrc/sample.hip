@@ -256,8 +256,8 @@ struct Row {
   }
 
   // g(index, logit) of four logits.  A block that streams its row goes through much code once, and what it reads of
-  // code costs it more than a loop over one copy of g does (64 rows of 131072 that go through passes: 94 us, with four
-  // copies 124; 48 either way where the parts' sums spare them); a row in LDS is passed over by less (32 rows of 8192:
+  // code costs it more than a loop over one copy of g does (64 rows of 131072: 94 us, with four copies 124, while
+  // two lists and a segment's weights were made for each; 48 either way where the parts' sums spare those); a row in LDS is passed over by less (32 rows of 8192:
   // 10.9 us by four copies, 11.7 by one).
   template <class G>
   static __device__ __forceinline__ void one_by_one(floatx4 v, int i, G g) {

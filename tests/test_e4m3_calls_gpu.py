@@ -403,3 +403,18 @@ def test_append_of_every_block(ctx, dh, block, kv):
         assert np.array_equal(a & 127 == 127, nan) and np.array_equal(a[~nan], w[~nan])
     assert np.array_equal(got[2], c.ks) and np.array_equal(got[3], c.vs)
     dev.free(), k.free(), v.free()
+
+
+@pytest.mark.parametrize("b,kv,group,prefix,dh", [(200, 2, 4, 300, 64), (70, 1, 5, 700, 128), (150, 3, 1, 900, 24),
+                                                  (20, 4, 16, 14500, 64), (20, 2, 16, 14500, 128)])
+def test_prefixes_of_many_rows(ctx, b, kv, group, prefix, dh):
+    """Prefixes read once for more than 128 rows, light ones by items of 64 rows beside the own ones, heavy ones by
+    larger items."""
+    rng = np.random.default_rng(b)
+    c = Case8(rng, [1] * b, [1 + 7 * i % 40 for i in range(b)], prefix, 32, kv, group, dh, 8, behind=1)
+    dev = Device8(ctx, c)
+    dev.attend()
+    out, lse = dev.result()
+    want, want_lse, tol, tol_lse = attention_blocks(c)
+    assert np.all(np.abs(out[:b] - want[:b]) <= tol[:b]) and np.all(np.abs(lse[:b] - want_lse[:b]) <= tol_lse[:b])
+    dev.free()
