@@ -42,8 +42,9 @@ constexpr int kItems16 = 768, kItemsWide = 512, kItems = 1024, kItems8 = 256;
 constexpr int kWhole16 = 384, kWhole = 256, kWholeFull = 512, kFill = 256;
 constexpr int kLeastKeys = 128, kMostRanges = 48;
 // e4m3 keys: a CU holds two of their larger items, which take their keys faster (tails of 66 to 122 on 2048, 16
-// heads of 64: 71 µs with 512 items, 78 with 1024), and ranges of 256 keys (the prefix of 4999 alone, 48
-// sequences of 16 heads on 4 of 128: 23 µs, with 128 keys 29; d_head 64 with their own keys 32.5 and 31.4).
+// heads of 64: 71 µs with 512 items, 78 with 1024), and ranges of 256 keys (48 sequences of 16 heads on 4 of
+// 128, prefix 4999, own 500: 26.7 µs, with 192 keys 30.5, with 384 27.6; d_head 64 20.5, 22.6 and 21.1; 36 of them
+// on 1500 17.4, 15.8 and 20.1).
 constexpr int kItemsE4m3 = 512, kLeastKeysE4m3 = 256;
 // With little work the time is a block's chain of tiles, not the products: smaller items then.  16 rows up
 // to so many items of 16 rows by 128 keys (5 sequences of 74 rows on 434 keys, 3 heads of 48, bf16, 300 of
