@@ -111,7 +111,8 @@ struct Series {
     double x = 1.0;
     for (int i = 1; i <= 11; ++i) c[11 - i] = x *= l / i;
   }
-  // In registers, where the compiler would copy each one there from a constant in every use: for loops of weights.
+  // In registers, where the compiler would copy each one there from a constant in every use (32 rows of 32768, top_p:
+  // 37 us, 42 without; the last kernel of wide rows has no registers left for them).
   __device__ __forceinline__ void keep() {
 #pragma unroll
     for (int i = 0; i < 11; ++i) asm("" : "+v"(c[i]));
@@ -189,11 +190,14 @@ struct Row {
   int n_chunks;
   double scale, inv_t;  // log2(e) / T, 1 / T
   float m, T;
+  Series series;
   bool infinite;  // the largest logit is +∞: such ones count as 0, all others as −∞
 
   __device__ __forceinline__ Row(const SampleArgs& a, SampleLds& lds, floatx4* held, int r)
       : a(a), lds(lds), held(held), x(a.logits + (size_t)r * a.ld), n_chunks((a.vocab + 4 * TH - 1) / (4 * TH)),
-        infinite(false) {}
+        infinite(false) {
+    if (ROW > 0) series.keep();
+  }
   __device__ __forceinline__ void take(float most, float t) {
     infinite = most == INFINITY;
     m = infinite ? 0.f : most;
@@ -272,7 +276,7 @@ struct Row {
       }
     }
   }
-  __device__ __forceinline__ u64 weight(float v) const { return weight_of(v, m, scale, a.frac, Series()); }
+  __device__ __forceinline__ u64 weight(float v) const { return weight_of(v, m, scale, a.frac, series); }
 
   __device__ __forceinline__ float block_max(float v) {
     v = aurlanes::group_reduce<1, 64, true>(v);
@@ -939,8 +943,8 @@ __global__ void __launch_bounds__(1024) sample_finish_kernel(SampleArgs a) {
   if (tid == 0) row.result(r, token, row.infinite ? 0.f : row.x[token], total);
 }
 
-// A row that fits is chosen from by one block out of LDS: at 32768 tokens that takes 18 us from all of them, 42 with
-// top_p and 17 with top_k = 50, three launches on segments of it 37, 53 and 57.
+// A row that fits is chosen from by one block out of LDS: at 32768 tokens that takes 16 us from all of them, 37 with
+// top_p and 17 with top_k = 50 and top_p, three launches on segments of 40000 35, 52 and 58.
 int segments_of(uint32_t vocab) { return vocab > (uint32_t)kStaged ? (int)((vocab + kSegment - 1) / kSegment) : 0; }
 
 }  // namespace
@@ -985,8 +989,8 @@ extern "C" int aur_sample(aur_ctx* ctx, const float* logits, uint32_t ld, const 
     return 0;
   }
   // More threads pass over a long row sooner, fewer meet each other sooner at its barriers (top_p 0.95 on 32 rows,
-  // us by 256, 512 and 1024 threads: 8.7, 9.6 and 11.1 at 1000 tokens, 15.5, 13.1 and 14.0 at 4096, 24.2, 18.5 and
-  // 18.3 at 8192; drawn from all tokens 10.0, 8.9 and 9.4 there).
+  // us by 256, 512 and 1024 threads: 8.3, 9.0 and 10.0 at 1000 tokens, 14.6, 11.8 and 12.1 at 4096, 22.7, 16.6 and
+  // 15.8 at 8192; drawn from all tokens 9.2, 7.9 and 7.8 there).
   auto* kernel = vocab <= 1024   ? sample_kernel<256, 256>
                  : vocab <= 8192 ? sample_kernel<512, 2048>
                                  : sample_kernel<1024, kStaged / 4>;
