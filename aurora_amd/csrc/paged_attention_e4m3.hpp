@@ -23,6 +23,9 @@ constexpr int kUp = 7, kSpread = 15 + kUp;
 constexpr int kLeastScale = 10;   // byte of 2^-117, the least that an append gives
 constexpr int kNothing = 60;      // byte of 2^-67: beside it such ones are 2^-30 of its smallest number at most
 constexpr float kAbove = 14.f;    // log2 of the largest weight
+// Sums that leave no room for this factor below fp32's largest number are left to exact_sums, whose weights are at
+// most 1: up to 96 ranges of four waves each are added up later.
+constexpr float kRoom = 0x1p10f;
 
 struct Halves8 {  // eight numbers in two fp16 parts; the first is cut, the second has what that left
   f16x8 h, l;
@@ -274,7 +277,11 @@ __device__ __forceinline__ bool byte_sums(const MhaArgs& a, const Item& it, int 
 #pragma unroll
   for (int b = 0; b < VB; ++b)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) s.acc[0][b][c] *= back;
+    for (int c = 0; c < 4; ++c) {
+      s.acc[0][b][c] *= back;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fits &= !(fabsf(s.acc[0][b][c][i] * kRoom) == INFINITY);
+    }
   return __ballot(!fits) == 0;
 }
 
@@ -554,14 +561,17 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (DT * 16 == a.dh || 16 * d + 4 * g + i < a.dh) z += 0.f * acc[r][d][i];
+        if (DT * 16 == a.dh || 16 * d + 4 * g + i < a.dh) {
+          acc[r][d][i] *= back;
+          z += 0.f * (acc[r][d][i] * kRoom);
+        }
     const int row = row0 + 16 * r + l16;
     if (!exact && __ballot(row < it.n_rows && z != 0.f) == 0) {
       const float L = rows4_sum(l[r]);
       if (row < it.n_rows) {
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          if (DT * 16 == a.dh || 16 * d + 4 * g < a.dh) store(a, it, row, 16 * d + 4 * g, acc[r][d] * back, m[r], L);
+          if (DT * 16 == a.dh || 16 * d + 4 * g < a.dh) store(a, it, row, 16 * d + 4 * g, acc[r][d], m[r], L);
       }
     } else {
       store_exact<e4m3, DT>(a, it, row0 + 16 * r);

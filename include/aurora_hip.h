@@ -303,7 +303,8 @@ int aur_kv_read_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_page
  * aur_mha_paged_ws_bytes(cache, batch, n_head) (0: it may be NULL), which goes
  * by the host's fields alone; calls that overlap in time need a scratch each.
  * Sums are fp32 and joined in a fixed order: the same call gives the same bits.
- * `out` may not overlap q.
+ * They hold weights of up to 1 each times V: where these add up to 2^128 and more
+ * the result is an infinity (or NaN), for any type of pool.  `out` may not overlap q.
  * Smallest values: rows that pass through the matrix cores as bf16 parts lose
  * what lies below 2^-126 of K, of the scaled queries, of V and of the softmax's
  * weights, since those take no subnormal bf16.  V below 2^-110 then has an error
