@@ -19,8 +19,11 @@
 // Where top_k leaves few tokens, those are compared with each other instead.
 #include "common.hpp"
 #include "lanes.hpp"
+#include "sample_ranges.hpp"
 
 #include <cmath>
+
+using namespace aursample;
 
 namespace {
 
@@ -43,10 +46,9 @@ struct SampleArgs {
 
 typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int kBins = 1024, kList = 1024, kPairs = 64;
+constexpr int kList = 1024, kPairs = 64;
 constexpr int kSuper = 8;          // chunks whose weights are added up together
 constexpr int kMaxVocab = 1 << 20;
-constexpr float kLeastLogit = -3.402823466e38f;  // that can be chosen
 constexpr int kStaged = 32768;     // logits of a row in LDS
 constexpr int kSegment = 16384;    // … of a block, where several share a row
 constexpr int kMaxSegments = kMaxVocab / kSegment;
@@ -99,10 +101,6 @@ __device__ __forceinline__ u64 quad_sum(u64 x) {  // of four neighbouring lanes
 // The order of falling logits, equal ones by rising index.
 __device__ __forceinline__ bool before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
-// To the nearest whole number by adding 1.5·2^52, whose sum has it in its last bits.
-constexpr double kWhole = 6755399441055744.0;
-__device__ __forceinline__ int low32(double x) { return (int)(uint32)__double_as_longlong(x); }
-
 // The coefficients of 2^r's series from r^11 down to r.
 struct Series {
   double c[11];
@@ -134,22 +132,6 @@ __device__ __forceinline__ u64 weight_of(float v, float m, double scale, int fra
   return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
 }
 
-// The first ranges of a histogram: kBins of them down to where weights end; all below share the last one.
-struct Ranges {
-  double hi, inv;
-  __device__ __forceinline__ int of(float v) const { return low32(fmin((hi - (double)v) * inv, kBins - 1.0) + kWhole); }
-  // The least logit of the ranges 0 .. bin.
-  __device__ __forceinline__ float edge(int bin) const {
-    if (bin >= kBins - 1) return kLeastLogit;
-    const double c = hi - (bin + 0.5) / inv;
-    float v = c > kLeastLogit ? fminf((float)c, (float)hi) : kLeastLogit;
-    while (of(v) > bin) v = nextafterf(v, INFINITY);
-    while (v > kLeastLogit && of(nextafterf(v, -INFINITY)) <= bin) v = nextafterf(v, -INFINITY);
-    return v;
-  }
-};
-__device__ __forceinline__ Ranges first_ranges(float m, float T) { return {m, kBins / (32.0 * (double)T)}; }
-
 // A row's filters, those that do nothing as values that say so (k = 0, p = 1, floor_y = −∞).
 struct Filters {
   float T, p;
@@ -166,13 +148,7 @@ struct Filters {
   }
   // The least logit that min_p keeps of a row with the largest one m.
   __device__ __forceinline__ float least(float m) const {
-    if (floor_y == -INFINITY) return -INFINITY;
-    const double inv_t = 1.0 / (double)T, c = (double)m + (double)T * floor_y;
-    auto passes = [&](float v) { return v >= m || ((double)v - (double)m) * inv_t >= floor_y; };
-    float v = c > kLeastLogit ? fminf((float)c, m) : kLeastLogit;
-    while (!passes(v)) v = nextafterf(v, INFINITY);
-    while (v > kLeastLogit && passes(nextafterf(v, -INFINITY))) v = nextafterf(v, -INFINITY);
-    return v;
+    return floor_y == -INFINITY ? -INFINITY : least_kept(m, T, floor_y);
   }
   __device__ __forceinline__ bool greedy() const { return !(T > 0.f) || k == 1 || p <= 0.f; }
 };
