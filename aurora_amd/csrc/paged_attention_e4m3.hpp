@@ -54,9 +54,9 @@ __device__ __forceinline__ uint2v widen4(unsigned x, float scale) {
 struct Reference {
   int k, v;
 };
-// 2^(byte − of + kUp), and whether an item can go on with it.
-__device__ __forceinline__ float relative(int byte, int of, bool& fits) {
-  fits &= byte != 255 && (of - byte <= kSpread || (byte <= kLeastScale && of >= kNothing));
+// 2^(byte − of + kUp), and whether an item can go on with it (always, where there is no key).
+__device__ __forceinline__ float relative(int byte, int of, bool there, bool& fits) {
+  fits &= !there || (byte != 255 && (of - byte <= kSpread || (byte <= kLeastScale && of >= kNothing)));
   return scale_of((unsigned)max(127 + kUp + byte - of, 0));
 }
 // The larger of k and v bytes, each packed in 16 bits, over lanes 0 .. 63 (or of each half alike).
@@ -197,7 +197,7 @@ __device__ __forceinline__ bool byte_sums(const MhaArgs& a, const Item& it, int 
       ref = Reference{k, v};
       q.relative_to(k);
     }
-    const float ks = relative(kb, ref.k, fits), vs = relative(vb, ref.v, fits);
+    const float ks = relative(kb, ref.k, at >= 0, fits), vs = relative(vb, ref.v, at >= 0, fits);
     floatx4 st[1][2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -335,6 +335,7 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
   const long long ld = (long long)a.Hkv * a.dh;
   int xp = it.x0 + tid;  // the key whose page is under way
   int k_scale = 0, v_scale = 0;
+  bool is = false;  // a key has them
   auto place = [&](int slot) {
     if (tid < KT) {
       const int last = slot == 0 ? 2 : slot - 1;
@@ -343,13 +344,14 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
         const unsigned top = __builtin_amdgcn_readfirstlane(wave_top((unsigned)k_scale << 16 | (unsigned)v_scale));
         next = Reference{max(ref.k, (int)(top >> 16)), max(ref.v, (int)(top & 0xffff))};
       }
-      lds.scale[last][0][tid] = relative(k_scale, next.k, fits);
-      lds.scale[last][1][tid] = relative(v_scale, next.v, fits);
+      lds.scale[last][0][tid] = relative(k_scale, next.k, is, fits);
+      lds.scale[last][1][tid] = relative(v_scale, next.v, is, fits);
       const int at = row_of(a, it, xp, page);
       const size_t s = scale_index(max(at, 0), it.hk, a.Hkv, a.sh, a.ssh);
       k_scale = a.k_scale[s];
       v_scale = a.v_scale[s];
-      if (at < 0) k_scale = v_scale = 0;
+      is = at >= 0;
+      if (!is) k_scale = v_scale = 0;
       lds.offset[slot][tid] = at < 0 ? 0 : at * ld;
       const unsigned long long have = __ballot(at >= 0);
       if (tid == 0) {

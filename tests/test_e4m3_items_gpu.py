@@ -31,3 +31,23 @@ def test_values_near_the_largest(ctx, n, prefix, group, v_e, equal):
     dev.attend()
     _check(c, *dev.result())
     dev.free()
+
+
+@pytest.mark.parametrize("n,prefix,group", ITEMS)
+@pytest.mark.parametrize("k_e,v_e", [(0, -100), (0, -70), (-100, 0), (-70, 0), (-90, -90), (60, 60)])
+def test_the_size_of_all_scales_changes_no_bit(ctx, n, prefix, group, k_e, v_e):
+    """Scales of one power of two more, for which the queries make up: the same products, so the same bits times that
+    power, whatever stands in a last tile's places without a key."""
+    c = Case8(np.random.default_rng(4), n, [x + 23 for x in n], prefix, 16, 1, group, 64, 8)
+    got = []
+    for k, v in ((0, 0), (k_e, v_e)):
+        c.ks = np.where(c.ks == 255, 255, c.ks.astype(int) + k).astype(np.uint8)
+        c.vs = np.where(c.vs == 255, 255, c.vs.astype(int) + v).astype(np.uint8)
+        c.q *= np.float32(2.0**-k)
+        dev = Device8(ctx, c)
+        dev.attend()
+        got.append(dev.result())
+        dev.free()
+    rows = int(c.off[-1])
+    assert np.array_equal(got[1][0][:rows], got[0][0][:rows] * np.float32(2.0**v_e))
+    assert np.array_equal(got[1][1], got[0][1])
