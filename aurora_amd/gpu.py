@@ -421,21 +421,25 @@ class SampleKernel(_Kernel):
     """The next token of each row of logits [b, vocab] from a random number u [b]: tokens [b] int32 and, unless
     0, logprob [b].  temperature, top_k (int32), top_p and min_p are arrays of b values, 0 for none.
 
-    For more than 32768 tokens the object keeps a scratch, allocated when a call needs a larger one (or ahead,
-    by `reserve`: a captured call cannot allocate); calls that overlap in time take an object each.  One that was
-    outgrown is kept until `free`, since a captured call may still use it."""
+    For more than 32768 tokens the object keeps a scratch for each context, allocated when a call needs a larger one
+    (or ahead, by `reserve`: a captured call cannot allocate); calls of a context that overlap in time take an object
+    each.  One that was outgrown is kept until `free`, since a captured call may still use it; the next is twice as
+    large at least, so all of them together are no more than twice the last."""
 
     def __init__(self):
-        self._scratch = []  # the last one is in use
+        self._scratch = []  # a context's last one is in use
 
     @staticmethod
     def scratch_bytes(b, vocab) -> int:
         return _lib.load().aur_sample_ws_bytes(b, vocab)
 
     def reserve(self, ctx, b, vocab) -> None:
-        n = self.scratch_bytes(b, vocab)
-        if n and not (self._scratch and self._scratch[-1].nbytes >= n and self._scratch[-1].ctx is ctx):
-            self._scratch.append(GpuBuffer.empty(ctx, n, np.uint8))
+        n, held = self.scratch_bytes(b, vocab), self._held(ctx)
+        if n and (held is None or held.nbytes < n):
+            self._scratch.append(GpuBuffer.empty(ctx, max(n, 2 * held.nbytes if held else 0), np.uint8))
+
+    def _held(self, ctx):
+        return next((s for s in reversed(self._scratch) if s.ctx is ctx), None)
 
     def free(self) -> None:
         while self._scratch:
@@ -451,6 +455,7 @@ class SampleKernel(_Kernel):
         scratch, nbytes = 0, 0
         if vocab > 32768:
             self.reserve(ctx, b, vocab)
-            if self._scratch:
-                scratch, nbytes = self._scratch[-1].ptr, self._scratch[-1].nbytes
+            held = self._held(ctx)
+            if held:
+                scratch, nbytes = held.ptr, held.nbytes
         ctx.call("aur_sample", logits, ld, u, temperature, top_k, top_p, min_p, tokens, logprob, scratch, nbytes, b, vocab)
