@@ -1,7 +1,9 @@
 // Items of 16 rows and more on pools of e4m3: what is included by paged_attention.hpp.
 //
 // An e4m3 number is an fp16 one, so K and V go into the fp16 MFMA as they are, and queries and weights as two
-// fp16 parts, which keep 2^-20 of them: two products where bf16 parts of the same accuracy take three.  Bound by
+// fp16 parts, both rounded to nearest: their error is at most 2^-23 of a number, one unit in fp32's last place, where
+// the three bf16 parts of the bf16 pools leave 2^-24 for a product more.  (Numbers below 2^-11 of the row's largest
+// are kept to 2^-34 of that.)  Parts cut toward zero left 2^-21, all on one side.  Bound by
 // the softmax's instructions and the MFMA's between them: 16 sequences of 512 tokens on a prefix of 4096, 16 heads
 // of 64, 309 us, 350 TFLOP/s of the 600 that a large library product's rate leaves for two (the first form, of three
 // bf16 products and two barriers a tile, 478); a step of 64 sequences of 1024 keys on 32768, 16 heads of 64, 71 us,
@@ -27,16 +29,16 @@ constexpr float kAbove = 14.f;    // log2 of the largest weight
 // most 1: up to 96 ranges of four waves each are added up later.
 constexpr float kRoom = 0x1p10f;
 
-struct Halves8 {  // eight numbers in two fp16 parts; the first is cut, the second has what that left
+struct Halves8 {  // eight numbers in two fp16 parts; the second has what rounding to the first left
   f16x8 h, l;
   __device__ __forceinline__ void set(int i, float x0, float x1) {
     // A factor that the compiler does not know to be -1 leaves x - (float)h one instruction of mixed operands, where
     // it would take two (16 sequences of 512 tokens on 4096, 16 heads of 64: 309 us, 326 without).
     float minus;
     asm("s_mov_b32 %0, -1.0" : "=s"(minus));
-    const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)a[0], minus, x0),
-                                                                         __builtin_fmaf((float)a[1], minus, x1)));
+    const f16x2 a = __builtin_convertvector(float2v{x0, x1}, f16x2);
+    const float2v rest = {__builtin_fmaf((float)a[0], minus, x0), __builtin_fmaf((float)a[1], minus, x1)};
+    const f16x2 b = __builtin_convertvector(rest, f16x2);
     h[i] = a[0], h[i + 1] = a[1];
     l[i] = b[0], l[i + 1] = b[1];
   }

@@ -312,10 +312,11 @@ int aur_kv_read_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_page
  * from a column of 2^-115 in a key of 64 and 2^115 in the query.  With fp32 pools
  * these are items of more than 16 query rows of a K/V head (a prefix read once for
  * all counts the rows of the whole batch), with bf16 pools all but single tokens of
- * one or two rows.  e4m3 pools: queries and weights are kept to 2^-20 of the largest
- * of their row in the same items; blocks of one item whose scales lie more than 2^22
- * apart are summed in fp32, some 50 times slower, but for scales of 2^-117 and
- * less (what an append gives to zeros), which count as 0 beside 2^-67 and more. */
+ * one or two rows.  e4m3 pools: in the same items queries and weights are kept to
+ * 2^-23 of each, or to 2^-34 of the largest of their row where that is more; blocks
+ * of one item whose scales lie more than 2^22 apart are summed in fp32, some 50
+ * times slower, but for scales of 2^-117 and less (what an append gives to zeros),
+ * which count as 0 beside 2^-67 and more. */
 size_t aur_mha_paged_ws_bytes(const aur_paged_cache* cache, const aur_paged_batch* batch,
                               uint32_t n_head);
 int aur_mha_paged(aur_ctx* ctx, const aur_paged_cache* cache, const aur_paged_batch* batch,
