@@ -626,7 +626,7 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
   if constexpr (sizeof(T) == 1) {
     if (x < it.x1) {
       const bool good = byte_sums<DT>(a, it, x, STRIDE, page, s);
-      if (!good || !finite(s, it.row0 + l16 < it.n_rows)) exact_sums<T, DT, RT>(a, it, it.row0, x, STRIDE, s);
+      if (!good) exact_sums<T, DT, RT>(a, it, it.row0, x, STRIDE, s);
     }
   } else if (x < it.x1) {
     Keys32<T, DT> keys;

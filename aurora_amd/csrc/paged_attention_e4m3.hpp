@@ -46,6 +46,10 @@ struct Halves8 {  // eight numbers in two fp16 parts; the second has what roundi
 __device__ __forceinline__ floatx4 mfma_f16(f16x8 a, f16x8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+// The largest of m and the sizes of x; NaN if one is.
+__device__ __forceinline__ float larger4(float m, floatx4 x) {
+  return max3(max3(m, fabsf(x[0]), fabsf(x[1])), fabsf(x[2]), fabsf(x[3]));
+}
 // Four e4m3 numbers times a power of two as two pairs of fp16.
 __device__ __forceinline__ uint2v widen4(unsigned x, float scale) {
   return uint2v{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, false)),
@@ -55,10 +59,11 @@ __device__ __forceinline__ uint2v widen4(unsigned x, float scale) {
 // Largest scales so far, as bytes; the same in all lanes.
 struct Reference {
   int k, v;
+  static __device__ __forceinline__ Reference none() { return {-2, -2}; }  // below a key's that is not there
 };
-// 2^(byte − of + kUp), and whether an item can go on with it (always, where there is no key).
-__device__ __forceinline__ float relative(int byte, int of, bool there, bool& fits) {
-  fits &= !there || (byte != 255 && (of - byte <= kSpread || (byte <= kLeastScale && of >= kNothing)));
+// 2^(byte − of + kUp), and whether an item can go on with it (byte −1: there is no key, always).
+__device__ __forceinline__ float relative(int byte, int of, bool& fits) {
+  fits &= byte < 0 || (byte != 255 && (of - byte <= kSpread || (byte <= kLeastScale && of >= kNothing)));
   return scale_of((unsigned)max(127 + kUp + byte - of, 0));
 }
 // The larger of k and v bytes, each packed in 16 bits, over lanes 0 .. 63 (or of each half alike).
@@ -128,7 +133,7 @@ struct Bytes32 {
   static constexpr int VB = (DT + 3) / 4, KC = (DT + 1) / 2;
   uint2v k[2][KC];
   unsigned v[2][4][VB];
-  int k_scale, v_scale;  // bytes, 0 where there is no key
+  int k_scale, v_scale;  // bytes (where there is no key, row 0's)
   __device__ __forceinline__ void load_k(const MhaArgs& a, int hk, int at, int g, int l16) {
     const size_t ld = (size_t)a.Hkv * a.dh;
     const uint8_t* kp = static_cast<const uint8_t*>(a.k) + (size_t)hk * a.dh;
@@ -179,15 +184,15 @@ __device__ __forceinline__ bool byte_sums(const MhaArgs& a, const Item& it, int 
   q.load(rows, a.dh, g, a.scale * LOG2E);
   keys.load_v(a, it.hk, at, g, l16);
   page = page_of(a, it.s, it.pre, x + stride + k32);
-  Reference ref{-1, -1};
+  Reference ref = Reference::none();
   bool fits = true;
   for (; x < it.x1; x += stride) {
     // the next keys' loads go out as soon as this step has used the registers
     const bool more = x + stride < it.x1;
     const unsigned there = (unsigned)__ballot(at >= 0);
-    const int kb = at >= 0 ? keys.k_scale : 0, vb = at >= 0 ? keys.v_scale : 0;
+    const int kb = at >= 0 ? keys.k_scale : -1, vb = at >= 0 ? keys.v_scale : -1;
     if (__ballot(kb > ref.k || vb > ref.v)) {  // a scale grew: rarely, after the first steps
-      const unsigned top = __builtin_amdgcn_readfirstlane(wave_top((unsigned)kb << 16 | (unsigned)vb));
+      const unsigned top = __builtin_amdgcn_readfirstlane(wave_top((unsigned)max(kb, 0) << 16 | (unsigned)max(vb, 0)));
       const int k = max(ref.k, (int)(top >> 16)), v = max(ref.v, (int)(top & 0xffff));
       if (v != ref.v && ref.v >= 0) {
         const float less = ldexpf(1.f, ref.v - v);
@@ -199,7 +204,7 @@ __device__ __forceinline__ bool byte_sums(const MhaArgs& a, const Item& it, int 
       ref = Reference{k, v};
       q.relative_to(k);
     }
-    const float ks = relative(kb, ref.k, at >= 0, fits), vs = relative(vb, ref.v, at >= 0, fits);
+    const float ks = relative(kb, ref.k, fits), vs = relative(vb, ref.v, fits);
     floatx4 st[1][2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -279,12 +284,13 @@ __device__ __forceinline__ bool byte_sums(const MhaArgs& a, const Item& it, int 
 #pragma unroll
   for (int b = 0; b < VB; ++b)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      s.acc[0][b][c] *= back;
+    for (int c = 0; c < 4; ++c) s.acc[0][b][c] *= back;
+  float top = s.l[0];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) fits &= !(fabsf(s.acc[0][b][c][i] * kRoom) == INFINITY);
-    }
-  return __ballot(!fits) == 0;
+  for (int b = 0; b < VB; ++b)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) top = larger4(top, s.acc[0][b][c]);
+  return __ballot(!fits || (it.row0 + l16 < it.n_rows && !(top * kRoom < INFINITY))) == 0;
 }
 
 // ---------------------------------------------------------------- many rows: keys through LDS
@@ -332,28 +338,26 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
 
   // Where a tile's keys lie; the first wave asks for the pages' numbers a tile before they are needed, and lays
   // the scales down a tile after it asked for them, relative to the reference that this tile will have.
-  Reference ref{-1, -1};
+  Reference ref = Reference::none();
   bool fits = true;
   const long long ld = (long long)a.Hkv * a.dh;
   int xp = it.x0 + tid;  // the key whose page is under way
-  int k_scale = 0, v_scale = 0;
-  bool is = false;  // a key has them
+  int k_scale = -1, v_scale = -1;
   auto place = [&](int slot) {
     if (tid < KT) {
       const int last = slot == 0 ? 2 : slot - 1;
       Reference next = ref;
       if (__ballot(k_scale > ref.k || v_scale > ref.v)) {
-        const unsigned top = __builtin_amdgcn_readfirstlane(wave_top((unsigned)k_scale << 16 | (unsigned)v_scale));
+        const unsigned top = __builtin_amdgcn_readfirstlane(wave_top((unsigned)max(k_scale, 0) << 16 | (unsigned)max(v_scale, 0)));
         next = Reference{max(ref.k, (int)(top >> 16)), max(ref.v, (int)(top & 0xffff))};
       }
-      lds.scale[last][0][tid] = relative(k_scale, next.k, is, fits);
-      lds.scale[last][1][tid] = relative(v_scale, next.v, is, fits);
+      lds.scale[last][0][tid] = relative(k_scale, next.k, fits);
+      lds.scale[last][1][tid] = relative(v_scale, next.v, fits);
       const int at = row_of(a, it, xp, page);
       const size_t s = scale_index(max(at, 0), it.hk, a.Hkv, a.sh, a.ssh);
       k_scale = a.k_scale[s];
       v_scale = a.v_scale[s];
-      is = at >= 0;
-      if (!is) k_scale = v_scale = 0;
+      if (at < 0) k_scale = v_scale = -1;
       lds.offset[slot][tid] = at < 0 ? 0 : at * ld;
       const unsigned long long have = __ballot(at >= 0);
       if (tid == 0) {
@@ -560,22 +564,17 @@ __device__ __forceinline__ void byte_tile_item(const MhaArgs& a, ByteLds<DT, W>&
 
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    float z = 0.f * l[r];
+    float top = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (DT * 16 == a.dh || 16 * d + 4 * g + i < a.dh) {
-          acc[r][d][i] *= back;
-          z += 0.f * (acc[r][d][i] * kRoom);
-        }
+      if (DT * 16 == a.dh || 16 * d + 4 * g < a.dh) top = larger4(top, acc[r][d]);
     const int row = row0 + 16 * r + l16;
-    if (!exact && __ballot(row < it.n_rows && z != 0.f) == 0) {
+    if (!exact && __ballot(row < it.n_rows && !(top * back * kRoom < INFINITY)) == 0) {
       const float L = rows4_sum(l[r]);
       if (row < it.n_rows) {
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          if (DT * 16 == a.dh || 16 * d + 4 * g < a.dh) store(a, it, row, 16 * d + 4 * g, acc[r][d], m[r], L);
+          if (DT * 16 == a.dh || 16 * d + 4 * g < a.dh) store(a, it, row, 16 * d + 4 * g, acc[r][d] * back, m[r], L);
       }
     } else {
       store_exact<e4m3, DT>(a, it, row0 + 16 * r);

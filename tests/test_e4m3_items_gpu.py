@@ -101,3 +101,15 @@ def test_queries_keep_their_last_bits(ctx, n, prefix, group, dh):
     err = np.abs(lse[: len(t)] - want)
     print(f"{err.max() / (2.0**-9 * np.log(2)):.2f} of 3.5")
     assert err.max() <= 3.5 * 2.0**-9 * np.log(2)
+
+
+@pytest.mark.parametrize("n,prefix,group", ITEMS)
+def test_items_whose_first_keys_are_not_there(ctx, n, prefix, group):
+    """Pages that are not there at the start of both axes, so that whole tiles and items have no key."""
+    c = Case8(np.random.default_rng(6), n, [x + 150 for x in n], prefix, 16, 1, group, 64, 8)
+    c.prefix_pages[: len(c.prefix_pages) // 2] = -1
+    c.pages[:, :8] = c.n_pages + 3
+    dev = Device8(ctx, c)
+    dev.attend()
+    _check(c, *dev.result())
+    dev.free()
