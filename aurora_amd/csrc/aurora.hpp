@@ -221,15 +221,17 @@ struct PagedKvCache<uint8_t> {
   aur_paged_cache raw;
   PagedKvCache(const GpuContext& c, uint32_t n_pages, uint32_t page_len, uint32_t n_kv_head, uint32_t d_head,
                uint32_t scale_len)
-      : k(GpuBuffer<uint8_t>::zeros(c, (size_t)n_pages * page_len * n_kv_head * d_head)),
+      : k(GpuBuffer<uint8_t>::zeros(c, scales(n_pages, page_len, n_kv_head, scale_len) * scale_len * d_head)),
         v(GpuBuffer<uint8_t>::zeros(c, (size_t)n_pages * page_len * n_kv_head * d_head)),
         k_scale(GpuBuffer<uint8_t>::zeros(c, scales(n_pages, page_len, n_kv_head, scale_len))),
         v_scale(GpuBuffer<uint8_t>::zeros(c, scales(n_pages, page_len, n_kv_head, scale_len))),
         raw{k.ptr(), v.ptr(), n_pages, page_len, n_kv_head, d_head, AUR_PAGED_E4M3, k_scale.ptr(), v_scale.ptr(), scale_len} {}
 
- private:
+  // How many there are of K, and of V; refuses a length that no call would take, before anything is allocated.
   static size_t scales(uint32_t n_pages, uint32_t page_len, uint32_t n_kv_head, uint32_t scale_len) {
-    if (scale_len == 0 || page_len % scale_len != 0) throw Error("PagedKvCache: bad scale_len", AUR_EINVAL);
+    if (scale_len == 0 || (scale_len & (scale_len - 1)) != 0 || page_len % scale_len != 0)
+      throw Error("PagedKvCache: bad scale_len", AUR_EINVAL);
+    if (scale_len > 128) throw Error("PagedKvCache: scale_len above 128", AUR_ELIMIT);
     return (size_t)n_pages * n_kv_head * (page_len / scale_len);
   }
 };

@@ -303,8 +303,8 @@ class PagedKvCache:
     def _check(cls, dtype, page_len, scale_len) -> None:
         if dtype not in cls.DTYPES:
             raise ValueError(f"PagedKvCache: dtype {dtype!r}, one of {sorted(cls.DTYPES)}")
-        if dtype == "e4m3" and not (0 < scale_len <= page_len and scale_len & (scale_len - 1) == 0):
-            raise ValueError(f"PagedKvCache: scale_len {scale_len}, a power of two up to page_len {page_len}")
+        if dtype == "e4m3" and not (0 < scale_len <= min(page_len, 128) and scale_len & (scale_len - 1) == 0):
+            raise ValueError(f"PagedKvCache: scale_len {scale_len}, a power of two up to 128 and page_len {page_len}")
 
     @property
     def elements(self) -> int:
