@@ -162,10 +162,11 @@ def _need(what: str, n: int, *bufs) -> None:
     """The kernels touch exactly the extents their dimensions name; a
     GpuBuffer shorter than that is refused before the launch (the reference's
     WGSL had wgpu's bounds-checked buffer access; an out-of-range access on the
-    GPU faults).  Raw device pointers carry no length and pass unchecked."""
+    GPU faults).  Their elements have 4 bytes each, whatever the buffer's type is.  Raw device pointers carry
+    no length and pass unchecked."""
     for b in bufs:
-        if isinstance(b, GpuBuffer) and b.len < n:
-            raise ValueError(f"{what}: buffer of {b.len} elements, {n} needed")
+        if isinstance(b, GpuBuffer) and (b.len < n or b.nbytes < 4 * n):
+            raise ValueError(f"{what}: buffer of {b.len} elements of {b.dtype.itemsize} bytes, {n} of 4 needed")
 
 
 class _Kernel:
