@@ -58,8 +58,9 @@ struct MhaArgs {
 
 // The dice take blocks in turn, and each has an L2 of its own with lines of 128 bytes.  Where a head's row is
 // shorter than that, the items of all K/V heads on the same keys go to one die, one after the other, so that a
-// line is fetched once and not by every die that wants a part of it (64 sequences of 1024 keys, 16 heads of 64 in
-// e4m3: 40 us without this order, 24 with it).  With fewer than kDice sets of such items some dice would have none.
+// line is fetched once and not by every die that wants a part of it (64 sequences of 512 to 1024 keys, 16 heads of 64
+// in e4m3, out of the chip's caches: 40 us without this order, 24 with it).  With fewer than kDice sets of such items
+// some dice would have none.
 constexpr int kDice = 8;
 inline bool heads_by_xcd(int row_bytes, uint64_t p_groups, uint64_t o_groups) {
   return row_bytes < 128 && o_groups >= kDice && (p_groups == 0 || p_groups >= kDice);
@@ -600,7 +601,7 @@ __device__ __forceinline__ void store_exact(const MhaArgs& a, const Item& it, in
 // which keep 2^-24 of each.  A wave's next K is under way while it works, its V from the scores on.  Bound
 // by the reading with the MFMA's cycles in between: 64 sequences of 512 to 1024 keys (768 on average), 16
 // K/V heads of 64, 4 rows each: 56 µs in bf16 (3.7 TB/s), 92 in fp32 (4.5 TB/s); with 1024 keys each 62 µs
-// in bf16 (4.3 TB/s), 38 in e4m3 (3.5 TB/s).  On widened keys the fp32 MFMA took bf16's own keys of 64 such sequences 160 µs in a
+// in bf16 (4.3 TB/s), 43 in e4m3 (3.1 TB/s).  On widened keys the fp32 MFMA took bf16's own keys of 64 such sequences 160 µs in a
 // first version, the bf16 one 60.
 template <int DT>
 __device__ bool byte_sums(const MhaArgs& a, const Item& it, int x, int stride, int page, Sums<DT, 1>& s);  // e4m3 keys
@@ -699,10 +700,10 @@ __device__ __forceinline__ void rows_item(const MhaArgs& a, RowsLds<DT>& lds) {
 // average), 16 K/V heads of 64, µs by vectors and by the MFMA: 1 row 67 and 85 (5.9 TB/s), 2 rows 73 and 84,
 // 4 rows 83 and 92; bf16 keys 1 row 40 and 53 (5.0 TB/s), 2 rows 43 and 54, 4 rows 55 and 56 (with a prefix
 // of 2048 beside it 40 and 38): so 4 rows in fp32, 2 in bf16.  With 1024 keys each, by vectors: fp32 85 µs
-// (6.3 TB/s), 88 and 94, bf16 48 µs (5.6 TB/s) and 49, e4m3 (out of the chip's caches, which hold them) 24 and 31,
-// by the MFMA 32 and 32, and 4 rows 43 against 33: so 2 rows in e4m3 as well.  LP lanes have a key's head, 16
-// bytes each (8 of e4m3), so that a load brings 64/LP whole keys; a score is added up over the LP lanes, l and the
-// columns over the key groups once at the end, all of it in fp32.  While one half of the registers is in use, the
+// (6.3 TB/s), 88 and 94, bf16 48 µs (5.6 TB/s) and 49, e4m3 33 µs (4.0 TB/s) and 41.  e4m3 keys of 512 to 1024 (out of
+// the chip's caches, which hold them) by vectors 24 and 31, by the MFMA 32 and 32, and 4 rows 43 against 33: so 2 rows
+// in e4m3 as well.  LP lanes have a key's head, 16 bytes each (8 of e4m3), so that a load brings 64/LP whole keys;
+// a score is added up over the LP lanes, l and the columns over the key groups once at the end, all of it in fp32.  While one half of the registers is in use, the
 // loads of the other are under way, and the page of the step after them.
 template <class T, int DT>
 struct FewRows {
@@ -1229,7 +1230,8 @@ union StepLds {
 // d_head 33 to 64.  µs with three and with two, 16 heads: 100 sequences on a prefix of 8192, d_head 64 39.6 and
 // 43.5; 30 of 32 heads on 8, prefix 4096 19.7 and 21.9; 64 on 32768 82 and 77.6, without own keys 48.6 and 51;
 // of d_head 48 on 16384 63.2 and 61.6; tails of 30 to 60 tokens on 2048 51.4 and 49.5.  e4m3 keys, whose tiles wait
-// in registers as bytes beside two parts of Q, want two: 64 on 32768 75 and 60, without own keys 46 and 52.
+// in registers as bytes beside two parts of Q, want two: 64 on 32768 94 and 64, without own keys, out of the chip's
+// caches, 48 and 50.
 template <class T, int DT, int NR>
 constexpr int kWaves = sizeof(T) == 2 && DT <= 4 && NR == 1 ? 3 : 2;
 

@@ -5,9 +5,9 @@
 // the three bf16 parts of the bf16 pools leave 2^-24 for a product more.  (Numbers below 2^-11 of the row's largest
 // are kept to 2^-34 of that.)  Parts cut toward zero left 2^-21, all on one side.  Bound by
 // the softmax's instructions and the MFMA's between them: 16 sequences of 512 tokens on a prefix of 4096, 16 heads
-// of 64, 309 us, 350 TFLOP/s of the 600 that a large library product's rate leaves for two (the first form, of three
-// bf16 products and two barriers a tile, 478); a step of 64 sequences of 1024 keys on 32768, 16 heads of 64, 71 us,
-// 52 of them for the prefix.  The weights' sums as products with ones: 313 us, d_head 128 354 instead of 337.
+// of 64, 310 us, 350 TFLOP/s of the 600 that a large library product's rate leaves for two (the first form, of three
+// bf16 products and two barriers a tile, 478); a step of 64 sequences of 512 to 1024 keys on 32768, 16 heads of 64,
+// 64 us, 50 of them for the prefix.  The weights' sums as products with ones: 4 us more, d_head 128 17 of 337.
 //   * Scales.  Relative to the largest scale 2^E seen so far, of K and of V, a key's scale is 2^(e − E + kUp), which
 //     the conversion to fp16 multiplies by: 448 times the largest one's is near fp16's end, and down to e − E =
 //     −kSpread, where the smallest e4m3 number is the smallest fp16 one, that is exact.  E goes into the factor of
@@ -33,7 +33,7 @@ struct Halves8 {  // eight numbers in two fp16 parts; the second has what roundi
   f16x8 h, l;
   __device__ __forceinline__ void set(int i, float x0, float x1) {
     // A factor that the compiler does not know to be -1 leaves x - (float)h one instruction of mixed operands, where
-    // it would take two (16 sequences of 512 tokens on 4096, 16 heads of 64: 309 us, 326 without).
+    // it would take two (16 sequences of 512 tokens on 4096, 16 heads of 64: 310 us, 327 without).
     float minus;
     asm("s_mov_b32 %0, -1.0" : "=s"(minus));
     const f16x2 a = __builtin_convertvector(float2v{x0, x1}, f16x2);
